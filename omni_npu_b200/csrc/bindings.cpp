@@ -105,6 +105,14 @@ int b200_gqa_decode_ex(const void* q, const void* k_cache, const void* v_cache, 
                        int persistent, int* work_counter, cudaStream_t stream);
 int b200_kv_p2p_copy(const void* tensors, int num_tensors, const int* src_blocks, const int* dst_blocks,
                      int num_pairs, long long max_block_bytes, cudaStream_t stream);
+int b200_cache_copy(const void* tensors, int num_tensors, const int* pairs, int num_pairs, int page, int max_vecs, int sms,
+                    cudaStream_t stream);
+int b200_lora_plan(const int* slots, int T, int L, int rows, int* order, int* tiles, int* num_tiles, int* status,
+                   cudaStream_t stream);
+int b200_lora(const void* x, long long x_stride, const void* y, long long y_stride, void* out, long long out_stride,
+              const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks, const float* scales,
+              const int* order, const int* tiles, const int* num_tiles, int max_tiles, int rows, int K, int slices,
+              const int* n, int max_rank, int act, float act_alpha, float act_limit, cudaStream_t stream);
 size_t b200_mla_decode_scratch_bytes(int total_tokens, int N, int splits);
 int b200_mla_decode(const void* q, const void* cache, void* out, float* lse, const int* block_tables,
                     const int* seq_lens, const int* topk_indices, int topk, int B, int q_len, int N,
@@ -712,6 +720,102 @@ void kv_p2p_copy(const Tensor& desc, const Tensor& src_blocks, const Tensor& dst
         "kv_p2p_copy");
 }
 
+// Copies of pages inside a cache.  desc: int64 [tensors, 4] = (base, page bytes, head bytes, heads | vectors of a row << 32);
+// pairs: (source, destination, rows) one after another.  Returns the number of launches.
+int64_t cache_copy(const Tensor& desc, at::IntArrayRef pairs, int64_t blocks, int64_t page, int64_t max_vecs) {
+  TORCH_CHECK(desc.is_cuda() && desc.scalar_type() == at::kLong && desc.dim() == 2 && desc.size(1) == 4 && desc.is_contiguous(),
+              "cache_copy: desc int64 [n,4] on the device");
+  TORCH_CHECK_VALUE(pairs.size() % 3 == 0, "cache_copy: triples");
+  std::vector<int> p(pairs.size());
+  std::vector<char> use(blocks, 0);                        // 1: read, 2: written
+  for (size_t i = 0; i < pairs.size(); i += 3) {
+    TORCH_CHECK_VALUE(pairs[i] >= 0 && pairs[i] < blocks && pairs[i + 1] >= 0 && pairs[i + 1] < blocks && pairs[i + 2] >= 0 &&
+                          pairs[i + 2] <= page,
+                      "copy_blocks: a page outside 0 .. ", blocks - 1, " or more than ", page, " rows");
+    use[pairs[i]] |= 1;
+    TORCH_CHECK_VALUE(!(use[pairs[i + 1]] & 2), "copy_blocks: a destination is named twice or is a source");
+    use[pairs[i + 1]] |= 2;
+    for (int j = 0; j < 3; ++j) p[i + j] = (int)pairs[i + j];
+  }
+  for (size_t i = 0; i < pairs.size(); i += 3)
+    TORCH_CHECK_VALUE(use[pairs[i + 1]] == 2, "copy_blocks: a destination is named twice or is a source");
+  c10::cuda::CUDAGuard guard(desc.device());
+  const int n = (int)(pairs.size() / 3);
+  check(b200_cache_copy(desc.data_ptr(), (int)desc.size(0), p.data(), n, (int)page, (int)max_vecs,
+                        at::cuda::getCurrentDeviceProperties()->multiProcessorCount, cur_stream()),
+        "cache_copy");
+  return (n + 2047) / 2048;
+}
+
+// Tokens grouped by adapter slot.
+void lora_plan(const Tensor& slots, int64_t num_slots, int64_t rows, const Tensor& order, const Tensor& tiles,
+               const Tensor& num_tiles, const Tensor& status) {
+  CHECK_I32(slots);
+  CHECK_I32(order);
+  CHECK_I32(tiles);
+  CHECK_I32(num_tiles);
+  CHECK_I32(status);
+  TORCH_CHECK(order.numel() >= slots.numel() &&
+                  tiles.numel() >= 4 * (slots.numel() / rows + std::min<int64_t>(slots.numel(), num_slots + 1)),
+              "lora_plan: buffers too small");
+  c10::cuda::CUDAGuard guard(slots.device());
+  check(b200_lora_plan(slots.data_ptr<int>(), (int)slots.numel(), (int)num_slots, (int)rows, order.data_ptr<int>(),
+                       tiles.data_ptr<int>(), num_tiles.data_ptr<int>(), status.data_ptr<int>(), cur_stream()),
+        "lora_plan");
+}
+
+// Whether two tensors of bf16 rows may share an element: not when their spans are apart, nor when they are column ranges apart
+// of rows at one pitch.
+bool share_memory(const Tensor& a, const Tensor& b) {
+  const int64_t T = a.size(0);
+  if (T == 0) return false;
+  const auto at = [](const Tensor& t) { return (int64_t)(reinterpret_cast<uintptr_t>(t.data_ptr()) / 2); };
+  const auto end = [&](const Tensor& t) { return at(t) + (T - 1) * t.stride(0) + t.size(1); };
+  if (end(a) <= at(b) || end(b) <= at(a)) return false;
+  const int64_t s = a.stride(0);
+  if (T < 2 || b.stride(0) != s || a.size(1) > s || b.size(1) > s) return true;
+  const int64_t d = ((at(b) - at(a)) % s + s) % s;
+  return d < a.size(1) || d + b.size(1) > s;
+}
+
+// out = y + scale * B (A x) per adapter, or the gated activation of it.
+void lora(const Tensor& x, const Tensor& y, const Tensor& out, const Tensor& a, const Tensor& b, const Tensor& ranks,
+          const Tensor& scales, const Tensor& order, const Tensor& tiles, const Tensor& num_tiles, int64_t max_tiles,
+          int64_t rows, at::IntArrayRef slices, int64_t max_rank, int64_t act, double act_alpha, double act_limit) {
+  int n[4] = {0, 0, 0, 0};
+  int64_t width = 0;
+  TORCH_CHECK(!slices.empty() && slices.size() <= 4, "lora: one to four slices");
+  for (size_t i = 0; i < slices.size(); ++i) width += n[i] = (int)slices[i];
+  const int64_t T = x.size(0), L = ranks.size(0), S = (int64_t)slices.size();
+  for (const Tensor* t : {&x, &y, &out, &a, &b}) CHECK_CUDA_BF16(*t);
+  for (const Tensor* t : {&x, &y, &out})
+    TORCH_CHECK(t->dim() == 2 && t->size(0) == T && t->stride(1) == 1 && (T < 2 || t->stride(0) % 8 == 0) &&
+                    (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0,
+                "lora: rows of x, y and out are contiguous and start at 16-byte boundaries");
+  TORCH_CHECK(y.size(1) == width && out.size(1) == (act ? slices[0] : width), "lora: widths of y and out");
+  TORCH_CHECK(a.is_contiguous() && b.is_contiguous() && a.dim() == 2 && b.dim() == 2 && a.size(0) == L && b.size(0) == L &&
+                  a.size(1) == S * max_rank * x.size(1) && b.size(1) == width * max_rank,
+              "lora: factors [slots, slices * rank * K] and [slots, columns * rank]");
+  CHECK_I32(ranks);
+  CHECK_I32(order);
+  CHECK_I32(tiles);
+  CHECK_I32(num_tiles);
+  TORCH_CHECK(ranks.dim() == 2 && ranks.size(1) == S && scales.is_cuda() && scales.scalar_type() == at::kFloat &&
+                  scales.is_contiguous() && scales.numel() == L,
+              "lora: ranks int32 [slots, slices], scales fp32 [slots]");
+  TORCH_CHECK(order.numel() >= T && tiles.numel() >= 4 * max_tiles, "lora: plan of another step");
+  TORCH_CHECK(!share_memory(out, x), "lora: out shares memory with x");
+  TORCH_CHECK(!share_memory(out, y) || (act == 0 && out.data_ptr() == y.data_ptr() && (T < 2 || out.stride(0) == y.stride(0))),
+              "lora: out is y itself or shares no memory with it");
+  TORCH_CHECK(T < 2 || out.stride(0) >= out.size(1), "lora: rows of out overlap");
+  c10::cuda::CUDAGuard guard(x.device());
+  check(b200_lora(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(), out.stride(0), a.data_ptr(), a.size(1),
+                  b.data_ptr(), b.size(1), ranks.data_ptr<int>(), scales.data_ptr<float>(), order.data_ptr<int>(),
+                  tiles.data_ptr<int>(), num_tiles.data_ptr<int>(), (int)max_tiles, (int)rows, (int)x.size(1), (int)S, n,
+                  (int)max_rank, (int)act, (float)act_alpha, (float)act_limit, cur_stream()),
+        "lora");
+}
+
 int64_t mla_decode_scratch_bytes(int64_t T, int64_t N, int64_t splits) {
   return (int64_t)b200_mla_decode_scratch_bytes((int)T, (int)N, (int)splits);
 }
@@ -789,6 +893,9 @@ TORCH_LIBRARY_FRAGMENT(omni_b200, m) {
   });
   m.def("gqa_decode", &gqa_decode);
   m.def("kv_p2p_copy", &kv_p2p_copy);
+  m.def("cache_copy", &cache_copy);
+  m.def("lora_plan", &lora_plan);
+  m.def("lora", &lora);
   m.def("mla_decode_scratch_bytes", &mla_decode_scratch_bytes);
   m.def("mla_decode", &mla_decode);
 }

@@ -1308,3 +1308,7 @@ def kv_p2p_copy(desc: torch.Tensor, src_blocks: torch.Tensor, dst_blocks: torch.
     bytes).  Sources may be another GPU's memory mapped through CUDA IPC."""
     _count(1)
     _C().kv_p2p_copy(desc, src_blocks, dst_blocks, int(max_block_bytes))
+
+
+from .lora import LoraPlan, LoraStack, lora_add, lora_gated, lora_plan  # noqa: E402
+from .pages import CacheBlocks, copy_blocks  # noqa: E402

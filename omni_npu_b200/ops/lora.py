@@ -1,0 +1,212 @@
+"""Low-rank adapters of many requests beside a shared projection.
+
+A projection's weights are shared; a request may bring factors A [r, K] and B [N, r] of its own that add
+``scale * B (A x)`` to the projection's result for its tokens.  :class:`LoraStack` holds the factors of one projection for
+every adapter slot of the server, :func:`lora_plan` groups a step's tokens by slot once, and :func:`lora_add` and
+:func:`lora_gated` apply them to the result of the shared product, one launch each.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+from . import SILU, _C, _act_kind, _count, device_state, ref
+
+MAX_SLOTS, MAX_SLICES, MAX_RANK = 512, 4, 256
+
+# Tokens of one adapter that a cluster of CTAs takes together.  Up to this many tokens a step is a decode batch, whose adapters
+# have few tokens each: tiles of 16, one matrix instruction high.
+FEW_TOKENS, FEW_ROWS, MANY_ROWS = 256, 16, 64
+
+
+class LoraStack:
+    """Factors of one projection [sum(slices), in_features] for ``num_slots`` adapters of rank up to ``max_rank``.
+
+    ``slices``: columns of the parts of a joined projection (query, key and value; gate and up), each with factors of its
+    own.  ``interleaved``: two equal slices whose columns alternate in groups of eight, gate first, as the gated products
+    store them.  Slots start empty: tokens of an empty slot get the shared product alone."""
+
+    def __init__(self, num_slots: int, max_rank: int, in_features: int, slices: Sequence[int], device=None,
+                 dtype: torch.dtype = torch.bfloat16, interleaved: bool = False) -> None:
+        slices = [int(n) for n in slices]
+        if not 1 <= num_slots <= MAX_SLOTS:
+            raise ValueError(f"LoraStack: {num_slots} slots, 1 to {MAX_SLOTS} are possible")
+        if not 1 <= max_rank <= MAX_RANK:
+            raise ValueError(f"LoraStack: rank {max_rank}, 1 to {MAX_RANK} are possible")
+        if not 1 <= len(slices) <= MAX_SLICES or any(n <= 0 or n % 8 for n in slices):
+            raise ValueError(f"LoraStack: slices {slices}, one to {MAX_SLICES} multiples of 8 are possible")
+        if in_features <= 0 or in_features % 8:
+            raise ValueError(f"LoraStack: {in_features} input features are not a multiple of 8")
+        if interleaved and (len(slices) != 2 or slices[0] != slices[1]):
+            raise ValueError("LoraStack: interleaved columns are those of two equal slices")
+        device = torch.device(device if device is not None else "cpu")
+        if device.type == "cuda" and dtype != torch.bfloat16:
+            raise ValueError("LoraStack: factors on a GPU are bf16")
+        self.num_slots, self.in_features, self.slices, self.interleaved = num_slots, in_features, slices, interleaved
+        self.out_features = sum(slices)
+        self.max_rank = (max_rank + 15) // 16 * 16
+        self.dtype = dtype
+        with torch.inference_mode(False):
+            # packed: A of a slot as [sum of its ranks, K], B as one [columns, rank] after another
+            self.a = torch.zeros(num_slots, len(slices) * self.max_rank * in_features, dtype=dtype, device=device)
+            self.b = torch.zeros(num_slots, self.out_features * self.max_rank, dtype=dtype, device=device)
+            self.ranks = torch.zeros(num_slots, len(slices), dtype=torch.int32, device=device)
+            self.scales = torch.zeros(num_slots, dtype=torch.float32, device=device)
+        self.device = self.a.device
+        self._ranks = [[0] * len(slices) for _ in range(num_slots)]
+
+    def load(self, slot: int, a: Sequence[Optional[torch.Tensor]], b: Sequence[Optional[torch.Tensor]],
+             scale: float = 1.0) -> None:
+        """Put an adapter into ``slot``: ``a[i]`` [r, in_features] and ``b[i]`` [slices[i], r] of each slice, or None for a
+        slice that it leaves as it is.  Steps launched before keep the slot's earlier contents, later ones see these
+        (stream order)."""
+        self._check_slot(slot)
+        if len(a) != len(self.slices) or len(b) != len(self.slices):
+            raise ValueError(f"LoraStack.load: {len(self.slices)} slices need as many factors")
+        ranks = []
+        for i, (p, q) in enumerate(zip(a, b)):
+            if (p is None) != (q is None):
+                raise ValueError(f"LoraStack.load: slice {i} has one factor of two")
+            if p is None:
+                ranks.append(0)
+                continue
+            r = p.shape[0] if p.dim() == 2 else -1
+            if p.dim() != 2 or q.dim() != 2 or p.shape[1] != self.in_features or tuple(q.shape) != (self.slices[i], r):
+                raise ValueError(f"LoraStack.load: slice {i} has factors {tuple(p.shape)} and {tuple(q.shape)}, expected "
+                                 f"(r, {self.in_features}) and ({self.slices[i]}, r)")
+            if not 1 <= r <= self.max_rank:
+                raise ValueError(f"LoraStack.load: rank {r}, at most {self.max_rank}")
+            ranks.append((r + 15) // 16 * 16)
+        with torch.inference_mode():
+            at = 0
+            for p, r in zip(a, ranks):
+                if r:
+                    rows = self.a[slot, at: at + r * self.in_features].view(r, self.in_features)
+                    rows[: p.shape[0]].copy_(p)
+                    rows[p.shape[0]:].zero_()
+                    at += r * self.in_features
+            at = 0
+            for q, r, n in zip(b, ranks, self.slices):
+                if r:
+                    cols = self.b[slot, at: at + n * r].view(n, r)
+                    cols[:, : q.shape[1]].copy_(q)
+                    cols[:, q.shape[1]:].zero_()
+                    at += n * r
+            self.scales[slot] = float(scale)
+            self.ranks[slot].copy_(torch.tensor(ranks, dtype=torch.int32))
+        self._ranks[slot] = ranks
+
+    def clear(self, slot: int) -> None:
+        """Empty a slot."""
+        self._check_slot(slot)
+        with torch.inference_mode():
+            self.ranks[slot].zero_()
+        self._ranks[slot] = [0] * len(self.slices)
+
+    def factors(self, slot: int):
+        """(A, B) of each slice of a slot (ranks padded to 16), None where it has none."""
+        out, pa, pb = [], 0, 0
+        for r, n in zip(self._ranks[slot], self.slices):
+            if not r:
+                out.append(None)
+                continue
+            out.append((self.a[slot, pa: pa + r * self.in_features].view(r, self.in_features),
+                        self.b[slot, pb: pb + n * r].view(n, r)))
+            pa += r * self.in_features
+            pb += n * r
+        return out
+
+    def columns(self, i: int) -> torch.Tensor:
+        """Where the columns of slice ``i`` lie in the projection's result."""
+        j = torch.arange(self.slices[i], device=self.device)
+        return j // 8 * 16 + i * 8 + j % 8 if self.interleaved else sum(self.slices[:i]) + j
+
+    def _check_slot(self, slot: int) -> None:
+        if not 0 <= slot < self.num_slots:
+            raise ValueError(f"LoraStack: slot {slot} of {self.num_slots}")
+
+
+class LoraPlan:
+    """A step's tokens grouped by adapter slot (:func:`lora_plan`); the buffers belong to the step."""
+
+    __slots__ = ("slots", "num_slots", "num_tokens", "rows", "order", "tiles", "num_tiles", "max_tiles")
+
+    def __init__(self, slots: torch.Tensor, num_slots: int, rows: int = 0) -> None:
+        self.slots, self.num_slots, self.num_tokens, self.rows = slots, num_slots, slots.shape[0], rows
+        self.order = self.tiles = self.num_tiles = None
+        self.max_tiles = 0
+
+
+def lora_plan(slots: torch.Tensor, num_slots: int) -> LoraPlan:
+    """Group tokens by adapter: ``slots`` int32 [T], the slot of each token or -1 for the shared weights alone.  The plan is
+    made on the device (it may be captured, and follows ``slots`` at every replay) and serves every projection of the step.
+    A slot outside -1 .. num_slots - 1 counts as -1 and is reported by :func:`check_status`."""
+    if slots.dim() != 1 or slots.dtype != torch.int32 or not slots.is_contiguous():
+        raise ValueError("lora_plan: slots are a contiguous int32 vector")
+    if not 1 <= num_slots <= MAX_SLOTS:
+        raise ValueError(f"lora_plan: {num_slots} slots, 1 to {MAX_SLOTS} are possible")
+    t = slots.shape[0]
+    if not slots.is_cuda:
+        if t and (int(slots.min()) < -1 or int(slots.max()) >= num_slots):
+            raise ValueError(f"lora_plan: slots outside -1 .. {num_slots - 1}")
+        return LoraPlan(slots, num_slots)
+    plan = LoraPlan(slots, num_slots, FEW_ROWS if t <= FEW_TOKENS else MANY_ROWS)
+    if t == 0:
+        return plan
+    plan.max_tiles = t // plan.rows + min(t, num_slots + 1)
+    # order, count of tiles and tiles (four ints each, 16-byte aligned)
+    at = (t + 1 + 3) // 4 * 4
+    buf = torch.empty(at + 4 * plan.max_tiles, dtype=torch.int32, device=slots.device)
+    plan.order, plan.num_tiles, plan.tiles = buf[:t], buf[t: t + 1], buf[at:]
+    _count(1)
+    _C().lora_plan(slots, num_slots, plan.rows, plan.order, plan.tiles, plan.num_tiles, device_state(slots.device).status)
+    return plan
+
+
+def _check(what: str, y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan) -> None:
+    if y.dim() != 2 or x.dim() != 2 or x.shape[1] != stack.in_features or y.shape[1] != stack.out_features \
+            or x.shape[0] != y.shape[0]:
+        raise ValueError(f"{what}: x {tuple(x.shape)} and y {tuple(y.shape)} do not fit a projection of "
+                         f"{stack.in_features} to {stack.out_features}")
+    if plan.num_tokens != x.shape[0] or plan.num_slots != stack.num_slots:
+        raise ValueError(f"{what}: a plan of {plan.num_tokens} tokens and {plan.num_slots} slots for {x.shape[0]} tokens and "
+                         f"{stack.num_slots} slots")
+    if not x.device == y.device == stack.device == plan.slots.device:
+        raise ValueError(f"{what}: tensors on {x.device}, {y.device}, {stack.device} and {plan.slots.device}")
+
+
+def _launch(y, x, stack: LoraStack, plan: LoraPlan, out, kind) -> torch.Tensor:
+    if x.shape[0] == 0:
+        return out
+    _count(1)
+    _C().lora(x, y, out, stack.a, stack.b, stack.ranks, stack.scales, plan.order, plan.tiles, plan.num_tiles, plan.max_tiles,
+              plan.rows, stack.slices, stack.max_rank, *kind)
+    return out
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan,
+             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y + scale * B (A x)`` with the factors of each token's adapter: y [T, sum(slices)] is the shared product of
+    x [T, in_features].  ``out`` may be ``y`` itself (rows without an adapter are then not touched)."""
+    _check("lora_add", y, x, stack, plan)
+    if stack.interleaved:
+        raise ValueError("lora_add: the stack's columns are interleaved (lora_gated)")
+    if out is not None and (out.shape != y.shape or out.dtype != y.dtype or out.device != y.device):
+        raise ValueError("lora_add: out has another shape, type or device than y")
+    if not x.is_cuda:
+        z = ref.lora_sum(y, x, stack, plan.slots).to(y.dtype)
+        return z if out is None else out.copy_(z)
+    return _launch(y, x, stack, plan, y.new_empty(y.shape) if out is None else out, (0, 0.0, 0.0))
+
+
+def lora_gated(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan, act=SILU) -> torch.Tensor:
+    """``act(gate) * up`` of z = y + scale * B (A x), y [T, 2 I] being the shared gate / up product without its activation
+    (columns in alternating groups of eight, an ``interleaved`` stack): [T, I].  ``act`` as in :func:`gemm`."""
+    _check("lora_gated", y, x, stack, plan)
+    if not stack.interleaved:
+        raise ValueError("lora_gated: the stack's columns are not interleaved")
+    if not x.is_cuda:
+        z = ref.lora_sum(y, x, stack, plan.slots).view(y.shape[0], -1, 2, 8)
+        return ref.gated_act(z[:, :, 0], z[:, :, 1], act).reshape(y.shape[0], -1).to(y.dtype)
+    return _launch(y, x, stack, plan, y.new_empty(y.shape[0], stack.slices[0]), _act_kind(True, act))

@@ -871,3 +871,17 @@ def latent_decode(q, cache, block_tables, seq_lens, num_seqs, heads, rank, scale
         kv = latent_gather(cache, block_tables[b:b + 1], seq_lens[b:b + 1], 1).float()
         p = torch.softmax(q[b].float() @ kv.t() * scale, dim=-1)
         out[b] = (p @ kv[:, :rank]).to(out.dtype)
+
+
+def lora_sum(y: torch.Tensor, x: torch.Tensor, stack, slots: torch.Tensor) -> torch.Tensor:
+    """``y + scale * B (A x)`` in fp32 with the factors of each token's slot (-1: y alone)."""
+    z = y.float().clone()
+    for s in slots.unique().tolist():
+        if s < 0:
+            continue
+        rows = (slots == s).nonzero().flatten()
+        for i, f in enumerate(stack.factors(s)):
+            if f is not None:
+                d = (x[rows].float() @ f[0].float().t()) @ f[1].float().t()
+                z[rows[:, None], stack.columns(i)[None, :]] += d * stack.scales[s]
+    return z
