@@ -8,12 +8,17 @@
 // [N_p, rank_p] after another; ranks are multiples of 16 (zero padded), 0 for a slice without an adapter.
 //
 // Tokens are grouped by adapter once a step (lora_plan_kernel: a stable counting sort, then tiles of up to `rows` tokens of one
-// adapter).  A cluster takes a tile: its CTAs share out K for h, sum their parts over distributed shared memory in rank order,
-// and share out the columns for z, so that x, y, A and B are read once per tile, in one launch, and h never leaves the SMs.
+// adapter).  Two launches apply the adapters, both bound by what they read and write:
+//   lora_shrink_kernel  parts of h in fp32: a CTA per (tile, 64 of the joined ranks, part of K)
+//   lora_expand_kernel  h as the sum of its parts, then z: a CTA per (tile, 256 columns of y)
+// so that many small pieces of work even out adapters of unlike ranks.  The second is launched while the first runs and
+// has y and its first factors in registers by the time h is there.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 #include "../common/device_once.h"
 #include "../common/pdl.cuh"
@@ -25,7 +30,7 @@ namespace b200 {
 static constexpr int kLoraThreads = 256;
 static constexpr int kLoraWarps = kLoraThreads / 32;
 static constexpr int kLoraMaxSlices = 4;
-static constexpr int kLoraChunk = 8;             // 8-wide tiles of h that are summed at a time
+static constexpr int kLoraChunk = 8;             // 8-wide tiles of h in a piece of work
 static constexpr int kPlanThreads = 1024;
 
 // ----------------------------------------------------------------------------------------------- grouping
@@ -128,9 +133,14 @@ struct LoraParams {
   const int* order;
   const LoraTile* tiles;
   const int* num_tiles;
-  int K, slices, subs;                           // subs: parts of a plan's tile, each for a cluster of its own
+  float* h;                                      // [parts][T][h_width], rows in the order of the plan
+  long long h_part;                              // T * h_width
+  int h_width;                                   // slices * largest rank
+  int K, slices, parts;
+  int subs_shrink, subs;                         // pieces of a plan's tile, each with CTAs of its own
+  int groups;                                    // of 64 columns of y
   int n[kLoraMaxSlices];
-  int h_pitch;                                   // elements between rows of h in shared memory
+  int pitch;                                     // elements between rows of h in shared memory
   int act;
   float act_alpha, act_limit;
 };
@@ -152,267 +162,481 @@ __device__ __forceinline__ uint2 load8(const void* p, bool ok) {
   return ok ? *static_cast<const uint2*>(p) : make_uint2(0, 0);
 }
 
-// MT 16-row tiles a warp, MW warps side by side on rows in the first product: 16 * MT * MW rows a cluster.  The second
-// product gives every warp all rows and its own columns.  In the first, a lane's 16 bytes of a row of x and of A stand for
-// the k of two matrix instructions: both operands use the same permutation of k, which the sum does not see.
-template <int MT, int MW, bool GATED>
-__global__ void __launch_bounds__(kLoraThreads) lora_kernel(const LoraParams p) {
-  constexpr int BM = 16 * MT * MW, KW = kLoraWarps / MW, NT = kLoraChunk, M2 = MT * MW;
-  extern __shared__ __align__(16) char smem[];
-  float* red = reinterpret_cast<float*>(smem);                         // [KW][BM][NT * 8] parts of the warps
-  float* part = red + KW * BM * NT * 8;                                // [2][BM][NT * 8] of this CTA
-  __nv_bfloat16* h_hi = reinterpret_cast<__nv_bfloat16*>(part + 2 * BM * NT * 8);
-  __nv_bfloat16* h_lo = h_hi + BM * p.h_pitch;
-  __shared__ int tok[BM];
+// The tile of a CTA, or false when there is none.  (Entries behind the last tile lie in the buffer.)
+__device__ __forceinline__ bool lora_tile(const LoraParams& p, int item, int subs, int rows, LoraTile& tl) {
+  const int tile = item / subs, sub = item % subs;
+  const int4 v = *reinterpret_cast<const int4*>(p.tiles + tile);
+  if (tile >= *p.num_tiles) return false;
+  tl = LoraTile{v.x, v.y + sub * rows, min(rows, v.z - sub * rows), 0};
+  return tl.count > 0;
+}
 
-  pdl_trigger();
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+// ---- h of few rows: 16 at most, K dealt to the parts and, in steps of 32, to the warps.  The factors are what is read: they go
+// from global memory into the registers of the matrix instructions, `U` steps of NT tiles at a time in flight.  A lane's 16 bytes
+// of a row of x and of A stand for the k of two matrix instructions: both operands use the same permutation of k, which the
+// sum does not see.
+template <int NT, int U>
+__device__ __forceinline__ void shrink_rows(const LoraParams& p, const __nv_bfloat16* x0, const __nv_bfloat16* x1,
+                                            const __nv_bfloat16* a, int s, int s_hi, int t4, float* d) {
+  float acc[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+  for (; s < s_hi; s += U * kLoraWarps) {
+    uint4 av[U][NT], v0[U], v1[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (s + u * kLoraWarps) * 32 + t4 * 8;
+      const bool in = s + u * kLoraWarps < s_hi && k < p.K;            // K is a multiple of 8
+#pragma unroll
+      for (int j = 0; j < NT; ++j) av[u][j] = load16(a + static_cast<long long>(j) * 8 * p.K + k, in);
+      v0[u] = load16(x0 + k, in && x0 != nullptr);
+      v1[u] = load16(x1 + k, in && x1 != nullptr);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        mma_bf16(acc[j], v0[u].x, v1[u].x, v0[u].y, v1[u].y, av[u][j].x, av[u][j].y);
+        mma_bf16(acc[j], v0[u].z, v1[u].z, v0[u].w, v1[u].w, av[u][j].z, av[u][j].w);
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    *reinterpret_cast<float2*>(d + j * 8) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2*>(d + 8 * kLoraChunk * 8 + j * 8) = make_float2(acc[j][2], acc[j][3]);
+  }
+}
+
+__global__ void __launch_bounds__(kLoraThreads, 3) lora_shrink_few_kernel(const LoraParams p) {
+  constexpr int BM = 16, W = kLoraChunk * 8;
+  __shared__ __align__(16) float red[kLoraWarps][BM][W];               // parts of the warps
   pdl_wait();
-  uint32_t C;
-  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
-  const int rank = static_cast<int>(cluster_ctarank());
-  const int item = blockIdx.x / C;
-  const int tile = item / p.subs;
-  if (tile >= *p.num_tiles) return;                                    // the whole cluster alike
-  LoraTile tl = p.tiles[tile];
-  tl.start += (item % p.subs) * BM;
-  tl.count = min(BM, tl.count - (item % p.subs) * BM);
-  if (tl.count <= 0) return;
+  pdl_trigger();                                                       // (the second kernel reads what was there before this one)
+  LoraTile tl;
+  if (!lora_tile(p, blockIdx.z, p.subs_shrink, BM, tl) || tl.slot < 0) return;
+  int sum_r = 0;
+  for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * p.slices + s];
+  const int n0 = blockIdx.y * W;
+  if (n0 >= sum_r) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int nt = min(kLoraChunk, (sum_r - n0) / 8);                    // even: ranks are multiples of 16
+  const int steps = (p.K + 31) / 32;
+  const int s_lo = static_cast<int>(static_cast<long long>(steps) * blockIdx.x / p.parts) + warp;
+  const int s_hi = static_cast<int>(static_cast<long long>(steps) * (blockIdx.x + 1) / p.parts);
+  const __nv_bfloat16* x0 = g < tl.count ? p.x + p.order[tl.start + g] * p.x_stride : nullptr;
+  const __nv_bfloat16* x1 = g + 8 < tl.count ? p.x + p.order[tl.start + g + 8] * p.x_stride : nullptr;
+  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + static_cast<long long>(n0 + g) * p.K;
+  float* d = &red[warp][g][t4 * 2];
+  if (nt == 2) shrink_rows<2, 4>(p, x0, x1, a, s_lo, s_hi, t4, d);
+  else if (nt == 4) shrink_rows<4, 2>(p, x0, x1, a, s_lo, s_hi, t4, d);
+  else if (nt == 6) shrink_rows<6, 1>(p, x0, x1, a, s_lo, s_hi, t4, d);
+  else shrink_rows<8, 1>(p, x0, x1, a, s_lo, s_hi, t4, d);
+  __syncthreads();
+  // the warps' parts in order, four columns a thread
+  float* h = p.h + blockIdx.x * p.h_part + static_cast<long long>(tl.start) * p.h_width + n0;
+  for (int i = threadIdx.x; i < tl.count * nt * 2; i += kLoraThreads) {
+    const int row = i / (nt * 2), col = i % (nt * 2) * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kLoraWarps; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(&red[w][row][col]);
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    *reinterpret_cast<float4*>(h + static_cast<long long>(row) * p.h_width + col) = sum;
+  }
+}
+
+// ---- h of many rows: 64 rows of x and 64 of the joined ranks, in slabs of 64 of K through a ring in shared memory, so that
+// what is in flight does not depend on registers.  Warps: two halves of every slab's K, then 32 rows x 32 ranks each (a fragment
+// of x and one of A serve two and two pairs of matrix instructions).
+static constexpr int kSlab = 64, kStages = 5, kStageBytes = 2 * 64 * kSlab * 2;
+
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_many_kernel(const LoraParams p) {
+  constexpr int BM = 64, W = kLoraChunk * 8;
+  extern __shared__ __align__(128) char smem[];
+  pdl_wait();
+  pdl_trigger();
+  LoraTile tl;
+  if (!lora_tile(p, blockIdx.z, p.subs_shrink, BM, tl) || tl.slot < 0) return;
+  int sum_r = 0;
+  for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * p.slices + s];
+  const int n0 = blockIdx.y * W;
+  if (n0 >= sum_r) return;
+  const int width = min(W, sum_r - n0);                                // a multiple of 16
+  const int slabs = (p.K + kSlab - 1) / kSlab;
+  const int s_lo = static_cast<int>(static_cast<long long>(slabs) * blockIdx.x / p.parts);
+  const int s_hi = static_cast<int>(static_cast<long long>(slabs) * (blockIdx.x + 1) / p.parts);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // copies: eight lanes a row of 128 bytes, its 16-byte pieces at (piece ^ row % 8); two rows of x and of A each
+  const int crow = threadIdx.x >> 3, piece = threadIdx.x & 7;
+  const __nv_bfloat16 *xs[2], *as[2];
+  bool xok[2], aok[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = crow + 32 * i;
+    xok[i] = row < tl.count;
+    aok[i] = row < width;
+    xs[i] = p.x + (xok[i] ? p.order[tl.start + row] : 0) * p.x_stride + piece * 8;
+    as[i] = p.a + tl.slot * p.a_slot + static_cast<long long>(n0 + (aok[i] ? row : 0)) * p.K + piece * 8;
+  }
+  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  const uint32_t cdst = base + crow * 128 + ((piece ^ (crow & 7)) << 4);
+  auto copy = [&](int s) {
+    if (s < s_hi) {
+      const uint32_t dst = cdst + (s - s_lo) % kStages * kStageBytes;
+      const bool in = s * kSlab + piece * 8 < p.K;                     // K is a multiple of 8
+      const int k = in ? s * kSlab : -piece * 8;                       // (nothing is read there)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        cp16(dst + i * 4096, xs[i] + k, in && xok[i]);
+        cp16(dst + 8192 + i * 4096, as[i] + k, in && aok[i]);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int i = 0; i < kStages - 1; ++i) copy(s_lo + i);
+
+  const int kw = warp >> 2, m0 = (warp & 1) * 32, j0 = (warp >> 1 & 1) * 32;
+  const bool live = j0 < width && m0 < tl.count;
+  float acc[2][4][4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
+  // rows of the four 8 x 8 matrices of a fragment: x rows 0-7, 8-15 at k, then at k + 8; A ranks 0-7 at k, k + 8, then 8-15
+  const int xr = m0 + (lane & 15), xk = lane >> 4;
+  const int arow = j0 + (lane & 7) + (lane >> 4) * 8, ak = lane >> 3 & 1;
+  for (int s = s_lo; s < s_hi; ++s) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncthreads();
+    copy(s + kStages - 1);
+    if (!live) continue;
+    const uint32_t st = base + (s - s_lo) % kStages * kStageBytes;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int kc = (kw * 2 + q) * 2;                                 // its first 16-byte piece
+      uint32_t xf[2][4], af[2][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int row = xr + m * 16;
+        ldmatrix4(xf[m], st + row * 128 + (((kc + xk) ^ (row & 7)) << 4));
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = arow + j * 16;
+        ldmatrix4(af[j], st + 8192 + row * 128 + (((kc + ak) ^ (row & 7)) << 4));
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma_bf16(acc[m][j], xf[m][0], xf[m][1], xf[m][2], xf[m][3], af[j >> 1][(j & 1) * 2], af[j >> 1][(j & 1) * 2 + 1]);
+    }
+  }
+  // the two halves of K in order
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);                         // [4 warps][32][32]
+  const int g = lane >> 2, t4 = lane & 3;
+  float* mine = red + (warp & 3) * 32 * 36;
+  if (kw == 1 && live) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        *reinterpret_cast<float2*>(mine + (m * 16 + g) * 36 + j * 8 + t4 * 2) = make_float2(acc[m][j][0], acc[m][j][1]);
+        *reinterpret_cast<float2*>(mine + (m * 16 + g + 8) * 36 + j * 8 + t4 * 2) = make_float2(acc[m][j][2], acc[m][j][3]);
+      }
+  }
+  __syncthreads();
+  if (kw == 0 && live) {
+    float* h = p.h + blockIdx.x * p.h_part + static_cast<long long>(tl.start) * p.h_width + n0;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = m * 16 + g + e * 8, col = j0 + j * 8 + t4 * 2;
+          const float2 o = *reinterpret_cast<const float2*>(mine + r * 36 + j * 8 + t4 * 2);
+          if (m0 + r < tl.count && col < width)
+            *reinterpret_cast<float2*>(h + static_cast<long long>(m0 + r) * p.h_width + col) =
+                make_float2(acc[m][j][2 * e] + o.x, acc[m][j][2 * e + 1] + o.y);
+        }
+  }
+}
+
+// ---- z: a CTA has a tile's rows and a run of column groups, 64 columns of y each; a warp takes every eighth group, 16 rows at a
+// time.  Columns of B are dealt to the matrix instructions so that a lane ends up with eight neighbouring columns twice (gated:
+// eight of gate and their eight of up): y and the result move 16 bytes a lane, 128 of a row at once.  y of the next 16 rows
+// and the next factors are on their way while these are multiplied.
+struct LoraGroup {
+  int slice, c0, h0, first;                      // slice, first column in it; of the slice: first rank in h, first column of y
+  long long off;                                 // of the slice in B
+};
+
+template <int MS, bool GATED>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const LoraParams p) {
+  constexpr int BM = 16 * MS;
+  extern __shared__ __align__(16) char smem[];
+  __nv_bfloat16* h_hi = reinterpret_cast<__nv_bfloat16*>(smem);        // [BM][pitch]
+  __nv_bfloat16* h_lo = h_hi + BM * p.pitch;
+  __shared__ int tok[BM];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const bool in_place = !GATED && p.out == p.y;
+  // Everything but h is older than the first kernel, which has started only behind it: no wait yet.
+  LoraTile tl;
+  if (!lora_tile(p, blockIdx.y, p.subs, BM, tl)) {
+    pdl_wait();
+    return;
+  }
   int r[kLoraMaxSlices], sum_r = 0;
 #pragma unroll
   for (int s = 0; s < kLoraMaxSlices; ++s) {
     r[s] = tl.slot >= 0 && s < p.slices ? p.ranks[tl.slot * p.slices + s] : 0;
     sum_r += r[s];
   }
-  const bool in_place = !GATED && p.out == p.y;
-  if (sum_r == 0 && in_place) return;
+  if (sum_r == 0 && in_place) {
+    pdl_wait();
+    return;
+  }
+  const float scale = tl.slot >= 0 ? p.scales[tl.slot] : 0.f;
   if (threadIdx.x < BM) tok[threadIdx.x] = threadIdx.x < tl.count ? p.order[tl.start + threadIdx.x] : -1;
-  __syncthreads();
-
-  // ---- h: this CTA's part of K, in chunks of 64 of the joined ranks
-  if (sum_r > 0) {
-    const int steps = (p.K + 31) / 32;
-    const int s_lo = static_cast<int>(static_cast<long long>(steps) * rank / C);
-    const int s_hi = static_cast<int>(static_cast<long long>(steps) * (rank + 1) / C);
-    const int mw = warp % MW, kw = warp / MW;
-    const __nv_bfloat16* xr[2 * MT];
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-      const int t = tok[mw * 16 * MT + i * 8 + g];
-      xr[i] = t >= 0 ? p.x + t * p.x_stride : nullptr;
-    }
-    const __nv_bfloat16* a = p.a + tl.slot * p.a_slot;
-    const float scale = p.scales[tl.slot];
-    int buf = 0;
-    for (int n0 = 0; n0 < sum_r; n0 += NT * 8, buf ^= 1) {
-      const int nt = min(NT, (sum_r - n0) / 8), width = nt * 8;
-      float acc[MT][NT][4];
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
-      const __nv_bfloat16* ar = a + static_cast<long long>(n0 + g) * p.K;
-#pragma unroll 2
-      for (int s = s_lo + kw; s < s_hi; s += KW) {
-        const int k = s * 32 + t4 * 8;
-        const bool in = k < p.K;                                       // K is a multiple of 8
-        uint4 xv[2 * MT];
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) xv[i] = load16(xr[i] + k, in && xr[i] != nullptr);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if (j >= nt) break;
-          const uint4 av = load16(ar + static_cast<long long>(j) * 8 * p.K + k, in);
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            mma_bf16(acc[m][j], xv[2 * m].x, xv[2 * m + 1].x, xv[2 * m].y, xv[2 * m + 1].y, av.x, av.y);
-            mma_bf16(acc[m][j], xv[2 * m].z, xv[2 * m + 1].z, xv[2 * m].w, xv[2 * m + 1].w, av.z, av.w);
-          }
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if (j >= nt) break;
-          float* d = red + (kw * BM + (mw * MT + m) * 16 + g) * (NT * 8) + j * 8 + t4 * 2;
-          *reinterpret_cast<float2*>(d) = make_float2(acc[m][j][0], acc[m][j][1]);
-          *reinterpret_cast<float2*>(d + 8 * NT * 8) = make_float2(acc[m][j][2], acc[m][j][3]);
-        }
-      __syncthreads();
-      float* pt = part + buf * BM * NT * 8;
-      for (int i = threadIdx.x; i < BM * width; i += kLoraThreads) {
-        const int row = i / width, col = i % width;
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < KW; ++w) sum += red[(w * BM + row) * (NT * 8) + col];
-        pt[row * (NT * 8) + col] = sum;
-      }
-      cluster_arrive_release();
-      cluster_wait_acquire();
-      // the parts of all CTAs in rank order; h as the sum of two bf16 (17 bits of the fp32 sum), so that the second
-      // product adds no rounding beside that of its result
-      const uint32_t base = smem_u32(pt);
-      for (int i = threadIdx.x; i < BM * width; i += kLoraThreads) {
-        const int row = i / width, col = i % width;
-        float sum = 0.f;
-        for (uint32_t c = 0; c < C; ++c) {
-          float v;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                       : "=f"(v)
-                       : "r"(mapa_shared(base + (row * (NT * 8) + col) * 4, c))
-                       : "memory");
-          sum += v;
-        }
-        sum *= scale;
-        const __nv_bfloat16 hi = __float2bfloat16(sum);
-        h_hi[row * p.h_pitch + n0 + col] = hi;
-        const float rest = sum - __bfloat162float(hi);
-        h_lo[row * p.h_pitch + n0 + col] = __float2bfloat16(rest - rest == 0.f ? rest : 0.f);      // (0 beside an infinity)
-      }
-      // (the buffer is written again two chunks on, behind the next chunk's barrier)
-    }
-    cluster_arrive_release();                                          // waited for before this CTA's memory goes
-    __syncthreads();
-  }
-
-  // ---- z: groups of 32 columns of y, each to one warp for all rows
-  int groups = 0;
-  if constexpr (GATED) {
-    groups = p.n[0] / 16 + (p.n[0] % 16 != 0);
-  } else {
-    for (int s = 0; s < p.slices; ++s) groups += (p.n[s] + 31) / 32;
-  }
-  const __nv_bfloat16* b0 = p.b + (tl.slot >= 0 ? tl.slot * p.b_slot : 0);
-  for (int gi = rank * kLoraWarps + warp; gi < groups; gi += C * kLoraWarps) {
-    float acc[M2][4][4];
-#pragma unroll
-    for (int m = 0; m < M2; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
-    if constexpr (!GATED) {
-      int s = 0, c0 = gi, h0 = 0, first = 0;                           // slice, its group, first rank and first column
-      long long off = 0;
-      while (s + 1 < p.slices && c0 >= (p.n[s] + 31) / 32) {
-        c0 -= (p.n[s] + 31) / 32;
-        h0 += r[s];
-        off += static_cast<long long>(p.n[s]) * r[s];
-        first += p.n[s];
-        ++s;
-      }
-      const int rs = r[s], N = p.n[s];
-      if (rs == 0 && in_place) continue;
-      c0 *= 32;
-      const int col = c0 + t4 * 8;
-      uint4 yv[2 * M2];
-#pragma unroll
-      for (int i = 0; i < 2 * M2; ++i) {
-        const int t = tok[i * 8 + g];
-        yv[i] = load16(p.y + t * p.y_stride + first + col, t >= 0 && col < N);
-      }
-      // columns 8 t + 2 j + e of the group are column 2 t + e of matrix tile j: a lane ends up with eight neighbours
-      const int bc = c0 + (g >> 1) * 8 + (g & 1);
-      const __nv_bfloat16* br = b0 + off + static_cast<long long>(bc) * rs + t4 * 4;
-      const bool bin = (c0 + (g >> 1) * 8) < N;
-      for (int k = 0; k < rs; k += 16) {
-        uint2 bv[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) bv[j] = load8(br + 2 * j * rs + k, bin);
-#pragma unroll
-        for (int m = 0; m < M2; ++m) {
-          const int at = (m * 16 + g) * p.h_pitch + h0 + k + t4 * 4;
-          const uint2 p0 = *reinterpret_cast<const uint2*>(h_hi + at), p1 = *reinterpret_cast<const uint2*>(h_hi + at + 8 * p.h_pitch);
-          const uint2 q0 = *reinterpret_cast<const uint2*>(h_lo + at), q1 = *reinterpret_cast<const uint2*>(h_lo + at + 8 * p.h_pitch);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mma_bf16(acc[m][j], p0.x, p1.x, p0.y, p1.y, bv[j].x, bv[j].y);
-            mma_bf16(acc[m][j], q0.x, q1.x, q0.y, q1.y, bv[j].x, bv[j].y);
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2 * M2; ++i) {
-        const int t = tok[i * 8 + g], m = i >> 1, e = (i & 1) * 2;
-        if (t < 0 || col >= N) continue;
-        const uint32_t w[4] = {yv[i].x, yv[i].y, yv[i].z, yv[i].w};
-        uint32_t o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(lo_f(w[j]) + acc[m][j][e], hi_f(w[j]) + acc[m][j][e + 1]);
-        *reinterpret_cast<uint4*>(p.out + t * p.out_stride + first + col) = make_uint4(o[0], o[1], o[2], o[3]);
-      }
+  const int ga = static_cast<int>(static_cast<long long>(p.groups) * blockIdx.x / gridDim.x);
+  const int gb = static_cast<int>(static_cast<long long>(p.groups) * (blockIdx.x + 1) / gridDim.x);
+  const long long slot_b = tl.slot >= 0 ? tl.slot * p.b_slot : 0;
+  auto locate = [&](int gi) {
+    LoraGroup q{0, gi, 0, 0, slot_b};
+    if constexpr (GATED) {
+      q.c0 *= 32;
     } else {
-      // 16 columns of the result: matrix tiles 0, 1 are their gate columns 4 t + 2 j + e, tiles 2, 3 the up columns
-      const int N = p.n[0], c0 = gi * 16, col = c0 + t4 * 4;
-      const int phys = col / 8 * 16 + col % 8;
-      uint2 gv[2 * M2], uv[2 * M2];
 #pragma unroll
-      for (int i = 0; i < 2 * M2; ++i) {
-        const int t = tok[i * 8 + g];
-        const __nv_bfloat16* yr = p.y + t * p.y_stride + phys;
-        gv[i] = load8(yr, t >= 0 && col < N);
-        uv[i] = load8(yr + 8, t >= 0 && col < N);
+      for (int s = 0; s < kLoraMaxSlices - 1; ++s) {
+        const int blocks = (p.n[s] + 63) / 64;
+        if (q.slice == s && s + 1 < p.slices && q.c0 >= blocks) {
+          q.c0 -= blocks;
+          q.h0 += r[s];
+          q.off += static_cast<long long>(p.n[s]) * r[s];
+          q.first += p.n[s];
+          q.slice = s + 1;
+        }
       }
-      const int bc = c0 + (g >> 1) * 4 + (g & 1);
-      const bool bin = bc < N;
+      q.c0 *= 64;
+    }
+    return q;
+  };
+  auto rank_of = [&](const LoraGroup& q) {
+    if constexpr (GATED) return max(r[0], r[1]);
+    int v = 0;
+#pragma unroll
+    for (int s = 0; s < kLoraMaxSlices; ++s) v = q.slice == s ? r[s] : v;
+    return v;
+  };
+  // y of 16 rows: rows g and g + 8, two times 16 bytes
+  auto load_y = [&](uint4 (&v)[4], const LoraGroup& q, int m) {
+    const int N = p.n[GATED ? 0 : q.slice], col = q.c0 + t4 * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = tok[m * 16 + i * 8 + g];
+      if constexpr (GATED) {
+        const __nv_bfloat16* src = p.y + t * p.y_stride + 2 * col;
+        v[2 * i] = load16(src, t >= 0 && col < N);
+        v[2 * i + 1] = load16(src + 8, t >= 0 && col < N);
+      } else {
+        const __nv_bfloat16* src = p.y + t * p.y_stride + q.first + col;
+        v[2 * i] = load16(src, t >= 0 && col < N);
+        v[2 * i + 1] = load16(src + 32, t >= 0 && col + 32 < N);
+      }
+    }
+  };
+  // 16 ranks of the group's columns of B for the eight matrix tiles
+  auto load_b = [&](uint2 (&v)[8], const LoraGroup& q, int k) {
+    const int N = p.n[GATED ? 0 : q.slice], bc = q.c0 + (g >> 1) * 8 + (g & 1);
+    if constexpr (GATED) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const int rs = r[s], h0 = s ? r[0] : 0;
-        const __nv_bfloat16* br = b0 + (s ? static_cast<long long>(N) * r[0] : 0) + static_cast<long long>(bc) * rs + t4 * 4;
-        for (int k = 0; k < rs; k += 16) {
-          uint2 bv[2];
+        const __nv_bfloat16* src = p.b + q.off + (s ? static_cast<long long>(N) * r[0] : 0) + static_cast<long long>(bc) * r[s] + t4 * 4 + k;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) bv[j] = load8(br + 2 * j * rs + k, bin);
+        for (int j = 0; j < 4; ++j) v[4 * s + j] = load8(src + 2 * j * r[s], bc < N && k < r[s]);
+      }
+    } else {
+      const int rs = rank_of(q);
+      const __nv_bfloat16* src = p.b + q.off + static_cast<long long>(bc) * rs + t4 * 4 + k;
 #pragma unroll
-          for (int m = 0; m < M2; ++m) {
-            const int at = (m * 16 + g) * p.h_pitch + h0 + k + t4 * 4;
-            const uint2 p0 = *reinterpret_cast<const uint2*>(h_hi + at), p1 = *reinterpret_cast<const uint2*>(h_hi + at + 8 * p.h_pitch);
-            const uint2 q0 = *reinterpret_cast<const uint2*>(h_lo + at), q1 = *reinterpret_cast<const uint2*>(h_lo + at + 8 * p.h_pitch);
+      for (int j = 0; j < 8; ++j)
+        v[j] = load8(src + ((j >> 2) * 32 + 2 * (j & 3)) * rs, bc + (j >> 2) * 32 < N && k < rs);
+    }
+  };
+  __syncthreads();
+  const int ms = (tl.count + 15) / 16;
+  uint4 yv[4];
+  uint2 bv[8];
+  LoraGroup cur = locate(min(ga + warp, p.groups - 1));
+  if (ga + warp < gb) {
+    load_y(yv, cur, 0);
+    load_b(bv, cur, 0);
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  // h of the slices that these groups belong to: the parts in order, times the scale, as the sum of two bf16 (17 bits of the fp32
+  // value), so that the product below adds no rounding beside that of its result
+  if (sum_r > 0) {
+    int lo = 0, hi = sum_r;
+    if constexpr (!GATED) {
+      const LoraGroup qa = locate(ga), qb = locate(gb - 1);
+      lo = qa.h0;
+      hi = qb.h0 + rank_of(qb);
+    }
+    const float* h = p.h + static_cast<long long>(tl.start) * p.h_width;
+    const int vecs = (hi - lo) / 4;
+    for (int i = threadIdx.x; i < BM * vecs; i += kLoraThreads) {
+      const int row = i / vecs, v = lo + i % vecs * 4;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < tl.count) {
+        const float* src = h + static_cast<long long>(row) * p.h_width + v;
+#pragma unroll 4
+        for (int c = 0; c < p.parts; ++c) {
+          const float4 q = *reinterpret_cast<const float4*>(src + c * p.h_part);
+          sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
+        }
+      }
+      const float f[4] = {sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale};
+      float up[4], rest[4];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              mma_bf16(acc[m][2 * s + j], p0.x, p1.x, p0.y, p1.y, bv[j].x, bv[j].y);
-              mma_bf16(acc[m][2 * s + j], q0.x, q1.x, q0.y, q1.y, bv[j].x, bv[j].y);
+      for (int e = 0; e < 4; ++e) {
+        up[e] = __bfloat162float(__float2bfloat16(f[e]));
+        rest[e] = f[e] - up[e];
+        if (!(rest[e] - rest[e] == 0.f)) rest[e] = 0.f;                // beside an infinity
+      }
+      *reinterpret_cast<uint2*>(h_hi + row * p.pitch + v) = make_uint2(pack_bf16x2(up[0], up[1]), pack_bf16x2(up[2], up[3]));
+      *reinterpret_cast<uint2*>(h_lo + row * p.pitch + v) = make_uint2(pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3]));
+    }
+  }
+  __syncthreads();
+  for (int gi = ga + warp; gi < gb; gi += kLoraWarps) {
+    const bool more = gi + kLoraWarps < gb;
+    const LoraGroup nxt = locate(more ? gi + kLoraWarps : gi);
+    const int rank = rank_of(cur);
+    for (int m = 0; m < ms; ++m) {
+      uint4 yn[4];
+      const bool last = m + 1 == ms;
+      if (!last || more) load_y(yn, last ? nxt : cur, last ? 0 : m + 1);
+      float acc[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+      int k = 0;
+      do {
+        uint2 bn[8];
+        if (k + 16 < rank) load_b(bn, cur, k + 16);
+        else if (!last && rank > 16) load_b(bn, cur, 0);
+        else if (last && more) load_b(bn, nxt, 0);
+        else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) bn[j] = bv[j];
+        }
+        if (k < rank) {
+#pragma unroll
+          for (int s = 0; s < (GATED ? 2 : 1); ++s) {
+            if (GATED && k >= r[s]) continue;
+            const int at = (m * 16 + g) * p.pitch + (GATED ? (s ? r[0] : 0) : cur.h0) + k + t4 * 4;
+            const uint2 p0 = *reinterpret_cast<const uint2*>(h_hi + at), p1 = *reinterpret_cast<const uint2*>(h_hi + at + 8 * p.pitch);
+            const uint2 q0 = *reinterpret_cast<const uint2*>(h_lo + at), q1 = *reinterpret_cast<const uint2*>(h_lo + at + 8 * p.pitch);
+#pragma unroll
+            for (int j = 0; j < (GATED ? 4 : 8); ++j) {
+              const int o = GATED ? 4 * s + j : j;
+              mma_bf16(acc[o], p0.x, p1.x, p0.y, p1.y, bv[o].x, bv[o].y);
+              mma_bf16(acc[o], q0.x, q1.x, q0.y, q1.y, bv[o].x, bv[o].y);
             }
           }
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bv[j] = bn[j];
+        k += 16;
+      } while (k < rank);
+      const int N = p.n[GATED ? 0 : cur.slice], col = cur.c0 + t4 * 8;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = tok[m * 16 + i * 8 + g], e = 2 * i;
+        const uint32_t w0[4] = {yv[2 * i].x, yv[2 * i].y, yv[2 * i].z, yv[2 * i].w};
+        const uint32_t w1[4] = {yv[2 * i + 1].x, yv[2 * i + 1].y, yv[2 * i + 1].z, yv[2 * i + 1].w};
+        uint32_t o0[4], o1[4];
+        if constexpr (GATED) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o0[j] = pack_bf16x2(gated_act(p.act, lo_f(w0[j]) + acc[j][e], lo_f(w1[j]) + acc[4 + j][e], p.act_alpha, p.act_limit),
+                                gated_act(p.act, hi_f(w0[j]) + acc[j][e + 1], hi_f(w1[j]) + acc[4 + j][e + 1], p.act_alpha,
+                                          p.act_limit));
+          if (t >= 0 && col < N)
+            *reinterpret_cast<uint4*>(p.out + t * p.out_stride + col) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            o0[j] = pack_bf16x2(lo_f(w0[j]) + acc[j][e], hi_f(w0[j]) + acc[j][e + 1]);
+            o1[j] = pack_bf16x2(lo_f(w1[j]) + acc[4 + j][e], hi_f(w1[j]) + acc[4 + j][e + 1]);
+          }
+          __nv_bfloat16* dst = p.out + t * p.out_stride + cur.first + col;
+          if (t >= 0 && col < N) *reinterpret_cast<uint4*>(dst) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+          if (t >= 0 && col + 32 < N) *reinterpret_cast<uint4*>(dst + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < 2 * M2; ++i) {
-        const int t = tok[i * 8 + g], m = i >> 1, e = (i & 1) * 2;
-        if (t < 0 || col >= N) continue;
-        const uint32_t gw[2] = {gv[i].x, gv[i].y}, uw[2] = {uv[i].x, uv[i].y};
-        uint32_t o[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          o[j] = pack_bf16x2(gated_act(p.act, lo_f(gw[j]) + acc[m][j][e], lo_f(uw[j]) + acc[m][2 + j][e], p.act_alpha, p.act_limit),
-                             gated_act(p.act, hi_f(gw[j]) + acc[m][j][e + 1], hi_f(uw[j]) + acc[m][2 + j][e + 1], p.act_alpha,
-                                       p.act_limit));
-        *reinterpret_cast<uint2*>(p.out + t * p.out_stride + col) = make_uint2(o[0], o[1]);
-      }
+      for (int i = 0; i < 4; ++i) yv[i] = yn[i];
     }
+    cur = nxt;
   }
-  if (sum_r > 0) cluster_wait_acquire();
 }
 
-template <int MT, int MW, bool GATED>
-static int launch_lora(const LoraParams& p, int clusters, int C, cudaStream_t stream) {
-  constexpr int BM = 16 * MT * MW, KW = kLoraWarps / MW;
-  const size_t smem = sizeof(float) * (KW + 2) * BM * kLoraChunk * 8 + 2 * sizeof(__nv_bfloat16) * BM * p.h_pitch;
-  if (smem > 227 * 1024 - 1024) return -2;
-  auto kern = lora_kernel<MT, MW, GATED>;
+static constexpr int kShrinkSmem = kStages * kStageBytes, kExpandSmem = 112 * 1024;
+
+template <bool GATED>
+static int launch_lora(const LoraParams& p, bool many, bool wide, unsigned tiles, unsigned chunks, unsigned blocks,
+                       cudaStream_t stream) {
+  auto expand = wide ? lora_expand_kernel<4, GATED> : lora_expand_kernel<1, GATED>;
   static DeviceOnce once;
   int dev;
   if (once.needed(&dev)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess) return -3;
+    const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    if (cudaFuncSetAttribute(lora_shrink_many_kernel, attr, kShrinkSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(lora_expand_kernel<4, GATED>, attr, kExpandSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(lora_expand_kernel<1, GATED>, attr, kExpandSmem) != cudaSuccess)
+      return -3;
     once.mark(dev);
   }
-  return launch_pdl(kern, dim3(static_cast<unsigned>(clusters) * C), dim3(kLoraThreads), smem, stream, C, p) == cudaSuccess ? 0 : -3;
+  const size_t smem = 2 * sizeof(__nv_bfloat16) * (wide ? 64 : 16) * p.pitch;
+  if (smem > kExpandSmem) return -2;
+  const dim3 grid(p.parts, chunks, tiles * p.subs_shrink);
+  if (grid.z > 65535 || tiles * p.subs > 65535) return -1;
+  const cudaError_t e = many ? launch_pdl(lora_shrink_many_kernel, grid, dim3(kLoraThreads), kShrinkSmem, stream, 1, p)
+                             : launch_pdl(lora_shrink_few_kernel, grid, dim3(kLoraThreads), 0, stream, 1, p);
+  if (e != cudaSuccess) return -3;
+  return launch_pdl(expand, dim3(blocks, tiles * p.subs), dim3(kLoraThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace b200
+
+// Parts of K that a step's h is summed from.  Few rows (tiles of 16): as many as the slots let be resident, whatever the number of
+// tokens, so that a row does not depend on it; many rows: as many as fill the SMs.
+extern "C" int b200_lora_parts(int K, int rows, int max_tiles, int num_slots) {
+  const int want = rows < 64 ? std::min((K + 511) / 512, 592 / num_slots) : std::min((K + 255) / 256, 296 / max_tiles);
+  return std::min(std::max(want, 1), 16);
+}
 
 // Groups tokens by adapter.  tiles: at least T / rows + min(T, L + 1) of four ints.
 extern "C" int b200_lora_plan(const int* slots, int T, int L, int rows, int* order, int* tiles, int* num_tiles, int* status,
@@ -432,15 +656,16 @@ extern "C" int b200_lora_plan(const int* slots, int T, int L, int rows, int* ord
                     reinterpret_cast<LoraTile*>(tiles), num_tiles, status) == cudaSuccess ? 0 : -3;
 }
 
-// n: columns of each slice.  max_tiles: tiles that the plan may have, of `rows` tokens each.  max_rank: bound of the ranks.
-// act: 0 adds, a gated kind of gemm/gated_act.cuh joins gate and up (alternating groups of eight columns of y).
+// n: columns of each slice.  h: fp32 [b200_lora_parts][T][slices * max_rank].  max_tiles: tiles that the plan may have, of `rows`
+// tokens each.  max_rank: bound of the ranks.  act: 0 adds, a gated kind of gemm/gated_act.cuh joins gate and up (alternating
+// groups of eight columns of y).
 extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long long y_stride, void* out, long long out_stride,
                          const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks,
                          const float* scales, const int* order, const int* tiles, const int* num_tiles, int max_tiles, int rows,
-                         int K, int slices, const int* n, int max_rank, int act, float act_alpha, float act_limit,
-                         cudaStream_t stream) {
+                         float* h, int T, int num_slots, int K, int slices, const int* n, int max_rank, int act,
+                         float act_alpha, float act_limit, cudaStream_t stream) {
   using namespace b200;
-  if (slices < 1 || slices > kLoraMaxSlices || (K & 7) || max_rank < 16 || (max_rank & 15) || max_tiles < 1) return -1;
+  if (slices < 1 || slices > kLoraMaxSlices || (K & 7) || max_rank < 16 || (max_rank & 15) || max_tiles < 1 || (rows & 15)) return -1;
   if (act != kActNone && (!act_is_gated(act) || slices != 2 || n[0] != n[1])) return -1;
   LoraParams p;
   p.x = static_cast<const __nv_bfloat16*>(x);
@@ -458,24 +683,31 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   p.order = order;
   p.tiles = reinterpret_cast<const LoraTile*>(tiles);
   p.num_tiles = num_tiles;
+  p.h = h;
+  p.h_width = slices * max_rank;
+  p.h_part = static_cast<long long>(T) * p.h_width;
   p.K = K;
   p.slices = slices;
+  p.groups = 0;
   for (int s = 0; s < kLoraMaxSlices; ++s) {
     p.n[s] = s < slices ? n[s] : 0;
     if (p.n[s] & 7) return -1;
+    p.groups += (p.n[s] + 63) / 64;
   }
+  if (act != kActNone) p.groups = (n[0] + 31) / 32;
   p.act = act;
   p.act_alpha = act_alpha;
   p.act_limit = act_limit;
   // rows of h are 32 or 96 bytes past a multiple of 128 apart: the eight-byte reads of a half warp touch every bank once
-  const int width = slices * max_rank;
-  p.h_pitch = width + (width % 32 ? 0 : 16);
-  const bool wide = rows >= 64 && p.h_pitch <= 400;
-  p.subs = wide ? rows / 64 : (rows + 15) / 16;
-  const long long clusters = static_cast<long long>(max_tiles) * p.subs;
-  if (clusters > (1 << 24)) return -1;
-  const int C = wide ? 4 : 8;
-  const int cl = static_cast<int>(clusters);
-  if (act != kActNone) return wide ? launch_lora<2, 2, true>(p, cl, C, stream) : launch_lora<1, 1, true>(p, cl, C, stream);
-  return wide ? launch_lora<2, 2, false>(p, cl, C, stream) : launch_lora<1, 1, false>(p, cl, C, stream);
+  p.pitch = p.h_width + (p.h_width % 32 ? 0 : 16);
+  const bool many = rows >= 64, wide = many && 4 * 64 * p.pitch <= kExpandSmem;
+  p.subs_shrink = many ? rows / 64 : rows / 16;
+  p.subs = wide ? rows / 64 : rows / 16;
+  p.parts = b200_lora_parts(K, rows, max_tiles, num_slots);
+  const unsigned chunks = (p.h_width + kLoraChunk * 8 - 1) / (kLoraChunk * 8), tiles_n = static_cast<unsigned>(max_tiles);
+  // column groups: one a warp, more where there are CTAs enough for two rounds of all SMs
+  const long long all = (p.groups + kLoraWarps - 1) / kLoraWarps, per = all * max_tiles * p.subs / (4 * 148);
+  const unsigned blocks = static_cast<unsigned>((all + std::max(per, 1LL) - 1) / std::max(per, 1LL));
+  return act != kActNone ? launch_lora<true>(p, many, wide, tiles_n, chunks, blocks, stream)
+                         : launch_lora<false>(p, many, wide, tiles_n, chunks, blocks, stream);
 }

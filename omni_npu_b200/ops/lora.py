@@ -3,7 +3,7 @@
 A projection's weights are shared; a request may bring factors A [r, K] and B [N, r] of its own that add
 ``scale * B (A x)`` to the projection's result for its tokens.  :class:`LoraStack` holds the factors of one projection for
 every adapter slot of the server, :func:`lora_plan` groups a step's tokens by slot once, and :func:`lora_add` and
-:func:`lora_gated` apply them to the result of the shared product, one launch each.
+:func:`lora_gated` apply them to the result of the shared product.
 """
 from __future__ import annotations
 
@@ -179,7 +179,7 @@ def _check(what: str, y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: 
 def _launch(y, x, stack: LoraStack, plan: LoraPlan, out, kind) -> torch.Tensor:
     if x.shape[0] == 0:
         return out
-    _count(1)
+    _count(2)
     _C().lora(x, y, out, stack.a, stack.b, stack.ranks, stack.scales, plan.order, plan.tiles, plan.num_tiles, plan.max_tiles,
               plan.rows, stack.slices, stack.max_rank, *kind)
     return out
