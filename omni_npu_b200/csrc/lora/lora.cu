@@ -386,12 +386,15 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_many_kernel(const
 // and the next factors are on their way while these are multiplied.
 struct LoraGroup {
   int slice, c0, h0, first;                      // slice, first column in it; of the slice: first rank in h, first column of y
-  long long off;                                 // of the slice in B
+  int rank;
+  const __nv_bfloat16* b;                        // the slice's factors
+  int left;                                      // columns from c0 on
 };
 
-template <int MS, bool GATED>
+template <int MS, int ACT>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const LoraParams p) {
   constexpr int BM = 16 * MS;
+  constexpr bool GATED = ACT != kActNone;
   extern __shared__ __align__(16) char smem[];
   __nv_bfloat16* h_hi = reinterpret_cast<__nv_bfloat16*>(smem);        // [BM][pitch]
   __nv_bfloat16* h_lo = h_hi + BM * p.pitch;
@@ -418,11 +421,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
   if (threadIdx.x < BM) tok[threadIdx.x] = threadIdx.x < tl.count ? p.order[tl.start + threadIdx.x] : -1;
   const int ga = static_cast<int>(static_cast<long long>(p.groups) * blockIdx.x / gridDim.x);
   const int gb = static_cast<int>(static_cast<long long>(p.groups) * (blockIdx.x + 1) / gridDim.x);
-  const long long slot_b = tl.slot >= 0 ? tl.slot * p.b_slot : 0;
+  const __nv_bfloat16* slot_b = p.b + (tl.slot >= 0 ? tl.slot * p.b_slot : 0);
   auto locate = [&](int gi) {
-    LoraGroup q{0, gi, 0, 0, slot_b};
+    LoraGroup q{0, gi, 0, 0, r[0], slot_b};
     if constexpr (GATED) {
       q.c0 *= 32;
+      q.rank = max(r[0], r[1]);
     } else {
 #pragma unroll
       for (int s = 0; s < kLoraMaxSlices - 1; ++s) {
@@ -430,81 +434,67 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
         if (q.slice == s && s + 1 < p.slices && q.c0 >= blocks) {
           q.c0 -= blocks;
           q.h0 += r[s];
-          q.off += static_cast<long long>(p.n[s]) * r[s];
+          q.b += static_cast<long long>(p.n[s]) * r[s];
           q.first += p.n[s];
           q.slice = s + 1;
+          q.rank = r[s + 1];
         }
       }
       q.c0 *= 64;
     }
+    q.left = p.n[GATED ? 0 : q.slice] - q.c0;
     return q;
-  };
-  auto rank_of = [&](const LoraGroup& q) {
-    if constexpr (GATED) return max(r[0], r[1]);
-    int v = 0;
-#pragma unroll
-    for (int s = 0; s < kLoraMaxSlices; ++s) v = q.slice == s ? r[s] : v;
-    return v;
   };
   // y of 16 rows: rows g and g + 8, two times 16 bytes
   auto load_y = [&](uint4 (&v)[4], const LoraGroup& q, int m) {
-    const int N = p.n[GATED ? 0 : q.slice], col = q.c0 + t4 * 8;
+    const __nv_bfloat16* src = p.y + q.first + (GATED ? 2 : 1) * (q.c0 + t4 * 8);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int t = tok[m * 16 + i * 8 + g];
-      if constexpr (GATED) {
-        const __nv_bfloat16* src = p.y + t * p.y_stride + 2 * col;
-        v[2 * i] = load16(src, t >= 0 && col < N);
-        v[2 * i + 1] = load16(src + 8, t >= 0 && col < N);
-      } else {
-        const __nv_bfloat16* src = p.y + t * p.y_stride + q.first + col;
-        v[2 * i] = load16(src, t >= 0 && col < N);
-        v[2 * i + 1] = load16(src + 32, t >= 0 && col + 32 < N);
-      }
+      const __nv_bfloat16* row = src + t * p.y_stride;
+      v[2 * i] = load16(row, t >= 0 && t4 * 8 < q.left);
+      v[2 * i + 1] = load16(row + (GATED ? 8 : 32), t >= 0 && t4 * 8 + (GATED ? 0 : 32) < q.left);
     }
   };
-  // 16 ranks of the group's columns of B for the eight matrix tiles
+  // 16 ranks, from k, of the group's columns of B for the eight matrix tiles
   auto load_b = [&](uint2 (&v)[8], const LoraGroup& q, int k) {
-    const int N = p.n[GATED ? 0 : q.slice], bc = q.c0 + (g >> 1) * 8 + (g & 1);
-    if constexpr (GATED) {
+    const int bc = (g >> 1) * 8 + (g & 1);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const __nv_bfloat16* src = p.b + q.off + (s ? static_cast<long long>(N) * r[0] : 0) + static_cast<long long>(bc) * r[s] + t4 * 4 + k;
+    for (int s = 0; s < 2; ++s) {                                      // gate and up, or the two halves of 64 columns
+      const int rs = GATED ? r[s] : q.rank;
+      const __nv_bfloat16* src = q.b + (GATED && s ? static_cast<long long>(p.n[0]) * r[0] : 0) +
+                                 static_cast<long long>(q.c0 + bc + (GATED ? 0 : 32 * s)) * rs + t4 * 4 + k;
+      const bool ok = k < rs && bc + (GATED ? 0 : 32 * s) < q.left;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * s + j] = load8(src + 2 * j * r[s], bc < N && k < r[s]);
-      }
-    } else {
-      const int rs = rank_of(q);
-      const __nv_bfloat16* src = p.b + q.off + static_cast<long long>(bc) * rs + t4 * 4 + k;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = load8(src + ((j >> 2) * 32 + 2 * (j & 3)) * rs, bc + (j >> 2) * 32 < N && k < rs);
+      for (int j = 0; j < 4; ++j) v[4 * s + j] = load8(src + 2 * j * rs, ok);
     }
   };
   __syncthreads();
   const int ms = (tl.count + 15) / 16;
   uint4 yv[4];
-  uint2 bv[8];
+  uint2 b0[8], b1[8];
   LoraGroup cur = locate(min(ga + warp, p.groups - 1));
   if (ga + warp < gb) {
     load_y(yv, cur, 0);
-    load_b(bv, cur, 0);
+    load_b(b0, cur, 0);
+    if (cur.rank > 16) load_b(b1, cur, 16);
   }
   pdl_wait();
   pdl_trigger();
 
   // h of the slices that these groups belong to: the parts in order, times the scale, as the sum of two bf16 (17 bits of the fp32
-  // value), so that the product below adds no rounding beside that of its result
+  // value), so that the product below adds no rounding beside that of its result.  Of 16 ranks, 4 q + e lies at 2 q + e for
+  // e = 0, 1 and at 8 + 2 q + e - 2 for e = 2, 3: a lane's eight bytes of a row of B are its two operands.
   if (sum_r > 0) {
     int lo = 0, hi = sum_r;
     if constexpr (!GATED) {
       const LoraGroup qa = locate(ga), qb = locate(gb - 1);
       lo = qa.h0;
-      hi = qb.h0 + rank_of(qb);
+      hi = qb.h0 + qb.rank;
     }
     const float* h = p.h + static_cast<long long>(tl.start) * p.h_width;
     const int vecs = (hi - lo) / 4;
-    for (int i = threadIdx.x; i < BM * vecs; i += kLoraThreads) {
+    for (int i = threadIdx.x; i < ms * 16 * vecs; i += kLoraThreads) {
       const int row = i / vecs, v = lo + i % vecs * 4;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < tl.count) {
@@ -523,15 +513,19 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
         rest[e] = f[e] - up[e];
         if (!(rest[e] - rest[e] == 0.f)) rest[e] = 0.f;                // beside an infinity
       }
-      *reinterpret_cast<uint2*>(h_hi + row * p.pitch + v) = make_uint2(pack_bf16x2(up[0], up[1]), pack_bf16x2(up[2], up[3]));
-      *reinterpret_cast<uint2*>(h_lo + row * p.pitch + v) = make_uint2(pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3]));
+      const int at = row * p.pitch + (v & ~15) + (v & 15) / 2;
+      *reinterpret_cast<uint32_t*>(h_hi + at) = pack_bf16x2(up[0], up[1]);
+      *reinterpret_cast<uint32_t*>(h_hi + at + 8) = pack_bf16x2(up[2], up[3]);
+      *reinterpret_cast<uint32_t*>(h_lo + at) = pack_bf16x2(rest[0], rest[1]);
+      *reinterpret_cast<uint32_t*>(h_lo + at + 8) = pack_bf16x2(rest[2], rest[3]);
     }
   }
   __syncthreads();
+  const uint32_t frag = static_cast<uint32_t>(__cvta_generic_to_shared(h_hi)) + ((lane & 15) * p.pitch + (lane >> 4) * 8) * 2;
+  const uint32_t lo_at = 2 * BM * p.pitch;
   for (int gi = ga + warp; gi < gb; gi += kLoraWarps) {
     const bool more = gi + kLoraWarps < gb;
     const LoraGroup nxt = locate(more ? gi + kLoraWarps : gi);
-    const int rank = rank_of(cur);
     for (int m = 0; m < ms; ++m) {
       uint4 yn[4];
       const bool last = m + 1 == ms;
@@ -541,36 +535,41 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-      int k = 0;
-      do {
-        uint2 bn[8];
-        if (k + 16 < rank) load_b(bn, cur, k + 16);
-        else if (!last && rank > 16) load_b(bn, cur, 0);
-        else if (last && more) load_b(bn, nxt, 0);
-        else {
+      auto multiply = [&](const uint2 (&b)[8], int k) {
+        const uint32_t at = frag + (m * 16 * p.pitch + (GATED ? 0 : cur.h0) + k) * 2;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) bn[j] = bv[j];
-        }
-        if (k < rank) {
+        for (int s = 0; s < (GATED ? 2 : 1); ++s) {
+          if (GATED && k >= r[s]) continue;
+          uint32_t hi[4], lo[4];
+          ldmatrix4(hi, at + (s ? r[0] * 2 : 0));
+          ldmatrix4(lo, at + (s ? r[0] * 2 : 0) + lo_at);
 #pragma unroll
-          for (int s = 0; s < (GATED ? 2 : 1); ++s) {
-            if (GATED && k >= r[s]) continue;
-            const int at = (m * 16 + g) * p.pitch + (GATED ? (s ? r[0] : 0) : cur.h0) + k + t4 * 4;
-            const uint2 p0 = *reinterpret_cast<const uint2*>(h_hi + at), p1 = *reinterpret_cast<const uint2*>(h_hi + at + 8 * p.pitch);
-            const uint2 q0 = *reinterpret_cast<const uint2*>(h_lo + at), q1 = *reinterpret_cast<const uint2*>(h_lo + at + 8 * p.pitch);
-#pragma unroll
-            for (int j = 0; j < (GATED ? 4 : 8); ++j) {
-              const int o = GATED ? 4 * s + j : j;
-              mma_bf16(acc[o], p0.x, p1.x, p0.y, p1.y, bv[o].x, bv[o].y);
-              mma_bf16(acc[o], q0.x, q1.x, q0.y, q1.y, bv[o].x, bv[o].y);
-            }
+          for (int j = 0; j < (GATED ? 4 : 8); ++j) {
+            const int o = 4 * s + j;
+            mma_bf16(acc[o], hi[0], hi[1], hi[2], hi[3], b[o].x, b[o].y);
+            mma_bf16(acc[o], lo[0], lo[1], lo[2], lo[3], b[o].x, b[o].y);
           }
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) bv[j] = bn[j];
-        k += 16;
-      } while (k < rank);
-      const int N = p.n[GATED ? 0 : cur.slice], col = cur.c0 + t4 * 8;
+      };
+      // two steps of 16 ranks at a time; their registers take the next two as soon as they have been used, and stay for
+      // the next 16 rows where there are no others
+      for (int k = 0; k < cur.rank; k += 32) {
+        const bool tail = k + 32 >= cur.rank;
+        const bool other = tail && last && more, again = tail && !last && cur.rank > 32;
+        multiply(b0, k);
+        if (!tail) load_b(b0, cur, k + 32);
+        else if (other) load_b(b0, nxt, 0);
+        else if (again) load_b(b0, cur, 0);
+        if (k + 16 < cur.rank) multiply(b1, k + 16);
+        if (!tail) load_b(b1, cur, k + 48);
+        else if (other) load_b(b1, nxt, 16);
+        else if (again) load_b(b1, cur, 16);
+      }
+      if (cur.rank == 0 && last && more) {
+        load_b(b0, nxt, 0);
+        load_b(b1, nxt, 16);
+      }
+      __nv_bfloat16* dst = p.out + cur.first + cur.c0 + t4 * 8;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int t = tok[m * 16 + i * 8 + g], e = 2 * i;
@@ -580,21 +579,19 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
         if constexpr (GATED) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            o0[j] = pack_bf16x2(gated_act(p.act, lo_f(w0[j]) + acc[j][e], lo_f(w1[j]) + acc[4 + j][e], p.act_alpha, p.act_limit),
-                                gated_act(p.act, hi_f(w0[j]) + acc[j][e + 1], hi_f(w1[j]) + acc[4 + j][e + 1], p.act_alpha,
+            o0[j] = pack_bf16x2(gated_act(ACT, lo_f(w0[j]) + acc[j][e], lo_f(w1[j]) + acc[4 + j][e], p.act_alpha, p.act_limit),
+                                gated_act(ACT, hi_f(w0[j]) + acc[j][e + 1], hi_f(w1[j]) + acc[4 + j][e + 1], p.act_alpha,
                                           p.act_limit));
-          if (t >= 0 && col < N)
-            *reinterpret_cast<uint4*>(p.out + t * p.out_stride + col) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             o0[j] = pack_bf16x2(lo_f(w0[j]) + acc[j][e], hi_f(w0[j]) + acc[j][e + 1]);
             o1[j] = pack_bf16x2(lo_f(w1[j]) + acc[4 + j][e], hi_f(w1[j]) + acc[4 + j][e + 1]);
           }
-          __nv_bfloat16* dst = p.out + t * p.out_stride + cur.first + col;
-          if (t >= 0 && col < N) *reinterpret_cast<uint4*>(dst) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
-          if (t >= 0 && col + 32 < N) *reinterpret_cast<uint4*>(dst + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
         }
+        __nv_bfloat16* row = dst + t * p.out_stride;
+        if (t >= 0 && t4 * 8 < cur.left) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+        if (!GATED && t >= 0 && t4 * 8 + 32 < cur.left) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) yv[i] = yn[i];
@@ -605,17 +602,17 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
 
 static constexpr int kShrinkSmem = kStages * kStageBytes, kExpandSmem = 112 * 1024;
 
-template <bool GATED>
+template <int ACT>
 static int launch_lora(const LoraParams& p, bool many, bool wide, unsigned tiles, unsigned chunks, unsigned blocks,
                        cudaStream_t stream) {
-  auto expand = wide ? lora_expand_kernel<4, GATED> : lora_expand_kernel<1, GATED>;
+  auto expand = wide ? lora_expand_kernel<4, ACT> : lora_expand_kernel<1, ACT>;
   static DeviceOnce once;
   int dev;
   if (once.needed(&dev)) {
     const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
     if (cudaFuncSetAttribute(lora_shrink_many_kernel, attr, kShrinkSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(lora_expand_kernel<4, GATED>, attr, kExpandSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(lora_expand_kernel<1, GATED>, attr, kExpandSmem) != cudaSuccess)
+        cudaFuncSetAttribute(lora_expand_kernel<4, ACT>, attr, kExpandSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(lora_expand_kernel<1, ACT>, attr, kExpandSmem) != cudaSuccess)
       return -3;
     once.mark(dev);
   }
@@ -698,8 +695,7 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   p.act = act;
   p.act_alpha = act_alpha;
   p.act_limit = act_limit;
-  // rows of h are 32 or 96 bytes past a multiple of 128 apart: the eight-byte reads of a half warp touch every bank once
-  p.pitch = p.h_width + (p.h_width % 32 ? 0 : 16);
+  p.pitch = p.h_width + 8;                       // eight rows of 16 bytes in banks of their own
   const bool many = rows >= 64, wide = many && 4 * 64 * p.pitch <= kExpandSmem;
   p.subs_shrink = many ? rows / 64 : rows / 16;
   p.subs = wide ? rows / 64 : rows / 16;
@@ -708,6 +704,11 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   // column groups: one a warp, more where there are CTAs enough for two rounds of all SMs
   const long long all = (p.groups + kLoraWarps - 1) / kLoraWarps, per = all * max_tiles * p.subs / (4 * 148);
   const unsigned blocks = static_cast<unsigned>((all + std::max(per, 1LL) - 1) / std::max(per, 1LL));
-  return act != kActNone ? launch_lora<true>(p, many, wide, tiles_n, chunks, blocks, stream)
-                         : launch_lora<false>(p, many, wide, tiles_n, chunks, blocks, stream);
+  switch (act) {
+    case kActNone: return launch_lora<kActNone>(p, many, wide, tiles_n, chunks, blocks, stream);
+    case kActSilu: return launch_lora<kActSilu>(p, many, wide, tiles_n, chunks, blocks, stream);
+    case kActClampedGlu: return launch_lora<kActClampedGlu>(p, many, wide, tiles_n, chunks, blocks, stream);
+    case kActGeluTanh: return launch_lora<kActGeluTanh>(p, many, wide, tiles_n, chunks, blocks, stream);
+    default: return launch_lora<kActReluGate>(p, many, wide, tiles_n, chunks, blocks, stream);
+  }
 }
