@@ -138,10 +138,10 @@ struct LoraParams {
   int h_width;                                   // slices * largest rank
   int K, slices, parts;
   int subs_shrink, subs;                         // pieces of a plan's tile, each with CTAs of its own
-  int groups;                                    // of 64 columns of y
+  int per;                                       // column groups of a CTA of the second kernel
+  int chunk;                                     // ranks in a stage of its ring
   int n[kLoraMaxSlices];
-  int pitch;                                     // elements between rows of h in shared memory
-  int act;
+  int h_pitch;                                   // elements between rows of h in shared memory
   float act_alpha, act_limit;
 };
 
@@ -155,13 +155,6 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 
 __device__ __forceinline__ float lo_f(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float hi_f(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
-__device__ __forceinline__ uint4 load16(const void* p, bool ok) {
-  return ok ? *static_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
-}
-__device__ __forceinline__ uint2 load8(const void* p, bool ok) {
-  return ok ? *static_cast<const uint2*>(p) : make_uint2(0, 0);
-}
-
 // The tile of a CTA, or false when there is none.  (Entries behind the last tile lie in the buffer.)
 __device__ __forceinline__ bool lora_tile(const LoraParams& p, int item, int subs, int rows, LoraTile& tl) {
   const int tile = item / subs, sub = item % subs;
@@ -180,36 +173,65 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr));
 }
 
-// ---- h of few rows: 16 at most, K dealt to the parts and, in steps of 32, to the warps.  The factors are what is read: they go
-// from global memory into the registers of the matrix instructions, `U` steps of NT tiles at a time in flight.  A lane's 16 bytes
-// of a row of x and of A stand for the k of two matrix instructions: both operands use the same permutation of k, which the
-// sum does not see.
-template <int NT, int U>
-__device__ __forceinline__ void shrink_rows(const LoraParams& p, const __nv_bfloat16* x0, const __nv_bfloat16* x1,
-                                            const __nv_bfloat16* a, int s, int s_hi, int t4, float* d) {
+// ---- h of few rows: 16 at most, K dealt to the parts and within one to the warps.  The factors are what is read: every warp has a
+// ring of its own in shared memory (no barrier between copy and product), with some 4 KB of A a stage however many ranks there
+// are: 128 of K for 16 of them, 64 for 32, 32 for 48 or 64.  Rows lie 16 bytes past their length apart, so that eight of them
+// are in banks of their own.
+static constexpr int kFewThreads = 128, kFewWarps = kFewThreads / 32, kFewStages = 3, kFewStageBytes = 2 * 16 * 272;
+
+template <int NT>
+__device__ __forceinline__ void shrink_rows(const LoraParams& p, const LoraTile& tl, const int* tok, int n0, int k_lo, int k_hi,
+                                            uint32_t ring, float* d) {
+  constexpr int KT = NT == 2 ? 128 : NT == 4 ? 64 : 32, PIECES = KT / 8, PITCH = KT * 2 + 16;
+  constexpr int X_AT = NT * 8 * PITCH;
+  static_assert(X_AT + 16 * PITCH <= kFewStageBytes, "stage");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + static_cast<long long>(n0) * p.K;
+  auto copy = [&](int i) {
+    const int k0 = k_lo + (i * kFewWarps + warp) * KT;
+    if (k0 < k_hi) {
+      const uint32_t st = ring + i % kFewStages * kFewStageBytes;
+#pragma unroll
+      for (int u = 0; u < NT * 8 * PIECES / 32; ++u) {
+        const int row = (lane + 32 * u) / PIECES, k = k0 + (lane + 32 * u) % PIECES * 8;
+        cp16(st + row * PITCH + (k - k0) * 2, a + static_cast<long long>(row) * p.K + (k < k_hi ? k : 0), k < k_hi);
+      }
+#pragma unroll
+      for (int u = 0; u < 16 * PIECES / 32; ++u) {
+        const int row = (lane + 32 * u) / PIECES, k = k0 + (lane + 32 * u) % PIECES * 8;
+        if (row < tl.count)                                            // (the other rows of h are not used)
+          cp16(st + X_AT + row * PITCH + (k - k0) * 2, p.x + tok[row] * p.x_stride + (k < k_hi ? k : 0), k < k_hi);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kFewStages - 1; ++i) copy(i);
   float acc[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-  for (; s < s_hi; s += U * kLoraWarps) {
-    uint4 av[U][NT], v0[U], v1[U];
+  const uint32_t xf = X_AT + (lane & 15) * PITCH + (lane >> 4) * 16;
+  const uint32_t af = ((lane & 7) + (lane >> 4) * 8) * PITCH + (lane >> 3 & 1) * 16;
+  for (int i = 0; k_lo + (i * kFewWarps + warp) * KT < k_hi; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
+    __syncwarp();
+    copy(i + kFewStages - 1);
+    const uint32_t st = ring + i % kFewStages * kFewStageBytes;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = (s + u * kLoraWarps) * 32 + t4 * 8;
-      const bool in = s + u * kLoraWarps < s_hi && k < p.K;            // K is a multiple of 8
+    for (int k = 0; k < KT; k += 16) {
+      uint32_t x[4];
+      ldmatrix4(x, st + xf + k * 2);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) av[u][j] = load16(a + static_cast<long long>(j) * 8 * p.K + k, in);
-      v0[u] = load16(x0 + k, in && x0 != nullptr);
-      v1[u] = load16(x1 + k, in && x1 != nullptr);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        mma_bf16(acc[j], v0[u].x, v1[u].x, v0[u].y, v1[u].y, av[u][j].x, av[u][j].y);
-        mma_bf16(acc[j], v0[u].z, v1[u].z, v0[u].w, v1[u].w, av[u][j].z, av[u][j].w);
+      for (int j = 0; j < NT; j += 2) {
+        uint32_t b[4];
+        ldmatrix4(b, st + af + j * 8 * PITCH + k * 2);
+        mma_bf16(acc[j], x[0], x[1], x[2], x[3], b[0], b[1]);
+        mma_bf16(acc[j + 1], x[0], x[1], x[2], x[3], b[2], b[3]);
       }
+    }
+    __syncwarp();
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
@@ -218,9 +240,10 @@ __device__ __forceinline__ void shrink_rows(const LoraParams& p, const __nv_bflo
   }
 }
 
-__global__ void __launch_bounds__(kLoraThreads, 3) lora_shrink_few_kernel(const LoraParams p) {
+__global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const LoraParams p) {
   constexpr int BM = 16, W = kLoraChunk * 8;
-  __shared__ __align__(16) float red[kLoraWarps][BM][W];               // parts of the warps
+  extern __shared__ __align__(128) char smem[];
+  __shared__ int tok[BM];
   pdl_wait();
   pdl_trigger();                                                       // (the second kernel reads what was there before this one)
   LoraTile tl;
@@ -229,28 +252,30 @@ __global__ void __launch_bounds__(kLoraThreads, 3) lora_shrink_few_kernel(const 
   for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * p.slices + s];
   const int n0 = blockIdx.y * W;
   if (n0 >= sum_r) return;
+  if (threadIdx.x < tl.count) tok[threadIdx.x] = p.order[tl.start + threadIdx.x];
+  __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int nt = min(kLoraChunk, (sum_r - n0) / 8);                    // even: ranks are multiples of 16
   const int steps = (p.K + 31) / 32;
-  const int s_lo = static_cast<int>(static_cast<long long>(steps) * blockIdx.x / p.parts) + warp;
-  const int s_hi = static_cast<int>(static_cast<long long>(steps) * (blockIdx.x + 1) / p.parts);
-  const __nv_bfloat16* x0 = g < tl.count ? p.x + p.order[tl.start + g] * p.x_stride : nullptr;
-  const __nv_bfloat16* x1 = g + 8 < tl.count ? p.x + p.order[tl.start + g + 8] * p.x_stride : nullptr;
-  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + static_cast<long long>(n0 + g) * p.K;
-  float* d = &red[warp][g][t4 * 2];
-  if (nt == 2) shrink_rows<2, 4>(p, x0, x1, a, s_lo, s_hi, t4, d);
-  else if (nt == 4) shrink_rows<4, 2>(p, x0, x1, a, s_lo, s_hi, t4, d);
-  else if (nt == 6) shrink_rows<6, 1>(p, x0, x1, a, s_lo, s_hi, t4, d);
-  else shrink_rows<8, 1>(p, x0, x1, a, s_lo, s_hi, t4, d);
+  const int k_lo = static_cast<int>(static_cast<long long>(steps) * blockIdx.x / p.parts) * 32;
+  const int k_hi = min(p.K, static_cast<int>(static_cast<long long>(steps) * (blockIdx.x + 1) / p.parts) * 32);
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kFewStages * kFewStageBytes;
+  // (a warp's part of h goes where its ring was)
+  const auto red = [&](int w) { return reinterpret_cast<float*>(smem + w * kFewStages * kFewStageBytes); };
+  float* d = red(warp) + g * W + t4 * 2;
+  if (nt == 2) shrink_rows<2>(p, tl, tok, n0, k_lo, k_hi, ring, d);
+  else if (nt == 4) shrink_rows<4>(p, tl, tok, n0, k_lo, k_hi, ring, d);
+  else if (nt == 6) shrink_rows<6>(p, tl, tok, n0, k_lo, k_hi, ring, d);
+  else shrink_rows<8>(p, tl, tok, n0, k_lo, k_hi, ring, d);
   __syncthreads();
   // the warps' parts in order, four columns a thread
   float* h = p.h + blockIdx.x * p.h_part + static_cast<long long>(tl.start) * p.h_width + n0;
-  for (int i = threadIdx.x; i < tl.count * nt * 2; i += kLoraThreads) {
+  for (int i = threadIdx.x; i < tl.count * nt * 2; i += kFewThreads) {
     const int row = i / (nt * 2), col = i % (nt * 2) * 4;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kLoraWarps; ++w) {
-      const float4 v = *reinterpret_cast<const float4*>(&red[w][row][col]);
+    for (int w = 0; w < kFewWarps; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(red(w) + row * W + col);
       sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
     *reinterpret_cast<float4*>(h + static_cast<long long>(row) * p.h_width + col) = sum;
@@ -380,26 +405,21 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_many_kernel(const
   }
 }
 
-// ---- z: a CTA has a tile's rows and a run of column groups, 64 columns of y each; a warp takes every eighth group, 16 rows at a
-// time.  Columns of B are dealt to the matrix instructions so that a lane ends up with eight neighbouring columns twice (gated:
-// eight of gate and their eight of up): y and the result move 16 bytes a lane, 128 of a row at once.  y of the next 16 rows
-// and the next factors are on their way while these are multiplied.
-struct LoraGroup {
-  int slice, c0, h0, first;                      // slice, first column in it; of the slice: first rank in h, first column of y
-  int rank;
-  const __nv_bfloat16* b;                        // the slice's factors
-  int left;                                      // columns from c0 on
-};
+// ---- z: a CTA has a tile's rows and a run of column groups of one slice, 64 columns of y each (gated: 32 of gate and their 32 of
+// up).  A team of RW warps, 16 rows each, takes a group; y and B come through a ring in shared memory (many rows: one team of
+// four, so that a group's B is read once for 64 rows; few rows: four teams of a warp).  Columns of B are dealt to the matrix
+// instructions so that a lane ends up with eight neighbouring columns twice: y and the result move 16 bytes a lane, 128 of a
+// row at once.
+static constexpr int kExpandThreads = 128, kExpandStages = 3;
 
-template <int MS, int ACT>
-__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const LoraParams p) {
-  constexpr int BM = 16 * MS;
+template <int RW, int ACT>
+__global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const LoraParams p) {
+  constexpr int BM = 16 * RW, TEAMS = kExpandThreads / 32 / RW, TEAM = 32 * RW;
   constexpr bool GATED = ACT != kActNone;
-  extern __shared__ __align__(16) char smem[];
-  __nv_bfloat16* h_hi = reinterpret_cast<__nv_bfloat16*>(smem);        // [BM][pitch]
-  __nv_bfloat16* h_lo = h_hi + BM * p.pitch;
+  extern __shared__ __align__(128) char smem[];
   __shared__ int tok[BM];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int team = warp / RW, member = threadIdx.x % TEAM, rows0 = warp % RW * 16;
   const bool in_place = !GATED && p.out == p.y;
   // Everything but h is older than the first kernel, which has started only behind it: no wait yet.
   LoraTile tl;
@@ -407,95 +427,95 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
     pdl_wait();
     return;
   }
-  int r[kLoraMaxSlices], sum_r = 0;
-#pragma unroll
-  for (int s = 0; s < kLoraMaxSlices; ++s) {
-    r[s] = tl.slot >= 0 && s < p.slices ? p.ranks[tl.slot * p.slices + s] : 0;
-    sum_r += r[s];
+  // this CTA's slice and groups in it; of the slice: first rank in h, first column of y, factors
+  int slice = 0, block = blockIdx.x, h0 = 0, first = 0, r0 = 0, r1 = 0;
+  const __nv_bfloat16* b = p.b + (tl.slot >= 0 ? tl.slot * p.b_slot : 0);
+  const int* ranks = p.ranks + max(tl.slot, 0) * p.slices;
+  if constexpr (GATED) {
+    r0 = tl.slot >= 0 ? ranks[0] : 0;
+    r1 = tl.slot >= 0 ? ranks[1] : 0;
+  } else {
+    for (;; ++slice) {
+      r0 = tl.slot >= 0 ? ranks[slice] : 0;
+      const int blocks = ((p.n[slice] + 63) / 64 + p.per - 1) / p.per;
+      if (block < blocks) break;
+      block -= blocks;
+      h0 += r0;
+      first += p.n[slice];
+      b += static_cast<long long>(p.n[slice]) * r0;
+    }
+    r1 = r0;
   }
-  if (sum_r == 0 && in_place) {
+  const int rank = max(r0, r1), N = p.n[slice];
+  if (rank == 0 && in_place) {
     pdl_wait();
     return;
   }
+  constexpr int GW = GATED ? 32 : 64;                                  // columns of a slice in a group
+  const int ga = block * p.per + team, gb = min((N + GW - 1) / GW, (block + 1) * p.per);
   const float scale = tl.slot >= 0 ? p.scales[tl.slot] : 0.f;
   if (threadIdx.x < BM) tok[threadIdx.x] = threadIdx.x < tl.count ? p.order[tl.start + threadIdx.x] : -1;
-  const int ga = static_cast<int>(static_cast<long long>(p.groups) * blockIdx.x / gridDim.x);
-  const int gb = static_cast<int>(static_cast<long long>(p.groups) * (blockIdx.x + 1) / gridDim.x);
-  const __nv_bfloat16* slot_b = p.b + (tl.slot >= 0 ? tl.slot * p.b_slot : 0);
-  auto locate = [&](int gi) {
-    LoraGroup q{0, gi, 0, 0, r[0], slot_b};
-    if constexpr (GATED) {
-      q.c0 *= 32;
-      q.rank = max(r[0], r[1]);
-    } else {
+  __syncthreads();
+
+  const int b_pitch = p.chunk * 2 + 16;                                // bytes; eight rows are in banks of their own
+  const int stage_bytes = 64 * b_pitch + RW * 2048;
+  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  const uint32_t ring = base + team * kExpandStages * stage_bytes;
+  const uint32_t h_at = base + TEAMS * kExpandStages * stage_bytes;
+  __nv_bfloat16* h_hi = reinterpret_cast<__nv_bfloat16*>(smem + TEAMS * kExpandStages * stage_bytes);   // [BM][h_pitch]
+  __nv_bfloat16* h_lo = h_hi + BM * p.h_pitch;
+  const uint32_t y_slot = 64 * b_pitch + (warp % RW * 128 + lane) * 16;
+  const int tok0 = tok[rows0 + g], tok1 = tok[rows0 + g + 8];
+  const int chunks = max(1, (rank + p.chunk - 1) / p.chunk);
+  // the ring's next item: chunk of ranks cc of group cg
+  int cg = ga, cc = 0, cs = 0;
+  auto copy = [&]() {
+    if (cg < gb) {
+      const uint32_t st = ring + cs * stage_bytes;
+      const int c0 = cg * GW;
 #pragma unroll
-      for (int s = 0; s < kLoraMaxSlices - 1; ++s) {
-        const int blocks = (p.n[s] + 63) / 64;
-        if (q.slice == s && s + 1 < p.slices && q.c0 >= blocks) {
-          q.c0 -= blocks;
-          q.h0 += r[s];
-          q.b += static_cast<long long>(p.n[s]) * r[s];
-          q.first += p.n[s];
-          q.slice = s + 1;
-          q.rank = r[s + 1];
+      for (int s = 0; s < (GATED ? 2 : 1); ++s) {
+        const int rs = s ? r1 : r0, kc = min(p.chunk, rs - cc * p.chunk), pieces = kc >> 3;
+        if (kc <= 0) continue;
+        const __nv_bfloat16* src = b + (s ? static_cast<long long>(N) * r0 : 0) + static_cast<long long>(c0) * rs + cc * p.chunk;
+        const uint32_t inv = 65536u / pieces + 1;                      // i / pieces for i < 512
+        for (int i = member; i < GW * pieces; i += TEAM) {
+          const int col = (i * inv) >> 16, piece = i - col * pieces, c = col & 31;
+          const int row = s * 32 + (col & 32) + ((c & 7) >> 1) * 8 + (c >> 3) * 2 + (c & 1);
+          if (c0 + col < N) cp16(st + row * b_pitch + piece * 16, src + col * rs + piece * 8, true);
         }
       }
-      q.c0 *= 64;
-    }
-    q.left = p.n[GATED ? 0 : q.slice] - q.c0;
-    return q;
-  };
-  // y of 16 rows: rows g and g + 8, two times 16 bytes
-  auto load_y = [&](uint4 (&v)[4], const LoraGroup& q, int m) {
-    const __nv_bfloat16* src = p.y + q.first + (GATED ? 2 : 1) * (q.c0 + t4 * 8);
+      if (cc == 0) {
+        const int col = c0 + t4 * 8;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = tok[m * 16 + i * 8 + g];
-      const __nv_bfloat16* row = src + t * p.y_stride;
-      v[2 * i] = load16(row, t >= 0 && t4 * 8 < q.left);
-      v[2 * i + 1] = load16(row + (GATED ? 8 : 32), t >= 0 && t4 * 8 + (GATED ? 0 : 32) < q.left);
+        for (int i = 0; i < 2; ++i) {
+          const int t = i ? tok1 : tok0;
+          const __nv_bfloat16* row = p.y + t * p.y_stride + first + (GATED ? 2 : 1) * col;
+          if (t >= 0 && col < N) cp16(st + y_slot + i * 1024, row, true);
+          if (t >= 0 && col + (GATED ? 0 : 32) < N) cp16(st + y_slot + i * 1024 + 512, row + (GATED ? 8 : 32), true);
+        }
+      }
+      if (++cc == chunks) {
+        cc = 0;
+        cg += TEAMS;
+      }
+      cs = cs + 1 == kExpandStages ? 0 : cs + 1;
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // 16 ranks, from k, of the group's columns of B for the eight matrix tiles
-  auto load_b = [&](uint2 (&v)[8], const LoraGroup& q, int k) {
-    const int bc = (g >> 1) * 8 + (g & 1);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {                                      // gate and up, or the two halves of 64 columns
-      const int rs = GATED ? r[s] : q.rank;
-      const __nv_bfloat16* src = q.b + (GATED && s ? static_cast<long long>(p.n[0]) * r[0] : 0) +
-                                 static_cast<long long>(q.c0 + bc + (GATED ? 0 : 32 * s)) * rs + t4 * 4 + k;
-      const bool ok = k < rs && bc + (GATED ? 0 : 32 * s) < q.left;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * s + j] = load8(src + 2 * j * rs, ok);
-    }
-  };
-  __syncthreads();
-  const int ms = (tl.count + 15) / 16;
-  uint4 yv[4];
-  uint2 b0[8], b1[8];
-  LoraGroup cur = locate(min(ga + warp, p.groups - 1));
-  if (ga + warp < gb) {
-    load_y(yv, cur, 0);
-    load_b(b0, cur, 0);
-    if (cur.rank > 16) load_b(b1, cur, 16);
-  }
+  for (int i = 0; i < kExpandStages - 1; ++i) copy();
   pdl_wait();
   pdl_trigger();
 
-  // h of the slices that these groups belong to: the parts in order, times the scale, as the sum of two bf16 (17 bits of the fp32
-  // value), so that the product below adds no rounding beside that of its result.  Of 16 ranks, 4 q + e lies at 2 q + e for
-  // e = 0, 1 and at 8 + 2 q + e - 2 for e = 2, 3: a lane's eight bytes of a row of B are its two operands.
+  // h: the parts in order, times the scale, as the sum of two bf16 (17 bits of the fp32 value), so that the product below adds
+  // no rounding beside that of its result
+  const int sum_r = GATED ? r0 + r1 : r0;
   if (sum_r > 0) {
-    int lo = 0, hi = sum_r;
-    if constexpr (!GATED) {
-      const LoraGroup qa = locate(ga), qb = locate(gb - 1);
-      lo = qa.h0;
-      hi = qb.h0 + qb.rank;
-    }
-    const float* h = p.h + static_cast<long long>(tl.start) * p.h_width;
-    const int vecs = (hi - lo) / 4;
-    for (int i = threadIdx.x; i < ms * 16 * vecs; i += kLoraThreads) {
-      const int row = i / vecs, v = lo + i % vecs * 4;
+    const float* h = p.h + static_cast<long long>(tl.start) * p.h_width + h0;
+    const int vecs = sum_r / 4;
+    for (int i = threadIdx.x; i < BM * vecs; i += kExpandThreads) {
+      const int row = i / vecs, v = i % vecs * 4;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < tl.count) {
         const float* src = h + static_cast<long long>(row) * p.h_width + v;
@@ -513,117 +533,119 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
         rest[e] = f[e] - up[e];
         if (!(rest[e] - rest[e] == 0.f)) rest[e] = 0.f;                // beside an infinity
       }
-      const int at = row * p.pitch + (v & ~15) + (v & 15) / 2;
-      *reinterpret_cast<uint32_t*>(h_hi + at) = pack_bf16x2(up[0], up[1]);
-      *reinterpret_cast<uint32_t*>(h_hi + at + 8) = pack_bf16x2(up[2], up[3]);
-      *reinterpret_cast<uint32_t*>(h_lo + at) = pack_bf16x2(rest[0], rest[1]);
-      *reinterpret_cast<uint32_t*>(h_lo + at + 8) = pack_bf16x2(rest[2], rest[3]);
+      *reinterpret_cast<uint2*>(h_hi + row * p.h_pitch + v) = make_uint2(pack_bf16x2(up[0], up[1]), pack_bf16x2(up[2], up[3]));
+      *reinterpret_cast<uint2*>(h_lo + row * p.h_pitch + v) = make_uint2(pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3]));
     }
   }
   __syncthreads();
-  const uint32_t frag = static_cast<uint32_t>(__cvta_generic_to_shared(h_hi)) + ((lane & 15) * p.pitch + (lane >> 4) * 8) * 2;
-  const uint32_t lo_at = 2 * BM * p.pitch;
-  for (int gi = ga + warp; gi < gb; gi += kLoraWarps) {
-    const bool more = gi + kLoraWarps < gb;
-    const LoraGroup nxt = locate(more ? gi + kLoraWarps : gi);
-    for (int m = 0; m < ms; ++m) {
-      uint4 yn[4];
-      const bool last = m + 1 == ms;
-      if (!last || more) load_y(yn, last ? nxt : cur, last ? 0 : m + 1);
-      float acc[8][4];
+  const uint32_t hf = h_at + ((rows0 + (lane & 15)) * p.h_pitch + (lane >> 4) * 8) * 2, lo_at = 2 * BM * p.h_pitch;
+  const uint32_t bf = ((lane & 7) + (lane >> 4) * 8) * b_pitch + (lane >> 3 & 1) * 16;
+  const bool live = rows0 < tl.count;
+  __nv_bfloat16* out0 = p.out + tok0 * p.out_stride + first + t4 * 8;
+  __nv_bfloat16* out1 = p.out + tok1 * p.out_stride + first + t4 * 8;
+  int rs = 0;                                                          // the ring's stage that is read
+  for (int gi = ga; gi < gb; gi += TEAMS) {
+    float acc[8][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-      auto multiply = [&](const uint2 (&b)[8], int k) {
-        const uint32_t at = frag + (m * 16 * p.pitch + (GATED ? 0 : cur.h0) + k) * 2;
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+    uint4 yv[4];
+    for (int c = 0; c < chunks; ++c) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kExpandStages - 2) : "memory");
+      if constexpr (RW > 1) __syncthreads();
+      else __syncwarp();
+      copy();
+      const uint32_t st = ring + rs * stage_bytes;
+      rs = rs + 1 == kExpandStages ? 0 : rs + 1;
+      if (!live) continue;
+      if (c == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(yv[i].x), "=r"(yv[i].y), "=r"(yv[i].z), "=r"(yv[i].w)
+                       : "r"(st + y_slot + i * 512)
+                       : "memory");
+      }
+      const int k0 = c * p.chunk;
+      for (int k = 0; k < min(p.chunk, rank - k0); k += 16) {
 #pragma unroll
         for (int s = 0; s < (GATED ? 2 : 1); ++s) {
-          if (GATED && k >= r[s]) continue;
+          if (GATED && k0 + k >= (s ? r1 : r0)) continue;
           uint32_t hi[4], lo[4];
-          ldmatrix4(hi, at + (s ? r[0] * 2 : 0));
-          ldmatrix4(lo, at + (s ? r[0] * 2 : 0) + lo_at);
+          const uint32_t at = hf + (k0 + k + (s ? r0 : 0)) * 2;
+          ldmatrix4(hi, at);
+          ldmatrix4(lo, at + lo_at);
 #pragma unroll
-          for (int j = 0; j < (GATED ? 4 : 8); ++j) {
+          for (int j = 0; j < (GATED ? 4 : 8); j += 2) {
+            uint32_t v[4];
             const int o = 4 * s + j;
-            mma_bf16(acc[o], hi[0], hi[1], hi[2], hi[3], b[o].x, b[o].y);
-            mma_bf16(acc[o], lo[0], lo[1], lo[2], lo[3], b[o].x, b[o].y);
+            ldmatrix4(v, st + bf + o * 8 * b_pitch + k * 2);
+            mma_bf16(acc[o], hi[0], hi[1], hi[2], hi[3], v[0], v[1]);
+            mma_bf16(acc[o + 1], hi[0], hi[1], hi[2], hi[3], v[2], v[3]);
+            mma_bf16(acc[o], lo[0], lo[1], lo[2], lo[3], v[0], v[1]);
+            mma_bf16(acc[o + 1], lo[0], lo[1], lo[2], lo[3], v[2], v[3]);
           }
         }
-      };
-      // two steps of 16 ranks at a time; their registers take the next two as soon as they have been used, and stay for
-      // the next 16 rows where there are no others
-      for (int k = 0; k < cur.rank; k += 32) {
-        const bool tail = k + 32 >= cur.rank;
-        const bool other = tail && last && more, again = tail && !last && cur.rank > 32;
-        multiply(b0, k);
-        if (!tail) load_b(b0, cur, k + 32);
-        else if (other) load_b(b0, nxt, 0);
-        else if (again) load_b(b0, cur, 0);
-        if (k + 16 < cur.rank) multiply(b1, k + 16);
-        if (!tail) load_b(b1, cur, k + 48);
-        else if (other) load_b(b1, nxt, 16);
-        else if (again) load_b(b1, cur, 16);
       }
-      if (cur.rank == 0 && last && more) {
-        load_b(b0, nxt, 0);
-        load_b(b1, nxt, 16);
-      }
-      __nv_bfloat16* dst = p.out + cur.first + cur.c0 + t4 * 8;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = tok[m * 16 + i * 8 + g], e = 2 * i;
-        const uint32_t w0[4] = {yv[2 * i].x, yv[2 * i].y, yv[2 * i].z, yv[2 * i].w};
-        const uint32_t w1[4] = {yv[2 * i + 1].x, yv[2 * i + 1].y, yv[2 * i + 1].z, yv[2 * i + 1].w};
-        uint32_t o0[4], o1[4];
-        if constexpr (GATED) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            o0[j] = pack_bf16x2(gated_act(ACT, lo_f(w0[j]) + acc[j][e], lo_f(w1[j]) + acc[4 + j][e], p.act_alpha, p.act_limit),
-                                gated_act(ACT, hi_f(w0[j]) + acc[j][e + 1], hi_f(w1[j]) + acc[4 + j][e + 1], p.act_alpha,
-                                          p.act_limit));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            o0[j] = pack_bf16x2(lo_f(w0[j]) + acc[j][e], hi_f(w0[j]) + acc[j][e + 1]);
-            o1[j] = pack_bf16x2(lo_f(w1[j]) + acc[4 + j][e], hi_f(w1[j]) + acc[4 + j][e + 1]);
-          }
-        }
-        __nv_bfloat16* row = dst + t * p.out_stride;
-        if (t >= 0 && t4 * 8 < cur.left) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
-        if (!GATED && t >= 0 && t4 * 8 + 32 < cur.left) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) yv[i] = yn[i];
     }
-    cur = nxt;
+    if (!live) continue;
+    const int c0 = gi * GW, left = N - c0 - t4 * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int e = 2 * i;
+      const uint32_t w0[4] = {yv[2 * i].x, yv[2 * i].y, yv[2 * i].z, yv[2 * i].w};
+      const uint32_t w1[4] = {yv[2 * i + 1].x, yv[2 * i + 1].y, yv[2 * i + 1].z, yv[2 * i + 1].w};
+      uint32_t o0[4], o1[4];
+      if constexpr (GATED) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          o0[j] = pack_bf16x2(gated_act(ACT, lo_f(w0[j]) + acc[j][e], lo_f(w1[j]) + acc[4 + j][e], p.act_alpha, p.act_limit),
+                              gated_act(ACT, hi_f(w0[j]) + acc[j][e + 1], hi_f(w1[j]) + acc[4 + j][e + 1], p.act_alpha,
+                                        p.act_limit));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          o0[j] = pack_bf16x2(lo_f(w0[j]) + acc[j][e], hi_f(w0[j]) + acc[j][e + 1]);
+          o1[j] = pack_bf16x2(lo_f(w1[j]) + acc[4 + j][e], hi_f(w1[j]) + acc[4 + j][e + 1]);
+        }
+      }
+      __nv_bfloat16* row = (i ? out1 : out0) + c0;
+      const bool ok = (i ? tok1 : tok0) >= 0;
+      if (ok && left > 0) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+      if (!GATED && ok && left > 32) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+    }
   }
 }
 
-static constexpr int kShrinkSmem = kStages * kStageBytes, kExpandSmem = 112 * 1024;
+static constexpr int kShrinkFewSmem = kFewWarps * kFewStages * kFewStageBytes, kShrinkSmem = kStages * kStageBytes,
+                     kExpandSmem = 200 * 1024;
 
 template <int ACT>
-static int launch_lora(const LoraParams& p, bool many, bool wide, unsigned tiles, unsigned chunks, unsigned blocks,
-                       cudaStream_t stream) {
-  auto expand = wide ? lora_expand_kernel<4, ACT> : lora_expand_kernel<1, ACT>;
+static int launch_lora(const LoraParams& p, bool many, unsigned tiles, unsigned chunks, unsigned blocks, cudaStream_t stream) {
+  auto expand = many ? lora_expand_kernel<4, ACT> : lora_expand_kernel<1, ACT>;
   static DeviceOnce once;
   int dev;
   if (once.needed(&dev)) {
     const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    if (cudaFuncSetAttribute(lora_shrink_many_kernel, attr, kShrinkSmem) != cudaSuccess ||
+    if (cudaFuncSetAttribute(lora_shrink_few_kernel, attr, kShrinkFewSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(lora_shrink_many_kernel, attr, kShrinkSmem) != cudaSuccess ||
         cudaFuncSetAttribute(lora_expand_kernel<4, ACT>, attr, kExpandSmem) != cudaSuccess ||
         cudaFuncSetAttribute(lora_expand_kernel<1, ACT>, attr, kExpandSmem) != cudaSuccess)
       return -3;
     once.mark(dev);
   }
-  const size_t smem = 2 * sizeof(__nv_bfloat16) * (wide ? 64 : 16) * p.pitch;
+  const int rw = many ? 4 : 1;
+  const size_t smem = static_cast<size_t>(4 / rw) * kExpandStages * (64 * (p.chunk * 2 + 16) + rw * 2048) +
+                      2 * sizeof(__nv_bfloat16) * rw * 16 * p.h_pitch;
   if (smem > kExpandSmem) return -2;
   const dim3 grid(p.parts, chunks, tiles * p.subs_shrink);
   if (grid.z > 65535 || tiles * p.subs > 65535) return -1;
-  const cudaError_t e = many ? launch_pdl(lora_shrink_many_kernel, grid, dim3(kLoraThreads), kShrinkSmem, stream, 1, p)
-                             : launch_pdl(lora_shrink_few_kernel, grid, dim3(kLoraThreads), 0, stream, 1, p);
+  const cudaError_t e =
+      many ? launch_pdl(lora_shrink_many_kernel, grid, dim3(kLoraThreads), kShrinkSmem, stream, 1, p)
+           : launch_pdl(lora_shrink_few_kernel, grid, dim3(kFewThreads), kShrinkFewSmem, stream, 1, p);
   if (e != cudaSuccess) return -3;
-  return launch_pdl(expand, dim3(blocks, tiles * p.subs), dim3(kLoraThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
+  return launch_pdl(expand, dim3(blocks, tiles * p.subs), dim3(kExpandThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace b200
@@ -685,30 +707,32 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   p.h_part = static_cast<long long>(T) * p.h_width;
   p.K = K;
   p.slices = slices;
-  p.groups = 0;
+  const bool many = rows >= 64, gated = act != kActNone;
+  p.act_alpha = act_alpha;
+  p.act_limit = act_limit;
+  p.subs_shrink = p.subs = many ? rows / 64 : rows / 16;
+  p.parts = b200_lora_parts(K, rows, max_tiles, num_slots);
+  p.chunk = std::min(max_rank, many ? 64 : 32);
+  p.h_pitch = (gated ? 2 : 1) * max_rank + 8;    // eight rows of 16 bytes are in banks of their own
+  const unsigned chunks = (p.h_width + kLoraChunk * 8 - 1) / (kLoraChunk * 8), tiles_n = static_cast<unsigned>(max_tiles);
+  // column groups of a CTA: a few rounds of the resident CTAs in all, a group a team at least
+  int groups = 0;
   for (int s = 0; s < kLoraMaxSlices; ++s) {
     p.n[s] = s < slices ? n[s] : 0;
     if (p.n[s] & 7) return -1;
-    p.groups += (p.n[s] + 63) / 64;
+    if (!gated || s == 0) groups += gated ? (p.n[s] + 31) / 32 : (p.n[s] + 63) / 64;
   }
-  if (act != kActNone) p.groups = (n[0] + 31) / 32;
-  p.act = act;
-  p.act_alpha = act_alpha;
-  p.act_limit = act_limit;
-  p.pitch = p.h_width + 8;                       // eight rows of 16 bytes in banks of their own
-  const bool many = rows >= 64, wide = many && 4 * 64 * p.pitch <= kExpandSmem;
-  p.subs_shrink = many ? rows / 64 : rows / 16;
-  p.subs = wide ? rows / 64 : rows / 16;
-  p.parts = b200_lora_parts(K, rows, max_tiles, num_slots);
-  const unsigned chunks = (p.h_width + kLoraChunk * 8 - 1) / (kLoraChunk * 8), tiles_n = static_cast<unsigned>(max_tiles);
-  // column groups: one a warp, more where there are CTAs enough for two rounds of all SMs
-  const long long all = (p.groups + kLoraWarps - 1) / kLoraWarps, per = all * max_tiles * p.subs / (4 * 148);
-  const unsigned blocks = static_cast<unsigned>((all + std::max(per, 1LL) - 1) / std::max(per, 1LL));
+  const int team = many ? 1 : 4;
+  const long long want = static_cast<long long>(groups) * max_tiles * p.subs / (148 * 8);
+  p.per = static_cast<int>(std::max(1LL, (want + team - 1) / team)) * team;
+  unsigned blocks = 0;
+  for (int s = 0; s < slices; ++s)
+    if (!gated || s == 0) blocks += ((gated ? (n[s] + 31) / 32 : (n[s] + 63) / 64) + p.per - 1) / p.per;
   switch (act) {
-    case kActNone: return launch_lora<kActNone>(p, many, wide, tiles_n, chunks, blocks, stream);
-    case kActSilu: return launch_lora<kActSilu>(p, many, wide, tiles_n, chunks, blocks, stream);
-    case kActClampedGlu: return launch_lora<kActClampedGlu>(p, many, wide, tiles_n, chunks, blocks, stream);
-    case kActGeluTanh: return launch_lora<kActGeluTanh>(p, many, wide, tiles_n, chunks, blocks, stream);
-    default: return launch_lora<kActReluGate>(p, many, wide, tiles_n, chunks, blocks, stream);
+    case kActNone: return launch_lora<kActNone>(p, many, tiles_n, chunks, blocks, stream);
+    case kActSilu: return launch_lora<kActSilu>(p, many, tiles_n, chunks, blocks, stream);
+    case kActClampedGlu: return launch_lora<kActClampedGlu>(p, many, tiles_n, chunks, blocks, stream);
+    case kActGeluTanh: return launch_lora<kActGeluTanh>(p, many, tiles_n, chunks, blocks, stream);
+    default: return launch_lora<kActReluGate>(p, many, tiles_n, chunks, blocks, stream);
   }
 }
