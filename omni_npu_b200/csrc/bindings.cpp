@@ -784,9 +784,12 @@ void lora(const Tensor& x, const Tensor& y, const Tensor& out, const Tensor& a, 
           const Tensor& scales, const Tensor& order, const Tensor& tiles, const Tensor& num_tiles, int64_t max_tiles,
           int64_t rows, at::IntArrayRef slices, int64_t max_rank, int64_t act, double act_alpha, double act_limit) {
   int n[4] = {0, 0, 0, 0};
-  int64_t width = 0;
+  int64_t width = 0, padded = 0;
   TORCH_CHECK(!slices.empty() && slices.size() <= 4, "lora: one to four slices");
-  for (size_t i = 0; i < slices.size(); ++i) width += n[i] = (int)slices[i];
+  for (size_t i = 0; i < slices.size(); ++i) {
+    width += n[i] = (int)slices[i];
+    padded += (slices[i] + 31) / 32 * 32;
+  }
   const int64_t T = x.size(0), L = ranks.size(0), S = (int64_t)slices.size();
   for (const Tensor* t : {&x, &y, &out, &a, &b}) CHECK_CUDA_BF16(*t);
   for (const Tensor* t : {&x, &y, &out})
@@ -795,8 +798,8 @@ void lora(const Tensor& x, const Tensor& y, const Tensor& out, const Tensor& a, 
                 "lora: rows of x, y and out are contiguous and start at 16-byte boundaries");
   TORCH_CHECK(y.size(1) == width && out.size(1) == (act ? slices[0] : width), "lora: widths of y and out");
   TORCH_CHECK(a.is_contiguous() && b.is_contiguous() && a.dim() == 2 && b.dim() == 2 && a.size(0) == L && b.size(0) == L &&
-                  a.size(1) == S * max_rank * x.size(1) && b.size(1) == width * max_rank,
-              "lora: factors [slots, slices * rank * K] and [slots, columns * rank]");
+                  a.size(1) == S * max_rank * ((x.size(1) + 31) / 32 * 32) && b.size(1) == padded * max_rank,
+              "lora: factors [slots, slices * rank * K] and [slots, columns * rank], K and columns in whole 32");
   CHECK_I32(ranks);
   CHECK_I32(order);
   CHECK_I32(tiles);

@@ -4,8 +4,16 @@
 //   out[t, n] = z[t, n],   or   act(z[t, gate n]) * z[t, up n]
 //
 // for tokens t with adapter s = slots[t] (none: z = y).  y is the shared product; p(n) is the slice of column n (query, key and
-// value of a joined projection have factors of their own).  A slot's factors lie packed: A as [sum of ranks, K], B as one
-// [N_p, rank_p] after another; ranks are multiples of 16 (zero padded), 0 for a slice without an adapter.
+// value of a joined projection have factors of their own).  Ranks are multiples of 16 (zero padded), 0 for a slice without an
+// adapter; the slices' A of a slot are joined along the rank.
+//
+// The factors lie in the order in which lanes of the matrix instructions hold them (g = lane / 4, q = lane % 4), so that they are
+// read in whole kilobytes and need no shuffling:
+//   A  [K / 32][rank / 16][u = 0, 1][lane][8]    ranks g, g + 8 of 16 times k = 8 q + 4 u + 0 .. 3 of 32
+//   B  [N / 32][rank / 16][v = 0, 1][lane][8]    columns 8 (g / 2) + 2 j + g % 2 of 32 for j = 2 v, 2 v + 1 times
+//                                                k = 2 q, 2 q + 1, 2 q + 8, 2 q + 9 of 16
+// K and N padded with zeros.  A lane's 16 bytes of a row of x then are its k of two instructions, and the columns of its
+// results are eight neighbours.
 //
 // Tokens are grouped by adapter once a step (lora_plan_kernel: a stable counting sort, then tiles of up to `rows` tokens of one
 // adapter).  Two launches apply the adapters, both bound by what they read and write:
@@ -27,8 +35,6 @@
 
 namespace b200 {
 
-static constexpr int kLoraThreads = 256;
-static constexpr int kLoraWarps = kLoraThreads / 32;
 static constexpr int kLoraMaxSlices = 4;
 static constexpr int kLoraChunk = 8;             // 8-wide tiles of h in a piece of work
 static constexpr int kPlanThreads = 1024;
@@ -137,9 +143,8 @@ struct LoraParams {
   long long h_part;                              // T * h_width
   int h_width;                                   // slices * largest rank
   int K, slices, parts;
-  int subs_shrink, subs;                         // pieces of a plan's tile, each with CTAs of its own
+  int subs;                                      // pieces of a plan's tile, each with CTAs of its own
   int per;                                       // column groups of a CTA of the second kernel
-  int chunk;                                     // ranks in a stage of its ring
   int n[kLoraMaxSlices];
   int h_pitch;                                   // elements between rows of h in shared memory
   float act_alpha, act_limit;
@@ -167,72 +172,70 @@ __device__ __forceinline__ bool lora_tile(const LoraParams& p, int item, int sub
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
 
-// ---- h of few rows: 16 at most, K dealt to the parts and within one to the warps.  The factors are what is read: every warp has a
-// ring of its own in shared memory (no barrier between copy and product), with some 4 KB of A a stage however many ranks there
-// are: 128 of K for 16 of them, 64 for 32, 32 for 48 or 64.  Rows lie 16 bytes past their length apart, so that eight of them
-// are in banks of their own.
-static constexpr int kFewThreads = 128, kFewWarps = kFewThreads / 32, kFewStages = 3, kFewStageBytes = 2 * 16 * 272;
+// ---- h of few rows: 16 at most, K dealt to the parts and, in steps of 32, to the warps.  The factors are what is read: every
+// lane has a ring of its own in shared memory for what it alone uses of A and x (no barrier between copy and product), 20 to
+// 24 KB a warp in flight however many ranks there are.
+static constexpr int kFewThreads = 128, kFewWarps = kFewThreads / 32, kFewRing = 24 * 1024;
 
 template <int NT>
-__device__ __forceinline__ void shrink_rows(const LoraParams& p, const LoraTile& tl, const int* tok, int n0, int k_lo, int k_hi,
+__device__ __forceinline__ void shrink_rows(const LoraParams& p, const LoraTile& tl, int n0, int sum_r, int s_lo, int s_hi,
                                             uint32_t ring, float* d) {
-  constexpr int KT = NT == 2 ? 128 : NT == 4 ? 64 : 32, PIECES = KT / 8, PITCH = KT * 2 + 16;
-  constexpr int X_AT = NT * 8 * PITCH;
-  static_assert(X_AT + 16 * PITCH <= kFewStageBytes, "stage");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + static_cast<long long>(n0) * p.K;
-  auto copy = [&](int i) {
-    const int k0 = k_lo + (i * kFewWarps + warp) * KT;
-    if (k0 < k_hi) {
-      const uint32_t st = ring + i % kFewStages * kFewStageBytes;
+  constexpr int STAGE = (NT + 2) * 512, D = kFewRing / STAGE;          // NT / 2 x 2 pieces of A, two rows of x
+  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + (n0 / 16) * 512 + lane * 8;
+  const long long a_step = sum_r * 32;
+  const bool ok0 = g < tl.count, ok1 = g + 8 < tl.count;               // (the other rows of h are not used)
+  const __nv_bfloat16* x0 = p.x + (ok0 ? p.order[tl.start + g] : 0) * p.x_stride + t4 * 8;
+  const __nv_bfloat16* x1 = p.x + (ok1 ? p.order[tl.start + g + 8] : 0) * p.x_stride + t4 * 8;
+  ring += lane * 16;
+  int put = 0;
+  auto copy = [&](int s) {
+    if (s < s_hi) {
+      const uint32_t st = ring + put * STAGE;
+      put = put + 1 == D ? 0 : put + 1;
 #pragma unroll
-      for (int u = 0; u < NT * 8 * PIECES / 32; ++u) {
-        const int row = (lane + 32 * u) / PIECES, k = k0 + (lane + 32 * u) % PIECES * 8;
-        cp16(st + row * PITCH + (k - k0) * 2, a + static_cast<long long>(row) * p.K + (k < k_hi ? k : 0), k < k_hi);
-      }
-#pragma unroll
-      for (int u = 0; u < 16 * PIECES / 32; ++u) {
-        const int row = (lane + 32 * u) / PIECES, k = k0 + (lane + 32 * u) % PIECES * 8;
-        if (row < tl.count)                                            // (the other rows of h are not used)
-          cp16(st + X_AT + row * PITCH + (k - k0) * 2, p.x + tok[row] * p.x_stride + (k < k_hi ? k : 0), k < k_hi);
-      }
+      for (int u = 0; u < NT; ++u) cp16(st + u * 512, a + s * a_step + u * 256, true);
+      const bool in = s * 32 + t4 * 8 < p.K;                           // K is a multiple of 8
+      const int k = in ? s * 32 : 0;
+      if (ok0) cp16(st + NT * 512, x0 + k, in);
+      if (ok1) cp16(st + NT * 512 + 512, x1 + k, in);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-#pragma unroll
-  for (int i = 0; i < kFewStages - 1; ++i) copy(i);
+  for (int i = 0; i < D - 1; ++i) copy(s_lo + i * kFewWarps);
   float acc[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-  const uint32_t xf = X_AT + (lane & 15) * PITCH + (lane >> 4) * 16;
-  const uint32_t af = ((lane & 7) + (lane >> 4) * 8) * PITCH + (lane >> 3 & 1) * 16;
-  for (int i = 0; k_lo + (i * kFewWarps + warp) * KT < k_hi; ++i) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
-    __syncwarp();
-    copy(i + kFewStages - 1);
-    const uint32_t st = ring + i % kFewStages * kFewStageBytes;
+  int get = 0;
+  for (int s = s_lo; s < s_hi; s += kFewWarps) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+    const uint32_t st = ring + get * STAGE;
+    get = get + 1 == D ? 0 : get + 1;
+    const uint4 v0 = lds16(st + NT * 512), v1 = lds16(st + NT * 512 + 512);
 #pragma unroll
-    for (int k = 0; k < KT; k += 16) {
-      uint32_t x[4];
-      ldmatrix4(x, st + xf + k * 2);
-#pragma unroll
-      for (int j = 0; j < NT; j += 2) {
-        uint32_t b[4];
-        ldmatrix4(b, st + af + j * 8 * PITCH + k * 2);
-        mma_bf16(acc[j], x[0], x[1], x[2], x[3], b[0], b[1]);
-        mma_bf16(acc[j + 1], x[0], x[1], x[2], x[3], b[2], b[3]);
-      }
+    for (int j = 0; j < NT; j += 2) {
+      const uint4 b = lds16(st + j * 512), c = lds16(st + j * 512 + 512);
+      mma_bf16(acc[j], v0.x, v1.x, v0.y, v1.y, b.x, b.y);
+      mma_bf16(acc[j + 1], v0.x, v1.x, v0.y, v1.y, b.z, b.w);
+      mma_bf16(acc[j], v0.z, v1.z, v0.w, v1.w, c.x, c.y);
+      mma_bf16(acc[j + 1], v0.z, v1.z, v0.w, v1.w, c.z, c.w);
     }
-    __syncwarp();
+    copy(s + (D - 1) * kFewWarps);                                     // where the stage before this one was
   }
+  __syncwarp();
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     *reinterpret_cast<float2*>(d + j * 8) = make_float2(acc[j][0], acc[j][1]);
@@ -243,30 +246,27 @@ __device__ __forceinline__ void shrink_rows(const LoraParams& p, const LoraTile&
 __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const LoraParams p) {
   constexpr int BM = 16, W = kLoraChunk * 8;
   extern __shared__ __align__(128) char smem[];
-  __shared__ int tok[BM];
   pdl_wait();
   pdl_trigger();                                                       // (the second kernel reads what was there before this one)
   LoraTile tl;
-  if (!lora_tile(p, blockIdx.z, p.subs_shrink, BM, tl) || tl.slot < 0) return;
+  if (!lora_tile(p, blockIdx.z, p.subs, BM, tl) || tl.slot < 0) return;
   int sum_r = 0;
   for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * p.slices + s];
   const int n0 = blockIdx.y * W;
   if (n0 >= sum_r) return;
-  if (threadIdx.x < tl.count) tok[threadIdx.x] = p.order[tl.start + threadIdx.x];
-  __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int nt = min(kLoraChunk, (sum_r - n0) / 8);                    // even: ranks are multiples of 16
   const int steps = (p.K + 31) / 32;
-  const int k_lo = static_cast<int>(static_cast<long long>(steps) * blockIdx.x / p.parts) * 32;
-  const int k_hi = min(p.K, static_cast<int>(static_cast<long long>(steps) * (blockIdx.x + 1) / p.parts) * 32);
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kFewStages * kFewStageBytes;
+  const int s_lo = static_cast<int>(static_cast<long long>(steps) * blockIdx.x / p.parts) + warp;
+  const int s_hi = static_cast<int>(static_cast<long long>(steps) * (blockIdx.x + 1) / p.parts);
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kFewRing;
   // (a warp's part of h goes where its ring was)
-  const auto red = [&](int w) { return reinterpret_cast<float*>(smem + w * kFewStages * kFewStageBytes); };
+  const auto red = [&](int w) { return reinterpret_cast<float*>(smem + w * kFewRing); };
   float* d = red(warp) + g * W + t4 * 2;
-  if (nt == 2) shrink_rows<2>(p, tl, tok, n0, k_lo, k_hi, ring, d);
-  else if (nt == 4) shrink_rows<4>(p, tl, tok, n0, k_lo, k_hi, ring, d);
-  else if (nt == 6) shrink_rows<6>(p, tl, tok, n0, k_lo, k_hi, ring, d);
-  else shrink_rows<8>(p, tl, tok, n0, k_lo, k_hi, ring, d);
+  if (nt == 2) shrink_rows<2>(p, tl, n0, sum_r, s_lo, s_hi, ring, d);
+  else if (nt == 4) shrink_rows<4>(p, tl, n0, sum_r, s_lo, s_hi, ring, d);
+  else if (nt == 6) shrink_rows<6>(p, tl, n0, sum_r, s_lo, s_hi, ring, d);
+  else shrink_rows<8>(p, tl, n0, sum_r, s_lo, s_hi, ring, d);
   __syncthreads();
   // the warps' parts in order, four columns a thread
   float* h = p.h + blockIdx.x * p.h_part + static_cast<long long>(tl.start) * p.h_width + n0;
@@ -282,51 +282,55 @@ __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const Lora
   }
 }
 
-// ---- h of many rows: 64 rows of x and 64 of the joined ranks, in slabs of 64 of K through a ring in shared memory, so that
+// ---- h of many rows: 64 rows of x and 64 of the joined ranks, in slabs of 128 of K through a ring in shared memory, so that
 // what is in flight does not depend on registers.  Warps: two halves of every slab's K, then 32 rows x 32 ranks each (a fragment
 // of x and one of A serve two and two pairs of matrix instructions).
-static constexpr int kSlab = 64, kStages = 5, kStageBytes = 2 * 64 * kSlab * 2;
+static constexpr int kManyThreads = 256, kSlab = 128, kStages = 3, kStageBytes = 2 * 64 * kSlab * 2;
 
-__global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_many_kernel(const LoraParams p) {
+__global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const LoraParams p) {
   constexpr int BM = 64, W = kLoraChunk * 8;
   extern __shared__ __align__(128) char smem[];
   pdl_wait();
   pdl_trigger();
   LoraTile tl;
-  if (!lora_tile(p, blockIdx.z, p.subs_shrink, BM, tl) || tl.slot < 0) return;
+  if (!lora_tile(p, blockIdx.z, p.subs, BM, tl) || tl.slot < 0) return;
   int sum_r = 0;
   for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * p.slices + s];
   const int n0 = blockIdx.y * W;
   if (n0 >= sum_r) return;
   const int width = min(W, sum_r - n0);                                // a multiple of 16
-  const int slabs = (p.K + kSlab - 1) / kSlab;
+  const int slabs = (p.K + kSlab - 1) / kSlab, blocks = (p.K + 31) / 32;
   const int s_lo = static_cast<int>(static_cast<long long>(slabs) * blockIdx.x / p.parts);
   const int s_hi = static_cast<int>(static_cast<long long>(slabs) * (blockIdx.x + 1) / p.parts);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
 
-  // copies: eight lanes a row of 128 bytes, its 16-byte pieces at (piece ^ row % 8); two rows of x and of A each
-  const int crow = threadIdx.x >> 3, piece = threadIdx.x & 7;
-  const __nv_bfloat16 *xs[2], *as[2];
-  bool xok[2], aok[2];
+  // copies: sixteen lanes a row of 256 bytes, its 16-byte pieces at piece ^ 4 (row % 2), so that the eight lanes that read two
+  // rows at once find 128 bytes in different banks; A as it lies
+  const int crow = threadIdx.x >> 4, piece = threadIdx.x & 15;
+  const __nv_bfloat16* xs[4];
+  bool xok[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = crow + 32 * i;
+  for (int i = 0; i < 4; ++i) {
+    const int row = crow + 16 * i;
     xok[i] = row < tl.count;
-    aok[i] = row < width;
     xs[i] = p.x + (xok[i] ? p.order[tl.start + row] : 0) * p.x_stride + piece * 8;
-    as[i] = p.a + tl.slot * p.a_slot + static_cast<long long>(n0 + (aok[i] ? row : 0)) * p.K + piece * 8;
   }
+  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + (n0 / 16) * 512 + threadIdx.x * 8;
+  const long long a_step = sum_r * 32;
+  const bool aok = threadIdx.x < width * 4;
   const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-  const uint32_t cdst = base + crow * 128 + ((piece ^ (crow & 7)) << 4);
+  const uint32_t xdst = base + crow * 256 + ((piece ^ (crow & 1) << 2) << 4), adst = base + 16384 + threadIdx.x * 16;
   auto copy = [&](int s) {
     if (s < s_hi) {
-      const uint32_t dst = cdst + (s - s_lo) % kStages * kStageBytes;
+      const uint32_t st = (s - s_lo) % kStages * kStageBytes;
       const bool in = s * kSlab + piece * 8 < p.K;                     // K is a multiple of 8
       const int k = in ? s * kSlab : -piece * 8;                       // (nothing is read there)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        cp16(dst + i * 4096, xs[i] + k, in && xok[i]);
-        cp16(dst + 8192 + i * 4096, as[i] + k, in && aok[i]);
+      for (int i = 0; i < 4; ++i) cp16(xdst + st + i * 4096, xs[i] + k, in && xok[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool kb = s * 4 + i < blocks;
+        if (aok) cp16(adst + st + i * 4096, a + (kb ? s * 4 + i : 0) * a_step, kb);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -342,42 +346,39 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_many_kernel(const
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
-  // rows of the four 8 x 8 matrices of a fragment: x rows 0-7, 8-15 at k, then at k + 8; A ranks 0-7 at k, k + 8, then 8-15
-  const int xr = m0 + (lane & 15), xk = lane >> 4;
-  const int arow = j0 + (lane & 7) + (lane >> 4) * 8, ak = lane >> 3 & 1;
+  const uint32_t xf = base + (m0 + g) * 256, af = base + 16384 + (j0 / 16) * 1024 + lane * 16;
   for (int s = s_lo; s < s_hi; ++s) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncthreads();
     copy(s + kStages - 1);
     if (!live) continue;
-    const uint32_t st = base + (s - s_lo) % kStages * kStageBytes;
+    const uint32_t st = (s - s_lo) % kStages * kStageBytes;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int kc = (kw * 2 + q) * 2;                                 // its first 16-byte piece
-      uint32_t xf[2][4], af[2][4];
+      const int kb = kw * 2 + q;
+      uint4 xv[4], av[2][2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const int row = xr + m * 16;
-        ldmatrix4(xf[m], st + row * 128 + (((kc + xk) ^ (row & 7)) << 4));
-      }
+      for (int i = 0; i < 4; ++i) xv[i] = lds16(xf + st + i * 2048 + ((kb * 4 + t4) ^ (g & 1) << 2) * 16);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int row = arow + j * 16;
-        ldmatrix4(af[j], st + 8192 + row * 128 + (((kc + ak) ^ (row & 7)) << 4));
-      }
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) av[j][u] = lds16(af + st + kb * 4096 + j * 1024 + u * 512);
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          mma_bf16(acc[m][j], xf[m][0], xf[m][1], xf[m][2], xf[m][3], af[j >> 1][(j & 1) * 2], af[j >> 1][(j & 1) * 2 + 1]);
+        for (int j = 0; j < 2; ++j) {
+          const uint4 &v = xv[2 * m], &w = xv[2 * m + 1];
+          mma_bf16(acc[m][2 * j], v.x, w.x, v.y, w.y, av[j][0].x, av[j][0].y);
+          mma_bf16(acc[m][2 * j + 1], v.x, w.x, v.y, w.y, av[j][0].z, av[j][0].w);
+          mma_bf16(acc[m][2 * j], v.z, w.z, v.w, w.w, av[j][1].x, av[j][1].y);
+          mma_bf16(acc[m][2 * j + 1], v.z, w.z, v.w, w.w, av[j][1].z, av[j][1].w);
+        }
     }
   }
   // the two halves of K in order
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  float* red = reinterpret_cast<float*>(smem);                         // [4 warps][32][32]
-  const int g = lane >> 2, t4 = lane & 3;
-  float* mine = red + (warp & 3) * 32 * 36;
+  float* mine = reinterpret_cast<float*>(smem) + (warp & 3) * 32 * 36;
   if (kw == 1 && live) {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -406,20 +407,21 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_many_kernel(const
 }
 
 // ---- z: a CTA has a tile's rows and a run of column groups of one slice, 64 columns of y each (gated: 32 of gate and their 32 of
-// up).  A team of RW warps, 16 rows each, takes a group; y and B come through a ring in shared memory (many rows: one team of
-// four, so that a group's B is read once for 64 rows; few rows: four teams of a warp).  Columns of B are dealt to the matrix
-// instructions so that a lane ends up with eight neighbouring columns twice: y and the result move 16 bytes a lane, 128 of a
-// row at once.
-static constexpr int kExpandThreads = 128, kExpandStages = 3;
+// up).  A warp takes 16 rows of a group: y, which comes through a ring of the lane's own, starts its accumulators; a lane's
+// results are eight neighbouring columns twice, so y and the result move 16 bytes a lane, 128 of a row at once.
+// Many rows: the four warps have 64 rows and the same groups, B goes from L1 into registers a step ahead.  Few rows: the
+// warps have the same 16 rows and every fourth group, B comes through the ring as well, 32 ranks a stage.
+static constexpr int kExpandThreads = 128;
 
-template <int RW, int ACT>
+template <bool MANY, int ACT>
 __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const LoraParams p) {
-  constexpr int BM = 16 * RW, TEAMS = kExpandThreads / 32 / RW, TEAM = 32 * RW;
   constexpr bool GATED = ACT != kActNone;
+  constexpr int BM = MANY ? 64 : 16, STEP = MANY ? 1 : 4, D = MANY ? 3 : 4;
+  constexpr int STAGE = MANY ? 2048 : 2048 + 4096;
+  constexpr int GW = GATED ? 32 : 64;                                  // columns of a slice in a group
   extern __shared__ __align__(128) char smem[];
-  __shared__ int tok[BM];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int team = warp / RW, member = threadIdx.x % TEAM, rows0 = warp % RW * 16;
+  const int rows0 = MANY ? warp * 16 : 0;
   const bool in_place = !GATED && p.out == p.y;
   // Everything but h is older than the first kernel, which has started only behind it: no wait yet.
   LoraTile tl;
@@ -427,9 +429,9 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
     pdl_wait();
     return;
   }
-  // this CTA's slice and groups in it; of the slice: first rank in h, first column of y, factors
+  // this CTA's slice and groups in it; of the slice: first rank in h, first column of y, factors (in blocks of 32 columns)
   int slice = 0, block = blockIdx.x, h0 = 0, first = 0, r0 = 0, r1 = 0;
-  const __nv_bfloat16* b = p.b + (tl.slot >= 0 ? tl.slot * p.b_slot : 0);
+  const __nv_bfloat16* b = p.b + max(tl.slot, 0) * p.b_slot + lane * 8;
   const int* ranks = p.ranks + max(tl.slot, 0) * p.slices;
   if constexpr (GATED) {
     r0 = tl.slot >= 0 ? ranks[0] : 0;
@@ -442,74 +444,83 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
       block -= blocks;
       h0 += r0;
       first += p.n[slice];
-      b += static_cast<long long>(p.n[slice]) * r0;
+      b += static_cast<long long>((p.n[slice] + 31) / 32) * r0 * 32;
     }
     r1 = r0;
   }
-  const int rank = max(r0, r1), N = p.n[slice];
-  if (rank == 0 && in_place) {
+  const int N = p.n[slice], b_last = (N + 31) / 32 - 1, k0 = r0 / 16, k1 = r1 / 16, ks = max(k0, k1);
+  if (ks == 0 && in_place) {
     pdl_wait();
     return;
   }
-  constexpr int GW = GATED ? 32 : 64;                                  // columns of a slice in a group
-  const int ga = block * p.per + team, gb = min((N + GW - 1) / GW, (block + 1) * p.per);
+  const __nv_bfloat16* b_up = b + (GATED ? static_cast<long long>(b_last + 1) * r0 * 32 : 0);
+  const int ga = block * p.per + (MANY ? 0 : warp), gb = min((N + GW - 1) / GW, (block + 1) * p.per);
   const float scale = tl.slot >= 0 ? p.scales[tl.slot] : 0.f;
-  if (threadIdx.x < BM) tok[threadIdx.x] = threadIdx.x < tl.count ? p.order[tl.start + threadIdx.x] : -1;
-  __syncthreads();
-
-  const int b_pitch = p.chunk * 2 + 16;                                // bytes; eight rows are in banks of their own
-  const int stage_bytes = 64 * b_pitch + RW * 2048;
-  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-  const uint32_t ring = base + team * kExpandStages * stage_bytes;
-  const uint32_t h_at = base + TEAMS * kExpandStages * stage_bytes;
-  __nv_bfloat16* h_hi = reinterpret_cast<__nv_bfloat16*>(smem + TEAMS * kExpandStages * stage_bytes);   // [BM][h_pitch]
-  __nv_bfloat16* h_lo = h_hi + BM * p.h_pitch;
-  const uint32_t y_slot = 64 * b_pitch + (warp % RW * 128 + lane) * 16;
-  const int tok0 = tok[rows0 + g], tok1 = tok[rows0 + g + 8];
-  const int chunks = max(1, (rank + p.chunk - 1) / p.chunk);
-  // the ring's next item: chunk of ranks cc of group cg
-  int cg = ga, cc = 0, cs = 0;
+  const int tok0 = rows0 + g < tl.count ? p.order[tl.start + rows0 + g] : -1;
+  const int tok1 = rows0 + g + 8 < tl.count ? p.order[tl.start + rows0 + g + 8] : -1;
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * D * STAGE + lane * 16;
+  const __nv_bfloat16* y0 = p.y + max(tok0, 0) * p.y_stride + first + (GATED ? 2 : 1) * t4 * 8;
+  const __nv_bfloat16* y1 = p.y + max(tok1, 0) * p.y_stride + first + (GATED ? 2 : 1) * t4 * 8;
+  // 16 ranks (step k) of 32 columns of group gi: its half s, or gate / up.  Past the end: any others, whose results are not used
+  auto b_at = [&](int gi, int s, int k) {
+    if constexpr (GATED) return (s ? b_up : b) + (static_cast<long long>(gi) * (s ? k1 : k0) + min(k, max((s ? k1 : k0) - 1, 0))) * 512;
+    return b + (static_cast<long long>(min(2 * gi + s, b_last)) * k0 + k) * 512;
+  };
+  // the ring's next stage: group cg (few rows: and steps ck, ck + 1)
+  int cg = ga, ck = 0, put = 0;
   auto copy = [&]() {
     if (cg < gb) {
-      const uint32_t st = ring + cs * stage_bytes;
-      const int c0 = cg * GW;
+      const uint32_t st = ring + put * STAGE;
+      put = put + 1 == D ? 0 : put + 1;
+      if (MANY || ck == 0) {
+        const int c0 = cg * GW, left = N - c0 - t4 * 8;
+        const int at = (GATED ? 2 : 1) * c0, half = GATED ? 8 : 32;
+        if (tok0 >= 0 && left > 0) cp16(st, y0 + at, true);
+        if (tok0 >= 0 && left > (GATED ? 0 : 32)) cp16(st + 512, y0 + at + half, true);
+        if (tok1 >= 0 && left > 0) cp16(st + 1024, y1 + at, true);
+        if (tok1 >= 0 && left > (GATED ? 0 : 32)) cp16(st + 1536, y1 + at + half, true);
+      }
+      if constexpr (MANY) {
+        cg += STEP;
+      } else {
 #pragma unroll
-      for (int s = 0; s < (GATED ? 2 : 1); ++s) {
-        const int rs = s ? r1 : r0, kc = min(p.chunk, rs - cc * p.chunk), pieces = kc >> 3;
-        if (kc <= 0) continue;
-        const __nv_bfloat16* src = b + (s ? static_cast<long long>(N) * r0 : 0) + static_cast<long long>(c0) * rs + cc * p.chunk;
-        const uint32_t inv = 65536u / pieces + 1;                      // i / pieces for i < 512
-        for (int i = member; i < GW * pieces; i += TEAM) {
-          const int col = (i * inv) >> 16, piece = i - col * pieces, c = col & 31;
-          const int row = s * 32 + (col & 32) + ((c & 7) >> 1) * 8 + (c >> 3) * 2 + (c & 1);
-          if (c0 + col < N) cp16(st + row * b_pitch + piece * 16, src + col * rs + piece * 8, true);
+        for (int k = 0; k < 2; ++k)
+          if (ck + k < ks) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const __nv_bfloat16* src = b_at(cg, s, ck + k);
+              cp16(st + 2048 + k * 2048 + s * 1024, src, true);
+              cp16(st + 2048 + k * 2048 + s * 1024 + 512, src + 256, true);
+            }
+          }
+        ck += 2;
+        if (ck >= ks) {
+          ck = 0;
+          cg += STEP;
         }
       }
-      if (cc == 0) {
-        const int col = c0 + t4 * 8;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int t = i ? tok1 : tok0;
-          const __nv_bfloat16* row = p.y + t * p.y_stride + first + (GATED ? 2 : 1) * col;
-          if (t >= 0 && col < N) cp16(st + y_slot + i * 1024, row, true);
-          if (t >= 0 && col + (GATED ? 0 : 32) < N) cp16(st + y_slot + i * 1024 + 512, row + (GATED ? 8 : 32), true);
-        }
-      }
-      if (++cc == chunks) {
-        cc = 0;
-        cg += TEAMS;
-      }
-      cs = cs + 1 == kExpandStages ? 0 : cs + 1;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int i = 0; i < kExpandStages - 1; ++i) copy();
+  for (int i = 0; i < D - 1; ++i) copy();
+  uint4 bv[4];                                                         // many rows: a step's B, half s at 2 s
+  auto load_b = [&](uint4 (&v)[4], int gi, int k) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const __nv_bfloat16* src = b_at(gi, s, k);
+      v[2 * s] = *reinterpret_cast<const uint4*>(src);
+      v[2 * s + 1] = *reinterpret_cast<const uint4*>(src + 256);
+    }
+  };
+  if (MANY && ks > 0) load_b(bv, ga, 0);
   pdl_wait();
   pdl_trigger();
 
   // h: the parts in order, times the scale, as the sum of two bf16 (17 bits of the fp32 value), so that the product below adds
   // no rounding beside that of its result
+  __nv_bfloat16* h_hi = reinterpret_cast<__nv_bfloat16*>(smem + 4 * D * STAGE);                 // [BM][h_pitch]
+  __nv_bfloat16* h_lo = h_hi + BM * p.h_pitch;
   const int sum_r = GATED ? r0 + r1 : r0;
   if (sum_r > 0) {
     const float* h = p.h + static_cast<long long>(tl.start) * p.h_width + h0;
@@ -538,76 +549,91 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
     }
   }
   __syncthreads();
-  const uint32_t hf = h_at + ((rows0 + (lane & 15)) * p.h_pitch + (lane >> 4) * 8) * 2, lo_at = 2 * BM * p.h_pitch;
-  const uint32_t bf = ((lane & 7) + (lane >> 4) * 8) * b_pitch + (lane >> 3 & 1) * 16;
-  const bool live = rows0 < tl.count;
+  if (rows0 >= tl.count) return;
+  const uint32_t hf = static_cast<uint32_t>(__cvta_generic_to_shared(h_hi)) + ((rows0 + (lane & 15)) * p.h_pitch + (lane >> 4) * 8) * 2;
+  const uint32_t lo_at = 2 * BM * p.h_pitch;
   __nv_bfloat16* out0 = p.out + tok0 * p.out_stride + first + t4 * 8;
   __nv_bfloat16* out1 = p.out + tok1 * p.out_stride + first + t4 * 8;
-  int rs = 0;                                                          // the ring's stage that is read
-  for (int gi = ga; gi < gb; gi += TEAMS) {
+  int get = 0;
+  for (int gi = ga; gi < gb; gi += STEP) {
     float acc[8][4];
+    uint32_t st;
+    auto next = [&]() {
+      asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+      st = ring + get * STAGE;
+      get = get + 1 == D ? 0 : get + 1;
+    };
+    // step k of h times its B
+    auto multiply = [&](int k, const uint4& p0, const uint4& p1, const uint4& q0, const uint4& q1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-    uint4 yv[4];
-    for (int c = 0; c < chunks; ++c) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kExpandStages - 2) : "memory");
-      if constexpr (RW > 1) __syncthreads();
-      else __syncwarp();
-      copy();
-      const uint32_t st = ring + rs * stage_bytes;
-      rs = rs + 1 == kExpandStages ? 0 : rs + 1;
-      if (!live) continue;
-      if (c == 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(yv[i].x), "=r"(yv[i].y), "=r"(yv[i].z), "=r"(yv[i].w)
-                       : "r"(st + y_slot + i * 512)
-                       : "memory");
+      for (int s = 0; s < 2; ++s) {
+        if (GATED && k >= (s ? k1 : k0)) continue;
+        const uint4 &v = s ? q0 : p0, &w = s ? q1 : p1;
+        uint32_t hi[4], lo[4];
+        const uint32_t at = hf + k * 32 + (GATED && s ? r0 * 2 : 0);
+        ldmatrix4(hi, at);
+        ldmatrix4(lo, at + lo_at);
+        float(*c)[4] = acc + 4 * s;
+        mma_bf16(c[0], hi[0], hi[1], hi[2], hi[3], v.x, v.y);
+        mma_bf16(c[1], hi[0], hi[1], hi[2], hi[3], v.z, v.w);
+        mma_bf16(c[2], hi[0], hi[1], hi[2], hi[3], w.x, w.y);
+        mma_bf16(c[3], hi[0], hi[1], hi[2], hi[3], w.z, w.w);
+        mma_bf16(c[0], lo[0], lo[1], lo[2], lo[3], v.x, v.y);
+        mma_bf16(c[1], lo[0], lo[1], lo[2], lo[3], v.z, v.w);
+        mma_bf16(c[2], lo[0], lo[1], lo[2], lo[3], w.x, w.y);
+        mma_bf16(c[3], lo[0], lo[1], lo[2], lo[3], w.z, w.w);
       }
-      const int k0 = c * p.chunk;
-      for (int k = 0; k < min(p.chunk, rank - k0); k += 16) {
+    };
+    next();
 #pragma unroll
-        for (int s = 0; s < (GATED ? 2 : 1); ++s) {
-          if (GATED && k0 + k >= (s ? r1 : r0)) continue;
-          uint32_t hi[4], lo[4];
-          const uint32_t at = hf + (k0 + k + (s ? r0 : 0)) * 2;
-          ldmatrix4(hi, at);
-          ldmatrix4(lo, at + lo_at);
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int j = 0; j < (GATED ? 4 : 8); j += 2) {
-            uint32_t v[4];
-            const int o = 4 * s + j;
-            ldmatrix4(v, st + bf + o * 8 * b_pitch + k * 2);
-            mma_bf16(acc[o], hi[0], hi[1], hi[2], hi[3], v[0], v[1]);
-            mma_bf16(acc[o + 1], hi[0], hi[1], hi[2], hi[3], v[2], v[3]);
-            mma_bf16(acc[o], lo[0], lo[1], lo[2], lo[3], v[0], v[1]);
-            mma_bf16(acc[o + 1], lo[0], lo[1], lo[2], lo[3], v[2], v[3]);
-          }
+      for (int s = 0; s < 2; ++s) {
+        const uint4 v = lds16(st + i * 1024 + s * 512);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[4 * s + j][2 * i] = lo_f(w[j]);
+          acc[4 * s + j][2 * i + 1] = hi_f(w[j]);
         }
       }
+    if constexpr (MANY) {
+      copy();
+      for (int k = 0; k < ks; ++k) {
+        uint4 bn[4];
+        const bool more = k + 1 < ks;
+        load_b(bn, more || gi + 1 >= gb ? gi : gi + 1, more ? k + 1 : 0);
+        multiply(k, bv[0], bv[1], bv[2], bv[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bv[i] = bn[i];
+      }
+    } else {
+      for (int k = 0;;) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (k + u < ks) {
+            const uint32_t at = st + 2048 + u * 2048;
+            multiply(k + u, lds16(at), lds16(at + 512), lds16(at + 1024), lds16(at + 1536));
+          }
+        copy();
+        k += 2;
+        if (k >= ks) break;
+        next();
+      }
     }
-    if (!live) continue;
     const int c0 = gi * GW, left = N - c0 - t4 * 8;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int e = 2 * i;
-      const uint32_t w0[4] = {yv[2 * i].x, yv[2 * i].y, yv[2 * i].z, yv[2 * i].w};
-      const uint32_t w1[4] = {yv[2 * i + 1].x, yv[2 * i + 1].y, yv[2 * i + 1].z, yv[2 * i + 1].w};
       uint32_t o0[4], o1[4];
-      if constexpr (GATED) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          o0[j] = pack_bf16x2(gated_act(ACT, lo_f(w0[j]) + acc[j][e], lo_f(w1[j]) + acc[4 + j][e], p.act_alpha, p.act_limit),
-                              gated_act(ACT, hi_f(w0[j]) + acc[j][e + 1], hi_f(w1[j]) + acc[4 + j][e + 1], p.act_alpha,
-                                        p.act_limit));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          o0[j] = pack_bf16x2(lo_f(w0[j]) + acc[j][e], hi_f(w0[j]) + acc[j][e + 1]);
-          o1[j] = pack_bf16x2(lo_f(w1[j]) + acc[4 + j][e], hi_f(w1[j]) + acc[4 + j][e + 1]);
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (GATED) {
+          o0[j] = pack_bf16x2(gated_act(ACT, acc[j][e], acc[4 + j][e], p.act_alpha, p.act_limit),
+                              gated_act(ACT, acc[j][e + 1], acc[4 + j][e + 1], p.act_alpha, p.act_limit));
+        } else {
+          o0[j] = pack_bf16x2(acc[j][e], acc[j][e + 1]);
+          o1[j] = pack_bf16x2(acc[4 + j][e], acc[4 + j][e + 1]);
         }
       }
       __nv_bfloat16* row = (i ? out1 : out0) + c0;
@@ -618,34 +644,33 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
   }
 }
 
-static constexpr int kShrinkFewSmem = kFewWarps * kFewStages * kFewStageBytes, kShrinkSmem = kStages * kStageBytes,
-                     kExpandSmem = 200 * 1024;
+static constexpr int kShrinkFewSmem = kFewWarps * kFewRing, kShrinkManySmem = kStages * kStageBytes, kExpandSmem = 168 * 1024;
 
-template <int ACT>
-static int launch_lora(const LoraParams& p, bool many, unsigned tiles, unsigned chunks, unsigned blocks, cudaStream_t stream) {
-  auto expand = many ? lora_expand_kernel<4, ACT> : lora_expand_kernel<1, ACT>;
+template <bool MANY, int ACT>
+static int launch_lora(const LoraParams& p, unsigned tiles, unsigned chunks, unsigned blocks, cudaStream_t stream) {
+  auto shrink = MANY ? lora_shrink_many_kernel : lora_shrink_few_kernel;
+  auto expand = lora_expand_kernel<MANY, ACT>;
   static DeviceOnce once;
   int dev;
   if (once.needed(&dev)) {
     const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    if (cudaFuncSetAttribute(lora_shrink_few_kernel, attr, kShrinkFewSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(lora_shrink_many_kernel, attr, kShrinkSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(lora_expand_kernel<4, ACT>, attr, kExpandSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(lora_expand_kernel<1, ACT>, attr, kExpandSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(shrink, attr, MANY ? kShrinkManySmem : kShrinkFewSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(expand, attr, kExpandSmem) != cudaSuccess)
       return -3;
     once.mark(dev);
   }
-  const int rw = many ? 4 : 1;
-  const size_t smem = static_cast<size_t>(4 / rw) * kExpandStages * (64 * (p.chunk * 2 + 16) + rw * 2048) +
-                      2 * sizeof(__nv_bfloat16) * rw * 16 * p.h_pitch;
-  if (smem > kExpandSmem) return -2;
-  const dim3 grid(p.parts, chunks, tiles * p.subs_shrink);
-  if (grid.z > 65535 || tiles * p.subs > 65535) return -1;
-  const cudaError_t e =
-      many ? launch_pdl(lora_shrink_many_kernel, grid, dim3(kLoraThreads), kShrinkSmem, stream, 1, p)
-           : launch_pdl(lora_shrink_few_kernel, grid, dim3(kFewThreads), kShrinkFewSmem, stream, 1, p);
-  if (e != cudaSuccess) return -3;
-  return launch_pdl(expand, dim3(blocks, tiles * p.subs), dim3(kExpandThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
+  const size_t smem = 4 * (MANY ? 3 * 2048 : 4 * 6144) + 2 * sizeof(__nv_bfloat16) * (MANY ? 64 : 16) * p.h_pitch;
+  const dim3 grid(p.parts, chunks, tiles * p.subs);
+  if (smem > kExpandSmem || grid.z > 65535) return -2;
+  if (launch_pdl(shrink, grid, dim3(MANY ? kManyThreads : kFewThreads), MANY ? kShrinkManySmem : kShrinkFewSmem, stream, 1, p) !=
+      cudaSuccess)
+    return -3;
+  return launch_pdl(expand, dim3(blocks, grid.z), dim3(kExpandThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
+}
+
+template <int ACT>
+static int launch_lora(const LoraParams& p, bool many, unsigned tiles, unsigned chunks, unsigned blocks, cudaStream_t stream) {
+  return many ? launch_lora<true, ACT>(p, tiles, chunks, blocks, stream) : launch_lora<false, ACT>(p, tiles, chunks, blocks, stream);
 }
 
 }  // namespace b200
@@ -710,9 +735,8 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   const bool many = rows >= 64, gated = act != kActNone;
   p.act_alpha = act_alpha;
   p.act_limit = act_limit;
-  p.subs_shrink = p.subs = many ? rows / 64 : rows / 16;
+  p.subs = many ? rows / 64 : rows / 16;
   p.parts = b200_lora_parts(K, rows, max_tiles, num_slots);
-  p.chunk = std::min(max_rank, many ? 64 : 32);
   p.h_pitch = (gated ? 2 : 1) * max_rank + 8;    // eight rows of 16 bytes are in banks of their own
   const unsigned chunks = (p.h_width + kLoraChunk * 8 - 1) / (kLoraChunk * 8), tiles_n = static_cast<unsigned>(max_tiles);
   // column groups of a CTA: a few rounds of the resident CTAs in all, a group a team at least

@@ -20,6 +20,12 @@ MAX_SLOTS, MAX_SLICES, MAX_RANK = 512, 4, 256
 FEW_TOKENS, FEW_ROWS, MANY_ROWS = 256, 16, 64
 
 
+def _padded(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    if tuple(t.shape) != (rows, cols):
+        t = torch.nn.functional.pad(t, (0, cols - t.shape[1], 0, rows - t.shape[0]))
+    return t.contiguous()
+
+
 class LoraStack:
     """Factors of one projection [sum(slices), in_features] for ``num_slots`` adapters of rank up to ``max_rank``.
 
@@ -48,9 +54,10 @@ class LoraStack:
         self.max_rank = (max_rank + 15) // 16 * 16
         self.dtype = dtype
         with torch.inference_mode(False):
-            # packed: A of a slot as [sum of its ranks, K], B as one [columns, rank] after another
-            self.a = torch.zeros(num_slots, len(slices) * self.max_rank * in_features, dtype=dtype, device=device)
-            self.b = torch.zeros(num_slots, self.out_features * self.max_rank, dtype=dtype, device=device)
+            # in the order of the matrix instructions' lanes (csrc/lora/lora.cu), K and columns in whole 32
+            self._k = (in_features + 31) // 32
+            self.a = torch.zeros(num_slots, len(slices) * self.max_rank * self._k * 32, dtype=dtype, device=device)
+            self.b = torch.zeros(num_slots, sum((n + 31) // 32 * 32 for n in slices) * self.max_rank, dtype=dtype, device=device)
             self.ranks = torch.zeros(num_slots, len(slices), dtype=torch.int32, device=device)
             self.scales = torch.zeros(num_slots, dtype=torch.float32, device=device)
         self.device = self.a.device
@@ -79,23 +86,34 @@ class LoraStack:
                 raise ValueError(f"LoraStack.load: rank {r}, at most {self.max_rank}")
             ranks.append((r + 15) // 16 * 16)
         with torch.inference_mode():
-            at = 0
-            for p, r in zip(a, ranks):
-                if r:
-                    rows = self.a[slot, at: at + r * self.in_features].view(r, self.in_features)
-                    rows[: p.shape[0]].copy_(p)
-                    rows[p.shape[0]:].zero_()
-                    at += r * self.in_features
-            at = 0
-            for q, r, n in zip(b, ranks, self.slices):
-                if r:
-                    cols = self.b[slot, at: at + n * r].view(n, r)
-                    cols[:, : q.shape[1]].copy_(q)
-                    cols[:, q.shape[1]:].zero_()
-                    at += n * r
+            for p, view in zip(a, self._views_a(slot, ranks)):
+                if view is not None:
+                    view.copy_(_padded(p, view.shape[0] * 16, self._k * 32).view(view.shape))
+            for q, view in zip(b, self._views_b(slot, ranks)):
+                if view is not None:
+                    view.copy_(_padded(q, view.shape[0] * 32, view.shape[5] * 16).view(view.shape))
             self.scales[slot] = float(scale)
             self.ranks[slot].copy_(torch.tensor(ranks, dtype=torch.int32))
         self._ranks[slot] = ranks
+
+    def _views_a(self, slot: int, ranks):
+        """A of each slice as [ranks, K] in the shape (rank / 16, 2, 8, K / 32, 4, 2, 4) over its packed place."""
+        total = sum(ranks) // 16
+        packed = self.a[slot, : total * 16 * self._k * 32].view(self._k, total, 2, 8, 4, 2, 4)   # k32, r16, u, g, q, half, 4
+        at = 0
+        for r in ranks:
+            yield packed[:, at: at + r // 16].permute(1, 5, 3, 0, 4, 2, 6) if r else None
+            at += r // 16
+
+    def _views_b(self, slot: int, ranks):
+        """B of each slice as [columns, rank] in the shape (columns / 32, 4, 2, 2, 2, rank / 16, 2, 4, 2) over its packed place."""
+        at = 0
+        for r, n in zip(ranks, self.slices):
+            c = (n + 31) // 32
+            # n32, r16, v, g / 2, g % 2, q, j % 2, half, 2
+            yield (self.b[slot, at: at + c * 32 * r].view(c, r // 16, 2, 4, 2, 4, 2, 2, 2).permute(0, 3, 2, 6, 4, 1, 7, 5, 8)
+                   if r else None)
+            at += c * 32 * r
 
     def clear(self, slot: int) -> None:
         """Empty a slot."""
@@ -106,16 +124,9 @@ class LoraStack:
 
     def factors(self, slot: int):
         """(A, B) of each slice of a slot (ranks padded to 16), None where it has none."""
-        out, pa, pb = [], 0, 0
-        for r, n in zip(self._ranks[slot], self.slices):
-            if not r:
-                out.append(None)
-                continue
-            out.append((self.a[slot, pa: pa + r * self.in_features].view(r, self.in_features),
-                        self.b[slot, pb: pb + n * r].view(n, r)))
-            pa += r * self.in_features
-            pb += n * r
-        return out
+        ranks = self._ranks[slot]
+        return [None if a is None else (a.reshape(r, -1)[:, : self.in_features], b.reshape(-1, r)[:n])
+                for a, b, r, n in zip(self._views_a(slot, ranks), self._views_b(slot, ranks), ranks, self.slices)]
 
     def columns(self, i: int) -> torch.Tensor:
         """Where the columns of slice ``i`` lie in the projection's result."""
