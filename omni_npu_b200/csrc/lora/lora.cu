@@ -170,7 +170,7 @@ __device__ __forceinline__ bool lora_tile(const LoraParams& p, int item, int sub
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   uint4 v;
@@ -407,21 +407,20 @@ __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const
 }
 
 // ---- z: a CTA has a tile's rows and a run of column groups of one slice, 64 columns of y each (gated: 32 of gate and their 32 of
-// up).  A warp takes 16 rows of a group: y, which comes through a ring of the lane's own, starts its accumulators; a lane's
-// results are eight neighbouring columns twice, so y and the result move 16 bytes a lane, 128 of a row at once.
-// Many rows: the four warps have 64 rows and the same groups, B goes from L1 into registers a step ahead.  Few rows: the
-// warps have the same 16 rows and every fourth group, B comes through the ring as well, 32 ranks a stage.
+// up).  A warp takes every fourth group, 16 rows at a time: y, which comes through a ring of the lane's own, starts its
+// accumulators; a lane's results are eight neighbouring columns twice, so y and the result move 16 bytes a lane, 512 of a row
+// by the four warps.  Many rows: B is read into registers once for the 64 rows (up to 32 ranks; above, two steps of 16
+// follow one another).  Few rows: B comes through the ring as well, 32 ranks a stage.
 static constexpr int kExpandThreads = 128;
 
 template <bool MANY, int ACT>
 __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const LoraParams p) {
   constexpr bool GATED = ACT != kActNone;
-  constexpr int BM = MANY ? 64 : 16, STEP = MANY ? 1 : 4, D = MANY ? 3 : 4;
-  constexpr int STAGE = MANY ? 2048 : 2048 + 4096;
+  constexpr int BM = MANY ? 64 : 16, STEP = 4, D = 4, STAGE = MANY ? 2048 : 2048 + 4096;
   constexpr int GW = GATED ? 32 : 64;                                  // columns of a slice in a group
   extern __shared__ __align__(128) char smem[];
+  __shared__ int tok[BM];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int rows0 = MANY ? warp * 16 : 0;
   const bool in_place = !GATED && p.out == p.y;
   // Everything but h is older than the first kernel, which has started only behind it: no wait yet.
   LoraTile tl;
@@ -429,6 +428,7 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
     pdl_wait();
     return;
   }
+  if (threadIdx.x < BM) tok[threadIdx.x] = threadIdx.x < tl.count ? p.order[tl.start + threadIdx.x] : -1;
   // this CTA's slice and groups in it; of the slice: first rank in h, first column of y, factors (in blocks of 32 columns)
   int slice = 0, block = blockIdx.x, h0 = 0, first = 0, r0 = 0, r1 = 0;
   const __nv_bfloat16* b = p.b + max(tl.slot, 0) * p.b_slot + lane * 8;
@@ -454,34 +454,40 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
     return;
   }
   const __nv_bfloat16* b_up = b + (GATED ? static_cast<long long>(b_last + 1) * r0 * 32 : 0);
-  const int ga = block * p.per + (MANY ? 0 : warp), gb = min((N + GW - 1) / GW, (block + 1) * p.per);
+  const int ga = block * p.per + warp, gb = min((N + GW - 1) / GW, (block + 1) * p.per);
+  const int ms = (tl.count + 15) / 16;
   const float scale = tl.slot >= 0 ? p.scales[tl.slot] : 0.f;
-  const int tok0 = rows0 + g < tl.count ? p.order[tl.start + rows0 + g] : -1;
-  const int tok1 = rows0 + g + 8 < tl.count ? p.order[tl.start + rows0 + g + 8] : -1;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * D * STAGE + lane * 16;
-  const __nv_bfloat16* y0 = p.y + max(tok0, 0) * p.y_stride + first + (GATED ? 2 : 1) * t4 * 8;
-  const __nv_bfloat16* y1 = p.y + max(tok1, 0) * p.y_stride + first + (GATED ? 2 : 1) * t4 * 8;
+  const __nv_bfloat16* y = p.y + first + (GATED ? 2 : 1) * t4 * 8;
+  __nv_bfloat16* out = p.out + first + t4 * 8;
   // 16 ranks (step k) of 32 columns of group gi: its half s, or gate / up.  Past the end: any others, whose results are not used
   auto b_at = [&](int gi, int s, int k) {
     if constexpr (GATED) return (s ? b_up : b) + (static_cast<long long>(gi) * (s ? k1 : k0) + min(k, max((s ? k1 : k0) - 1, 0))) * 512;
-    return b + (static_cast<long long>(min(2 * gi + s, b_last)) * k0 + k) * 512;
+    return b + (static_cast<long long>(min(2 * gi + s, b_last)) * k0 + min(k, k0 - 1)) * 512;
   };
-  // the ring's next stage: group cg (few rows: and steps ck, ck + 1)
-  int cg = ga, ck = 0, put = 0;
+  __syncthreads();
+  // the ring's next stage: group cg and its rows cm (few rows: steps ck, ck + 1)
+  int cg = ga, cm = 0, ck = 0, put = 0;
   auto copy = [&]() {
     if (cg < gb) {
       const uint32_t st = ring + put * STAGE;
       put = put + 1 == D ? 0 : put + 1;
       if (MANY || ck == 0) {
-        const int c0 = cg * GW, left = N - c0 - t4 * 8;
-        const int at = (GATED ? 2 : 1) * c0, half = GATED ? 8 : 32;
-        if (tok0 >= 0 && left > 0) cp16(st, y0 + at, true);
-        if (tok0 >= 0 && left > (GATED ? 0 : 32)) cp16(st + 512, y0 + at + half, true);
-        if (tok1 >= 0 && left > 0) cp16(st + 1024, y1 + at, true);
-        if (tok1 >= 0 && left > (GATED ? 0 : 32)) cp16(st + 1536, y1 + at + half, true);
+        const int left = N - cg * GW - t4 * 8;
+        const __nv_bfloat16* src = y + (GATED ? 2 : 1) * GW * cg;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int t = tok[cm * 16 + i * 8 + g];
+          const __nv_bfloat16* row = src + t * p.y_stride;
+          if (t >= 0 && left > 0) cp16(st + i * 1024, row, true);
+          if (t >= 0 && left > (GATED ? 0 : 32)) cp16(st + i * 1024 + 512, row + (GATED ? 8 : 32), true);
+        }
       }
       if constexpr (MANY) {
-        cg += STEP;
+        if (++cm == ms) {
+          cm = 0;
+          cg += STEP;
+        }
       } else {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -504,7 +510,7 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
   };
 #pragma unroll
   for (int i = 0; i < D - 1; ++i) copy();
-  uint4 bv[4];                                                         // many rows: a step's B, half s at 2 s
+  uint4 bv[2][4];                                                      // many rows: B of two steps, half s at 2 s
   auto load_b = [&](uint4 (&v)[4], int gi, int k) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -513,7 +519,10 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
       v[2 * s + 1] = *reinterpret_cast<const uint4*>(src + 256);
     }
   };
-  if (MANY && ks > 0) load_b(bv, ga, 0);
+  if (MANY && ks > 0 && ga < gb) {
+    load_b(bv[0], ga, 0);
+    if (ks > 1) load_b(bv[1], ga, 1);
+  }
   pdl_wait();
   pdl_trigger();
 
@@ -525,7 +534,7 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
   if (sum_r > 0) {
     const float* h = p.h + static_cast<long long>(tl.start) * p.h_width + h0;
     const int vecs = sum_r / 4;
-    for (int i = threadIdx.x; i < BM * vecs; i += kExpandThreads) {
+    for (int i = threadIdx.x; i < ms * 16 * vecs; i += kExpandThreads) {
       const int row = i / vecs, v = i % vecs * 4;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < tl.count) {
@@ -549,97 +558,98 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
     }
   }
   __syncthreads();
-  if (rows0 >= tl.count) return;
-  const uint32_t hf = static_cast<uint32_t>(__cvta_generic_to_shared(h_hi)) + ((rows0 + (lane & 15)) * p.h_pitch + (lane >> 4) * 8) * 2;
-  const uint32_t lo_at = 2 * BM * p.h_pitch;
-  __nv_bfloat16* out0 = p.out + tok0 * p.out_stride + first + t4 * 8;
-  __nv_bfloat16* out1 = p.out + tok1 * p.out_stride + first + t4 * 8;
+  const uint32_t hf = static_cast<uint32_t>(__cvta_generic_to_shared(h_hi)) + ((lane & 15) * p.h_pitch + (lane >> 4) * 8) * 2;
+  const uint32_t lo_at = 2 * BM * p.h_pitch, m_step = 32 * p.h_pitch;
   int get = 0;
   for (int gi = ga; gi < gb; gi += STEP) {
-    float acc[8][4];
-    uint32_t st;
-    auto next = [&]() {
-      asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
-      st = ring + get * STAGE;
-      get = get + 1 == D ? 0 : get + 1;
-    };
-    // step k of h times its B
-    auto multiply = [&](int k, const uint4& p0, const uint4& p1, const uint4& q0, const uint4& q1) {
+    const int left = N - gi * GW - t4 * 8;
+    for (int m = 0; m < ms; ++m) {
+      float acc[8][4];
+      uint32_t st;
+      auto next = [&]() {
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+        st = ring + get * STAGE;
+        get = get + 1 == D ? 0 : get + 1;
+      };
+      // step k of h times its B
+      auto multiply = [&](int k, const uint4& p0, const uint4& p1, const uint4& q0, const uint4& q1) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (GATED && k >= (s ? k1 : k0)) continue;
-        const uint4 &v = s ? q0 : p0, &w = s ? q1 : p1;
-        uint32_t hi[4], lo[4];
-        const uint32_t at = hf + k * 32 + (GATED && s ? r0 * 2 : 0);
-        ldmatrix4(hi, at);
-        ldmatrix4(lo, at + lo_at);
-        float(*c)[4] = acc + 4 * s;
-        mma_bf16(c[0], hi[0], hi[1], hi[2], hi[3], v.x, v.y);
-        mma_bf16(c[1], hi[0], hi[1], hi[2], hi[3], v.z, v.w);
-        mma_bf16(c[2], hi[0], hi[1], hi[2], hi[3], w.x, w.y);
-        mma_bf16(c[3], hi[0], hi[1], hi[2], hi[3], w.z, w.w);
-        mma_bf16(c[0], lo[0], lo[1], lo[2], lo[3], v.x, v.y);
-        mma_bf16(c[1], lo[0], lo[1], lo[2], lo[3], v.z, v.w);
-        mma_bf16(c[2], lo[0], lo[1], lo[2], lo[3], w.x, w.y);
-        mma_bf16(c[3], lo[0], lo[1], lo[2], lo[3], w.z, w.w);
+        for (int s = 0; s < 2; ++s) {
+          if (GATED && k >= (s ? k1 : k0)) continue;
+          const uint4 &v = s ? q0 : p0, &w = s ? q1 : p1;
+          uint32_t hi[4], lo[4];
+          const uint32_t at = hf + m * m_step + k * 32 + (GATED && s ? r0 * 2 : 0);
+          ldmatrix4(hi, at);
+          ldmatrix4(lo, at + lo_at);
+          float(*c)[4] = acc + 4 * s;
+          mma_bf16(c[0], hi[0], hi[1], hi[2], hi[3], v.x, v.y);
+          mma_bf16(c[1], hi[0], hi[1], hi[2], hi[3], v.z, v.w);
+          mma_bf16(c[2], hi[0], hi[1], hi[2], hi[3], w.x, w.y);
+          mma_bf16(c[3], hi[0], hi[1], hi[2], hi[3], w.z, w.w);
+          mma_bf16(c[0], lo[0], lo[1], lo[2], lo[3], v.x, v.y);
+          mma_bf16(c[1], lo[0], lo[1], lo[2], lo[3], v.z, v.w);
+          mma_bf16(c[2], lo[0], lo[1], lo[2], lo[3], w.x, w.y);
+          mma_bf16(c[3], lo[0], lo[1], lo[2], lo[3], w.z, w.w);
+        }
+      };
+      next();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint4 v = lds16(st + i * 1024 + s * 512);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            acc[4 * s + j][2 * i] = lo_f(w[j]);
+            acc[4 * s + j][2 * i + 1] = hi_f(w[j]);
+          }
+        }
+      if constexpr (MANY) {
+        copy();
+        const bool last = m + 1 == ms, more = last && gi + STEP < gb;
+        for (int k = 0; k < ks; k += 2) {
+          // the registers take the next steps as soon as they have been used, and keep what the next rows need
+          const bool tail = k + 2 >= ks;
+          const bool fill = !tail || more || (!last && ks > 2);
+          const int ng = tail && more ? gi + STEP : gi, nk = tail ? 0 : k + 2;
+          multiply(k, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
+          if (fill) load_b(bv[0], ng, nk);
+          if (k + 1 < ks) multiply(k + 1, bv[1][0], bv[1][1], bv[1][2], bv[1][3]);
+          if (fill && ks > 1) load_b(bv[1], ng, nk + 1);
+        }
+      } else {
+        for (int k = 0;;) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (k + u < ks) {
+              const uint32_t at = st + 2048 + u * 2048;
+              multiply(k + u, lds16(at), lds16(at + 512), lds16(at + 1024), lds16(at + 1536));
+            }
+          copy();
+          k += 2;
+          if (k >= ks) break;
+          next();
+        }
       }
-    };
-    next();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const uint4 v = lds16(st + i * 1024 + s * 512);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      for (int i = 0; i < 2; ++i) {
+        const int e = 2 * i, t = tok[m * 16 + i * 8 + g];
+        uint32_t o0[4], o1[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          acc[4 * s + j][2 * i] = lo_f(w[j]);
-          acc[4 * s + j][2 * i + 1] = hi_f(w[j]);
-        }
-      }
-    if constexpr (MANY) {
-      copy();
-      for (int k = 0; k < ks; ++k) {
-        uint4 bn[4];
-        const bool more = k + 1 < ks;
-        load_b(bn, more || gi + 1 >= gb ? gi : gi + 1, more ? k + 1 : 0);
-        multiply(k, bv[0], bv[1], bv[2], bv[3]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bv[i] = bn[i];
-      }
-    } else {
-      for (int k = 0;;) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (k + u < ks) {
-            const uint32_t at = st + 2048 + u * 2048;
-            multiply(k + u, lds16(at), lds16(at + 512), lds16(at + 1024), lds16(at + 1536));
+          if constexpr (GATED) {
+            o0[j] = pack_bf16x2(gated_act(ACT, acc[j][e], acc[4 + j][e], p.act_alpha, p.act_limit),
+                                gated_act(ACT, acc[j][e + 1], acc[4 + j][e + 1], p.act_alpha, p.act_limit));
+          } else {
+            o0[j] = pack_bf16x2(acc[j][e], acc[j][e + 1]);
+            o1[j] = pack_bf16x2(acc[4 + j][e], acc[4 + j][e + 1]);
           }
-        copy();
-        k += 2;
-        if (k >= ks) break;
-        next();
-      }
-    }
-    const int c0 = gi * GW, left = N - c0 - t4 * 8;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int e = 2 * i;
-      uint32_t o0[4], o1[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (GATED) {
-          o0[j] = pack_bf16x2(gated_act(ACT, acc[j][e], acc[4 + j][e], p.act_alpha, p.act_limit),
-                              gated_act(ACT, acc[j][e + 1], acc[4 + j][e + 1], p.act_alpha, p.act_limit));
-        } else {
-          o0[j] = pack_bf16x2(acc[j][e], acc[j][e + 1]);
-          o1[j] = pack_bf16x2(acc[4 + j][e], acc[4 + j][e + 1]);
         }
+        __nv_bfloat16* row = out + t * p.out_stride + gi * GW;
+        if (t >= 0 && left > 0) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+        if (!GATED && t >= 0 && left > 32) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
       }
-      __nv_bfloat16* row = (i ? out1 : out0) + c0;
-      const bool ok = (i ? tok1 : tok0) >= 0;
-      if (ok && left > 0) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
-      if (!GATED && ok && left > 32) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
     }
   }
 }
@@ -659,7 +669,7 @@ static int launch_lora(const LoraParams& p, unsigned tiles, unsigned chunks, uns
       return -3;
     once.mark(dev);
   }
-  const size_t smem = 4 * (MANY ? 3 * 2048 : 4 * 6144) + 2 * sizeof(__nv_bfloat16) * (MANY ? 64 : 16) * p.h_pitch;
+  const size_t smem = 4 * 4 * (MANY ? 2048 : 6144) + 2 * sizeof(__nv_bfloat16) * (MANY ? 64 : 16) * p.h_pitch;
   const dim3 grid(p.parts, chunks, tiles * p.subs);
   if (smem > kExpandSmem || grid.z > 65535) return -2;
   if (launch_pdl(shrink, grid, dim3(MANY ? kManyThreads : kFewThreads), MANY ? kShrinkManySmem : kShrinkFewSmem, stream, 1, p) !=
@@ -746,7 +756,7 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
     if (p.n[s] & 7) return -1;
     if (!gated || s == 0) groups += gated ? (p.n[s] + 31) / 32 : (p.n[s] + 63) / 64;
   }
-  const int team = many ? 1 : 4;
+  const int team = 4;
   const long long want = static_cast<long long>(groups) * max_tiles * p.subs / (148 * 8);
   p.per = static_cast<int>(std::max(1LL, (want + team - 1) / team)) * team;
   unsigned blocks = 0;
