@@ -109,10 +109,10 @@ int b200_cache_copy(const void* tensors, int num_tensors, const int* pairs, int 
                     cudaStream_t stream);
 int b200_lora_plan(const int* slots, int T, int L, int rows, int* order, int* tiles, int* num_tiles, int* status,
                    cudaStream_t stream);
-int b200_lora_parts(int K, int rows, int max_tiles, int num_slots);
+long long b200_lora_scratch_bytes(int T, int K, int rows, int max_tiles, int num_slots, int slices, int max_rank);
 int b200_lora(const void* x, long long x_stride, const void* y, long long y_stride, void* out, long long out_stride,
               const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks, const float* scales,
-              const int* order, const int* tiles, const int* num_tiles, int max_tiles, int rows, float* h, int T,
+              const int* order, const int* tiles, const int* num_tiles, int max_tiles, int rows, void* h, int T,
               int num_slots, int K, int slices, const int* n, int max_rank, int act, float act_alpha, float act_limit, cudaStream_t stream);
 size_t b200_mla_decode_scratch_bytes(int total_tokens, int N, int splits);
 int b200_mla_decode(const void* q, const void* cache, void* out, float* lse, const int* block_tables,
@@ -813,10 +813,12 @@ void lora(const Tensor& x, const Tensor& y, const Tensor& out, const Tensor& a, 
               "lora: out is y itself or shares no memory with it");
   TORCH_CHECK(T < 2 || out.stride(0) >= out.size(1), "lora: rows of out overlap");
   c10::cuda::CUDAGuard guard(x.device());
-  const Tensor h = torch::empty({b200_lora_parts((int)x.size(1), (int)rows, (int)max_tiles, (int)L), T, S * max_rank}, scales.options());
+  const Tensor h = torch::empty(
+      {b200_lora_scratch_bytes((int)T, (int)x.size(1), (int)rows, (int)max_tiles, (int)L, (int)S, (int)max_rank)},
+      x.options().dtype(at::kByte));
   check(b200_lora(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(), out.stride(0), a.data_ptr(), a.size(1),
                   b.data_ptr(), b.size(1), ranks.data_ptr<int>(), scales.data_ptr<float>(), order.data_ptr<int>(),
-                  tiles.data_ptr<int>(), num_tiles.data_ptr<int>(), (int)max_tiles, (int)rows, h.data_ptr<float>(), (int)T,
+                  tiles.data_ptr<int>(), num_tiles.data_ptr<int>(), (int)max_tiles, (int)rows, h.data_ptr(), (int)T,
                   (int)L, (int)x.size(1), (int)S, n,
                   (int)max_rank, (int)act, (float)act_alpha, (float)act_limit, cur_stream()),
         "lora");

@@ -17,10 +17,10 @@
 //
 // Tokens are grouped by adapter once a step (lora_plan_kernel: a stable counting sort, then tiles of up to `rows` tokens of one
 // adapter).  Two launches apply the adapters, both bound by what they read and write:
-//   lora_shrink_kernel  parts of h in fp32: a CTA per (tile, 64 of the joined ranks, part of K)
-//   lora_expand_kernel  h as the sum of its parts, then z: a CTA per (tile, 256 columns of y)
+//   lora_shrink_*_kernel  h: a cluster per (tile, 64 of the joined ranks), its CTAs sharing K
+//   lora_expand_kernel    z: a CTA per (tile, run of column groups)
 // so that many small pieces of work even out adapters of unlike ranks.  The second is launched while the first runs and
-// has y and its first factors in registers by the time h is there.
+// has its first y and factors at hand by the time h is there.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -30,6 +30,7 @@
 
 #include "../common/device_once.h"
 #include "../common/pdl.cuh"
+#include "../common/ptx.cuh"
 #include "../common/ptx.cuh"
 #include "../gemm/gated_act.cuh"
 
@@ -139,8 +140,10 @@ struct LoraParams {
   const int* order;
   const LoraTile* tiles;
   const int* num_tiles;
-  float* h;                                      // [parts][T][h_width], rows in the order of the plan
-  long long h_part;                              // T * h_width
+  // h, rows in the order of the plan: few rows fp32 [parts][T][h_width], to be summed; many rows bf16 [2][T][h_width], h times the
+  // scale rounded and what that leaves
+  void* h;
+  long long h_plane;                             // T * h_width
   int h_width;                                   // slices * largest rank
   int K, slices, parts;
   int subs;                                      // pieces of a plan's tile, each with CTAs of its own
@@ -181,6 +184,21 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
+}
+
+// Four of h times the scale as the sum of two bf16 (17 bits of the fp32 values), so that the product with B adds no rounding
+// beside that of its result.
+__device__ __forceinline__ void split_h(const float4& s, float scale, uint2& hi, uint2& lo) {
+  const float f[4] = {s.x * scale, s.y * scale, s.z * scale, s.w * scale};
+  float up[4], rest[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    up[e] = __bfloat162float(__float2bfloat16(f[e]));
+    rest[e] = f[e] - up[e];
+    if (!(rest[e] - rest[e] == 0.f)) rest[e] = 0.f;                    // beside an infinity
+  }
+  hi = make_uint2(pack_bf16x2(up[0], up[1]), pack_bf16x2(up[2], up[3]));
+  lo = make_uint2(pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3]));
 }
 
 // ---- h of few rows: 16 at most, K dealt to the parts and, in steps of 32, to the warps.  The factors are what is read: every
@@ -269,7 +287,7 @@ __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const Lora
   else shrink_rows<8>(p, tl, n0, sum_r, s_lo, s_hi, ring, d);
   __syncthreads();
   // the warps' parts in order, four columns a thread
-  float* h = p.h + blockIdx.x * p.h_part + static_cast<long long>(tl.start) * p.h_width + n0;
+  float* h = static_cast<float*>(p.h) + blockIdx.x * p.h_plane + static_cast<long long>(tl.start) * p.h_width + n0;
   for (int i = threadIdx.x; i < tl.count * nt * 2; i += kFewThreads) {
     const int row = i / (nt * 2), col = i % (nt * 2) * 4;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -379,6 +397,7 @@ __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   float* mine = reinterpret_cast<float*>(smem) + (warp & 3) * 32 * 36;
+  float* part = reinterpret_cast<float*>(smem) + 4 * 32 * 36;
   if (kw == 1 && live) {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -390,20 +409,40 @@ __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const
   }
   __syncthreads();
   if (kw == 0 && live) {
-    float* h = p.h + blockIdx.x * p.h_part + static_cast<long long>(tl.start) * p.h_width + n0;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = m * 16 + g + e * 8, col = j0 + j * 8 + t4 * 2;
-          const float2 o = *reinterpret_cast<const float2*>(mine + r * 36 + j * 8 + t4 * 2);
-          if (m0 + r < tl.count && col < width)
-            *reinterpret_cast<float2*>(h + static_cast<long long>(m0 + r) * p.h_width + col) =
-                make_float2(acc[m][j][2 * e] + o.x, acc[m][j][2 * e + 1] + o.y);
+          const int r = m * 16 + g + e * 8, col = j * 8 + t4 * 2;
+          const float2 o = *reinterpret_cast<const float2*>(mine + r * 36 + col);
+          *reinterpret_cast<float2*>(part + (m0 + r) * W + j0 + col) =
+              make_float2(acc[m][j][2 * e] + o.x, acc[m][j][2 * e + 1] + o.y);
         }
   }
+  // The cluster's CTAs have summed a part of K each.  Every one adds up its share of the elements in the order of the parts and
+  // leaves them ready for the second kernel, whose many CTAs then need no more than copy them.
+  cluster_arrive_release();
+  cluster_wait_acquire();
+  const int C = p.parts, rank = blockIdx.x, vecs = width / 4;
+  const float scale = p.scales[tl.slot];
+  __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p.h) + static_cast<long long>(tl.start) * p.h_width + n0;
+  for (int i = rank * kManyThreads + threadIdx.x; i < tl.count * vecs; i += C * kManyThreads) {
+    const int row = i / vecs, v = i % vecs * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < C; ++c) {
+      const float4 q = ld_shared_cluster_f4(mapa_shared(smem_u32(part + row * W + v), c));
+      sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
+    }
+    uint2 hi, lo;
+    split_h(sum, scale, hi, lo);
+    __nv_bfloat16* dst = h + static_cast<long long>(row) * p.h_width + v;
+    *reinterpret_cast<uint2*>(dst) = hi;
+    *reinterpret_cast<uint2*>(dst + p.h_plane) = lo;
+  }
+  cluster_arrive_release();                                            // no CTA leaves while its part is read
+  cluster_wait_acquire();
 }
 
 // ---- z: a CTA has a tile's rows and a run of column groups of one slice, 64 columns of y each (gated: 32 of gate and their 32 of
@@ -411,10 +450,16 @@ __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const
 // accumulators; a lane's results are eight neighbouring columns twice, so y and the result move 16 bytes a lane, 512 of a row
 // by the four warps.  Many rows: B is read into registers once for the 64 rows (up to 32 ranks; above, two steps of 16
 // follow one another).  Few rows: B comes through the ring as well, 32 ranks a stage.
+#ifndef LORA_OCC
+#define LORA_OCC 4
+#endif
+#ifndef LORA_WAVES
+#define LORA_WAVES 4
+#endif
 static constexpr int kExpandThreads = 128;
 
 template <bool MANY, int ACT>
-__global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const LoraParams p) {
+__global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(const LoraParams p) {
   constexpr bool GATED = ACT != kActNone;
   constexpr int BM = MANY ? 64 : 16, STEP = 4, D = 4, STAGE = MANY ? 2048 : 2048 + 4096;
   constexpr int GW = GATED ? 32 : 64;                                  // columns of a slice in a group
@@ -456,7 +501,7 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
   const __nv_bfloat16* b_up = b + (GATED ? static_cast<long long>(b_last + 1) * r0 * 32 : 0);
   const int ga = block * p.per + warp, gb = min((N + GW - 1) / GW, (block + 1) * p.per);
   const int ms = (tl.count + 15) / 16;
-  const float scale = tl.slot >= 0 ? p.scales[tl.slot] : 0.f;
+  const float scale = !MANY && tl.slot >= 0 ? p.scales[tl.slot] : 0.f;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * D * STAGE + lane * 16;
   const __nv_bfloat16* y = p.y + first + (GATED ? 2 : 1) * t4 * 8;
   __nv_bfloat16* out = p.out + first + t4 * 8;
@@ -526,39 +571,39 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
   pdl_wait();
   pdl_trigger();
 
-  // h: the parts in order, times the scale, as the sum of two bf16 (17 bits of the fp32 value), so that the product below adds
-  // no rounding beside that of its result
-  __nv_bfloat16* h_hi = reinterpret_cast<__nv_bfloat16*>(smem + 4 * D * STAGE);                 // [BM][h_pitch]
-  __nv_bfloat16* h_lo = h_hi + BM * p.h_pitch;
+  // h of this slice (gated: of both) into shared memory, [2][BM][h_pitch]
+  const uint32_t h_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + 4 * D * STAGE;
   const int sum_r = GATED ? r0 + r1 : r0;
-  if (sum_r > 0) {
-    const float* h = p.h + static_cast<long long>(tl.start) * p.h_width + h0;
+  if constexpr (MANY) {
+    const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(p.h) + static_cast<long long>(tl.start) * p.h_width + h0;
+    const int pieces = sum_r / 8;
+    for (int i = threadIdx.x; i < 2 * tl.count * pieces; i += kExpandThreads) {
+      const int piece = i % pieces, row = i / pieces >> 1, rest = i / pieces & 1;
+      cp16(h_at + ((rest * BM + row) * p.h_pitch + piece * 8) * 2,
+           h + rest * p.h_plane + static_cast<long long>(row) * p.h_width + piece * 8, true);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    const float* h = static_cast<const float*>(p.h) + static_cast<long long>(tl.start) * p.h_width + h0;
+    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(smem + 4 * D * STAGE);
     const int vecs = sum_r / 4;
-    for (int i = threadIdx.x; i < ms * 16 * vecs; i += kExpandThreads) {
+    for (int i = threadIdx.x; i < tl.count * vecs; i += kExpandThreads) {
       const int row = i / vecs, v = i % vecs * 4;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < tl.count) {
-        const float* src = h + static_cast<long long>(row) * p.h_width + v;
+      const float* src = h + static_cast<long long>(row) * p.h_width + v;
 #pragma unroll 4
-        for (int c = 0; c < p.parts; ++c) {
-          const float4 q = *reinterpret_cast<const float4*>(src + c * p.h_part);
-          sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
-        }
+      for (int c = 0; c < p.parts; ++c) {
+        const float4 q = *reinterpret_cast<const float4*>(src + c * p.h_plane);
+        sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
       }
-      const float f[4] = {sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale};
-      float up[4], rest[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        up[e] = __bfloat162float(__float2bfloat16(f[e]));
-        rest[e] = f[e] - up[e];
-        if (!(rest[e] - rest[e] == 0.f)) rest[e] = 0.f;                // beside an infinity
-      }
-      *reinterpret_cast<uint2*>(h_hi + row * p.h_pitch + v) = make_uint2(pack_bf16x2(up[0], up[1]), pack_bf16x2(up[2], up[3]));
-      *reinterpret_cast<uint2*>(h_lo + row * p.h_pitch + v) = make_uint2(pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3]));
+      uint2 hi, lo;
+      split_h(sum, scale, hi, lo);
+      *reinterpret_cast<uint2*>(dst + row * p.h_pitch + v) = hi;
+      *reinterpret_cast<uint2*>(dst + (BM + row) * p.h_pitch + v) = lo;
     }
   }
   __syncthreads();
-  const uint32_t hf = static_cast<uint32_t>(__cvta_generic_to_shared(h_hi)) + ((lane & 15) * p.h_pitch + (lane >> 4) * 8) * 2;
+  const uint32_t hf = h_at + ((lane & 15) * p.h_pitch + (lane >> 4) * 8) * 2;
   const uint32_t lo_at = 2 * BM * p.h_pitch, m_step = 32 * p.h_pitch;
   int get = 0;
   for (int gi = ga; gi < gb; gi += STEP) {
@@ -607,16 +652,27 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
         }
       if constexpr (MANY) {
         copy();
-        const bool last = m + 1 == ms, more = last && gi + STEP < gb;
-        for (int k = 0; k < ks; k += 2) {
-          // the registers take the next steps as soon as they have been used, and keep what the next rows need
-          const bool tail = k + 2 >= ks;
-          const bool fill = !tail || more || (!last && ks > 2);
-          const int ng = tail && more ? gi + STEP : gi, nk = tail ? 0 : k + 2;
-          multiply(k, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
-          if (fill) load_b(bv[0], ng, nk);
-          if (k + 1 < ks) multiply(k + 1, bv[1][0], bv[1][1], bv[1][2], bv[1][3]);
-          if (fill && ks > 1) load_b(bv[1], ng, nk + 1);
+        const bool more = m + 1 == ms && gi + STEP < gb;
+        if (ks == 1) {
+          multiply(0, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
+          if (more) load_b(bv[0], gi + STEP, 0);
+        } else if (ks == 2) {
+          multiply(0, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
+          multiply(1, bv[1][0], bv[1][1], bv[1][2], bv[1][3]);
+          if (more) {
+            load_b(bv[0], gi + STEP, 0);
+            load_b(bv[1], gi + STEP, 1);
+          }
+        } else {
+          for (int k = 0; k < ks; k += 2) {
+            // the registers take the steps after these as soon as they have been used
+            const bool tail = k + 2 >= ks;
+            const int ng = tail && more ? gi + STEP : gi, nk = tail ? 0 : k + 2;
+            multiply(k, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
+            load_b(bv[0], ng, nk);
+            if (k + 1 < ks) multiply(k + 1, bv[1][0], bv[1][1], bv[1][2], bv[1][3]);
+            load_b(bv[1], ng, nk + 1);
+          }
         }
       } else {
         for (int k = 0;;) {
@@ -672,7 +728,7 @@ static int launch_lora(const LoraParams& p, unsigned tiles, unsigned chunks, uns
   const size_t smem = 4 * 4 * (MANY ? 2048 : 6144) + 2 * sizeof(__nv_bfloat16) * (MANY ? 64 : 16) * p.h_pitch;
   const dim3 grid(p.parts, chunks, tiles * p.subs);
   if (smem > kExpandSmem || grid.z > 65535) return -2;
-  if (launch_pdl(shrink, grid, dim3(MANY ? kManyThreads : kFewThreads), MANY ? kShrinkManySmem : kShrinkFewSmem, stream, 1, p) !=
+  if (launch_pdl(shrink, grid, dim3(MANY ? kManyThreads : kFewThreads), MANY ? kShrinkManySmem : kShrinkFewSmem, stream, MANY ? p.parts : 1, p) !=
       cudaSuccess)
     return -3;
   return launch_pdl(expand, dim3(blocks, grid.z), dim3(kExpandThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
@@ -685,11 +741,16 @@ static int launch_lora(const LoraParams& p, bool many, unsigned tiles, unsigned 
 
 }  // namespace b200
 
-// Parts of K that a step's h is summed from.  Few rows (tiles of 16): as many as the slots let be resident, whatever the number of
+// Parts of K that a step's h is summed from, a CTA each (many rows: of a cluster).  Few rows (tiles of 16): as many as the slots let be resident, whatever the number of
 // tokens, so that a row does not depend on it; many rows: as many as fill the SMs.
-extern "C" int b200_lora_parts(int K, int rows, int max_tiles, int num_slots) {
+static int lora_parts(int K, int rows, int max_tiles, int num_slots) {
   const int want = rows < 64 ? std::min((K + 511) / 512, 592 / num_slots) : std::min((K + 255) / 256, 296 / max_tiles);
-  return std::min(std::max(want, 1), 16);
+  return std::min(std::max(want, 1), rows < 64 ? 16 : 8);
+}
+
+// Bytes of scratch for a step's h.
+extern "C" long long b200_lora_scratch_bytes(int T, int K, int rows, int max_tiles, int num_slots, int slices, int max_rank) {
+  return 4LL * T * slices * max_rank * (rows < 64 ? lora_parts(K, rows, max_tiles, num_slots) : 1);
 }
 
 // Groups tokens by adapter.  tiles: at least T / rows + min(T, L + 1) of four ints.
@@ -710,13 +771,13 @@ extern "C" int b200_lora_plan(const int* slots, int T, int L, int rows, int* ord
                     reinterpret_cast<LoraTile*>(tiles), num_tiles, status) == cudaSuccess ? 0 : -3;
 }
 
-// n: columns of each slice.  h: fp32 [b200_lora_parts][T][slices * max_rank].  max_tiles: tiles that the plan may have, of `rows`
+// n: columns of each slice.  h: scratch of b200_lora_scratch_bytes.  max_tiles: tiles that the plan may have, of `rows`
 // tokens each.  max_rank: bound of the ranks.  act: 0 adds, a gated kind of gemm/gated_act.cuh joins gate and up (alternating
 // groups of eight columns of y).
 extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long long y_stride, void* out, long long out_stride,
                          const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks,
                          const float* scales, const int* order, const int* tiles, const int* num_tiles, int max_tiles, int rows,
-                         float* h, int T, int num_slots, int K, int slices, const int* n, int max_rank, int act,
+                         void* h, int T, int num_slots, int K, int slices, const int* n, int max_rank, int act,
                          float act_alpha, float act_limit, cudaStream_t stream) {
   using namespace b200;
   if (slices < 1 || slices > kLoraMaxSlices || (K & 7) || max_rank < 16 || (max_rank & 15) || max_tiles < 1 || (rows & 15)) return -1;
@@ -739,14 +800,14 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   p.num_tiles = num_tiles;
   p.h = h;
   p.h_width = slices * max_rank;
-  p.h_part = static_cast<long long>(T) * p.h_width;
+  p.h_plane = static_cast<long long>(T) * p.h_width;
   p.K = K;
   p.slices = slices;
   const bool many = rows >= 64, gated = act != kActNone;
   p.act_alpha = act_alpha;
   p.act_limit = act_limit;
   p.subs = many ? rows / 64 : rows / 16;
-  p.parts = b200_lora_parts(K, rows, max_tiles, num_slots);
+  p.parts = lora_parts(K, rows, max_tiles, num_slots);
   p.h_pitch = (gated ? 2 : 1) * max_rank + 8;    // eight rows of 16 bytes are in banks of their own
   const unsigned chunks = (p.h_width + kLoraChunk * 8 - 1) / (kLoraChunk * 8), tiles_n = static_cast<unsigned>(max_tiles);
   // column groups of a CTA: a few rounds of the resident CTAs in all, a group a team at least
@@ -757,7 +818,7 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
     if (!gated || s == 0) groups += gated ? (p.n[s] + 31) / 32 : (p.n[s] + 63) / 64;
   }
   const int team = 4;
-  const long long want = static_cast<long long>(groups) * max_tiles * p.subs / (148 * 8);
+  const long long want = static_cast<long long>(groups) * max_tiles * p.subs / (148 * 4 * LORA_WAVES);
   p.per = static_cast<int>(std::max(1LL, (want + team - 1) / team)) * team;
   unsigned blocks = 0;
   for (int s = 0; s < slices; ++s)
