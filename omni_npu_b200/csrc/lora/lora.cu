@@ -172,8 +172,11 @@ __device__ __forceinline__ bool lora_tile(const LoraParams& p, int item, int sub
   return tl.count > 0;
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   uint4 v;
@@ -223,11 +226,11 @@ __device__ __forceinline__ void shrink_rows(const LoraParams& p, const LoraTile&
       const uint32_t st = ring + put * STAGE;
       put = put + 1 == D ? 0 : put + 1;
 #pragma unroll
-      for (int u = 0; u < NT; ++u) cp16(st + u * 512, a + s * a_step + u * 256, true);
+      for (int u = 0; u < NT; ++u) cp16(st + u * 512, a + s * a_step + u * 256);
       const bool in = s * 32 + t4 * 8 < p.K;                           // K is a multiple of 8
       const int k = in ? s * 32 : 0;
-      if (ok0) cp16(st + NT * 512, x0 + k, in);
-      if (ok1) cp16(st + NT * 512 + 512, x1 + k, in);
+      if (ok0) cp16_or_zero(st + NT * 512, x0 + k, in);
+      if (ok1) cp16_or_zero(st + NT * 512 + 512, x1 + k, in);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -323,37 +326,47 @@ __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
 
   // copies: sixteen lanes a row of 256 bytes, its 16-byte pieces at piece ^ 4 (row % 2), so that the eight lanes that read two
-  // rows at once find 128 bytes in different banks; A as it lies
+  // rows at once find 128 bytes in different banks; A as it lies.  (Rows behind the tile's last are copies of its first.)
   const int crow = threadIdx.x >> 4, piece = threadIdx.x & 15;
   const __nv_bfloat16* xs[4];
-  bool xok[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = crow + 16 * i;
-    xok[i] = row < tl.count;
-    xs[i] = p.x + (xok[i] ? p.order[tl.start + row] : 0) * p.x_stride + piece * 8;
+    xs[i] = p.x + p.order[tl.start + (row < tl.count ? row : 0)] * p.x_stride + s_lo * kSlab + piece * 8;
   }
-  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + (n0 / 16) * 512 + threadIdx.x * 8;
   const long long a_step = sum_r * 32;
+  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + (n0 / 16) * 512 + threadIdx.x * 8 + s_lo * 4 * a_step;
   const bool aok = threadIdx.x < width * 4;
-  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  const uint32_t base = smem_u32(smem);
   const uint32_t xdst = base + crow * 256 + ((piece ^ (crow & 1) << 2) << 4), adst = base + 16384 + threadIdx.x * 16;
-  auto copy = [&](int s) {
-    if (s < s_hi) {
-      const uint32_t st = (s - s_lo) % kStages * kStageBytes;
-      const bool in = s * kSlab + piece * 8 < p.K;                     // K is a multiple of 8
-      const int k = in ? s * kSlab : -piece * 8;                       // (nothing is read there)
+  uint32_t put = 0;
+  int next = s_lo;                                                     // slab that is copied next
+  auto copy = [&]() {
+    if (next < s_hi) {
+      if (next * kSlab + kSlab <= p.K) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) cp16(xdst + st + i * 4096, xs[i] + k, in && xok[i]);
+        for (int i = 0; i < 4; ++i) cp16(xdst + put + i * 4096, xs[i]);
+        if (aok) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool kb = s * 4 + i < blocks;
-        if (aok) cp16(adst + st + i * 4096, a + (kb ? s * 4 + i : 0) * a_step, kb);
+          for (int i = 0; i < 4; ++i) cp16(adst + put + i * 4096, a + i * a_step);
+        }
+      } else {                                                         // the end of K, a multiple of 8
+        const bool in = next * kSlab + piece * 8 < p.K;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cp16_or_zero(xdst + put + i * 4096, in ? xs[i] : p.x, in);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (aok) cp16_or_zero(adst + put + i * 4096, next * 4 + i < blocks ? a + i * a_step : p.a, next * 4 + i < blocks);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xs[i] += kSlab;
+      a += 4 * a_step;
+      put = put + kStageBytes == kStages * kStageBytes ? 0 : put + kStageBytes;
+      ++next;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  for (int i = 0; i < kStages - 1; ++i) copy(s_lo + i);
+  for (int i = 0; i < kStages - 1; ++i) copy();
 
   const int kw = warp >> 2, m0 = (warp & 1) * 32, j0 = (warp >> 1 & 1) * 32;
   const bool live = j0 < width && m0 < tl.count;
@@ -364,34 +377,37 @@ __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
-  const uint32_t xf = base + (m0 + g) * 256, af = base + 16384 + (j0 / 16) * 1024 + lane * 16;
+  // (32 of K at 4 pieces; the exchange of pieces swaps neighbouring 32 in odd rows)
+  const uint32_t xf = base + (m0 + g) * 256 + kw * 128 + t4 * 16, x_swap = (g & 1) * 64;
+  const uint32_t af = base + 16384 + kw * 8192 + (j0 / 16) * 1024 + lane * 16;
+  uint32_t get = 0;
   for (int s = s_lo; s < s_hi; ++s) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncthreads();
-    copy(s + kStages - 1);
-    if (!live) continue;
-    const uint32_t st = (s - s_lo) % kStages * kStageBytes;
+    copy();
+    if (live) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int kb = kw * 2 + q;
-      uint4 xv[4], av[2][2];
+      for (int q = 0; q < 2; ++q) {
+        uint4 xv[4], av[2][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) xv[i] = lds16(xf + st + i * 2048 + ((kb * 4 + t4) ^ (g & 1) << 2) * 16);
+        for (int i = 0; i < 4; ++i) xv[i] = lds16(xf + get + (q * 64 ^ x_swap) + i * 2048);
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) av[j][u] = lds16(af + st + kb * 4096 + j * 1024 + u * 512);
+          for (int u = 0; u < 2; ++u) av[j][u] = lds16(af + get + q * 4096 + j * 1024 + u * 512);
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint4 &v = xv[2 * m], &w = xv[2 * m + 1];
-          mma_bf16(acc[m][2 * j], v.x, w.x, v.y, w.y, av[j][0].x, av[j][0].y);
-          mma_bf16(acc[m][2 * j + 1], v.x, w.x, v.y, w.y, av[j][0].z, av[j][0].w);
-          mma_bf16(acc[m][2 * j], v.z, w.z, v.w, w.w, av[j][1].x, av[j][1].y);
-          mma_bf16(acc[m][2 * j + 1], v.z, w.z, v.w, w.w, av[j][1].z, av[j][1].w);
-        }
+          for (int j = 0; j < 2; ++j) {
+            const uint4 &v = xv[2 * m], &w = xv[2 * m + 1];
+            mma_bf16(acc[m][2 * j], v.x, w.x, v.y, w.y, av[j][0].x, av[j][0].y);
+            mma_bf16(acc[m][2 * j + 1], v.x, w.x, v.y, w.y, av[j][0].z, av[j][0].w);
+            mma_bf16(acc[m][2 * j], v.z, w.z, v.w, w.w, av[j][1].x, av[j][1].y);
+            mma_bf16(acc[m][2 * j + 1], v.z, w.z, v.w, w.w, av[j][1].z, av[j][1].w);
+          }
+      }
     }
+    get = get + kStageBytes == kStages * kStageBytes ? 0 : get + kStageBytes;
   }
   // the two halves of K in order
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -450,21 +466,15 @@ __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const
 // accumulators; a lane's results are eight neighbouring columns twice, so y and the result move 16 bytes a lane, 512 of a row
 // by the four warps.  Many rows: B is read into registers once for the 64 rows (up to 32 ranks; above, two steps of 16
 // follow one another).  Few rows: B comes through the ring as well, 32 ranks a stage.
-#ifndef LORA_OCC
-#define LORA_OCC 4
-#endif
-#ifndef LORA_WAVES
-#define LORA_WAVES 4
-#endif
 static constexpr int kExpandThreads = 128;
 
 template <bool MANY, int ACT>
-__global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(const LoraParams p) {
+__global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const LoraParams p) {
   constexpr bool GATED = ACT != kActNone;
   constexpr int BM = MANY ? 64 : 16, STEP = 4, D = 4, STAGE = MANY ? 2048 : 2048 + 4096;
   constexpr int GW = GATED ? 32 : 64;                                  // columns of a slice in a group
   extern __shared__ __align__(128) char smem[];
-  __shared__ int tok[BM];
+  __shared__ long long y_row[BM], out_row[BM];                         // where a row of the tile starts; out_row -1: none
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const bool in_place = !GATED && p.out == p.y;
   // Everything but h is older than the first kernel, which has started only behind it: no wait yet.
@@ -473,7 +483,12 @@ __global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(c
     pdl_wait();
     return;
   }
-  if (threadIdx.x < BM) tok[threadIdx.x] = threadIdx.x < tl.count ? p.order[tl.start + threadIdx.x] : -1;
+  if (threadIdx.x < BM) {
+    const bool ok = threadIdx.x < tl.count;
+    const int t = p.order[tl.start + (ok ? threadIdx.x : 0)];          // (rows behind the last read what the first does)
+    y_row[threadIdx.x] = t * p.y_stride;
+    out_row[threadIdx.x] = ok ? t * p.out_stride : -1;
+  }
   // this CTA's slice and groups in it; of the slice: first rank in h, first column of y, factors (in blocks of 32 columns)
   int slice = 0, block = blockIdx.x, h0 = 0, first = 0, r0 = 0, r1 = 0;
   const __nv_bfloat16* b = p.b + max(tl.slot, 0) * p.b_slot + lane * 8;
@@ -503,7 +518,7 @@ __global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(c
   const int ms = (tl.count + 15) / 16;
   const float scale = !MANY && tl.slot >= 0 ? p.scales[tl.slot] : 0.f;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * D * STAGE + lane * 16;
-  const __nv_bfloat16* y = p.y + first + (GATED ? 2 : 1) * t4 * 8;
+  const __nv_bfloat16* y = p.y + first;
   __nv_bfloat16* out = p.out + first + t4 * 8;
   // 16 ranks (step k) of 32 columns of group gi: its half s, or gate / up.  Past the end: any others, whose results are not used
   auto b_at = [&](int gi, int s, int k) {
@@ -511,22 +526,23 @@ __global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(c
     return b + (static_cast<long long>(min(2 * gi + s, b_last)) * k0 + min(k, k0 - 1)) * 512;
   };
   __syncthreads();
-  // the ring's next stage: group cg and its rows cm (few rows: steps ck, ck + 1)
-  int cg = ga, cm = 0, ck = 0, put = 0;
+  // the ring's next stage: group cg and its rows cm (few rows: steps ck, ck + 1).  Columns behind the slice's last eight are read
+  // there; their results are not stored.
+  int cg = ga, cm = 0, ck = 0;
+  uint32_t put = ring;
   auto copy = [&]() {
     if (cg < gb) {
-      const uint32_t st = ring + put * STAGE;
-      put = put + 1 == D ? 0 : put + 1;
+      const uint32_t st = put;
+      put = put + STAGE == ring + D * STAGE ? ring : put + STAGE;
       if (MANY || ck == 0) {
-        const int left = N - cg * GW - t4 * 8;
-        const __nv_bfloat16* src = y + (GATED ? 2 : 1) * GW * cg;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int t = tok[cm * 16 + i * 8 + g];
-          const __nv_bfloat16* row = src + t * p.y_stride;
-          if (t >= 0 && left > 0) cp16(st + i * 1024, row, true);
-          if (t >= 0 && left > (GATED ? 0 : 32)) cp16(st + i * 1024 + 512, row + (GATED ? 8 : 32), true);
-        }
+        const int col = cg * GW + t4 * 8;
+        const __nv_bfloat16* src0 = y + (GATED ? 2 : 1) * min(col, N - 8);
+        const __nv_bfloat16* src1 = GATED ? src0 + 8 : y + min(col + 32, N - 8);
+        const long long at0 = y_row[cm * 16 + g], at1 = y_row[cm * 16 + g + 8];
+        cp16(st, src0 + at0);
+        cp16(st + 512, src1 + at0);
+        cp16(st + 1024, src0 + at1);
+        cp16(st + 1536, src1 + at1);
       }
       if constexpr (MANY) {
         if (++cm == ms) {
@@ -540,8 +556,8 @@ __global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(c
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
               const __nv_bfloat16* src = b_at(cg, s, ck + k);
-              cp16(st + 2048 + k * 2048 + s * 1024, src, true);
-              cp16(st + 2048 + k * 2048 + s * 1024 + 512, src + 256, true);
+              cp16(st + 2048 + k * 2048 + s * 1024, src);
+              cp16(st + 2048 + k * 2048 + s * 1024 + 512, src + 256);
             }
           }
         ck += 2;
@@ -580,7 +596,7 @@ __global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(c
     for (int i = threadIdx.x; i < 2 * tl.count * pieces; i += kExpandThreads) {
       const int piece = i % pieces, row = i / pieces >> 1, rest = i / pieces & 1;
       cp16(h_at + ((rest * BM + row) * p.h_pitch + piece * 8) * 2,
-           h + rest * p.h_plane + static_cast<long long>(row) * p.h_width + piece * 8, true);
+           h + rest * p.h_plane + static_cast<long long>(row) * p.h_width + piece * 8);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
@@ -605,7 +621,7 @@ __global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(c
   __syncthreads();
   const uint32_t hf = h_at + ((lane & 15) * p.h_pitch + (lane >> 4) * 8) * 2;
   const uint32_t lo_at = 2 * BM * p.h_pitch, m_step = 32 * p.h_pitch;
-  int get = 0;
+  uint32_t get = ring;
   for (int gi = ga; gi < gb; gi += STEP) {
     const int left = N - gi * GW - t4 * 8;
     for (int m = 0; m < ms; ++m) {
@@ -613,8 +629,8 @@ __global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(c
       uint32_t st;
       auto next = [&]() {
         asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
-        st = ring + get * STAGE;
-        get = get + 1 == D ? 0 : get + 1;
+        st = get;
+        get = get + STAGE == ring + D * STAGE ? ring : get + STAGE;
       };
       // step k of h times its B
       auto multiply = [&](int k, const uint4& p0, const uint4& p1, const uint4& q0, const uint4& q1) {
@@ -690,7 +706,8 @@ __global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(c
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int e = 2 * i, t = tok[m * 16 + i * 8 + g];
+        const int e = 2 * i;
+        const long long at = out_row[m * 16 + i * 8 + g];
         uint32_t o0[4], o1[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -702,9 +719,9 @@ __global__ void __launch_bounds__(kExpandThreads, LORA_OCC) lora_expand_kernel(c
             o1[j] = pack_bf16x2(acc[4 + j][e], acc[4 + j][e + 1]);
           }
         }
-        __nv_bfloat16* row = out + t * p.out_stride + gi * GW;
-        if (t >= 0 && left > 0) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
-        if (!GATED && t >= 0 && left > 32) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+        __nv_bfloat16* row = out + at + gi * GW;
+        if (at >= 0 && left > 0) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+        if (!GATED && at >= 0 && left > 32) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
       }
     }
   }
@@ -743,14 +760,14 @@ static int launch_lora(const LoraParams& p, bool many, unsigned tiles, unsigned 
 
 // Parts of K that a step's h is summed from, a CTA each (many rows: of a cluster).  Few rows (tiles of 16): as many as the slots let be resident, whatever the number of
 // tokens, so that a row does not depend on it; many rows: as many as fill the SMs.
-static int lora_parts(int K, int rows, int max_tiles, int num_slots) {
-  const int want = rows < 64 ? std::min((K + 511) / 512, 592 / num_slots) : std::min((K + 255) / 256, 296 / max_tiles);
+static int lora_parts(int K, int rows, int max_tiles, int num_slots, int chunks) {
+  const int want = rows < 64 ? std::min((K + 511) / 512, 592 / num_slots) : std::min((K + 255) / 256, 296 / (max_tiles * chunks));
   return std::min(std::max(want, 1), rows < 64 ? 16 : 8);
 }
 
 // Bytes of scratch for a step's h.
 extern "C" long long b200_lora_scratch_bytes(int T, int K, int rows, int max_tiles, int num_slots, int slices, int max_rank) {
-  return 4LL * T * slices * max_rank * (rows < 64 ? lora_parts(K, rows, max_tiles, num_slots) : 1);
+  return 4LL * T * slices * max_rank * (rows < 64 ? lora_parts(K, rows, max_tiles, num_slots, 1) : 1);
 }
 
 // Groups tokens by adapter.  tiles: at least T / rows + min(T, L + 1) of four ints.
@@ -807,9 +824,9 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   p.act_alpha = act_alpha;
   p.act_limit = act_limit;
   p.subs = many ? rows / 64 : rows / 16;
-  p.parts = lora_parts(K, rows, max_tiles, num_slots);
-  p.h_pitch = (gated ? 2 : 1) * max_rank + 8;    // eight rows of 16 bytes are in banks of their own
   const unsigned chunks = (p.h_width + kLoraChunk * 8 - 1) / (kLoraChunk * 8), tiles_n = static_cast<unsigned>(max_tiles);
+  p.parts = lora_parts(K, rows, max_tiles, num_slots, chunks);
+  p.h_pitch = (gated ? 2 : 1) * max_rank + 8;    // eight rows of 16 bytes are in banks of their own
   // column groups of a CTA: a few rounds of the resident CTAs in all, a group a team at least
   int groups = 0;
   for (int s = 0; s < kLoraMaxSlices; ++s) {
@@ -818,7 +835,7 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
     if (!gated || s == 0) groups += gated ? (p.n[s] + 31) / 32 : (p.n[s] + 63) / 64;
   }
   const int team = 4;
-  const long long want = static_cast<long long>(groups) * max_tiles * p.subs / (148 * 4 * LORA_WAVES);
+  const long long want = static_cast<long long>(groups) * max_tiles * p.subs / (148 * 4 * (many ? 4 : 2));
   p.per = static_cast<int>(std::max(1LL, (want + team - 1) / team)) * team;
   unsigned blocks = 0;
   for (int s = 0; s < slices; ++s)
