@@ -111,9 +111,9 @@ int b200_lora_plan(const int* slots, int T, int L, int rows, int* order, int* ti
                    cudaStream_t stream);
 long long b200_lora_scratch_bytes(int T, int K, int rows, int max_tiles, int num_slots, int slices, int max_rank);
 int b200_lora(const void* x, long long x_stride, const void* y, long long y_stride, void* out, long long out_stride,
-              const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks, const float* scales,
-              const int* order, const int* tiles, const int* num_tiles, int max_tiles, int rows, void* h, int T,
-              int num_slots, int K, int slices, const int* n, int max_rank, int act, float act_alpha, float act_limit, cudaStream_t stream);
+              const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks, const int* order,
+              const int* tiles, const int* num_tiles, int max_tiles, int rows, void* h, int T, int num_slots, int K, int slices,
+              const int* n, int max_rank, int mean_rank, int act, float act_alpha, float act_limit, cudaStream_t stream);
 size_t b200_mla_decode_scratch_bytes(int total_tokens, int N, int splits);
 int b200_mla_decode(const void* q, const void* cache, void* out, float* lse, const int* block_tables,
                     const int* seq_lens, const int* topk_indices, int topk, int B, int q_len, int N,
@@ -748,21 +748,22 @@ int64_t cache_copy(const Tensor& desc, at::IntArrayRef pairs, int64_t blocks, in
   return (n + 2047) / 2048;
 }
 
-// Tokens grouped by adapter slot.
-void lora_plan(const Tensor& slots, int64_t num_slots, int64_t rows, const Tensor& order, const Tensor& tiles,
-               const Tensor& num_tiles, const Tensor& status) {
+// A plan is one int32 buffer: the tokens in order, from T the number of tiles, from the next multiple of four the tiles.
+int64_t lora_tiles_at(int64_t T) { return (T + 1 + 3) / 4 * 4; }
+int64_t lora_max_tiles(int64_t T, int64_t num_slots, int64_t rows) { return T / rows + std::min(T, num_slots + 1); }
+
+// Tokens grouped by adapter slot, in tiles of up to `rows`.
+Tensor lora_plan(const Tensor& slots, int64_t num_slots, int64_t rows, const Tensor& status) {
   CHECK_I32(slots);
-  CHECK_I32(order);
-  CHECK_I32(tiles);
-  CHECK_I32(num_tiles);
   CHECK_I32(status);
-  TORCH_CHECK(order.numel() >= slots.numel() &&
-                  tiles.numel() >= 4 * (slots.numel() / rows + std::min<int64_t>(slots.numel(), num_slots + 1)),
-              "lora_plan: buffers too small");
+  const int64_t T = slots.numel(), at = lora_tiles_at(T);
   c10::cuda::CUDAGuard guard(slots.device());
-  check(b200_lora_plan(slots.data_ptr<int>(), (int)slots.numel(), (int)num_slots, (int)rows, order.data_ptr<int>(),
-                       tiles.data_ptr<int>(), num_tiles.data_ptr<int>(), status.data_ptr<int>(), cur_stream()),
+  Tensor plan = torch::empty({at + 4 * lora_max_tiles(T, num_slots, rows)}, slots.options());
+  int* p = plan.data_ptr<int>();
+  check(b200_lora_plan(slots.data_ptr<int>(), (int)T, (int)num_slots, (int)rows, p, p + at, p + T, status.data_ptr<int>(),
+                       cur_stream()),
         "lora_plan");
+  return plan;
 }
 
 // Whether two tensors of bf16 rows may share an element: not when their spans are apart, nor when they are column ranges apart
@@ -779,49 +780,53 @@ bool share_memory(const Tensor& a, const Tensor& b) {
   return d < a.size(1) || d + b.size(1) > s;
 }
 
-// out = y + scale * B (A x) per adapter, or the gated activation of it.
-void lora(const Tensor& x, const Tensor& y, const Tensor& out, const Tensor& a, const Tensor& b, const Tensor& ranks,
-          const Tensor& scales, const Tensor& order, const Tensor& tiles, const Tensor& num_tiles, int64_t max_tiles,
-          int64_t rows, at::IntArrayRef slices, int64_t max_rank, int64_t act, double act_alpha, double act_limit) {
+// y + scale * B (A x) per adapter, or the gated activation of it (a new tensor unless `out` is given).  ranks: int32 [slots,
+// slices + 1], each slot's ranks and the bits of its scale.  sizes: rows of the plan's tiles, largest rank, mean of the joined
+// ranks, activation, then the columns of each slice.
+Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given, const Tensor& a, const Tensor& b,
+            const Tensor& ranks, const Tensor& plan, at::IntArrayRef sizes, double act_alpha, double act_limit) {
+  TORCH_CHECK(sizes.size() > 4 && sizes.size() <= 8, "lora: one to four slices");
+  const int64_t rows = sizes[0], max_rank = sizes[1], mean_rank = sizes[2], act = sizes[3], S = (int64_t)sizes.size() - 4;
   int n[4] = {0, 0, 0, 0};
   int64_t width = 0, padded = 0;
-  TORCH_CHECK(!slices.empty() && slices.size() <= 4, "lora: one to four slices");
-  for (size_t i = 0; i < slices.size(); ++i) {
-    width += n[i] = (int)slices[i];
-    padded += (slices[i] + 31) / 32 * 32;
+  for (int64_t i = 0; i < S; ++i) {
+    width += n[i] = (int)sizes[4 + i];
+    padded += (sizes[4 + i] + 31) / 32 * 32;
   }
-  const int64_t T = x.size(0), L = ranks.size(0), S = (int64_t)slices.size();
+  const int64_t T = x.size(0), L = ranks.size(0), K = x.dim() == 2 ? x.size(1) : 0;
+  c10::cuda::CUDAGuard guard(x.device());
+  const Tensor out = given.has_value() ? *given : torch::empty({T, act ? sizes[4] : width}, y.options());
   for (const Tensor* t : {&x, &y, &out, &a, &b}) CHECK_CUDA_BF16(*t);
   for (const Tensor* t : {&x, &y, &out})
     TORCH_CHECK(t->dim() == 2 && t->size(0) == T && t->stride(1) == 1 && (T < 2 || t->stride(0) % 8 == 0) &&
                     (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0,
                 "lora: rows of x, y and out are contiguous and start at 16-byte boundaries");
-  TORCH_CHECK(y.size(1) == width && out.size(1) == (act ? slices[0] : width), "lora: widths of y and out");
+  TORCH_CHECK(y.size(1) == width && out.size(1) == (act ? sizes[4] : width), "lora: widths of y and out");
   TORCH_CHECK(a.is_contiguous() && b.is_contiguous() && a.dim() == 2 && b.dim() == 2 && a.size(0) == L && b.size(0) == L &&
-                  a.size(1) == S * max_rank * ((x.size(1) + 31) / 32 * 32) && b.size(1) == padded * max_rank,
+                  a.size(1) == S * max_rank * ((K + 31) / 32 * 32) && b.size(1) == padded * max_rank,
               "lora: factors [slots, slices * rank * K] and [slots, columns * rank], K and columns in whole 32");
   CHECK_I32(ranks);
-  CHECK_I32(order);
-  CHECK_I32(tiles);
-  CHECK_I32(num_tiles);
-  TORCH_CHECK(ranks.dim() == 2 && ranks.size(1) == S && scales.is_cuda() && scales.scalar_type() == at::kFloat &&
-                  scales.is_contiguous() && scales.numel() == L,
-              "lora: ranks int32 [slots, slices], scales fp32 [slots]");
-  TORCH_CHECK(order.numel() >= T && tiles.numel() >= 4 * max_tiles, "lora: plan of another step");
-  TORCH_CHECK(!share_memory(out, x), "lora: out shares memory with x");
-  TORCH_CHECK(!share_memory(out, y) || (act == 0 && out.data_ptr() == y.data_ptr() && (T < 2 || out.stride(0) == y.stride(0))),
-              "lora: out is y itself or shares no memory with it");
-  TORCH_CHECK(T < 2 || out.stride(0) >= out.size(1), "lora: rows of out overlap");
-  c10::cuda::CUDAGuard guard(x.device());
+  CHECK_I32(plan);
+  const int64_t at = lora_tiles_at(T), max_tiles = lora_max_tiles(T, L, rows);
+  TORCH_CHECK(ranks.dim() == 2 && ranks.size(1) == S + 1, "lora: ranks int32 [slots, slices + 1]");
+  TORCH_CHECK(plan.numel() == at + 4 * max_tiles && max_tiles <= 65535, "lora: plan of another step, or of too many tokens");
+  if (given.has_value()) {
+    TORCH_CHECK(!share_memory(out, x), "lora: out shares memory with x");
+    TORCH_CHECK(!share_memory(out, y) || (act == 0 && out.data_ptr() == y.data_ptr() && (T < 2 || out.stride(0) == y.stride(0))),
+                "lora: out is y itself or shares no memory with it");
+    TORCH_CHECK(T < 2 || out.stride(0) >= out.size(1), "lora: rows of out overlap");
+  }
+  if (T == 0) return out;
   const Tensor h = torch::empty(
-      {b200_lora_scratch_bytes((int)T, (int)x.size(1), (int)rows, (int)max_tiles, (int)L, (int)S, (int)max_rank)},
+      {b200_lora_scratch_bytes((int)T, (int)K, (int)rows, (int)max_tiles, (int)L, (int)S, (int)max_rank)},
       x.options().dtype(at::kByte));
+  const int* p = plan.data_ptr<int>();
   check(b200_lora(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(), out.stride(0), a.data_ptr(), a.size(1),
-                  b.data_ptr(), b.size(1), ranks.data_ptr<int>(), scales.data_ptr<float>(), order.data_ptr<int>(),
-                  tiles.data_ptr<int>(), num_tiles.data_ptr<int>(), (int)max_tiles, (int)rows, h.data_ptr(), (int)T,
-                  (int)L, (int)x.size(1), (int)S, n,
-                  (int)max_rank, (int)act, (float)act_alpha, (float)act_limit, cur_stream()),
+                  b.data_ptr(), b.size(1), ranks.data_ptr<int>(), p, p + at, p + T, (int)max_tiles, (int)rows, h.data_ptr(),
+                  (int)T, (int)L, (int)K, (int)S, n, (int)max_rank, (int)std::max<int64_t>(mean_rank, 16), (int)act,
+                  (float)act_alpha, (float)act_limit, cur_stream()),
         "lora");
+  return out;
 }
 
 int64_t mla_decode_scratch_bytes(int64_t T, int64_t N, int64_t splits) {

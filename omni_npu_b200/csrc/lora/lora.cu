@@ -135,8 +135,7 @@ struct LoraParams {
   const __nv_bfloat16* a;                        // [L, a_slot]
   const __nv_bfloat16* b;                        // [L, b_slot]
   long long a_slot, b_slot;
-  const int* ranks;                              // [L, slices]
-  const float* scales;                           // [L]
+  const int* ranks;                              // [L, slices + 1]: of each slice, then the scale's bits
   const int* order;
   const LoraTile* tiles;
   const int* num_tiles;
@@ -146,7 +145,6 @@ struct LoraParams {
   long long h_plane;                             // T * h_width
   int h_width;                                   // slices * largest rank
   int K, slices, parts;
-  int subs;                                      // pieces of a plan's tile, each with CTAs of its own
   int per;                                       // column groups of a CTA of the second kernel
   int n[kLoraMaxSlices];
   int h_pitch;                                   // elements between rows of h in shared memory
@@ -155,7 +153,7 @@ struct LoraParams {
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -163,13 +161,16 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 
 __device__ __forceinline__ float lo_f(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float hi_f(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+__device__ __forceinline__ float lora_scale(const LoraParams& p, int slot) {
+  return __int_as_float(p.ranks[slot * (p.slices + 1) + p.slices]);
+}
+
 // The tile of a CTA, or false when there is none.  (Entries behind the last tile lie in the buffer.)
-__device__ __forceinline__ bool lora_tile(const LoraParams& p, int item, int subs, int rows, LoraTile& tl) {
-  const int tile = item / subs, sub = item % subs;
+__device__ __forceinline__ bool lora_tile(const LoraParams& p, int tile, LoraTile& tl) {
   const int4 v = *reinterpret_cast<const int4*>(p.tiles + tile);
   if (tile >= *p.num_tiles) return false;
-  tl = LoraTile{v.x, v.y + sub * rows, min(rows, v.z - sub * rows), 0};
-  return tl.count > 0;
+  tl = LoraTile{v.x, v.y, v.z, 0};
+  return true;
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -205,9 +206,10 @@ __device__ __forceinline__ void split_h(const float4& s, float scale, uint2& hi,
 }
 
 // ---- h of few rows: 16 at most, K dealt to the parts and, in steps of 32, to the warps.  The factors are what is read: every
-// lane has a ring of its own in shared memory for what it alone uses of A and x (no barrier between copy and product), 20 to
-// 24 KB a warp in flight however many ranks there are.
-static constexpr int kFewThreads = 128, kFewWarps = kFewThreads / 32, kFewRing = 24 * 1024;
+// lane has a ring of its own in shared memory for what it alone uses of A and x (no barrier between copy and product), 12 KB a
+// warp however many ranks there are, so that four CTAs are resident (128 adapters of rank 16, K 14336: 13.2 us, with 24 KB
+// and two CTAs 15.8).
+static constexpr int kFewThreads = 128, kFewWarps = kFewThreads / 32, kFewRing = 12 * 1024;
 
 template <int NT>
 __device__ __forceinline__ void shrink_rows(const LoraParams& p, const LoraTile& tl, int n0, int sum_r, int s_lo, int s_hi,
@@ -270,9 +272,9 @@ __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const Lora
   pdl_wait();
   pdl_trigger();                                                       // (the second kernel reads what was there before this one)
   LoraTile tl;
-  if (!lora_tile(p, blockIdx.z, p.subs, BM, tl) || tl.slot < 0) return;
+  if (!lora_tile(p, blockIdx.z, tl) || tl.slot < 0) return;
   int sum_r = 0;
-  for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * p.slices + s];
+  for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * (p.slices + 1) + s];
   const int n0 = blockIdx.y * W;
   if (n0 >= sum_r) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
@@ -306,17 +308,17 @@ __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const Lora
 // ---- h of many rows: 64 rows of x and 64 of the joined ranks, in slabs of 128 of K through a ring in shared memory, so that
 // what is in flight does not depend on registers.  Warps: two halves of every slab's K, then 32 rows x 32 ranks each (a fragment
 // of x and one of A serve two and two pairs of matrix instructions).
-static constexpr int kManyThreads = 256, kSlab = 128, kStages = 3, kStageBytes = 2 * 64 * kSlab * 2;
+static constexpr int kManyThreads = 256, kManyRows = 64, kSlab = 128, kStages = 3, kStageBytes = 2 * 64 * kSlab * 2;
 
 __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const LoraParams p) {
-  constexpr int BM = 64, W = kLoraChunk * 8;
+  constexpr int BM = kManyRows, W = kLoraChunk * 8;
   extern __shared__ __align__(128) char smem[];
   pdl_wait();
   pdl_trigger();
   LoraTile tl;
-  if (!lora_tile(p, blockIdx.z, p.subs, BM, tl) || tl.slot < 0) return;
+  if (!lora_tile(p, blockIdx.z, tl) || tl.slot < 0) return;
   int sum_r = 0;
-  for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * p.slices + s];
+  for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * (p.slices + 1) + s];
   const int n0 = blockIdx.y * W;
   if (n0 >= sum_r) return;
   const int width = min(W, sum_r - n0);                                // a multiple of 16
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const
   cluster_arrive_release();
   cluster_wait_acquire();
   const int C = p.parts, rank = blockIdx.x, vecs = width / 4;
-  const float scale = p.scales[tl.slot];
+  const float scale = lora_scale(p, tl.slot);
   __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p.h) + static_cast<long long>(tl.start) * p.h_width + n0;
   for (int i = rank * kManyThreads + threadIdx.x; i < tl.count * vecs; i += C * kManyThreads) {
     const int row = i / vecs, v = i % vecs * 4;
@@ -479,7 +481,7 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
   const bool in_place = !GATED && p.out == p.y;
   // Everything but h is older than the first kernel, which has started only behind it: no wait yet.
   LoraTile tl;
-  if (!lora_tile(p, blockIdx.y, p.subs, BM, tl)) {
+  if (!lora_tile(p, blockIdx.y, tl)) {
     pdl_wait();
     return;
   }
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
   // this CTA's slice and groups in it; of the slice: first rank in h, first column of y, factors (in blocks of 32 columns)
   int slice = 0, block = blockIdx.x, h0 = 0, first = 0, r0 = 0, r1 = 0;
   const __nv_bfloat16* b = p.b + max(tl.slot, 0) * p.b_slot + lane * 8;
-  const int* ranks = p.ranks + max(tl.slot, 0) * p.slices;
+  const int* ranks = p.ranks + max(tl.slot, 0) * (p.slices + 1);
   if constexpr (GATED) {
     r0 = tl.slot >= 0 ? ranks[0] : 0;
     r1 = tl.slot >= 0 ? ranks[1] : 0;
@@ -516,10 +518,15 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
   const __nv_bfloat16* b_up = b + (GATED ? static_cast<long long>(b_last + 1) * r0 * 32 : 0);
   const int ga = block * p.per + warp, gb = min((N + GW - 1) / GW, (block + 1) * p.per);
   const int ms = (tl.count + 15) / 16;
-  const float scale = !MANY && tl.slot >= 0 ? p.scales[tl.slot] : 0.f;
+  const float scale = !MANY && tl.slot >= 0 ? lora_scale(p, tl.slot) : 0.f;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * D * STAGE + lane * 16;
   const __nv_bfloat16* y = p.y + first;
   __nv_bfloat16* out = p.out + first + t4 * 8;
+  // Gated: the eight pieces of 16 bytes of a row are gate and up in turn, and a lane needs two neighbours; copied so, every
+  // request would be for halves of sectors, twice.  So lane q copies pieces q and 4 + q, the latter one place off, and finds
+  // its own without bank conflicts at y_at and y_at ^ 16.
+  constexpr uint32_t y_swap = GATED ? 16 : 0;
+  const uint32_t y_at = GATED ? (t4 >> 1) * 512 + ((t4 & 1) * 2 ^ t4 >> 1) * 16 - t4 * 16 : 0;
   // 16 ranks (step k) of 32 columns of group gi: its half s, or gate / up.  Past the end: any others, whose results are not used
   auto b_at = [&](int gi, int s, int k) {
     if constexpr (GATED) return (s ? b_up : b) + (static_cast<long long>(gi) * (s ? k1 : k0) + min(k, max((s ? k1 : k0) - 1, 0))) * 512;
@@ -535,14 +542,13 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
       const uint32_t st = put;
       put = put + STAGE == ring + D * STAGE ? ring : put + STAGE;
       if (MANY || ck == 0) {
-        const int col = cg * GW + t4 * 8;
-        const __nv_bfloat16* src0 = y + (GATED ? 2 : 1) * min(col, N - 8);
-        const __nv_bfloat16* src1 = GATED ? src0 + 8 : y + min(col + 32, N - 8);
+        const int col = cg * 64 + t4 * 8, end = (GATED ? 2 : 1) * N - 8;
+        const __nv_bfloat16 *src0 = y + min(col, end), *src1 = y + min(col + 32, end);
         const long long at0 = y_row[cm * 16 + g], at1 = y_row[cm * 16 + g + 8];
         cp16(st, src0 + at0);
-        cp16(st + 512, src1 + at0);
+        cp16((st + 512) ^ y_swap, src1 + at0);
         cp16(st + 1024, src0 + at1);
-        cp16(st + 1536, src1 + at1);
+        cp16((st + 1536) ^ y_swap, src1 + at1);
       }
       if constexpr (MANY) {
         if (++cm == ms) {
@@ -622,109 +628,116 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
   const uint32_t hf = h_at + ((lane & 15) * p.h_pitch + (lane >> 4) * 8) * 2;
   const uint32_t lo_at = 2 * BM * p.h_pitch, m_step = 32 * p.h_pitch;
   uint32_t get = ring;
-  for (int gi = ga; gi < gb; gi += STEP) {
-    const int left = N - gi * GW - t4 * 8;
-    for (int m = 0; m < ms; ++m) {
-      float acc[8][4];
-      uint32_t st;
-      auto next = [&]() {
-        asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
-        st = get;
-        get = get + STAGE == ring + D * STAGE ? ring : get + STAGE;
-      };
-      // step k of h times its B
-      auto multiply = [&](int k, const uint4& p0, const uint4& p1, const uint4& q0, const uint4& q1) {
+  auto next = [&]() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+    if (GATED) __syncwarp();
+    const uint32_t st = get;
+    get = get + STAGE == ring + D * STAGE ? ring : get + STAGE;
+    return st;
+  };
+  // rows m of group gi: z in `acc`
+  auto compute = [&](float (&acc)[8][4], int gi, int m) {
+    // step k of h times its B
+    auto multiply = [&](int k, const uint4& p0, const uint4& p1, const uint4& q0, const uint4& q1) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          if (GATED && k >= (s ? k1 : k0)) continue;
-          const uint4 &v = s ? q0 : p0, &w = s ? q1 : p1;
-          uint32_t hi[4], lo[4];
-          const uint32_t at = hf + m * m_step + k * 32 + (GATED && s ? r0 * 2 : 0);
-          ldmatrix4(hi, at);
-          ldmatrix4(lo, at + lo_at);
-          float(*c)[4] = acc + 4 * s;
-          mma_bf16(c[0], hi[0], hi[1], hi[2], hi[3], v.x, v.y);
-          mma_bf16(c[1], hi[0], hi[1], hi[2], hi[3], v.z, v.w);
-          mma_bf16(c[2], hi[0], hi[1], hi[2], hi[3], w.x, w.y);
-          mma_bf16(c[3], hi[0], hi[1], hi[2], hi[3], w.z, w.w);
-          mma_bf16(c[0], lo[0], lo[1], lo[2], lo[3], v.x, v.y);
-          mma_bf16(c[1], lo[0], lo[1], lo[2], lo[3], v.z, v.w);
-          mma_bf16(c[2], lo[0], lo[1], lo[2], lo[3], w.x, w.y);
-          mma_bf16(c[3], lo[0], lo[1], lo[2], lo[3], w.z, w.w);
-        }
-      };
-      next();
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const uint4 v = lds16(st + i * 1024 + s * 512);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            acc[4 * s + j][2 * i] = lo_f(w[j]);
-            acc[4 * s + j][2 * i + 1] = hi_f(w[j]);
-          }
-        }
-      if constexpr (MANY) {
-        copy();
-        const bool more = m + 1 == ms && gi + STEP < gb;
-        if (ks == 1) {
-          multiply(0, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
-          if (more) load_b(bv[0], gi + STEP, 0);
-        } else if (ks == 2) {
-          multiply(0, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
-          multiply(1, bv[1][0], bv[1][1], bv[1][2], bv[1][3]);
-          if (more) {
-            load_b(bv[0], gi + STEP, 0);
-            load_b(bv[1], gi + STEP, 1);
-          }
-        } else {
-          for (int k = 0; k < ks; k += 2) {
-            // the registers take the steps after these as soon as they have been used
-            const bool tail = k + 2 >= ks;
-            const int ng = tail && more ? gi + STEP : gi, nk = tail ? 0 : k + 2;
-            multiply(k, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
-            load_b(bv[0], ng, nk);
-            if (k + 1 < ks) multiply(k + 1, bv[1][0], bv[1][1], bv[1][2], bv[1][3]);
-            load_b(bv[1], ng, nk + 1);
-          }
-        }
-      } else {
-        for (int k = 0;;) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            if (k + u < ks) {
-              const uint32_t at = st + 2048 + u * 2048;
-              multiply(k + u, lds16(at), lds16(at + 512), lds16(at + 1024), lds16(at + 1536));
-            }
-          copy();
-          k += 2;
-          if (k >= ks) break;
-          next();
-        }
+      for (int s = 0; s < 2; ++s) {
+        if (GATED && k >= (s ? k1 : k0)) continue;
+        const uint4 &v = s ? q0 : p0, &w = s ? q1 : p1;
+        uint32_t hi[4], lo[4];
+        const uint32_t at = hf + m * m_step + k * 32 + (GATED && s ? r0 * 2 : 0);
+        ldmatrix4(hi, at);
+        ldmatrix4(lo, at + lo_at);
+        float(*c)[4] = acc + 4 * s;
+        mma_bf16(c[0], hi[0], hi[1], hi[2], hi[3], v.x, v.y);
+        mma_bf16(c[1], hi[0], hi[1], hi[2], hi[3], v.z, v.w);
+        mma_bf16(c[2], hi[0], hi[1], hi[2], hi[3], w.x, w.y);
+        mma_bf16(c[3], hi[0], hi[1], hi[2], hi[3], w.z, w.w);
+        mma_bf16(c[0], lo[0], lo[1], lo[2], lo[3], v.x, v.y);
+        mma_bf16(c[1], lo[0], lo[1], lo[2], lo[3], v.z, v.w);
+        mma_bf16(c[2], lo[0], lo[1], lo[2], lo[3], w.x, w.y);
+        mma_bf16(c[3], lo[0], lo[1], lo[2], lo[3], w.z, w.w);
       }
+    };
+    uint32_t st = next();
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int e = 2 * i;
-        const long long at = out_row[m * 16 + i * 8 + g];
-        uint32_t o0[4], o1[4];
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint4 v = lds16(GATED ? (st + y_at + i * 1024) ^ s * 16 : st + i * 1024 + s * 512);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if constexpr (GATED) {
-            o0[j] = pack_bf16x2(gated_act(ACT, acc[j][e], acc[4 + j][e], p.act_alpha, p.act_limit),
-                                gated_act(ACT, acc[j][e + 1], acc[4 + j][e + 1], p.act_alpha, p.act_limit));
-          } else {
-            o0[j] = pack_bf16x2(acc[j][e], acc[j][e + 1]);
-            o1[j] = pack_bf16x2(acc[4 + j][e], acc[4 + j][e + 1]);
-          }
+          acc[4 * s + j][2 * i] = lo_f(w[j]);
+          acc[4 * s + j][2 * i + 1] = hi_f(w[j]);
         }
-        __nv_bfloat16* row = out + at + gi * GW;
-        if (at >= 0 && left > 0) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
-        if (!GATED && at >= 0 && left > 32) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+      }
+    if constexpr (MANY) {
+      copy();
+      const bool more = m + 1 == ms && gi + STEP < gb;
+      if (ks == 1) {
+        multiply(0, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
+        if (more) load_b(bv[0], gi + STEP, 0);
+      } else if (ks == 2) {
+        multiply(0, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
+        multiply(1, bv[1][0], bv[1][1], bv[1][2], bv[1][3]);
+        if (more) {
+          load_b(bv[0], gi + STEP, 0);
+          load_b(bv[1], gi + STEP, 1);
+        }
+      } else {
+        for (int k = 0; k < ks; k += 2) {
+          // the registers take the steps after these as soon as they have been used
+          const bool tail = k + 2 >= ks;
+          const int ng = tail && more ? gi + STEP : gi, nk = tail ? 0 : k + 2;
+          multiply(k, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
+          load_b(bv[0], ng, nk);
+          if (k + 1 < ks) multiply(k + 1, bv[1][0], bv[1][1], bv[1][2], bv[1][3]);
+          load_b(bv[1], ng, nk + 1);
+        }
+      }
+    } else {
+      for (int k = 0;;) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (k + u < ks) {
+            const uint32_t at = st + 2048 + u * 2048;
+            multiply(k + u, lds16(at), lds16(at + 512), lds16(at + 1024), lds16(at + 1536));
+          }
+        copy();
+        k += 2;
+        if (k >= ks) break;
+        st = next();
       }
     }
-  }
+  };
+  auto store = [&](const float (&acc)[8][4], int gi, int m) {
+    const int left = N - gi * GW - t4 * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int e = 2 * i;
+      const long long at = out_row[m * 16 + i * 8 + g];
+      uint32_t o0[4], o1[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (GATED) {
+          o0[j] = pack_bf16x2(gated_act(ACT, acc[j][e], acc[4 + j][e], p.act_alpha, p.act_limit),
+                              gated_act(ACT, acc[j][e + 1], acc[4 + j][e + 1], p.act_alpha, p.act_limit));
+        } else {
+          o0[j] = pack_bf16x2(acc[j][e], acc[j][e + 1]);
+          o1[j] = pack_bf16x2(acc[4 + j][e], acc[4 + j][e + 1]);
+        }
+      }
+      __nv_bfloat16* row = out + at + gi * GW;
+      if (at >= 0 && left > 0) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+      if (!GATED && at >= 0 && left > 32) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+    }
+  };
+  for (int gi = ga; gi < gb; gi += STEP)
+    for (int m = 0; m < ms; ++m) {
+      float acc[8][4];
+      compute(acc, gi, m);
+      store(acc, gi, m);
+    }
 }
 
 static constexpr int kShrinkFewSmem = kFewWarps * kFewRing, kShrinkManySmem = kStages * kStageBytes, kExpandSmem = 168 * 1024;
@@ -743,12 +756,12 @@ static int launch_lora(const LoraParams& p, unsigned tiles, unsigned chunks, uns
     once.mark(dev);
   }
   const size_t smem = 4 * 4 * (MANY ? 2048 : 6144) + 2 * sizeof(__nv_bfloat16) * (MANY ? 64 : 16) * p.h_pitch;
-  const dim3 grid(p.parts, chunks, tiles * p.subs);
-  if (smem > kExpandSmem || grid.z > 65535) return -2;
+  const dim3 grid(p.parts, chunks, tiles);
+  if (smem > kExpandSmem || tiles > 65535) return -2;
   if (launch_pdl(shrink, grid, dim3(MANY ? kManyThreads : kFewThreads), MANY ? kShrinkManySmem : kShrinkFewSmem, stream, MANY ? p.parts : 1, p) !=
       cudaSuccess)
     return -3;
-  return launch_pdl(expand, dim3(blocks, grid.z), dim3(kExpandThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
+  return launch_pdl(expand, dim3(blocks, tiles), dim3(kExpandThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
 }
 
 template <int ACT>
@@ -756,18 +769,21 @@ static int launch_lora(const LoraParams& p, bool many, unsigned tiles, unsigned 
   return many ? launch_lora<true, ACT>(p, tiles, chunks, blocks, stream) : launch_lora<false, ACT>(p, tiles, chunks, blocks, stream);
 }
 
-}  // namespace b200
-
-// Parts of K that a step's h is summed from, a CTA each (many rows: of a cluster).  Few rows (tiles of 16): as many as the slots let be resident, whatever the number of
-// tokens, so that a row does not depend on it; many rows: as many as fill the SMs.
+// Parts of K that a step's h is summed from, a CTA each (many rows: of a cluster).  Few rows (tiles of 16): as many as the slots
+// let be resident, whatever the number of tokens, so that a row does not depend on it.  Many rows: as many as fill the SMs, given
+// the pieces of 64 ranks that a tile has on average.
 static int lora_parts(int K, int rows, int max_tiles, int num_slots, int chunks) {
-  const int want = rows < 64 ? std::min((K + 511) / 512, 592 / num_slots) : std::min((K + 255) / 256, 296 / (max_tiles * chunks));
-  return std::min(std::max(want, 1), rows < 64 ? 16 : 8);
+  const int pieces = max_tiles * chunks;
+  const int want = rows < kManyRows ? std::min((K + 511) / 512, 592 / num_slots)
+                                    : std::min((K + 127) / 128, (296 + pieces / 2) / pieces);
+  return std::min(std::max(want, 1), rows < kManyRows ? 16 : 8);
 }
+
+}  // namespace b200
 
 // Bytes of scratch for a step's h.
 extern "C" long long b200_lora_scratch_bytes(int T, int K, int rows, int max_tiles, int num_slots, int slices, int max_rank) {
-  return 4LL * T * slices * max_rank * (rows < 64 ? lora_parts(K, rows, max_tiles, num_slots, 1) : 1);
+  return 4LL * T * slices * max_rank * (rows < b200::kManyRows ? b200::lora_parts(K, rows, max_tiles, num_slots, 1) : 1);
 }
 
 // Groups tokens by adapter.  tiles: at least T / rows + min(T, L + 1) of four ints.
@@ -788,16 +804,18 @@ extern "C" int b200_lora_plan(const int* slots, int T, int L, int rows, int* ord
                     reinterpret_cast<LoraTile*>(tiles), num_tiles, status) == cudaSuccess ? 0 : -3;
 }
 
-// n: columns of each slice.  h: scratch of b200_lora_scratch_bytes.  max_tiles: tiles that the plan may have, of `rows`
-// tokens each.  max_rank: bound of the ranks.  act: 0 adds, a gated kind of gemm/gated_act.cuh joins gate and up (alternating
+// ranks: [L, slices + 1], a slot's ranks and the bits of its scale.  n: columns of each slice.  h: scratch of b200_lora_scratch_bytes.  max_tiles: tiles that the plan may have, of `rows`
+// tokens each.  max_rank: bound of the ranks; mean_rank: about what a
+// tile's joined ranks are (16 at least).  act: 0 adds, a gated kind of gemm/gated_act.cuh joins gate and up (alternating
 // groups of eight columns of y).
 extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long long y_stride, void* out, long long out_stride,
-                         const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks,
-                         const float* scales, const int* order, const int* tiles, const int* num_tiles, int max_tiles, int rows,
-                         void* h, int T, int num_slots, int K, int slices, const int* n, int max_rank, int act,
-                         float act_alpha, float act_limit, cudaStream_t stream) {
+                         const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks, const int* order, const int* tiles, const int* num_tiles, int max_tiles, int rows,
+                         void* h, int T, int num_slots, int K, int slices, const int* n, int max_rank, int mean_rank,
+                         int act, float act_alpha, float act_limit, cudaStream_t stream) {
   using namespace b200;
-  if (slices < 1 || slices > kLoraMaxSlices || (K & 7) || max_rank < 16 || (max_rank & 15) || max_tiles < 1 || (rows & 15)) return -1;
+  if (slices < 1 || slices > kLoraMaxSlices || (K & 7) || max_rank < 16 || mean_rank < 16 || (max_rank & 15) || max_tiles < 1 ||
+      (rows != 16 && rows != kManyRows))
+    return -1;
   if (act != kActNone && (!act_is_gated(act) || slices != 2 || n[0] != n[1])) return -1;
   LoraParams p;
   p.x = static_cast<const __nv_bfloat16*>(x);
@@ -811,7 +829,6 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   p.a_slot = a_slot;
   p.b_slot = b_slot;
   p.ranks = ranks;
-  p.scales = scales;
   p.order = order;
   p.tiles = reinterpret_cast<const LoraTile*>(tiles);
   p.num_tiles = num_tiles;
@@ -820,14 +837,14 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   p.h_plane = static_cast<long long>(T) * p.h_width;
   p.K = K;
   p.slices = slices;
-  const bool many = rows >= 64, gated = act != kActNone;
+  const bool many = rows == kManyRows, gated = act != kActNone;
   p.act_alpha = act_alpha;
   p.act_limit = act_limit;
-  p.subs = many ? rows / 64 : rows / 16;
   const unsigned chunks = (p.h_width + kLoraChunk * 8 - 1) / (kLoraChunk * 8), tiles_n = static_cast<unsigned>(max_tiles);
-  p.parts = lora_parts(K, rows, max_tiles, num_slots, chunks);
+  p.parts = lora_parts(K, rows, max_tiles, num_slots, (mean_rank + kLoraChunk * 8 - 1) / (kLoraChunk * 8));
   p.h_pitch = (gated ? 2 : 1) * max_rank + 8;    // eight rows of 16 bytes are in banks of their own
-  // column groups of a CTA: a few rounds of the resident CTAs in all, a group a team at least
+  // column groups of a CTA: four rounds of the resident CTAs in all, or for few rows one, where a CTA's start is most of its
+  // time (128 adapters of rank 16, 4096 columns: 7.7 us, with four rounds 12.9); a group a warp at least
   int groups = 0;
   for (int s = 0; s < kLoraMaxSlices; ++s) {
     p.n[s] = s < slices ? n[s] : 0;
@@ -835,7 +852,7 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
     if (!gated || s == 0) groups += gated ? (p.n[s] + 31) / 32 : (p.n[s] + 63) / 64;
   }
   const int team = 4;
-  const long long want = static_cast<long long>(groups) * max_tiles * p.subs / (148 * 4 * (many ? 4 : 2));
+  const long long want = static_cast<long long>(groups) * max_tiles / (148 * (many ? 16 : 2));
   p.per = static_cast<int>(std::max(1LL, (want + team - 1) / team)) * team;
   unsigned blocks = 0;
   for (int s = 0; s < slices; ++s)

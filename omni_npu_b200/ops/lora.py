@@ -58,10 +58,12 @@ class LoraStack:
             self._k = (in_features + 31) // 32
             self.a = torch.zeros(num_slots, len(slices) * self.max_rank * self._k * 32, dtype=dtype, device=device)
             self.b = torch.zeros(num_slots, sum((n + 31) // 32 * 32 for n in slices) * self.max_rank, dtype=dtype, device=device)
-            self.ranks = torch.zeros(num_slots, len(slices), dtype=torch.int32, device=device)
-            self.scales = torch.zeros(num_slots, dtype=torch.float32, device=device)
+            # of every slot the ranks (in whole 16) and the bits of the scale
+            self.ranks = torch.zeros(num_slots, len(slices) + 1, dtype=torch.int32, device=device)
         self.device = self.a.device
         self._ranks = [[0] * len(slices) for _ in range(num_slots)]
+        self._scales = [0.0] * num_slots
+        self.mean_rank = 0
 
     def load(self, slot: int, a: Sequence[Optional[torch.Tensor]], b: Sequence[Optional[torch.Tensor]],
              scale: float = 1.0) -> None:
@@ -92,9 +94,11 @@ class LoraStack:
             for q, view in zip(b, self._views_b(slot, ranks)):
                 if view is not None:
                     view.copy_(_padded(q, view.shape[0] * 32, view.shape[5] * 16).view(view.shape))
-            self.scales[slot] = float(scale)
-            self.ranks[slot].copy_(torch.tensor(ranks, dtype=torch.int32))
-        self._ranks[slot] = ranks
+            row = torch.tensor(ranks + [0], dtype=torch.int32)
+            row[-1:].view(torch.float32).fill_(scale)
+            self.ranks[slot].copy_(row)
+        self._scales[slot] = float(scale)
+        self._set_ranks(slot, ranks)
 
     def _views_a(self, slot: int, ranks):
         """A of each slice as [ranks, K] in the shape (rank / 16, 2, 8, K / 32, 4, 2, 4) over its packed place."""
@@ -120,7 +124,7 @@ class LoraStack:
         self._check_slot(slot)
         with torch.inference_mode():
             self.ranks[slot].zero_()
-        self._ranks[slot] = [0] * len(self.slices)
+        self._set_ranks(slot, [0] * len(self.slices))
 
     def factors(self, slot: int):
         """(A, B) of each slice of a slot (ranks padded to 16), None where it has none."""
@@ -133,20 +137,35 @@ class LoraStack:
         j = torch.arange(self.slices[i], device=self.device)
         return j // 8 * 16 + i * 8 + j % 8 if self.interleaved else sum(self.slices[:i]) + j
 
+    def _set_ranks(self, slot: int, ranks) -> None:
+        self._ranks[slot] = ranks
+        used = [sum(r) for r in self._ranks if any(r)]
+        self.mean_rank = sum(used) // max(1, len(used))        # of the loaded adapters, the slices' together: only speed depends on it
+
     def _check_slot(self, slot: int) -> None:
         if not 0 <= slot < self.num_slots:
             raise ValueError(f"LoraStack: slot {slot} of {self.num_slots}")
 
 
 class LoraPlan:
-    """A step's tokens grouped by adapter slot (:func:`lora_plan`); the buffers belong to the step."""
+    """A step's tokens grouped by adapter slot (:func:`lora_plan`)."""
 
-    __slots__ = ("slots", "num_slots", "num_tokens", "rows", "order", "tiles", "num_tiles", "max_tiles")
+    __slots__ = ("slots", "num_slots", "num_tokens", "rows", "buffer")
 
-    def __init__(self, slots: torch.Tensor, num_slots: int, rows: int = 0) -> None:
-        self.slots, self.num_slots, self.num_tokens, self.rows = slots, num_slots, slots.shape[0], rows
-        self.order = self.tiles = self.num_tiles = None
-        self.max_tiles = 0
+    def __init__(self, slots: torch.Tensor, num_slots: int, rows: int = 0, buffer: Optional[torch.Tensor] = None) -> None:
+        self.slots, self.num_slots, self.num_tokens, self.rows, self.buffer = slots, num_slots, slots.shape[0], rows, buffer
+
+    @property
+    def order(self) -> torch.Tensor:
+        """Tokens by slot, those without an adapter last (on a GPU)."""
+        return self.buffer[: self.num_tokens]
+
+    @property
+    def tiles(self) -> torch.Tensor:
+        """[tiles, 4]: slot, first place in ``order`` and number of tokens of every tile (on a GPU; reads their number back)."""
+        t = self.num_tokens
+        at = (t + 1 + 3) // 4 * 4
+        return self.buffer[at: at + 4 * int(self.buffer[t])].view(-1, 4)
 
 
 def lora_plan(slots: torch.Tensor, num_slots: int) -> LoraPlan:
@@ -162,17 +181,11 @@ def lora_plan(slots: torch.Tensor, num_slots: int) -> LoraPlan:
         if t and (int(slots.min()) < -1 or int(slots.max()) >= num_slots):
             raise ValueError(f"lora_plan: slots outside -1 .. {num_slots - 1}")
         return LoraPlan(slots, num_slots)
-    plan = LoraPlan(slots, num_slots, FEW_ROWS if t <= FEW_TOKENS else MANY_ROWS)
+    rows = FEW_ROWS if t <= FEW_TOKENS else MANY_ROWS
     if t == 0:
-        return plan
-    plan.max_tiles = t // plan.rows + min(t, num_slots + 1)
-    # order, count of tiles and tiles (four ints each, 16-byte aligned)
-    at = (t + 1 + 3) // 4 * 4
-    buf = torch.empty(at + 4 * plan.max_tiles, dtype=torch.int32, device=slots.device)
-    plan.order, plan.num_tiles, plan.tiles = buf[:t], buf[t: t + 1], buf[at:]
+        return LoraPlan(slots, num_slots, rows, slots.new_empty(4))
     _count(1)
-    _C().lora_plan(slots, num_slots, plan.rows, plan.order, plan.tiles, plan.num_tiles, device_state(slots.device).status)
-    return plan
+    return LoraPlan(slots, num_slots, rows, _C().lora_plan(slots, num_slots, rows, device_state(slots.device).status))
 
 
 def _check(what: str, y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan) -> None:
@@ -187,13 +200,10 @@ def _check(what: str, y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: 
         raise ValueError(f"{what}: tensors on {x.device}, {y.device}, {stack.device} and {plan.slots.device}")
 
 
-def _launch(y, x, stack: LoraStack, plan: LoraPlan, out, kind) -> torch.Tensor:
-    if x.shape[0] == 0:
-        return out
-    _count(2)
-    _C().lora(x, y, out, stack.a, stack.b, stack.ranks, stack.scales, plan.order, plan.tiles, plan.num_tiles, plan.max_tiles,
-              plan.rows, stack.slices, stack.max_rank, *kind)
-    return out
+def _launch(y, x, stack: LoraStack, plan: LoraPlan, out, kind, alpha, limit) -> torch.Tensor:
+    _count(2 if plan.num_tokens else 0)
+    return _C().lora(x, y, out, stack.a, stack.b, stack.ranks, plan.buffer,
+                     [plan.rows, stack.max_rank, stack.mean_rank, kind, *stack.slices], alpha, limit)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan,
@@ -208,7 +218,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan,
     if not x.is_cuda:
         z = ref.lora_sum(y, x, stack, plan.slots).to(y.dtype)
         return z if out is None else out.copy_(z)
-    return _launch(y, x, stack, plan, y.new_empty(y.shape) if out is None else out, (0, 0.0, 0.0))
+    return _launch(y, x, stack, plan, out, 0, 0.0, 0.0)
 
 
 def lora_gated(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan, act=SILU) -> torch.Tensor:
@@ -220,4 +230,4 @@ def lora_gated(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPla
     if not x.is_cuda:
         z = ref.lora_sum(y, x, stack, plan.slots).view(y.shape[0], -1, 2, 8)
         return ref.gated_act(z[:, :, 0], z[:, :, 1], act).reshape(y.shape[0], -1).to(y.dtype)
-    return _launch(y, x, stack, plan, y.new_empty(y.shape[0], stack.slices[0]), _act_kind(True, act))
+    return _launch(y, x, stack, plan, None, *_act_kind(True, act))

@@ -883,5 +883,5 @@ def lora_sum(y: torch.Tensor, x: torch.Tensor, stack, slots: torch.Tensor) -> to
         for i, f in enumerate(stack.factors(s)):
             if f is not None:
                 d = (x[rows].float() @ f[0].float().t()) @ f[1].float().t()
-                z[rows[:, None], stack.columns(i)[None, :]] += d * stack.scales[s]
+                z[rows[:, None], stack.columns(i)[None, :]] += d * stack._scales[s]
     return z
