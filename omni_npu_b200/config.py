@@ -504,6 +504,13 @@ class SpeculativeConfig:
 
 
 @dataclass
+class AdapterConfig:
+    """Low-rank adapters: slots for adapters loaded at once (0 = off) and their largest rank."""
+    max_loras: int = 0
+    max_lora_rank: int = 16
+
+
+@dataclass
 class EngineConfig:
     model: ModelConfig = field(default_factory=ModelConfig)
     cache: CacheConfig = field(default_factory=CacheConfig)
@@ -512,6 +519,7 @@ class EngineConfig:
     compilation: CompilationConfig = field(default_factory=CompilationConfig)
     kv_transfer: Optional[KVTransferConfig] = None
     speculative: SpeculativeConfig = field(default_factory=SpeculativeConfig)
+    adapters: AdapterConfig = field(default_factory=AdapterConfig)
     model_path: Optional[str] = None          # HF directory with safetensors; None = random init
     load_format: str = "auto"                 # auto | dummy
     seed: int = 0
@@ -546,6 +554,15 @@ class EngineConfig:
                 raise ValueError("speculative decoding is not supported with pipeline_parallel_size > 1")
             if self.kv_transfer is not None:
                 raise ValueError("KV transfer connectors are not supported with pipeline_parallel_size > 1")
+
+        if self.adapters.max_loras > 0:
+            p = self.parallel
+            if p.world_size > 1 or p.decode_context_parallel_size > 1 or p.sequence_parallel_residual:
+                raise ValueError("low-rank adapters run on one GPU: no tensor, pipeline, data or context parallelism")
+            if self.speculative.method in ("mtp", "deepseek_mtp") and self.speculative.num_speculative_tokens > 0:
+                raise ValueError("low-rank adapters are not supported together with a draft head")
+            if self.kv_transfer is not None:
+                raise ValueError("low-rank adapters are not supported together with KV transfer connectors")
 
     def resolved_device(self) -> torch.device:
         if self.device == "cpu":

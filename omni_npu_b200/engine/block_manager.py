@@ -16,10 +16,11 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 
 def chain_block_hashes(token_ids: Sequence[int], block_size: int, prev: Optional[List[bytes]] = None,
-                       upto_blocks: Optional[int] = None) -> List[bytes]:
+                       upto_blocks: Optional[int] = None, salt: bytes = b"") -> List[bytes]:
     """Content hashes of the full blocks of ``token_ids``: block i hashes (hash of block i - 1, its
     tokens), so equal hashes mean equal prefixes.  ``prev`` are hashes already known (extended in
-    place and returned); a block holding a negative token id (a placeholder) ends the chain."""
+    place and returned); a block holding a negative token id (a placeholder) ends the chain.  ``salt``: what besides the
+    tokens decides the blocks' contents."""
     import hashlib
     import struct
     out = prev if prev is not None else []
@@ -30,14 +31,14 @@ def chain_block_hashes(token_ids: Sequence[int], block_size: int, prev: Optional
         blk = token_ids[i * block_size: (i + 1) * block_size]
         if min(blk) < 0:
             break
-        h = hashlib.blake2b(out[i - 1] if i else b"", digest_size=16)
+        h = hashlib.blake2b(out[i - 1] if i else salt, digest_size=16)
         h.update(struct.pack(f"<{block_size}q", *blk))
         out.append(h.digest())
     return out
 
 
 class BlockPool:
-    """Free list of KV blocks.  With ``prefix_caching`` a block may be shared by several requests
+    """Free list of KV blocks.  A block may be shared (``share``): it returns with its last user.  With ``prefix_caching`` a block may be shared by several requests
     (reference counts) and a full block whose content hash was registered stays findable after its
     last user frees it, until the block is needed again (least recently freed first)."""
 
@@ -50,7 +51,7 @@ class BlockPool:
         self._free: List[int] = list(range(num_blocks - 1, num_reserved - 1, -1))
         self._delayed: Dict[str, Tuple[float, List[int]]] = {}
         self.prefix_caching = prefix_caching
-        self._ref: Dict[int, int] = {}                 # users of a block in use (prefix caching only)
+        self._ref: Dict[int, int] = {}                 # users of a block in use (without prefix caching: of shared blocks only)
         self._hash_of: Dict[int, bytes] = {}           # block -> registered content hash
         self._block_of: Dict[bytes, int] = {}          # content hash -> block
         self._cached_free: Dict[int, None] = {}        # unused blocks that still hold registered content, oldest first
@@ -90,7 +91,15 @@ class BlockPool:
 
     def free(self, blocks: Sequence[int]) -> None:
         if not self.prefix_caching:
-            self._free.extend(reversed(list(blocks)))
+            if not self._ref:
+                self._free.extend(reversed(list(blocks)))
+                return
+            for b in reversed(list(blocks)):
+                users = self._ref.pop(b, 1)
+                if users > 2:
+                    self._ref[b] = users - 1
+                elif users == 1:
+                    self._free.append(b)
             return
         for b in reversed(list(blocks)):
             left = self._ref.get(b, 1) - 1
@@ -102,6 +111,14 @@ class BlockPool:
                 self._cached_free[b] = None
             else:
                 self._free.append(b)
+
+    def share(self, blocks: Sequence[int]) -> None:
+        """One more user of blocks in use."""
+        if self.prefix_caching:
+            self.acquire(blocks)
+            return
+        for b in blocks:
+            self._ref[b] = self._ref.get(b, 1) + 1
 
     # ---- prefix caching
     def register(self, block: int, content_hash: bytes) -> None:

@@ -8,6 +8,7 @@ the model's collectives); rank 0's outputs are the result.
 """
 from __future__ import annotations
 
+import dataclasses
 import itertools
 import time
 from typing import Dict, Iterable, List, Optional, Sequence, Union
@@ -67,6 +68,9 @@ class LLMEngine:
                              "newest token of a sequence only")
         self.scheduler = Scheduler(config.scheduler, config.cache, num_blocks, reserved, connector,
                                    context_parallel_size=dcp, num_state_slots=state_slots)
+        # (a pipeline stage may hold no layers: its pages could not say what the others do)
+        self.scheduler.copies_pages = (self.worker.model_runner.page_cache is not None
+                                       and config.parallel.pipeline_parallel_size == 1)
         self._ids = itertools.count()
         self.stats = {"steps": 0, "prefill_steps": 0, "decode_steps": 0, "spec_decode_steps": 0,
                       "h2d_bytes": 0, "d2h_bytes": 0, "output_tokens": 0}
@@ -91,13 +95,41 @@ class LLMEngine:
 
     def add_request(self, prompt_token_ids: Sequence[int], sampling_params: Optional[SamplingParams] = None,
                     request_id: Optional[str] = None, kv_transfer_params=None,
-                    arrival_time: Optional[float] = None) -> str:
+                    arrival_time: Optional[float] = None, adapter: Optional[str] = None,
+                    fork_of: Optional[str] = None) -> str:
+        """``adapter``: name of a loaded low-rank adapter.  ``fork_of``: an earlier request with the same prompt and adapter,
+        of which this is a further sample; it shares that request's prompt blocks instead of computing them again."""
         rid = request_id or f"req-{next(self._ids)}"
         self.validate_sampling_params(sampling_params)
         req = Request(rid, prompt_token_ids, sampling_params, self.config.model.eos_token_id,
                       arrival_time, kv_transfer_params)
-        self.scheduler.add_request(req)
+        if adapter is not None:
+            adapters = self.adapters()
+            req.adapter, req.lora_slot, req.cache_salt = adapter, adapters.slot(adapter), adapters.keys[adapter]
+        if fork_of is not None:
+            self.scheduler.add_fork(req, fork_of)
+        else:
+            self.scheduler.add_request(req)
         return rid
+
+    def adapters(self):
+        """The adapter slots (``layers.lora.AdapterManager``)."""
+        manager = self.worker.model_runner.adapters
+        if manager is None:
+            raise ValueError("low-rank adapters are off (enable_lora=True turns them on)")
+        return manager
+
+    def load_adapter(self, name: str, path: str) -> int:
+        """Load a low-rank adapter (a directory in the PEFT layout) into a free slot; returns the slot."""
+        return self.adapters().load(name, path)
+
+    def unload_adapter(self, name: str) -> None:
+        """Empty an adapter's slot; refused while requests use it."""
+        self.adapters().slot(name)
+        users = sum(r.adapter == name for r in self.scheduler.requests.values())
+        if users or self._inflight is not None and any(r.adapter == name for r in self._inflight[1]["reqs"]):
+            raise ValueError(f"adapter {name!r} is in use by {max(users, 1)} requests")
+        self.adapters().unload(name)
 
     def validate_sampling_params(self, sp: Optional[SamplingParams]) -> None:
         """Refuse (ValueError) what the sampler cannot honour rather than ignore it."""
@@ -140,7 +172,7 @@ class LLMEngine:
         finish_reason "abort" and their blocks return to the pool."""
         self._inflight = None
         outs = []
-        for req in list(self.scheduler.running) + list(self.scheduler.waiting):
+        for req in list(self.scheduler.requests.values()):
             self.scheduler.abort_request(req.request_id)
             self.worker.model_runner.input_batch.remove_request(req.request_id)
             outs.append(RequestOutput.from_request(req))
@@ -388,11 +420,21 @@ class LLM:
     def wake_up(self, tags=None) -> int:
         return self.engine.worker.wake_up(tags)
 
+    def load_adapter(self, name: str, path: str) -> int:
+        """Load a low-rank adapter (a directory with ``adapter_config.json`` and ``adapter_model.safetensors``) under a name
+        that requests may ask for (needs ``enable_lora=True``); returns its slot."""
+        return self.engine.load_adapter(name, path)
+
+    def unload_adapter(self, name: str) -> None:
+        self.engine.unload_adapter(name)
+
     def generate(self, prompts: Sequence[Union[str, Sequence[int]]],
                  sampling_params: Union[SamplingParams, Sequence[SamplingParams], None] = None,
-                 ) -> List[RequestOutput]:
+                 adapter: Union[str, Sequence[Optional[str]], None] = None) -> List[RequestOutput]:
         """Run the prompts to completion.  A prompt is a list of token ids, or text when the model
-        directory has a tokenizer (the outputs then carry ``text`` as well)."""
+        directory has a tokenizer (the outputs then carry ``text`` as well).  ``adapter``: a loaded adapter's name for all
+        prompts, or one (or None) for each.  With ``SamplingParams.n`` > 1 a prompt is computed once for its n samples; an
+        output carries the second to the n-th as ``others``."""
         tok = self.tokenizer
         if any(isinstance(p, str) for p in prompts):
             tok = self.get_tokenizer()
@@ -400,11 +442,24 @@ class LLM:
                 raise ValueError("text prompts need a tokenizer in the model directory; pass token ids instead")
             prompts = [tok.encode(p) if isinstance(p, str) else p for p in prompts]
         sps = sampling_params if isinstance(sampling_params, (list, tuple)) else [sampling_params] * len(prompts)
+        names = [adapter] * len(prompts) if adapter is None or isinstance(adapter, str) else list(adapter)
+        if len(names) != len(prompts):
+            raise ValueError(f"{len(names)} adapters for {len(prompts)} prompts")
+        for name in {n for n in names if n is not None}:
+            self.engine.adapters().slot(name)            # an unknown one is refused before anything is queued
+        if any(sp is not None and int(sp.n) < 1 for sp in sps):
+            raise ValueError("n must be 1 at least")
         order: Dict[str, int] = {}
+        further: List[tuple] = []
         now = time.monotonic()
-        for i, (p, sp) in enumerate(zip(prompts, sps)):
-            order[self.engine.add_request(p, sp, arrival_time=now)] = i
-        results: List[Optional[RequestOutput]] = [None] * len(prompts)
+        for i, (p, sp, name) in enumerate(zip(prompts, sps, names)):
+            first = self.engine.add_request(p, sp, arrival_time=now, adapter=name)
+            order[first] = i
+            for j in range(1, sp.n if sp is not None else 1):
+                again = dataclasses.replace(sp, seed=None if sp.seed is None else sp.seed + j)
+                order[self.engine.add_request(p, again, arrival_time=now, adapter=name, fork_of=first)] = len(prompts) + len(further)
+                further.append((i, j))
+        results: List[Optional[RequestOutput]] = [None] * (len(prompts) + len(further))
         if self.engine.dp_group is not None:
             # replicas finish at different times; keep stepping (dummy batches) until all are done
             while True:
@@ -421,13 +476,16 @@ class LLM:
             for o in results:
                 if o is not None:
                     o.text = tok.decode(o.output_token_ids)
-        return results  # type: ignore[return-value]
+        for (i, _), o in zip(further, results[len(prompts):]):
+            if results[i] is not None:
+                results[i].others.append(o)
+        return results[: len(prompts)]  # type: ignore[return-value]
 
 
 def build_engine_config(model: ModelConfig, model_path: Optional[str] = None, **kw) -> EngineConfig:
     """Keyword-style construction mirroring the usual serving flags
     (tensor_parallel_size, max_num_seqs, block_size, ...)."""
-    from ..config import (CacheConfig, CompilationConfig, KVTransferConfig, ParallelConfig,
+    from ..config import (AdapterConfig, CacheConfig, CompilationConfig, KVTransferConfig, ParallelConfig,
                           SchedulerConfig, SpeculativeConfig)
     cache = CacheConfig(block_size=kw.pop("block_size", 16),
                         gpu_memory_utilization=kw.pop("gpu_memory_utilization", 0.9),
@@ -462,7 +520,9 @@ def build_engine_config(model: ModelConfig, model_path: Optional[str] = None, **
                                  num_speculative_tokens=spec.get("num_speculative_tokens", 0),
                                  prompt_lookup_max=spec.get("prompt_lookup_max", 4),
                                  prompt_lookup_min=spec.get("prompt_lookup_min", 2))
-    cfg = EngineConfig(model=model, cache=cache, parallel=par, scheduler=sched,
+    max_loras, max_rank = kw.pop("max_loras", 8), kw.pop("max_lora_rank", 16)
+    adapters = AdapterConfig(max_loras if kw.pop("enable_lora", False) else 0, max_rank)
+    cfg = EngineConfig(model=model, cache=cache, adapters=adapters, parallel=par, scheduler=sched,
                        compilation=comp or CompilationConfig(), kv_transfer=kvt,
                        speculative=spec or SpeculativeConfig(), model_path=model_path,
                        load_format=kw.pop("load_format", "auto"), seed=kw.pop("seed", 0),

@@ -35,6 +35,8 @@ class SamplingParams:
     # token sequences that must not appear in the output: once the output ends with all but the last
     # token of one of them, that last token cannot be sampled
     bad_words_token_ids: Optional[Sequence[Sequence[int]]] = None
+    # samples drawn from this prompt (offline front end); each has a seed of its own
+    n: int = 1
     # scheduling priority under SchedulerConfig.policy == "priority": lower values are admitted first
     # and preempted last (ties: earlier arrival first)
     priority: int = 0
@@ -72,7 +74,8 @@ class Request:
                  "block_ids", "num_computed_tokens", "arrival_time", "first_token_time",
                  "finish_time", "kv_transfer_params", "eos_token_id", "num_preemptions",
                  "spec_token_ids", "client_index", "num_external_tokens", "_block_hashes",
-                 "_registered_blocks", "logprobs", "prompt_logprobs", "state_slot")
+                 "_registered_blocks", "logprobs", "prompt_logprobs", "state_slot", "adapter", "lora_slot",
+                 "cache_salt", "forks", "fork_source")
 
     def __init__(self, request_id: str, prompt_token_ids: Sequence[int],
                  sampling_params: Optional[SamplingParams] = None,
@@ -85,6 +88,13 @@ class Request:
         self.status = RequestStatus.WAITING
         self.block_ids: List[int] = []
         self.state_slot = -1                  # slot of the recurrent state while running (models that have one)
+        self.adapter: Optional[str] = None    # low-rank adapter: its name and slot, and what tells its blocks apart in the cache
+        self.lora_slot = -1
+        self.cache_salt = b""
+        # further samples of this prompt that wait for its blocks; of such a sample, until it runs: (block, rows) whose
+        # rows it takes into a block of its own
+        self.forks: List["Request"] = []
+        self.fork_source: Optional[Tuple[int, int]] = None
         self.num_computed_tokens = 0
         self.arrival_time = time.monotonic() if arrival_time is None else arrival_time
         self.first_token_time: Optional[float] = None
@@ -161,6 +171,7 @@ class RequestOutput:
     logprobs: Optional[List[Tuple[float, List[Tuple[int, float]]]]] = None    # per output token, when asked for
     text: Optional[str] = None             # decoded output, when a tokenizer is at hand
     prompt_logprobs: Optional[List[Optional[Tuple[float, List[Tuple[int, float]]]]]] = None   # per prompt token
+    others: List["RequestOutput"] = field(default_factory=list)    # the prompt's further samples (SamplingParams.n > 1)
 
     @classmethod
     def from_request(cls, r: Request) -> "RequestOutput":

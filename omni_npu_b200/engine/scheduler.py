@@ -40,6 +40,8 @@ class SchedulerOutput:
     preempted: List[str] = field(default_factory=list)
     finished_req_ids: List[str] = field(default_factory=list)
     kv_connector_metadata: Any = None
+    # cache pages to copy before the step: (source, destination, rows)
+    block_copies: List[Tuple[int, int, int]] = field(default_factory=list)
     step_index: int = 0
     pending_pos: List[int] = field(default_factory=list)   # asynchronous scheduling: output index of each placeholder
 
@@ -64,6 +66,13 @@ class Scheduler:
         # models with recurrent state: every running request owns a slot (as many as it can run at once)
         self.state_pool = StateSlotPool(num_state_slots) if num_state_slots else None
         self.prefix_stats = {"requests": 0, "hit_tokens": 0}
+        # further samples of a prompt take over its blocks when it has been computed; the partly filled one only where the
+        # runner can copy pages (set by the engine)
+        self.can_fork = kv_connector is None and self.state_pool is None and context_parallel_size <= 1
+        self.copies_pages = False
+        self.held: Dict[str, Request] = {}             # samples that wait for their prompt
+        self._fork_release: List[int] = []             # sources of the last step's page copies
+        self.fork_stats = {"requests": 0, "shared_tokens": 0}
         self.waiting: Deque[Request] = deque()
         self.running: List[Request] = []
         self.requests: Dict[str, Request] = {}
@@ -84,6 +93,22 @@ class Scheduler:
             raise ValueError(f"prompt of {req.num_prompt_tokens} tokens does not fit the KV cache "
                              f"({usable} blocks of {self.block_size} tokens)")
         self.requests[req.request_id] = req
+        self._enqueue(req)
+
+    def add_fork(self, req: Request, parent_id: str) -> None:
+        """A request with the prompt of another one: it waits until that prompt has been computed and then shares its
+        blocks, computing the last token alone.  Without such a parent, or where blocks cannot be shared, an ordinary
+        request."""
+        parent = self.requests.get(parent_id)
+        if (not self.can_fork or parent is None or parent.is_finished or parent.num_computed_tokens >= parent.num_prompt_tokens
+                or parent.prompt_token_ids != req.prompt_token_ids or parent.adapter != req.adapter
+                or req.sampling_params.prompt_logprobs is not None or parent.request_id in self.held):
+            return self.add_request(req)
+        self.requests[req.request_id] = req
+        self.held[req.request_id] = req
+        parent.forks.append(req)
+
+    def _enqueue(self, req: Request) -> None:
         if self.cfg.policy == "priority":
             # keep the queue ordered by (priority, arrival): behind every request that is at least as urgent
             key = (req.sampling_params.priority, req.arrival_time)
@@ -106,14 +131,72 @@ class Scheduler:
             self.running.remove(req)
         elif req in self.waiting:
             self.waiting.remove(req)
+        elif self.held.pop(req.request_id, None) is not None:
+            for parent in self.requests.values():
+                if req in parent.forks:
+                    parent.forks.remove(req)
+        if req.forks:
+            # its samples wait for a prompt that will not be computed: the first of them takes its place
+            first, *rest = req.forks
+            req.forks = []
+            first.forks = rest
+            del self.held[first.request_id]
+            self._enqueue(first)
         self._release(req)
 
     def has_unfinished(self) -> bool:
-        return bool(self.waiting or self.running)
+        return bool(self.waiting or self.running or self.held)
 
     @property
     def num_unfinished(self) -> int:
-        return len(self.waiting) + len(self.running)
+        return len(self.waiting) + len(self.running) + len(self.held)
+
+    # ------------------------------------------------- several samples of one prompt
+    def _fork_prompt(self, parent: Request) -> None:
+        """The prompt of ``parent`` has been computed: its further samples take its blocks over and may be admitted.  They share
+        the whole blocks; of the last one they get a copy of the rows before the prompt's last token, which
+        each computes itself (it writes there, and its logits are what the sample is drawn from)."""
+        forks, parent.forks = parent.forks, []
+        front = self.cfg.policy != "priority"          # they arrived with their parent, before what waits now
+        full, rows = divmod(parent.num_prompt_tokens - 1, self.block_size)
+        for req in reversed(forks) if front else forks:
+            del self.held[req.request_id]
+            req.block_ids = parent.block_ids[:full]
+            self.pool.share(req.block_ids)
+            req.num_computed_tokens = full * self.block_size
+            if rows and self.copies_pages:
+                req.fork_source = (parent.block_ids[full], rows)
+                self.pool.share([parent.block_ids[full]])
+                req.num_computed_tokens += rows
+            self.fork_stats["requests"] += 1
+            self.fork_stats["shared_tokens"] += req.num_computed_tokens
+            if front:
+                self.waiting.appendleft(req)
+            else:
+                self._enqueue(req)
+
+    def _release_fork_sources(self) -> None:
+        """The last step's page copies have been launched: what they read may be given out again."""
+        if self._fork_release:
+            self.pool.free(self._fork_release)
+            self._fork_release = []
+
+    def _drop_fork_source(self, req: Request) -> None:
+        if req.fork_source is not None:
+            self.pool.free([req.fork_source[0]])
+            req.fork_source = None
+
+    def _drop_waiting_forks(self) -> bool:
+        """Take the shared blocks back from samples that wait for admission (they compute the prompt then)."""
+        dropped = False
+        for req in self.waiting if self.can_fork else ():
+            if req.block_ids or req.fork_source is not None:
+                dropped = True
+                self._drop_fork_source(req)
+                self.pool.free(req.block_ids)
+                req.block_ids = []
+                req.num_computed_tokens = 0
+        return dropped
 
     # ---------------------------------------------------------------- blocks
     def _ensure_blocks(self, req: Request, total_tokens: int) -> bool:
@@ -152,7 +235,8 @@ class Scheduler:
         if usable <= 0 or req.sampling_params.prompt_logprobs is not None:
             return False
         toks = req.all_token_ids
-        req._block_hashes = chain_block_hashes(toks, bs, getattr(req, "_block_hashes", None), upto_blocks=usable)
+        req._block_hashes = chain_block_hashes(toks, bs, getattr(req, "_block_hashes", None), upto_blocks=usable,
+                                               salt=req.cache_salt)
         hit = self.pool.match_prefix(req._block_hashes[:usable])
         self.prefix_stats["requests"] += 1
         if not hit:
@@ -181,7 +265,8 @@ class Scheduler:
         if nfull <= done or nfull > len(req.block_ids):
             return
         from .block_manager import chain_block_hashes
-        hashes = chain_block_hashes(req.all_token_ids, bs, getattr(req, "_block_hashes", None), upto_blocks=nfull)
+        hashes = chain_block_hashes(req.all_token_ids, bs, getattr(req, "_block_hashes", None), upto_blocks=nfull,
+                                    salt=req.cache_salt)
         req._block_hashes = hashes
         upto = min(len(hashes), nfull)
         for i in range(done, upto):
@@ -207,6 +292,7 @@ class Scheduler:
             self.pool.park(req.request_id, req.block_ids, delay)
         else:
             self.pool.free(req.block_ids)
+        self._drop_fork_source(req)
         req.block_ids = []
         self._release_state(req)
         self._finished_since_last.append(req.request_id)
@@ -295,6 +381,7 @@ class Scheduler:
         self._step += 1
         out = SchedulerOutput(step_index=self._step)
         self.pool.expire_parked()
+        self._release_fork_sources()
         if self.kv_connector is not None:
             for rid in self.kv_connector.take_released_requests():
                 self.pool.release_parked(rid)
@@ -338,6 +425,9 @@ class Scheduler:
                 while not fits:
                     victim = self.running[-1]
                     if victim is req:
+                        if self._drop_waiting_forks():
+                            fits = self._ensure_blocks(req, req.num_computed_tokens + n)
+                            continue
                         if len(self.running) == 1 and not prefill:
                             raise RuntimeError("KV cache too small for a single sequence")
                         self.preempt_for_recompute(req)
@@ -410,6 +500,11 @@ class Scheduler:
                 break
             self.waiting.popleft()
             self._admit(req)
+            if req.fork_source is not None:
+                block, rows = req.fork_source
+                out.block_copies.append((block, req.block_ids[req.num_computed_tokens // self.block_size], rows))
+                self._fork_release.append(block)
+                req.fork_source = None
             prefill.append(ScheduledSeq(req, req.num_computed_tokens, n, n == remaining))
             budget -= n
         if prefill:
@@ -436,6 +531,8 @@ class Scheduler:
             drafts = req.spec_token_ids[: max(0, room)] if req.spec_token_ids else []
             while not self._ensure_blocks(req, req.num_tokens + len(drafts)):
                 victim = self._preempt_one(protect=req)
+                if victim is None and self._drop_waiting_forks():
+                    continue
                 if victim is None:
                     raise RuntimeError("KV cache too small for a single sequence")
                 out.preempted.append(victim.request_id)
@@ -449,6 +546,8 @@ class Scheduler:
             out.kind = "spec_decode" if spec else "decode"
             out.seqs = decode
             out.num_tokens = sum(s.num_new_tokens for s in decode)
+        elif not self.running and not out.preempted and self._drop_waiting_forks():
+            return self.schedule()                     # the blocks that they held back were all that was missing
         self._finish_output(out)
         return out
 
@@ -525,6 +624,7 @@ class Scheduler:
         finished in this step."""
         finished: List[Request] = []
         now = time.monotonic() if now is None else now
+        self._release_fork_sources()
         for idx, (seq, tok) in enumerate(zip(out.seqs, sampled)):
             req = seq.request
             if req.is_finished:
@@ -540,6 +640,8 @@ class Scheduler:
                 req.num_computed_tokens = seq.start + seq.num_new_tokens
             req.spec_token_ids = []
             self._register_full_blocks(req)
+            if req.forks and req.num_computed_tokens >= req.num_prompt_tokens:
+                self._fork_prompt(req)
             if not seq.samples:
                 continue
             done = False

@@ -210,6 +210,7 @@ class LlamaModel(nn.Module):
 
 
 class LlamaForCausalLM(nn.Module):
+    supports_adapters = True
     stacked_params_mapping = [
         # (fused parameter, checkpoint name, shard id)
         (".qkv_proj", ".q_proj", "q"), (".qkv_proj", ".k_proj", "k"), (".qkv_proj", ".v_proj", "v"),

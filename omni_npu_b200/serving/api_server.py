@@ -66,9 +66,10 @@ class EngineLoop:
         self.counters = {"requests": 0, "finished": 0, "output_tokens": 0, "steps": 0}
 
     def submit(self, prompt_ids: List[int], sp: SamplingParams, kv_transfer_params=None,
-               stop: Optional[List[str]] = None) -> str:
+               stop: Optional[List[str]] = None, adapter: Optional[str] = None, fork_of: Optional[str] = None) -> str:
         """``stop``: strings that end the request when they appear in its decoded output (needs
-        ``self.tokenizer``); the answer's text is cut before the first of them."""
+        ``self.tokenizer``); the answer's text is cut before the first of them.  ``adapter``, ``fork_of``: as in
+        ``LLMEngine.add_request``."""
         self.engine.validate_sampling_params(sp)        # ValueError -> HTTP 400, before anything is queued
         if stop and self.tokenizer is None:
             raise ValueError("stop strings need a tokenizer (use stop_token_ids on a server without one)")
@@ -78,10 +79,15 @@ class EngineLoop:
         with self.lock:
             self.waiters[rid] = slot
             if self.group is None:
-                self.engine.add_request(prompt_ids, sp, request_id=rid, kv_transfer_params=kv_transfer_params)
+                try:
+                    self.engine.add_request(prompt_ids, sp, request_id=rid, kv_transfer_params=kv_transfer_params,
+                                            adapter=adapter, fork_of=fork_of)
+                except ValueError:
+                    del self.waiters[rid]
+                    raise
                 slot["request"] = self.engine.scheduler.requests[rid]
             else:                                   # added on every rank by the next broadcast
-                self._new.append((rid, list(prompt_ids), sp, kv_transfer_params))
+                self._new.append((rid, list(prompt_ids), sp, kv_transfer_params, fork_of))
             self.counters["requests"] += 1
         self.wake.set()
         return rid
@@ -175,8 +181,8 @@ class EngineLoop:
     KEEPALIVE_S = 5.0        # idle leaders still broadcast, so followers never sit in a receive for long
 
     def _apply(self, new, aborts) -> None:
-        for rid, prompt_ids, sp, kvp in new:
-            self.engine.add_request(prompt_ids, sp, request_id=rid, kv_transfer_params=kvp)
+        for rid, prompt_ids, sp, kvp, fork_of in new:
+            self.engine.add_request(prompt_ids, sp, request_id=rid, kv_transfer_params=kvp, fork_of=fork_of)
             slot = self.waiters.get(rid)
             if slot is not None:
                 slot["request"] = self.engine.scheduler.requests[rid]
@@ -352,7 +358,28 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
 
     @app.get("/v1/models")
     def models():
-        return {"object": "list", "data": [{"id": model_name, "object": "model"}]}
+        manager = llm.engine.worker.model_runner.adapters
+        return {"object": "list", "data": [{"id": model_name, "object": "model"}]
+                + [{"id": name, "object": "model", "parent": model_name} for name in (manager.slots if manager else ())]}
+
+    @app.post("/v1/load_lora_adapter")
+    def load_adapter(body: Dict[str, Any]):
+        """Load a low-rank adapter: ``lora_name`` as requests will ask for it (``model``), ``lora_path`` its directory."""
+        try:
+            with loop.lock:
+                slot = llm.load_adapter(str(body.get("lora_name") or ""), str(body.get("lora_path") or ""))
+        except (ValueError, KeyError, OSError) as e:
+            raise HTTPException(400, str(e))
+        return {"status": "loaded", "slot": slot}
+
+    @app.post("/v1/unload_lora_adapter")
+    def unload_adapter(body: Dict[str, Any]):
+        try:
+            with loop.lock:
+                llm.unload_adapter(str(body.get("lora_name") or ""))
+        except ValueError as e:
+            raise HTTPException(400, str(e))
+        return {"status": "unloaded"}
 
     @app.get("/metrics")
     def metrics():
@@ -370,16 +397,22 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
                  f"omni_b200_preemptions_total {sch.num_preemptions}",
                  f"omni_b200_prefix_cache_queries_total {sch.prefix_stats['requests']}",
                  f"omni_b200_prefix_cache_hit_tokens_total {sch.prefix_stats['hit_tokens']}",
+                 f"omni_b200_forked_requests_total {sch.fork_stats['requests']}",
+                 f"omni_b200_forked_tokens_total {sch.fork_stats['shared_tokens']}",
                  f"omni_b200_spec_draft_tokens_total {sch.spec_stats['drafted']}",
                  f"omni_b200_spec_accepted_tokens_total {sch.spec_stats['accepted']}",
                  f"omni_b200_failed_steps_total {c.get('failed_steps', 0)}"]
         return PlainTextResponse("\n".join(lines) + "\n")
 
-    def _submit(ids, body) -> str:
+    def _submit(ids, body, fork_of: Optional[str] = None) -> str:
         stop = body.get("stop")
         stop = [stop] if isinstance(stop, str) else list(stop or [])
+        # a request names an adapter as its model; any other name stands for the served model
+        manager = llm.engine.worker.model_runner.adapters
+        adapter = body.get("model") if manager is not None and body.get("model") in manager.slots else None
         try:
-            return loop.submit(ids, sampling_from_body(body, tokenizer), body.get("kv_transfer_params"), stop=stop)
+            return loop.submit(ids, sampling_from_body(body, tokenizer), body.get("kv_transfer_params"), stop=stop,
+                               adapter=adapter, fork_of=fork_of)
         except ValueError as e:
             raise HTTPException(400, str(e))
 
@@ -443,9 +476,11 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
         ids = encode(body.get("prompt"))
         n = _n_choices(body)
         if n > 1:
-            # n independent requests (each draws from its own default seed, or from seed + index)
-            rids = [_submit(ids, dict(body, seed=body["seed"] + i) if body.get("seed") is not None else body)
-                    for i in range(n)]
+            # n requests that share the first one's prompt (each draws from its own default seed, or from seed + index)
+            rids: List[str] = []
+            for i in range(n):
+                rids.append(_submit(ids, dict(body, seed=body["seed"] + i) if body.get("seed") is not None else body,
+                                    rids[0] if rids else None))
             outs = [await _finish(r) for r in rids]
             done = sum(len(o.output_token_ids) for o in outs)
             return JSONResponse({
@@ -545,6 +580,10 @@ def make_parser() -> argparse.ArgumentParser:
                     help="reuse the KV blocks of a cached token prefix for new requests")
     ap.add_argument("--enable-mixed-batches", action="store_true",
                     help="decoding requests ride along in the prefill steps of other requests")
+    ap.add_argument("--enable-lora", action="store_true", help="take low-rank adapters beside the model's weights")
+    ap.add_argument("--max-loras", type=int, default=8, help="adapters loaded at once")
+    ap.add_argument("--max-lora-rank", type=int, default=16)
+    ap.add_argument("--lora-modules", nargs="*", default=[], metavar="NAME=PATH", help="adapters to load at the start")
     ap.add_argument("--compilation-config", type=json.loads, default=None)
     ap.add_argument("--kv-transfer-config", type=json.loads, default=None)
     ap.add_argument("--speculative-config", type=json.loads, default=None)
@@ -577,10 +616,14 @@ def main(argv=None) -> None:
               enable_prefix_caching=args.enable_prefix_caching, scheduling_policy=args.scheduling_policy,
               compilation_config=args.compilation_config, kv_transfer_config=args.kv_transfer_config,
               speculative_config=args.speculative_config, additional_config=args.additional_config,
-              load_format=args.load_format, seed=args.seed)
+              load_format=args.load_format, seed=args.seed, enable_lora=args.enable_lora, max_loras=args.max_loras,
+              max_lora_rank=args.max_lora_rank)
     if args.reasoning_config:
         kw["additional_config"] = dict(kw["additional_config"] or {}, reasoning_config=args.reasoning_config)
     llm = LLM(model=args.model, **kw)
+    for item in args.lora_modules:
+        name, _, path = item.partition("=")
+        llm.load_adapter(name, path)
     tokenizer = None
     tok_dir = args.tokenizer or (args.model if os.path.isdir(args.model) else None)
     if tok_dir:

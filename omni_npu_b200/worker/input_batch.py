@@ -5,7 +5,8 @@ of computed tokens, sampling parameters).  A step's device inputs are built with
 vectorised numpy operations into ONE pinned int32 staging buffer laid out as
 
     [ input_ids | positions | slot_mapping | seq_lens | cu_q | temperature(f32 bits)
-      | top_k | top_p(f32 bits) | sequence of each token | state slots | block_table rows ]
+      | top_k | top_p(f32 bits) | sequence of each token | state slots | adapter slot of each token (engines with
+      adapters) | block_table rows ]
 
 and shipped with a single host-to-device copy.  For every CUDA-graph batch size
 the section offsets are fixed, so the captured graph reads the same device
@@ -41,16 +42,18 @@ class StepLayout:
     next_ids: int = 0
     seq: int = 0
     state: int = 0
+    lora: int = 0
     bt: int = 0
     total: int = 0
 
     @classmethod
-    def make(cls, T: int, S: int, max_blocks: int) -> "StepLayout":
+    def make(cls, T: int, S: int, max_blocks: int, lora: bool = False) -> "StepLayout":
         lay = cls(T, S, max_blocks)
         off = 0
         for name, n in (("ids", T), ("pos", T), ("slot", T), ("seq_lens", S), ("cu_q", S + 1),
                         ("temp", S), ("top_k", S), ("top_p", S), ("seeds", 2 * S),
-                        ("logits_idx", S), ("next_ids", T), ("seq", T), ("state", S), ("bt", S * max_blocks)):
+                        ("logits_idx", S), ("next_ids", T), ("seq", T), ("state", S), ("lora", T if lora else 0),
+                        ("bt", S * max_blocks)):
             off = (off + 3) // 4 * 4           # 16-byte aligned sections
             setattr(lay, name, off)
             off += n
@@ -72,7 +75,8 @@ def default_seed(request_id: str, base_seed: int = 0) -> int:
 
 class InputBatch:
     def __init__(self, max_num_seqs: int, max_model_len: int, block_size: int,
-                 max_num_batched_tokens: int, device: torch.device, cp_world: int = 1, cp_rank: int = 0) -> None:
+                 max_num_batched_tokens: int, device: torch.device, cp_world: int = 1, cp_rank: int = 0,
+                 adapters: bool = False) -> None:
         self.max_num_seqs = max_num_seqs
         self.block_size = block_size
         # decode context parallelism: token p of a sequence is stored on rank p % cp_world at local
@@ -89,9 +93,10 @@ class InputBatch:
         self.top_k = np.zeros(max_num_seqs, dtype=np.int32)
         self.top_p = np.ones(max_num_seqs, dtype=np.float32)
         self.seeds = np.zeros(max_num_seqs, dtype=np.int64)
+        self.adapters = adapters
         self.base_seed = 0              # engine seed, mixed into the default per-request seeds
         cap_T = max(max_num_batched_tokens, max_num_seqs)
-        self.capacity = StepLayout.make(cap_T, max_num_seqs, self.max_blocks)
+        self.capacity = StepLayout.make(cap_T, max_num_seqs, self.max_blocks, adapters)
         pin = device.type == "cuda"
         self.host = torch.zeros(self.capacity.total, dtype=torch.int32, pin_memory=pin)
         self.host_np = self.host.numpy()
@@ -145,7 +150,7 @@ class InputBatch:
 
     # ----------------------------------------------------------------- staging
     def layout_for(self, T: int, S: int) -> StepLayout:
-        return StepLayout.make(T, S, self.max_blocks)
+        return StepLayout.make(T, S, self.max_blocks, self.adapters)
 
     def views(self, lay: StepLayout, buf: torch.Tensor) -> Dict[str, torch.Tensor]:
         """Typed views into ``buf`` (host or device) for a layout."""
@@ -164,6 +169,7 @@ class InputBatch:
             "next_ids": buf[lay.next_ids: lay.next_ids + T],
             "seq": buf[lay.seq: lay.seq + T],
             "state": buf[lay.state: lay.state + S],
+            "lora": buf[lay.lora: lay.lora + (T if self.adapters else 0)],
             "bt": buf[lay.bt: lay.bt + S * mb].view(S, mb),
         }
 
@@ -249,6 +255,9 @@ class InputBatch:
         h[lay.seq: lay.seq + lay.T] = np.arange(lay.T, dtype=np.int32) // q_len
         h[lay.state: lay.state + lay.S] = -1
         h[lay.state: lay.state + n] = np.fromiter((r.state_slot for r in reqs), dtype=np.int32, count=n)
+        if self.adapters:
+            h[lay.lora: lay.lora + lay.T] = -1
+            h[lay.lora: lay.lora + n * q_len] = np.repeat([r.lora_slot for r in reqs], q_len)
         self._fill_sampling(lay, rows, n, [len(r.output_token_ids) for r in reqs])
         bt = h[lay.bt: lay.bt + lay.S * lay.max_blocks].reshape(lay.S, lay.max_blocks)
         bt[:n] = self.block_table[rows]
@@ -285,6 +294,8 @@ class InputBatch:
             h[lay.seq_lens + i] = s.start + q
             h[lay.seq + off: lay.seq + off + q] = i
             h[lay.state + i] = req.state_slot
+            if self.adapters:
+                h[lay.lora + off: lay.lora + off + q] = req.lora_slot
             off += q
             cu[i + 1] = off
             h[lay.logits_idx + i] = off - 1
@@ -332,6 +343,8 @@ class InputBatch:
             h[lay.next_ids + off + q - 1] = req.token_at(nxt) if nxt < req.num_tokens else -1
             h[lay.seq + off: lay.seq + off + q] = i
             h[lay.state + i] = req.state_slot
+            if self.adapters:
+                h[lay.lora + off: lay.lora + off + q] = req.lora_slot
             off += q
             cu[i + 1] = off
             h[lay.logits_idx + i] = off - 1

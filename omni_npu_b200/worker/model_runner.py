@@ -59,11 +59,15 @@ class ModelRunner:
         dcp = config.parallel.decode_context_parallel_size
         self.input_batch = InputBatch(sc.max_num_seqs, sc.max_model_len, config.cache.block_size,
                                       sc.max_num_batched_tokens, device, cp_world=dcp,
-                                      cp_rank=pstate.get_tp_group().rank_in_group if dcp > 1 else 0)
+                                      cp_rank=pstate.get_tp_group().rank_in_group if dcp > 1 else 0,
+                                      adapters=config.adapters.max_loras > 0)
         self.input_batch.base_seed = int(config.seed or 0)
         self.sampler = Sampler(config, device)
         self.rejection_sampler = RejectionSampler(self.sampler)
         self.graphs: Dict[int, CUDAGraphRunner] = {}
+        self.lora_graphs: Dict[int, CUDAGraphRunner] = {}      # the same steps with the requests' adapters
+        self.adapters = None                                   # layers/lora.py manager, when adapters are on
+        self.page_cache: Optional[ops.CacheBlocks] = None      # the cache's tensors as page copies address them
         self.capture_sizes: List[int] = []
         pin = device.type == "cuda"
         self.sampled_host = torch.zeros(max(sc.max_num_seqs, 1), dtype=torch.int32, pin_memory=pin)
@@ -139,6 +143,10 @@ class ModelRunner:
         post = getattr(self.model, "post_load", None)
         if callable(post):
             post()
+        if cfg.adapters.max_loras > 0:
+            from ..layers.lora import AdapterManager
+            self.adapters = AdapterManager(self.model, cfg.adapters.max_loras, cfg.adapters.max_lora_rank, cfg.model.dtype,
+                                           self.device)
         self.model.eval()
         if cfg.speculative.method in ("mtp", "deepseek_mtp") and cfg.speculative.num_speculative_tokens > 0:
             self.mtp = getattr(self.model, "mtp", None)
@@ -229,8 +237,26 @@ class ModelRunner:
 
     def initialize_kv_cache(self, num_blocks: int) -> None:
         self._init_kv_cache_tensors(num_blocks)
+        self.page_cache = self._page_cache()
         if self.kv_connector is not None:
             self.kv_connector.register_kv_caches(self.kv_caches)
+
+    def _page_cache(self) -> Optional[ops.CacheBlocks]:
+        """The cache's tensors for page copies; None when a model's cache is not made of pages of token rows."""
+        tensors: Dict[int, torch.Tensor] = {}
+
+        def collect(item) -> None:
+            if isinstance(item, torch.Tensor):
+                tensors[item.data_ptr()] = item                # (layers may share a tensor)
+            elif isinstance(item, (tuple, list)):
+                for x in item:
+                    collect(x)
+        collect(self.kv_caches)
+        try:
+            cache = ops.CacheBlocks(list(tensors.values()))
+        except ValueError:
+            return None
+        return cache if cache.num_blocks == self.num_blocks and cache.block_size == self.config.cache.block_size else None
 
     # ------------------------------------------------------------- execution
     def _metadata(self, lay: StepLayout, views, is_prefill: bool, num_seqs: int, num_tokens: int,
@@ -247,6 +273,8 @@ class ModelRunner:
         """Model forward + LM head + sampling for the staged step (device side only).
         Returns the sampled tokens [num_samples]; with an MTP head int32 [num_samples, 1 + k]:
         the sampled token and the k drafts for the tokens after it."""
+        if md.extra.get("adapters"):
+            md.extra["lora"] = self.adapters.plan(views["lora"])
         if self.pp_group is not None:
             return self._forward_and_sample_pipeline(views, md, num_samples)
         with set_forward_context(md, self.kv_caches, self.config, states=self.states):
@@ -481,6 +509,8 @@ class ModelRunner:
         [n, max_k + 2 (+k)]: the settled tokens (-1 padded), their count and, with an MTP
         head, the k drafts for the next step."""
         n = len(seqs)
+        if md.extra.get("adapters"):
+            md.extra["lora"] = self.adapters.plan(views["lora"])
         with set_forward_context(md, self.kv_caches, self.config):
             hidden = self.model(views["ids"], views["pos"])
             logits = self.model.compute_logits(hidden)
@@ -703,6 +733,9 @@ class ModelRunner:
         top_v, top_i, picked = top_v.cpu().tolist(), top_i.cpu().tolist(), picked.cpu().tolist()
         return {i: (picked[j], list(zip(top_i[j][: ks[j]], top_v[j][: ks[j]])), rank[j]) for j, i in enumerate(rows)}
 
+    def _uses_adapters(self, seqs) -> bool:
+        return self.adapters is not None and any(s.request.lora_slot >= 0 for s in seqs)
+
     def _pad_decode_size(self, n: int) -> Optional[int]:
         for s in self.capture_sizes:
             if s >= n:
@@ -727,6 +760,8 @@ class ModelRunner:
             self.kv_connector.start_load_kv(out.kv_connector_metadata)
         if out.kind == "idle" or not out.seqs:
             return []
+        if out.block_copies:
+            ops.copy_blocks(self.page_cache, out.block_copies)
         n = len(out.seqs)
         ev = None
         self.last_logprobs = {}
@@ -774,6 +809,7 @@ class ModelRunner:
             views = ib.views(lay, ib.dev)
             max_seq = max(s.start + s.num_new_tokens for s in out.seqs)
             md = self._metadata(lay, views, True, n, T, max_q, max_seq, 0, T, n)
+            md.extra["adapters"] = self._uses_adapters(out.seqs)
             packed = self._forward_and_verify(views, md, out.seqs)
             self.step_counter += max_q
             self._event_stop(ev, "spec_decode")
@@ -796,11 +832,12 @@ class ModelRunner:
             ib.upload(lay)
             ev = self._event_start()
             if padded is not None:
-                sampled = self.graphs[padded].replay()
+                sampled = (self.lora_graphs if self._uses_adapters(out.seqs) else self.graphs)[padded].replay()
             else:
                 views = ib.views(lay, ib.dev)
                 md = self._metadata(lay, views, False, S, S, 1, self.config.scheduler.max_model_len,
                                     1, n, n)
+                md.extra["adapters"] = self._uses_adapters(out.seqs)
                 sampled = self._forward_and_sample(views, md, S)
         else:
             T = out.num_tokens
@@ -812,6 +849,7 @@ class ModelRunner:
             max_seq = max(s.start + s.num_new_tokens for s in out.seqs)
             md = self._metadata(lay, views, True, n, T, max_q, max_seq, 0, T, n)
             md.extra["seq_lens_host"] = [s.start + s.num_new_tokens for s in out.seqs]
+            md.extra["adapters"] = self._uses_adapters(out.seqs)
             if self.pcp_group is not None and T >= 2 * self.pcp_group.world_size:
                 sampled = self._forward_and_sample_pcp(views, out.seqs, T, max_seq)
                 self.step_counter += 1
@@ -902,9 +940,10 @@ class ModelRunner:
                 ids.copy_(torch.where(fb_dev >= 0, src.index_select(0, fb_dev.clamp_min(0)), ids))
         ev = self._event_start()
         if padded is not None:
-            sampled = self.graphs[padded].replay()
+            sampled = (self.lora_graphs if self._uses_adapters(out.seqs) else self.graphs)[padded].replay()
         else:
             md = self._metadata(lay, views, False, S, S, 1, self.config.scheduler.max_model_len, 1, n, n)
+            md.extra["adapters"] = self._uses_adapters(out.seqs)
             sampled = self._forward_and_sample(views, md, S)
         self.step_counter += 1
         self._event_stop(ev, "decode")
@@ -990,6 +1029,7 @@ class ModelRunner:
             h[lay.temp: lay.temp + n_seq] = 0
             h[lay.top_k: lay.top_k + n_seq] = 0
             h[lay.top_p: lay.top_p + n_seq] = np.float32(1.0).view(np.int32)
+            h[lay.lora: lay.lora + (T if ib.adapters else 0)] = -1
             bt = h[lay.bt: lay.bt + n_seq * lay.max_blocks].reshape(n_seq, lay.max_blocks)
             nb = (per + bs * ib.cp_world - 1) // (bs * ib.cp_world)
             bt[:, :nb] = np.arange(nb, dtype=np.int32) % max(1, self.num_blocks)
@@ -997,6 +1037,7 @@ class ModelRunner:
             views = ib.views(lay, ib.dev)
             md = self._metadata(lay, views, True, n_seq, T, per, per, 0, T, n_seq)
             md.extra["seq_lens_host"] = [per] * n_seq
+            md.extra["adapters"] = self.adapters is not None   # (the larger step; no token has an adapter)
             self._forward_and_sample(views, md, n_seq)
         else:
             S = num_tokens
@@ -1029,12 +1070,14 @@ class ModelRunner:
             ib.stage_decode(lay, [])
             ib.upload(lay)
             views = ib.views(lay, ib.dev)
-            md = self._metadata(lay, views, False, S, S, 1, self.config.scheduler.max_model_len, 1, 0, 0)
-            runner = CUDAGraphRunner(lambda v=views, m=md, s=S: self._forward_and_sample(v, m, s),
-                                     self.device, pool)
-            runner.capture(warmup=2)
-            pool = runner.pool
-            self.graphs[S] = runner
+            for graphs in (self.graphs, self.lora_graphs)[: 1 if self.adapters is None else 2]:
+                md = self._metadata(lay, views, False, S, S, 1, self.config.scheduler.max_model_len, 1, 0, 0)
+                md.extra["adapters"] = graphs is self.lora_graphs
+                runner = CUDAGraphRunner(lambda v=views, m=md, s=S: self._forward_and_sample(v, m, s),
+                                         self.device, pool)
+                runner.capture(warmup=2)
+                pool = runner.pool
+                graphs[S] = runner
         torch.cuda.synchronize(self.device)
         self.timings["capture_s"] = time.time() - t0
         logger.info("captured %d decode graphs in %.1f s", len(self.graphs), time.time() - t0)
