@@ -781,40 +781,50 @@ bool share_memory(const Tensor& a, const Tensor& b) {
 }
 
 // y + scale * B (A x) per adapter, or the gated activation of it (a new tensor unless `out` is given).  ranks: int32 [slots,
-// slices + 1], each slot's ranks and the bits of its scale.  sizes: rows of the plan's tiles, largest rank, mean of the joined
-// ranks, activation, then the columns of each slice.
+// slices + 1], each slot's ranks and the bits of its scale.  sizes: slots and rows of the plan's tiles, activation, then of the
+// stack: largest rank, mean of the joined ranks, columns of each slice.
 Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given, const Tensor& a, const Tensor& b,
             const Tensor& ranks, const Tensor& plan, at::IntArrayRef sizes, double act_alpha, double act_limit) {
-  TORCH_CHECK(sizes.size() > 4 && sizes.size() <= 8, "lora: one to four slices");
-  const int64_t rows = sizes[0], max_rank = sizes[1], mean_rank = sizes[2], act = sizes[3], S = (int64_t)sizes.size() - 4;
+  TORCH_CHECK(sizes.size() > 5 && sizes.size() <= 9, "lora: one to four slices");
+  const int64_t rows = sizes[1], act = sizes[2], max_rank = sizes[3], mean_rank = sizes[4], S = (int64_t)sizes.size() - 5;
+  const int64_t* slices = sizes.data() + 5;
   int n[4] = {0, 0, 0, 0};
   int64_t width = 0, padded = 0;
   for (int64_t i = 0; i < S; ++i) {
-    width += n[i] = (int)sizes[4 + i];
-    padded += (sizes[4 + i] + 31) / 32 * 32;
+    width += n[i] = (int)slices[i];
+    padded += (slices[i] + 31) / 32 * 32;
   }
-  const int64_t T = x.size(0), L = ranks.size(0), K = x.dim() == 2 ? x.size(1) : 0;
-  c10::cuda::CUDAGuard guard(x.device());
-  const Tensor out = given.has_value() ? *given : torch::empty({T, act ? sizes[4] : width}, y.options());
-  for (const Tensor* t : {&x, &y, &out, &a, &b}) CHECK_CUDA_BF16(*t);
-  for (const Tensor* t : {&x, &y, &out})
-    TORCH_CHECK(t->dim() == 2 && t->size(0) == T && t->stride(1) == 1 && (T < 2 || t->stride(0) % 8 == 0) &&
-                    (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0,
-                "lora: rows of x, y and out are contiguous and start at 16-byte boundaries");
-  TORCH_CHECK(y.size(1) == width && out.size(1) == (act ? sizes[4] : width), "lora: widths of y and out");
-  TORCH_CHECK(a.is_contiguous() && b.is_contiguous() && a.dim() == 2 && b.dim() == 2 && a.size(0) == L && b.size(0) == L &&
-                  a.size(1) == S * max_rank * ((K + 31) / 32 * 32) && b.size(1) == padded * max_rank,
-              "lora: factors [slots, slices * rank * K] and [slots, columns * rank], K and columns in whole 32");
+  TORCH_CHECK_VALUE(x.dim() == 2 && y.dim() == 2 && x.size(0) == y.size(0) && y.size(1) == width,
+                    "lora: x ", x.sizes(), " and y ", y.sizes(), " do not fit a projection to ", width, " columns");
+  const int64_t T = x.size(0), L = ranks.size(0), K = x.size(1);
+  for (const Tensor* t : {&x, &y, &a, &b})
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kBFloat16, "lora: x, y and the factors are bf16");
+  for (const Tensor* t : {&y, &a, &b, &ranks, &plan})
+    TORCH_CHECK_VALUE(t->device() == x.device(), "lora: tensors on ", x.device(), " and ", t->device());
+  TORCH_CHECK_VALUE(a.is_contiguous() && b.is_contiguous() && a.dim() == 2 && b.dim() == 2 && a.size(0) == L && b.size(0) == L &&
+                        a.size(1) == S * max_rank * ((K + 31) / 32 * 32) && b.size(1) == padded * max_rank,
+                    "lora: ", K, " columns of x do not fit the stack's factors");
   CHECK_I32(ranks);
   CHECK_I32(plan);
   const int64_t at = lora_tiles_at(T), max_tiles = lora_max_tiles(T, L, rows);
   TORCH_CHECK(ranks.dim() == 2 && ranks.size(1) == S + 1, "lora: ranks int32 [slots, slices + 1]");
-  TORCH_CHECK(plan.numel() == at + 4 * max_tiles && max_tiles <= 65535, "lora: plan of another step, or of too many tokens");
+  TORCH_CHECK_VALUE(sizes[0] == L && plan.numel() == std::max<int64_t>(at + 4 * max_tiles, 4),
+                    "lora: a plan of other tokens or slots than ", T, " and ", L);
+  TORCH_CHECK_VALUE(max_tiles <= 65535, "lora: ", T, " tokens are too many at once");
+  c10::cuda::CUDAGuard guard(x.device());
+  const int64_t cols = act ? slices[0] : width;
+  const Tensor out = given.has_value() ? *given : torch::empty({T, cols}, y.options());
+  for (const Tensor* t : {&x, &y, &out})
+    TORCH_CHECK_VALUE(t->stride(1) == 1 && (T < 2 || t->stride(0) % 8 == 0) && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0,
+                      "lora: rows of x, y and out are contiguous and start at 16-byte boundaries");
   if (given.has_value()) {
-    TORCH_CHECK(!share_memory(out, x), "lora: out shares memory with x");
-    TORCH_CHECK(!share_memory(out, y) || (act == 0 && out.data_ptr() == y.data_ptr() && (T < 2 || out.stride(0) == y.stride(0))),
-                "lora: out is y itself or shares no memory with it");
-    TORCH_CHECK(T < 2 || out.stride(0) >= out.size(1), "lora: rows of out overlap");
+    TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == T && out.size(1) == cols && out.scalar_type() == at::kBFloat16 &&
+                          out.device() == x.device(),
+                      "lora: out has another shape, type or device than y");
+    TORCH_CHECK_VALUE(!share_memory(out, x), "lora: out shares memory with x");
+    TORCH_CHECK_VALUE(!share_memory(out, y) || (act == 0 && out.data_ptr() == y.data_ptr() && (T < 2 || out.stride(0) == y.stride(0))),
+                      "lora: out is y itself or shares no memory with it");
+    TORCH_CHECK_VALUE(T < 2 || out.stride(0) >= out.size(1), "lora: rows of out overlap");
   }
   if (T == 0) return out;
   const Tensor h = torch::empty(

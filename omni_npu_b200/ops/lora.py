@@ -63,7 +63,7 @@ class LoraStack:
         self.device = self.a.device
         self._ranks = [[0] * len(slices) for _ in range(num_slots)]
         self._scales = [0.0] * num_slots
-        self.mean_rank = 0
+        self.sizes = [self.max_rank, 0, *slices]
 
     def load(self, slot: int, a: Sequence[Optional[torch.Tensor]], b: Sequence[Optional[torch.Tensor]],
              scale: float = 1.0) -> None:
@@ -140,7 +140,8 @@ class LoraStack:
     def _set_ranks(self, slot: int, ranks) -> None:
         self._ranks[slot] = ranks
         used = [sum(r) for r in self._ranks if any(r)]
-        self.mean_rank = sum(used) // max(1, len(used))        # of the loaded adapters, the slices' together: only speed depends on it
+        # largest rank; mean of the loaded adapters' ranks, the slices' together (only speed depends on it); slices
+        self.sizes = [self.max_rank, sum(used) // max(1, len(used)), *self.slices]
 
     def _check_slot(self, slot: int) -> None:
         if not 0 <= slot < self.num_slots:
@@ -201,33 +202,34 @@ def _check(what: str, y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: 
 
 
 def _launch(y, x, stack: LoraStack, plan: LoraPlan, out, kind, alpha, limit) -> torch.Tensor:
-    _count(2 if plan.num_tokens else 0)
-    return _C().lora(x, y, out, stack.a, stack.b, stack.ranks, plan.buffer,
-                     [plan.rows, stack.max_rank, stack.mean_rank, kind, *stack.slices], alpha, limit)
+    if plan.num_tokens:
+        _count(2)
+    return _C().lora(x, y, out, stack.a, stack.b, stack.ranks, plan.buffer, [plan.num_slots, plan.rows, kind] + stack.sizes,
+                     alpha, limit)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan,
              out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``y + scale * B (A x)`` with the factors of each token's adapter: y [T, sum(slices)] is the shared product of
     x [T, in_features].  ``out`` may be ``y`` itself (rows without an adapter are then not touched)."""
-    _check("lora_add", y, x, stack, plan)
     if stack.interleaved:
         raise ValueError("lora_add: the stack's columns are interleaved (lora_gated)")
+    if x.is_cuda and plan.buffer is not None:
+        return _launch(y, x, stack, plan, out, 0, 0.0, 0.0)
+    _check("lora_add", y, x, stack, plan)
     if out is not None and (out.shape != y.shape or out.dtype != y.dtype or out.device != y.device):
         raise ValueError("lora_add: out has another shape, type or device than y")
-    if not x.is_cuda:
-        z = ref.lora_sum(y, x, stack, plan.slots).to(y.dtype)
-        return z if out is None else out.copy_(z)
-    return _launch(y, x, stack, plan, out, 0, 0.0, 0.0)
+    z = ref.lora_sum(y, x, stack, plan.slots).to(y.dtype)
+    return z if out is None else out.copy_(z)
 
 
 def lora_gated(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan, act=SILU) -> torch.Tensor:
     """``act(gate) * up`` of z = y + scale * B (A x), y [T, 2 I] being the shared gate / up product without its activation
     (columns in alternating groups of eight, an ``interleaved`` stack): [T, I].  ``act`` as in :func:`gemm`."""
-    _check("lora_gated", y, x, stack, plan)
     if not stack.interleaved:
         raise ValueError("lora_gated: the stack's columns are not interleaved")
-    if not x.is_cuda:
-        z = ref.lora_sum(y, x, stack, plan.slots).view(y.shape[0], -1, 2, 8)
-        return ref.gated_act(z[:, :, 0], z[:, :, 1], act).reshape(y.shape[0], -1).to(y.dtype)
-    return _launch(y, x, stack, plan, None, *_act_kind(True, act))
+    if x.is_cuda and plan.buffer is not None:
+        return _launch(y, x, stack, plan, None, *_act_kind(True, act))
+    _check("lora_gated", y, x, stack, plan)
+    z = ref.lora_sum(y, x, stack, plan.slots).view(y.shape[0], -1, 2, 8)
+    return ref.gated_act(z[:, :, 0], z[:, :, 1], act).reshape(y.shape[0], -1).to(y.dtype)
