@@ -470,10 +470,10 @@ __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const
 // follow one another).  Few rows: B comes through the ring as well, 32 ranks a stage.
 static constexpr int kExpandThreads = 128;
 
-template <bool MANY, int ACT>
-__global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const LoraParams p) {
+template <bool MANY, int ACT, bool PAIRS>
+__global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_kernel(const LoraParams p) {
   constexpr bool GATED = ACT != kActNone;
-  constexpr int BM = MANY ? 64 : 16, STEP = 4, D = 4, STAGE = MANY ? 2048 : 2048 + 4096;
+  constexpr int BM = MANY ? 64 : 16, STEP = 4, D = PAIRS ? 6 : 4, STAGE = MANY ? 2048 : 2048 + 4096;
   constexpr int GW = GATED ? 32 : 64;                                  // columns of a slice in a group
   extern __shared__ __align__(128) char smem[];
   __shared__ long long y_row[BM], out_row[BM];                         // where a row of the tile starts; out_row -1: none
@@ -635,30 +635,8 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
     get = get + STAGE == ring + D * STAGE ? ring : get + STAGE;
     return st;
   };
-  // rows m of group gi: z in `acc`
-  auto compute = [&](float (&acc)[8][4], int gi, int m) {
-    // step k of h times its B
-    auto multiply = [&](int k, const uint4& p0, const uint4& p1, const uint4& q0, const uint4& q1) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (GATED && k >= (s ? k1 : k0)) continue;
-        const uint4 &v = s ? q0 : p0, &w = s ? q1 : p1;
-        uint32_t hi[4], lo[4];
-        const uint32_t at = hf + m * m_step + k * 32 + (GATED && s ? r0 * 2 : 0);
-        ldmatrix4(hi, at);
-        ldmatrix4(lo, at + lo_at);
-        float(*c)[4] = acc + 4 * s;
-        mma_bf16(c[0], hi[0], hi[1], hi[2], hi[3], v.x, v.y);
-        mma_bf16(c[1], hi[0], hi[1], hi[2], hi[3], v.z, v.w);
-        mma_bf16(c[2], hi[0], hi[1], hi[2], hi[3], w.x, w.y);
-        mma_bf16(c[3], hi[0], hi[1], hi[2], hi[3], w.z, w.w);
-        mma_bf16(c[0], lo[0], lo[1], lo[2], lo[3], v.x, v.y);
-        mma_bf16(c[1], lo[0], lo[1], lo[2], lo[3], v.z, v.w);
-        mma_bf16(c[2], lo[0], lo[1], lo[2], lo[3], w.x, w.y);
-        mma_bf16(c[3], lo[0], lo[1], lo[2], lo[3], w.z, w.w);
-      }
-    };
-    uint32_t st = next();
+  // the accumulators of 16 rows, from a stage of the ring
+  auto start = [&](float (&acc)[8][4], uint32_t st) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -671,43 +649,26 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
           acc[4 * s + j][2 * i + 1] = hi_f(w[j]);
         }
       }
-    if constexpr (MANY) {
-      copy();
-      const bool more = m + 1 == ms && gi + STEP < gb;
-      if (ks == 1) {
-        multiply(0, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
-        if (more) load_b(bv[0], gi + STEP, 0);
-      } else if (ks == 2) {
-        multiply(0, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
-        multiply(1, bv[1][0], bv[1][1], bv[1][2], bv[1][3]);
-        if (more) {
-          load_b(bv[0], gi + STEP, 0);
-          load_b(bv[1], gi + STEP, 1);
-        }
-      } else {
-        for (int k = 0; k < ks; k += 2) {
-          // the registers take the steps after these as soon as they have been used
-          const bool tail = k + 2 >= ks;
-          const int ng = tail && more ? gi + STEP : gi, nk = tail ? 0 : k + 2;
-          multiply(k, bv[0][0], bv[0][1], bv[0][2], bv[0][3]);
-          load_b(bv[0], ng, nk);
-          if (k + 1 < ks) multiply(k + 1, bv[1][0], bv[1][1], bv[1][2], bv[1][3]);
-          load_b(bv[1], ng, nk + 1);
-        }
-      }
-    } else {
-      for (int k = 0;;) {
+  };
+  // step k of h of rows m times its B
+  auto multiply = [&](float (&acc)[8][4], int m, int k, const uint4& p0, const uint4& p1, const uint4& q0, const uint4& q1) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (k + u < ks) {
-            const uint32_t at = st + 2048 + u * 2048;
-            multiply(k + u, lds16(at), lds16(at + 512), lds16(at + 1024), lds16(at + 1536));
-          }
-        copy();
-        k += 2;
-        if (k >= ks) break;
-        st = next();
-      }
+    for (int s = 0; s < 2; ++s) {
+      if (GATED && k >= (s ? k1 : k0)) continue;
+      const uint4 &v = s ? q0 : p0, &w = s ? q1 : p1;
+      uint32_t hi[4], lo[4];
+      const uint32_t at = hf + m * m_step + k * 32 + (GATED && s ? r0 * 2 : 0);
+      ldmatrix4(hi, at);
+      ldmatrix4(lo, at + lo_at);
+      float(*c)[4] = acc + 4 * s;
+      mma_bf16(c[0], hi[0], hi[1], hi[2], hi[3], v.x, v.y);
+      mma_bf16(c[1], hi[0], hi[1], hi[2], hi[3], v.z, v.w);
+      mma_bf16(c[2], hi[0], hi[1], hi[2], hi[3], w.x, w.y);
+      mma_bf16(c[3], hi[0], hi[1], hi[2], hi[3], w.z, w.w);
+      mma_bf16(c[0], lo[0], lo[1], lo[2], lo[3], v.x, v.y);
+      mma_bf16(c[1], lo[0], lo[1], lo[2], lo[3], v.z, v.w);
+      mma_bf16(c[2], lo[0], lo[1], lo[2], lo[3], w.x, w.y);
+      mma_bf16(c[3], lo[0], lo[1], lo[2], lo[3], w.z, w.w);
     }
   };
   auto store = [&](const float (&acc)[8][4], int gi, int m) {
@@ -732,20 +693,74 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_kernel(const Lo
       if (!GATED && at >= 0 && left > 32) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
     }
   };
-  for (int gi = ga; gi < gb; gi += STEP)
-    for (int m = 0; m < ms; ++m) {
-      float acc[8][4];
-      compute(acc, gi, m);
-      store(acc, gi, m);
+  for (int gi = ga; gi < gb; gi += STEP) {
+    const bool more = gi + STEP < gb;
+    if constexpr (PAIRS) {
+      // 32 rows at a time for every step's B, whose registers take the steps after it as soon as it has been used
+      for (int m = 0; m < ms; m += 2) {
+        const bool two = m + 1 < ms, last = m + 2 >= ms;
+        float acc[2][8][4];
+        start(acc[0], next());
+        copy();
+        if (two) {
+          start(acc[1], next());
+          copy();
+        }
+        for (int k = 0; k < ks; k += 2) {
+          const bool tail = k + 2 >= ks;
+          const int ng = tail && last && more ? gi + STEP : gi, nk = tail ? 0 : k + 2;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (k + u < ks) {
+              multiply(acc[0], m, k + u, bv[u][0], bv[u][1], bv[u][2], bv[u][3]);
+              if (two) multiply(acc[1], m + 1, k + u, bv[u][0], bv[u][1], bv[u][2], bv[u][3]);
+            }
+            load_b(bv[u], ng, nk + u);
+          }
+        }
+        store(acc[0], gi, m);
+        if (two) store(acc[1], gi, m + 1);
+      }
+    } else {
+      for (int m = 0; m < ms; ++m) {
+        float acc[8][4];
+        uint32_t st = next();
+        start(acc, st);
+        if constexpr (MANY) {
+          copy();
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (u < ks) multiply(acc, m, u, bv[u][0], bv[u][1], bv[u][2], bv[u][3]);
+          if (m + 1 == ms && more)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              if (u < ks) load_b(bv[u], gi + STEP, u);
+        } else {
+          for (int k = 0;;) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              if (k + u < ks) {
+                const uint32_t at = st + 2048 + u * 2048;
+                multiply(acc, m, k + u, lds16(at), lds16(at + 512), lds16(at + 1024), lds16(at + 1536));
+              }
+            copy();
+            k += 2;
+            if (k >= ks) break;
+            st = next();
+          }
+        }
+        store(acc, gi, m);
+      }
     }
+  }
 }
 
 static constexpr int kShrinkFewSmem = kFewWarps * kFewRing, kShrinkManySmem = kStages * kStageBytes, kExpandSmem = 168 * 1024;
 
-template <bool MANY, int ACT>
+template <bool MANY, int ACT, bool PAIRS>
 static int launch_lora(const LoraParams& p, unsigned tiles, unsigned chunks, unsigned blocks, cudaStream_t stream) {
   auto shrink = MANY ? lora_shrink_many_kernel : lora_shrink_few_kernel;
-  auto expand = lora_expand_kernel<MANY, ACT>;
+  auto expand = lora_expand_kernel<MANY, ACT, PAIRS>;
   static DeviceOnce once;
   int dev;
   if (once.needed(&dev)) {
@@ -755,7 +770,7 @@ static int launch_lora(const LoraParams& p, unsigned tiles, unsigned chunks, uns
       return -3;
     once.mark(dev);
   }
-  const size_t smem = 4 * 4 * (MANY ? 2048 : 6144) + 2 * sizeof(__nv_bfloat16) * (MANY ? 64 : 16) * p.h_pitch;
+  const size_t smem = 4 * (PAIRS ? 6 : 4) * (MANY ? 2048 : 6144) + 2 * sizeof(__nv_bfloat16) * (MANY ? 64 : 16) * p.h_pitch;
   const dim3 grid(p.parts, chunks, tiles);
   if (smem > kExpandSmem || tiles > 65535) return -2;
   if (launch_pdl(shrink, grid, dim3(MANY ? kManyThreads : kFewThreads), MANY ? kShrinkManySmem : kShrinkFewSmem, stream, MANY ? p.parts : 1, p) !=
@@ -765,8 +780,11 @@ static int launch_lora(const LoraParams& p, unsigned tiles, unsigned chunks, uns
 }
 
 template <int ACT>
-static int launch_lora(const LoraParams& p, bool many, unsigned tiles, unsigned chunks, unsigned blocks, cudaStream_t stream) {
-  return many ? launch_lora<true, ACT>(p, tiles, chunks, blocks, stream) : launch_lora<false, ACT>(p, tiles, chunks, blocks, stream);
+static int launch_lora(const LoraParams& p, bool many, int max_rank, unsigned tiles, unsigned chunks, unsigned blocks,
+                       cudaStream_t stream) {
+  if (!many) return launch_lora<false, ACT, false>(p, tiles, chunks, blocks, stream);
+  return max_rank > 32 ? launch_lora<true, ACT, true>(p, tiles, chunks, blocks, stream)
+                       : launch_lora<true, ACT, false>(p, tiles, chunks, blocks, stream);
 }
 
 // Parts of K that a step's h is summed from, a CTA each (many rows: of a cluster).  Few rows (tiles of 16): as many as the slots
@@ -843,8 +861,8 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   const unsigned chunks = (p.h_width + kLoraChunk * 8 - 1) / (kLoraChunk * 8), tiles_n = static_cast<unsigned>(max_tiles);
   p.parts = lora_parts(K, rows, max_tiles, num_slots, (mean_rank + kLoraChunk * 8 - 1) / (kLoraChunk * 8));
   p.h_pitch = (gated ? 2 : 1) * max_rank + 8;    // eight rows of 16 bytes are in banks of their own
-  // column groups of a CTA: four rounds of the resident CTAs in all, or for few rows one, where a CTA's start is most of its
-  // time (128 adapters of rank 16, 4096 columns: 7.7 us, with four rounds 12.9); a group a warp at least
+  // column groups of a CTA: two rounds of the resident CTAs in all, or for few rows one, where a CTA's start is most of its
+  // time (128 adapters of rank 16, 4096 columns: 7.7 us, with two rounds 9.6); a group a warp at least
   int groups = 0;
   for (int s = 0; s < kLoraMaxSlices; ++s) {
     p.n[s] = s < slices ? n[s] : 0;
@@ -852,16 +870,16 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
     if (!gated || s == 0) groups += gated ? (p.n[s] + 31) / 32 : (p.n[s] + 63) / 64;
   }
   const int team = 4;
-  const long long want = static_cast<long long>(groups) * max_tiles / (148 * (many ? 16 : 2));
+  const long long want = static_cast<long long>(groups) * max_tiles / (148 * (many ? 8 : 2));
   p.per = static_cast<int>(std::max(1LL, (want + team - 1) / team)) * team;
   unsigned blocks = 0;
   for (int s = 0; s < slices; ++s)
     if (!gated || s == 0) blocks += ((gated ? (n[s] + 31) / 32 : (n[s] + 63) / 64) + p.per - 1) / p.per;
   switch (act) {
-    case kActNone: return launch_lora<kActNone>(p, many, tiles_n, chunks, blocks, stream);
-    case kActSilu: return launch_lora<kActSilu>(p, many, tiles_n, chunks, blocks, stream);
-    case kActClampedGlu: return launch_lora<kActClampedGlu>(p, many, tiles_n, chunks, blocks, stream);
-    case kActGeluTanh: return launch_lora<kActGeluTanh>(p, many, tiles_n, chunks, blocks, stream);
-    default: return launch_lora<kActReluGate>(p, many, tiles_n, chunks, blocks, stream);
+    case kActNone: return launch_lora<kActNone>(p, many, max_rank, tiles_n, chunks, blocks, stream);
+    case kActSilu: return launch_lora<kActSilu>(p, many, max_rank, tiles_n, chunks, blocks, stream);
+    case kActClampedGlu: return launch_lora<kActClampedGlu>(p, many, max_rank, tiles_n, chunks, blocks, stream);
+    case kActGeluTanh: return launch_lora<kActGeluTanh>(p, many, max_rank, tiles_n, chunks, blocks, stream);
+    default: return launch_lora<kActReluGate>(p, many, max_rank, tiles_n, chunks, blocks, stream);
   }
 }
