@@ -17,10 +17,14 @@
 //
 // Tokens are grouped by adapter once a step (lora_plan_kernel: a stable counting sort, then tiles of up to `rows` tokens of one
 // adapter).  Two launches apply the adapters, both bound by what they read and write:
-//   lora_shrink_*_kernel  h: a cluster per (tile, 64 of the joined ranks), its CTAs sharing K
+//   lora_shrink_*_kernel  h: CTAs that share K per (tile, 64 of the joined ranks)
 //   lora_expand_kernel    z: a CTA per (tile, run of column groups)
-// so that many small pieces of work even out adapters of unlike ranks.  The second is launched while the first runs and
-// has its first y and factors at hand by the time h is there.
+// so that many small pieces of work even out adapters of unlike ranks (one cluster per tile for both, h in distributed shared
+// memory, took 56 us where this takes 15: 128 tokens of 31 adapters of ranks 8 to 64).  The second is launched while the first
+// runs and has its first y and factors at hand by the time h is there.  Measured (us, and the time of the bytes at 6.56 TB/s):
+// one token 4.6; 128 tokens of 128 adapters of rank 16, 14336 to 4096 18.3 / 12.4; 8192 tokens of 8, 4096 to 6144 56 / 42;
+// the same to 2 x 14336 with silu, rank 32 167 / 121.  Ranks above some 32 are bound by the matrix instructions and what
+// they read from shared memory: 8192 tokens of rank 64, 4096 to 6144 117 / 42.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -31,13 +35,12 @@
 #include "../common/device_once.h"
 #include "../common/pdl.cuh"
 #include "../common/ptx.cuh"
-#include "../common/ptx.cuh"
 #include "../gemm/gated_act.cuh"
 
 namespace b200 {
 
 static constexpr int kLoraMaxSlices = 4;
-static constexpr int kLoraChunk = 8;             // 8-wide tiles of h in a piece of work
+static constexpr int kLoraChunk = 8;             // 8-wide tiles of h that a CTA computes
 static constexpr int kPlanThreads = 1024;
 
 // ----------------------------------------------------------------------------------------------- grouping
@@ -307,11 +310,14 @@ __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const Lora
 
 // ---- h of many rows: 64 rows of x and 64 of the joined ranks, in slabs of 128 of K through a ring in shared memory, so that
 // what is in flight does not depend on registers.  Warps: two halves of every slab's K, then 32 rows x 32 ranks each (a fragment
-// of x and one of A serve two and two pairs of matrix instructions).
-static constexpr int kManyThreads = 256, kManyRows = 64, kSlab = 128, kStages = 3, kStageBytes = 2 * 64 * kSlab * 2;
+// of x and one of A serve two and two pairs of matrix instructions).  128 rows a CTA, or 128 ranks, halve what is read once more
+// from L2 but were no faster (8192 tokens, K 4096, 48 ranks: 26.2 us, 25.3 so; 192 ranks 60 and 61), nor were 64 of K a slab.
+// The parts of K meet in distributed shared memory: with fp32 parts in global memory that every CTA of the second kernel
+// adds up, 2847 tokens of ranks 33 to 128 took 66 us, 57 so.
+static constexpr int kManyThreads = 256, kManyRows = 64, kSlab = 128, kStages = 3, kStageBytes = 2 * kManyRows * kSlab * 2;
 
 __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const LoraParams p) {
-  constexpr int BM = kManyRows, W = kLoraChunk * 8;
+  constexpr int W = kLoraChunk * 8;
   extern __shared__ __align__(128) char smem[];
   pdl_wait();
   pdl_trigger();
@@ -466,8 +472,9 @@ __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const
 // ---- z: a CTA has a tile's rows and a run of column groups of one slice, 64 columns of y each (gated: 32 of gate and their 32 of
 // up).  A warp takes every fourth group, 16 rows at a time: y, which comes through a ring of the lane's own, starts its
 // accumulators; a lane's results are eight neighbouring columns twice, so y and the result move 16 bytes a lane, 512 of a row
-// by the four warps.  Many rows: B is read into registers once for the 64 rows (up to 32 ranks; above, two steps of 16
-// follow one another).  Few rows: B comes through the ring as well, 32 ranks a stage.
+// by the four warps.  Many rows: up to 32 ranks B stays in registers for the 64 rows; above (PAIRS), every step of 16 ranks
+// is used for 32 rows, and the registers take the step after next meanwhile (8192 tokens of rank 64, 4096 columns: 43.6 us,
+// with 16 rows 47.3).  Few rows: B comes through the ring as well, 32 ranks a stage.
 static constexpr int kExpandThreads = 128;
 
 template <bool MANY, int ACT, bool PAIRS>
@@ -773,8 +780,8 @@ static int launch_lora(const LoraParams& p, unsigned tiles, unsigned chunks, uns
   const size_t smem = 4 * (PAIRS ? 6 : 4) * (MANY ? 2048 : 6144) + 2 * sizeof(__nv_bfloat16) * (MANY ? 64 : 16) * p.h_pitch;
   const dim3 grid(p.parts, chunks, tiles);
   if (smem > kExpandSmem || tiles > 65535) return -2;
-  if (launch_pdl(shrink, grid, dim3(MANY ? kManyThreads : kFewThreads), MANY ? kShrinkManySmem : kShrinkFewSmem, stream, MANY ? p.parts : 1, p) !=
-      cudaSuccess)
+  if (launch_pdl(shrink, grid, dim3(MANY ? kManyThreads : kFewThreads), MANY ? kShrinkManySmem : kShrinkFewSmem, stream,
+                 MANY ? p.parts : 1, p) != cudaSuccess)
     return -3;
   return launch_pdl(expand, dim3(blocks, tiles), dim3(kExpandThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
 }
@@ -822,14 +829,15 @@ extern "C" int b200_lora_plan(const int* slots, int T, int L, int rows, int* ord
                     reinterpret_cast<LoraTile*>(tiles), num_tiles, status) == cudaSuccess ? 0 : -3;
 }
 
-// ranks: [L, slices + 1], a slot's ranks and the bits of its scale.  n: columns of each slice.  h: scratch of b200_lora_scratch_bytes.  max_tiles: tiles that the plan may have, of `rows`
-// tokens each.  max_rank: bound of the ranks; mean_rank: about what a
-// tile's joined ranks are (16 at least).  act: 0 adds, a gated kind of gemm/gated_act.cuh joins gate and up (alternating
+// ranks: [L, slices + 1], a slot's ranks and the bits of its scale.  max_tiles: tiles that the plan may have, of `rows` (16 or 64)
+// tokens each.  h: scratch of b200_lora_scratch_bytes.  n: columns of each slice.  max_rank: bound of the ranks; mean_rank: about
+// what a tile's joined ranks are (16 at least).  act: 0 adds, a gated kind of gemm/gated_act.cuh joins gate and up (alternating
 // groups of eight columns of y).
 extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long long y_stride, void* out, long long out_stride,
-                         const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks, const int* order, const int* tiles, const int* num_tiles, int max_tiles, int rows,
-                         void* h, int T, int num_slots, int K, int slices, const int* n, int max_rank, int mean_rank,
-                         int act, float act_alpha, float act_limit, cudaStream_t stream) {
+                         const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks, const int* order,
+                         const int* tiles, const int* num_tiles, int max_tiles, int rows, void* h, int T, int num_slots, int K,
+                         int slices, const int* n, int max_rank, int mean_rank, int act, float act_alpha, float act_limit,
+                         cudaStream_t stream) {
   using namespace b200;
   if (slices < 1 || slices > kLoraMaxSlices || (K & 7) || max_rank < 16 || mean_rank < 16 || (max_rank & 15) || max_tiles < 1 ||
       (rows != 16 && rows != kManyRows))
@@ -869,9 +877,8 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
     if (p.n[s] & 7) return -1;
     if (!gated || s == 0) groups += gated ? (p.n[s] + 31) / 32 : (p.n[s] + 63) / 64;
   }
-  const int team = 4;
   const long long want = static_cast<long long>(groups) * max_tiles / (148 * (many ? 8 : 2));
-  p.per = static_cast<int>(std::max(1LL, (want + team - 1) / team)) * team;
+  p.per = static_cast<int>(std::max(1LL, (want + 3) / 4)) * 4;
   unsigned blocks = 0;
   for (int s = 0; s < slices; ++s)
     if (!gated || s == 0) blocks += ((gated ? (n[s] + 31) / 32 : (n[s] + 63) / 64) + p.per - 1) / p.per;

@@ -15,9 +15,11 @@ from . import SILU, _C, _act_kind, _count, device_state, ref
 
 MAX_SLOTS, MAX_SLICES, MAX_RANK = 512, 4, 256
 
-# Tokens of one adapter that a cluster of CTAs takes together.  Up to this many tokens a step is a decode batch, whose adapters
-# have few tokens each: tiles of 16, one matrix instruction high.
-FEW_TOKENS, FEW_ROWS, MANY_ROWS = 256, 16, 64
+# Tokens of one adapter that are taken together.  Up to this many tokens of a step: tiles of 16, one matrix instruction high,
+# through kernels that stream the factors; above, tiles of 64.  Us, tiles of 64 / 16: 200 tokens of 32 adapters of rank 16,
+# 4096 to 4096 + 1024 + 1024 13.3 / 9.7, 14336 to 4096 18.2 / 9.0; 700 tokens 15.2 / 15.2 and 18.2 / 13.5; 1000 tokens of 4 of
+# rank 64 22.9 / 34.1 and 28.4 / 26.5.  A row's result does not depend on the rows beside it as long as these are no more.
+FEW_TOKENS, FEW_ROWS, MANY_ROWS = 768, 16, 64
 
 
 def _padded(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
