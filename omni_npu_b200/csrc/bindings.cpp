@@ -781,34 +781,35 @@ bool share_memory(const Tensor& a, const Tensor& b) {
 }
 
 // y + scale * B (A x) per adapter, or the gated activation of it (a new tensor unless `out` is given).  ranks: int32 [slots,
-// slices + 1], each slot's ranks and the bits of its scale.  sizes: slots and rows of the plan's tiles, activation, then of the
-// stack: largest rank, mean of the joined ranks, columns of each slice.
+// slices + 1], each slot's ranks and the bits of its scale.  sizes: of the plan tokens, slots and
+// rows of a tile; activation; of the stack input features, largest rank, mean of the joined ranks, columns of each slice.
 Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given, const Tensor& a, const Tensor& b,
             const Tensor& ranks, const Tensor& plan, at::IntArrayRef sizes, double act_alpha, double act_limit) {
-  TORCH_CHECK(sizes.size() > 5 && sizes.size() <= 9, "lora: one to four slices");
-  const int64_t rows = sizes[1], act = sizes[2], max_rank = sizes[3], mean_rank = sizes[4], S = (int64_t)sizes.size() - 5;
-  const int64_t* slices = sizes.data() + 5;
+  TORCH_CHECK(sizes.size() > 7 && sizes.size() <= 11, "lora: one to four slices");
+  const int64_t rows = sizes[2], act = sizes[3], K = sizes[4], max_rank = sizes[5], mean_rank = sizes[6];
+  const int64_t S = (int64_t)sizes.size() - 7;
+  const int64_t* slices = sizes.data() + 7;
   int n[4] = {0, 0, 0, 0};
   int64_t width = 0, padded = 0;
   for (int64_t i = 0; i < S; ++i) {
     width += n[i] = (int)slices[i];
     padded += (slices[i] + 31) / 32 * 32;
   }
-  TORCH_CHECK_VALUE(x.dim() == 2 && y.dim() == 2 && x.size(0) == y.size(0) && y.size(1) == width,
-                    "lora: x ", x.sizes(), " and y ", y.sizes(), " do not fit a projection to ", width, " columns");
-  const int64_t T = x.size(0), L = ranks.size(0), K = x.size(1);
+  TORCH_CHECK_VALUE(x.dim() == 2 && y.dim() == 2 && x.size(0) == y.size(0) && x.size(1) == K && y.size(1) == width,
+                    "lora: x ", x.sizes(), " and y ", y.sizes(), " do not fit a projection of ", K, " to ", width);
+  const int64_t T = x.size(0), L = ranks.size(0);
   for (const Tensor* t : {&x, &y, &a, &b})
     TORCH_CHECK_VALUE(t->scalar_type() == at::kBFloat16, "lora: x, y and the factors are bf16");
   for (const Tensor* t : {&y, &a, &b, &ranks, &plan})
     TORCH_CHECK_VALUE(t->device() == x.device(), "lora: tensors on ", x.device(), " and ", t->device());
-  TORCH_CHECK_VALUE(a.is_contiguous() && b.is_contiguous() && a.dim() == 2 && b.dim() == 2 && a.size(0) == L && b.size(0) == L &&
+  TORCH_CHECK(a.is_contiguous() && b.is_contiguous() && a.dim() == 2 && b.dim() == 2 && a.size(0) == L && b.size(0) == L &&
                         a.size(1) == S * max_rank * ((K + 31) / 32 * 32) && b.size(1) == padded * max_rank,
-                    "lora: ", K, " columns of x do not fit the stack's factors");
+              "lora: factors [slots, slices * rank * K] and [slots, columns * rank], K and columns in whole 32");
   CHECK_I32(ranks);
   CHECK_I32(plan);
   const int64_t at = lora_tiles_at(T), max_tiles = lora_max_tiles(T, L, rows);
   TORCH_CHECK(ranks.dim() == 2 && ranks.size(1) == S + 1, "lora: ranks int32 [slots, slices + 1]");
-  TORCH_CHECK_VALUE(sizes[0] == L && plan.numel() == std::max<int64_t>(at + 4 * max_tiles, 4),
+  TORCH_CHECK_VALUE(sizes[0] == T && sizes[1] == L && plan.numel() == std::max<int64_t>(at + 4 * max_tiles, 4),
                     "lora: a plan of other tokens or slots than ", T, " and ", L);
   TORCH_CHECK_VALUE(max_tiles <= 65535, "lora: ", T, " tokens are too many at once");
   c10::cuda::CUDAGuard guard(x.device());

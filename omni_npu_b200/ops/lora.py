@@ -65,7 +65,7 @@ class LoraStack:
         self.device = self.a.device
         self._ranks = [[0] * len(slices) for _ in range(num_slots)]
         self._scales = [0.0] * num_slots
-        self.sizes = [self.max_rank, 0, *slices]
+        self.sizes = [in_features, self.max_rank, 0, *slices]
 
     def load(self, slot: int, a: Sequence[Optional[torch.Tensor]], b: Sequence[Optional[torch.Tensor]],
              scale: float = 1.0) -> None:
@@ -142,8 +142,8 @@ class LoraStack:
     def _set_ranks(self, slot: int, ranks) -> None:
         self._ranks[slot] = ranks
         used = [sum(r) for r in self._ranks if any(r)]
-        # largest rank; mean of the loaded adapters' ranks, the slices' together (only speed depends on it); slices
-        self.sizes = [self.max_rank, sum(used) // max(1, len(used)), *self.slices]
+        # input features; largest rank; mean of the loaded adapters' ranks, the slices' together (only speed depends on it); slices
+        self.sizes = [self.in_features, self.max_rank, sum(used) // max(1, len(used)), *self.slices]
 
     def _check_slot(self, slot: int) -> None:
         if not 0 <= slot < self.num_slots:
@@ -206,8 +206,8 @@ def _check(what: str, y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: 
 def _launch(y, x, stack: LoraStack, plan: LoraPlan, out, kind, alpha, limit) -> torch.Tensor:
     if plan.num_tokens:
         _count(2)
-    return _C().lora(x, y, out, stack.a, stack.b, stack.ranks, plan.buffer, [plan.num_slots, plan.rows, kind] + stack.sizes,
-                     alpha, limit)
+    return _C().lora(x, y, out, stack.a, stack.b, stack.ranks, plan.buffer,
+                     [plan.num_tokens, plan.num_slots, plan.rows, kind] + stack.sizes, alpha, limit)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan,

@@ -28,8 +28,8 @@ class CacheBlocks:
             row, heads = t.shape[-1] * size, t.shape[1] if t.dim() == 4 else 1
             head = (t.stride(1) if t.dim() == 4 else t.stride(0)) * size
             if t.stride(-1) != 1 or t.stride(-2) != t.shape[-1] or row % 16 or head % 16 or t.stride(0) * size % 16 \
-                    or t.data_ptr() % 16:
-                raise ValueError("CacheBlocks: rows of a head lie one after another and are multiples of 16 bytes")
+                    or t.data_ptr() % 16 or t.numel() == 0:
+                raise ValueError("CacheBlocks: rows of a head lie one after another and are multiples of 16 bytes, not none")
             desc.append([t.data_ptr(), t.stride(0) * size, head, heads | (row // 16) << 32])
             self._max_vecs = max(self._max_vecs, heads * self.block_size * (row // 16))
         self._desc = torch.tensor(desc, dtype=torch.int64, device=self.device) if first.is_cuda else None

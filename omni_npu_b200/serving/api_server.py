@@ -404,12 +404,15 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
                  f"omni_b200_failed_steps_total {c.get('failed_steps', 0)}"]
         return PlainTextResponse("\n".join(lines) + "\n")
 
+    def _adapter(body) -> Optional[str]:
+        """A request names an adapter as its model; any other name stands for the served model."""
+        manager = llm.engine.worker.model_runner.adapters
+        return body.get("model") if manager is not None and body.get("model") in manager.slots else None
+
     def _submit(ids, body, fork_of: Optional[str] = None) -> str:
         stop = body.get("stop")
         stop = [stop] if isinstance(stop, str) else list(stop or [])
-        # a request names an adapter as its model; any other name stands for the served model
-        manager = llm.engine.worker.model_runner.adapters
-        adapter = body.get("model") if manager is not None and body.get("model") in manager.slots else None
+        adapter = _adapter(body)
         try:
             return loop.submit(ids, sampling_from_body(body, tokenizer), body.get("kv_transfer_params"), stop=stop,
                                adapter=adapter, fork_of=fork_of)
@@ -474,6 +477,7 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
     @app.post("/v1/completions")
     async def completions(body: Dict[str, Any]):
         ids = encode(body.get("prompt"))
+        name = _adapter(body) or model_name
         n = _n_choices(body)
         if n > 1:
             # n requests that share the first one's prompt (each draws from its own default seed, or from seed + index)
@@ -484,19 +488,19 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
             outs = [await _finish(r) for r in rids]
             done = sum(len(o.output_token_ids) for o in outs)
             return JSONResponse({
-                "id": rids[0], "object": "text_completion", "created": int(time.time()), "model": model_name,
+                "id": rids[0], "object": "text_completion", "created": int(time.time()), "model": name,
                 "choices": [_completion_choice(i, o) for i, o in enumerate(outs)],
                 "usage": {"prompt_tokens": len(ids), "completion_tokens": done, "total_tokens": len(ids) + done}})
         rid = _submit(ids, body)
         created = int(time.time())
         if body.get("stream"):
             def chunk(toks, finish):
-                return {"id": rid, "object": "text_completion", "created": created, "model": model_name,
+                return {"id": rid, "object": "text_completion", "created": created, "model": name,
                         "choices": [{"index": 0, "text": decode(toks), "token_ids": toks, "finish_reason": finish}]}
             return StreamingResponse(_stream(rid, chunk), media_type="text/event-stream")
         out = await _finish(rid)
         return JSONResponse({
-            "id": rid, "object": "text_completion", "created": created, "model": model_name,
+            "id": rid, "object": "text_completion", "created": created, "model": name,
             "choices": [_completion_choice(0, out)],
             "usage": {"prompt_tokens": len(ids), "completion_tokens": len(out.output_token_ids),
                       "total_tokens": len(ids) + len(out.output_token_ids)},
@@ -511,6 +515,7 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
             ids = msgs[-1]["content"]                      # token ids in the last message (no tokenizer)
         else:
             raise HTTPException(400, "chat needs a tokenizer with a chat template")
+        name = _adapter(body) or model_name
         rid = _submit(ids, body)
         if body.get("stream"):
             # chat.completion.chunk events: the role first, then the text of the new tokens as they
@@ -523,7 +528,7 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
                 if state["first"]:
                     delta["role"] = "assistant"
                     state["first"] = False
-                return {"id": rid, "object": "chat.completion.chunk", "created": created, "model": model_name,
+                return {"id": rid, "object": "chat.completion.chunk", "created": created, "model": name,
                         "choices": [{"index": 0, "delta": delta, "token_ids": toks, "finish_reason": finish}]}
             return StreamingResponse(_stream(rid, chunk), media_type="text/event-stream")
         out = await _finish(rid)
@@ -540,7 +545,7 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
                                          for tc in info.tool_calls]
                 message["content"] = info.content
         return JSONResponse({
-            "id": rid, "object": "chat.completion", "created": int(time.time()), "model": model_name,
+            "id": rid, "object": "chat.completion", "created": int(time.time()), "model": name,
             "choices": [{"index": 0, "message": message, "finish_reason": out.finish_reason or "stop",
                          # the chat form: one entry per output token with its alternatives
                          "logprobs": None if out.logprobs is None else {"content": [

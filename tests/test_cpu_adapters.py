@@ -215,6 +215,7 @@ def test_the_server_takes_an_adapter_as_model(tmp_path):
         assert [m["id"] for m in client.get("/v1/models").json()["data"]] == ["base", "a"]
         with_a = client.post("/v1/completions", json={**body, "model": "a"}).json()["choices"][0]["token_ids"]
         assert with_a != base
+        assert client.post("/v1/completions", json={**body, "model": "a"}).json()["model"] == "a"
         assert client.post("/v1/completions", json={**body, "model": "base"}).json()["choices"][0]["token_ids"] == base
         three = client.post("/v1/completions", json={**body, "model": "a", "n": 3}).json()["choices"]
         assert [c["token_ids"] for c in three] == [with_a] * 3

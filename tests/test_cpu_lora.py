@@ -99,6 +99,6 @@ def test_copy_blocks_refusals(pairs):
 def test_cache_blocks_refusals():
     t = torch.zeros(6, 2, 4, 8).bfloat16()
     for tensors in ([], [t, t[:5]], [t, torch.zeros(6, 2, 3, 8).bfloat16()], [torch.zeros(6, 2, 4, 4).bfloat16()], [t.transpose(1, 2)],
-                    [torch.zeros(6, 4)], [t[..., :4]]):
+                    [torch.zeros(6, 4)], [t[..., :4]], [torch.zeros(0, 2, 4, 8)], [torch.zeros(6, 2, 0, 8)], [torch.zeros(6, 2, 4, 0)]):
         with pytest.raises(ValueError):
             ops.CacheBlocks(tensors)

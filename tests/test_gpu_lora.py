@@ -180,8 +180,23 @@ def test_refusals_on_the_device():
     for bad_y, bad_x, out in ((y.float(), x, None), (y, x.float(), None), (y, wide[:, 4:68], None), (y, wide[:, 1:65], None),
                               (y.t().contiguous().t(), x, None), (y, wide[:, :64], wide[:, 8:40]),
                               (wide[:, :32], x, wide[:, 8:40])):
-        with pytest.raises((RuntimeError, ValueError)):
+        with pytest.raises(ValueError):
             ops.lora_add(bad_y, bad_x, st, plan, out=out)
+    # a plan of other tokens or slots, x of another width (the buffers' sizes are the same), another device's plan
+    other = ops.LoraStack(2, 16, 56, [32], device=DEV)
+    for t, n in ((5, 2), (7, 2), (6, 1), (6, 3)):
+        with pytest.raises(ValueError):
+            ops.lora_add(y, x, st, ops.lora_plan(torch.zeros(t, dtype=torch.int32, device=DEV), n))
+    with pytest.raises(ValueError):
+        ops.lora_add(y, x, other, plan)
+    with pytest.raises(ValueError):
+        ops.lora_add(y, x, st, ops.lora_plan(torch.zeros(6, dtype=torch.int32), 2))
+    both = ops.LoraStack(2, 16, 64, [16, 16], device=DEV, interleaved=True)
+    with pytest.raises(ValueError):
+        ops.lora_add(y, x, both, plan)
+    with pytest.raises(ValueError):
+        ops.lora_gated(y, x, st, plan)
+    torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("shape,dims", [((9, 2, 16), (64, 64)), ((30, 4, 64), (192, 128)), ((7, 1, 1), (8, 8)), ((12, 8, 16), (128, 128))])
