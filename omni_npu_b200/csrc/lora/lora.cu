@@ -40,7 +40,7 @@
 namespace b200 {
 
 static constexpr int kLoraMaxSlices = 4;
-static constexpr int kLoraChunk = 8;             // 8-wide tiles of h that a CTA computes
+static constexpr int kFewChunk = 4, kManyChunk = 8;   // 8-wide tiles of h that a CTA computes
 static constexpr int kPlanThreads = 1024;
 
 // ----------------------------------------------------------------------------------------------- grouping
@@ -211,7 +211,9 @@ __device__ __forceinline__ void split_h(const float4& s, float scale, uint2& hi,
 // ---- h of few rows: 16 at most, K dealt to the parts and, in steps of 32, to the warps.  The factors are what is read: every
 // lane has a ring of its own in shared memory for what it alone uses of A and x (no barrier between copy and product), 12 KB a
 // warp however many ranks there are, so that four CTAs are resident (128 adapters of rank 16, K 14336: 13.2 us, with 24 KB
-// and two CTAs 15.8).
+// and two CTAs 15.8).  A CTA computes 32 of the joined ranks: with 64, a ring of 12 KB has two stages only (both kernels, one
+// token, three slices, rank 16: 4.5 us, 4.7 with 64 ranks; over ranks 8 to 64 and 1 to 128 tokens 4% more); with a ring of 9 KB
+// 128 adapters take 20.1 us for both kernels, 18.4 so.
 static constexpr int kFewThreads = 128, kFewWarps = kFewThreads / 32, kFewRing = 12 * 1024;
 
 template <int NT>
@@ -265,12 +267,12 @@ __device__ __forceinline__ void shrink_rows(const LoraParams& p, const LoraTile&
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     *reinterpret_cast<float2*>(d + j * 8) = make_float2(acc[j][0], acc[j][1]);
-    *reinterpret_cast<float2*>(d + 8 * kLoraChunk * 8 + j * 8) = make_float2(acc[j][2], acc[j][3]);
+    *reinterpret_cast<float2*>(d + 8 * kFewChunk * 8 + j * 8) = make_float2(acc[j][2], acc[j][3]);
   }
 }
 
 __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const LoraParams p) {
-  constexpr int BM = 16, W = kLoraChunk * 8;
+  constexpr int W = kFewChunk * 8;
   extern __shared__ __align__(128) char smem[];
   pdl_wait();
   pdl_trigger();                                                       // (the second kernel reads what was there before this one)
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const Lora
   const int n0 = blockIdx.y * W;
   if (n0 >= sum_r) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int nt = min(kLoraChunk, (sum_r - n0) / 8);                    // even: ranks are multiples of 16
+  const int nt = min(kFewChunk, (sum_r - n0) / 8);                     // even: ranks are multiples of 16
   const int steps = (p.K + 31) / 32;
   const int s_lo = static_cast<int>(static_cast<long long>(steps) * blockIdx.x / p.parts) + warp;
   const int s_hi = static_cast<int>(static_cast<long long>(steps) * (blockIdx.x + 1) / p.parts);
@@ -290,9 +292,7 @@ __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const Lora
   const auto red = [&](int w) { return reinterpret_cast<float*>(smem + w * kFewRing); };
   float* d = red(warp) + g * W + t4 * 2;
   if (nt == 2) shrink_rows<2>(p, tl, n0, sum_r, s_lo, s_hi, ring, d);
-  else if (nt == 4) shrink_rows<4>(p, tl, n0, sum_r, s_lo, s_hi, ring, d);
-  else if (nt == 6) shrink_rows<6>(p, tl, n0, sum_r, s_lo, s_hi, ring, d);
-  else shrink_rows<8>(p, tl, n0, sum_r, s_lo, s_hi, ring, d);
+  else shrink_rows<4>(p, tl, n0, sum_r, s_lo, s_hi, ring, d);
   __syncthreads();
   // the warps' parts in order, four columns a thread
   float* h = static_cast<float*>(p.h) + blockIdx.x * p.h_plane + static_cast<long long>(tl.start) * p.h_width + n0;
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const Lora
 static constexpr int kManyThreads = 256, kManyRows = 64, kSlab = 128, kStages = 3, kStageBytes = 2 * kManyRows * kSlab * 2;
 
 __global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const LoraParams p) {
-  constexpr int W = kLoraChunk * 8;
+  constexpr int W = kManyChunk * 8;
   extern __shared__ __align__(128) char smem[];
   pdl_wait();
   pdl_trigger();
@@ -866,8 +866,9 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   const bool many = rows == kManyRows, gated = act != kActNone;
   p.act_alpha = act_alpha;
   p.act_limit = act_limit;
-  const unsigned chunks = (p.h_width + kLoraChunk * 8 - 1) / (kLoraChunk * 8), tiles_n = static_cast<unsigned>(max_tiles);
-  p.parts = lora_parts(K, rows, max_tiles, num_slots, (mean_rank + kLoraChunk * 8 - 1) / (kLoraChunk * 8));
+  const int width = (many ? kManyChunk : kFewChunk) * 8;
+  const unsigned chunks = (p.h_width + width - 1) / width, tiles_n = static_cast<unsigned>(max_tiles);
+  p.parts = lora_parts(K, rows, max_tiles, num_slots, (mean_rank + width - 1) / width);
   p.h_pitch = (gated ? 2 : 1) * max_rank + 8;    // eight rows of 16 bytes are in banks of their own
   // column groups of a CTA: two rounds of the resident CTAs in all, or for few rows one, where a CTA's start is most of its
   // time (128 adapters of rank 16, 4096 columns: 7.7 us, with two rounds 9.6); a group a warp at least
