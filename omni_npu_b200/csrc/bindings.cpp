@@ -113,7 +113,8 @@ long long b200_lora_scratch_bytes(int T, int K, int rows, int max_tiles, int num
 int b200_lora(const void* x, long long x_stride, const void* y, long long y_stride, void* out, long long out_stride,
               const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks, const int* order,
               const int* tiles, const int* num_tiles, int max_tiles, int rows, void* h, int T, int num_slots, int K, int slices,
-              const int* n, int max_rank, int mean_rank, int act, float act_alpha, float act_limit, cudaStream_t stream);
+              const int* n, int max_rank, int mean_rank, int act, float act_alpha, float act_limit, int* status,
+              cudaStream_t stream);
 size_t b200_mla_decode_scratch_bytes(int total_tokens, int N, int splits);
 int b200_mla_decode(const void* q, const void* cache, void* out, float* lse, const int* block_tables,
                     const int* seq_lens, const int* topk_indices, int topk, int B, int q_len, int N,
@@ -784,7 +785,7 @@ bool share_memory(const Tensor& a, const Tensor& b) {
 // slices + 1], each slot's ranks and the bits of its scale.  sizes: of the plan tokens, slots and
 // rows of a tile; activation; of the stack input features, largest rank, mean of the joined ranks, columns of each slice.
 Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given, const Tensor& a, const Tensor& b,
-            const Tensor& ranks, const Tensor& plan, at::IntArrayRef sizes, double act_alpha, double act_limit) {
+            const Tensor& ranks, const Tensor& plan, at::IntArrayRef sizes, double act_alpha, double act_limit, const Tensor& status) {
   TORCH_CHECK(sizes.size() > 7 && sizes.size() <= 11, "lora: one to four slices");
   const int64_t rows = sizes[2], act = sizes[3], K = sizes[4], max_rank = sizes[5], mean_rank = sizes[6];
   const int64_t S = (int64_t)sizes.size() - 7;
@@ -807,11 +808,12 @@ Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given
               "lora: factors [slots, slices * rank * K] and [slots, columns * rank], K and columns in whole 32");
   CHECK_I32(ranks);
   CHECK_I32(plan);
+  CHECK_I32(status);
   const int64_t at = lora_tiles_at(T), max_tiles = lora_max_tiles(T, L, rows);
   TORCH_CHECK(ranks.dim() == 2 && ranks.size(1) == S + 1, "lora: ranks int32 [slots, slices + 1]");
   TORCH_CHECK_VALUE(sizes[0] == T && sizes[1] == L && plan.numel() == std::max<int64_t>(at + 4 * max_tiles, 4),
                     "lora: a plan of other tokens or slots than ", T, " and ", L);
-  TORCH_CHECK_VALUE(max_tiles <= 65535, "lora: ", T, " tokens are too many at once");
+  TORCH_CHECK_VALUE(max_tiles <= (rows == 16 ? 65535 : 32767), "lora: ", T, " tokens are too many at once");
   c10::cuda::CUDAGuard guard(x.device());
   const int64_t cols = act ? slices[0] : width;
   const Tensor out = given.has_value() ? *given : torch::empty({T, cols}, y.options());
@@ -835,7 +837,7 @@ Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given
   check(b200_lora(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(), out.stride(0), a.data_ptr(), a.size(1),
                   b.data_ptr(), b.size(1), ranks.data_ptr<int>(), p, p + at, p + T, (int)max_tiles, (int)rows, h.data_ptr(),
                   (int)T, (int)L, (int)K, (int)S, n, (int)max_rank, (int)std::max<int64_t>(mean_rank, 16), (int)act,
-                  (float)act_alpha, (float)act_limit, cur_stream()),
+                  (float)act_alpha, (float)act_limit, status.data_ptr<int>(), cur_stream()),
         "lora");
   return out;
 }

@@ -7,24 +7,23 @@
 // value of a joined projection have factors of their own).  Ranks are multiples of 16 (zero padded), 0 for a slice without an
 // adapter; the slices' A of a slot are joined along the rank.
 //
-// The factors lie in the order in which lanes of the matrix instructions hold them (g = lane / 4, q = lane % 4), so that they are
-// read in whole kilobytes and need no shuffling:
-//   A  [K / 32][rank / 16][u = 0, 1][lane][8]    ranks g, g + 8 of 16 times k = 8 q + 4 u + 0 .. 3 of 32
+// The factors lie in the order in which the matrix instructions take them, so that they are read in whole kilobytes and need no
+// shuffling: A as 8 x 8 matrices (rows of ldmatrix, unswizzled operands of tcgen05), B as lanes hold it (g = lane / 4, q = lane % 4):
+//   A  [K / 32][rank / 8][4][rank % 8][8]        8 of K each of eight ranks, four times
 //   B  [N / 32][rank / 16][v = 0, 1][lane][8]    columns 8 (g / 2) + 2 j + g % 2 of 32 for j = 2 v, 2 v + 1 times
 //                                                k = 2 q, 2 q + 1, 2 q + 8, 2 q + 9 of 16
-// K and N padded with zeros.  A lane's 16 bytes of a row of x then are its k of two instructions, and the columns of its
-// results are eight neighbours.
+// K and N padded with zeros.  The columns of a lane's results are eight neighbours.
 //
 // Tokens are grouped by adapter once a step (lora_plan_kernel: a stable counting sort, then tiles of up to `rows` tokens of one
 // adapter).  Two launches apply the adapters, both bound by what they read and write:
-//   lora_shrink_*_kernel  h: CTAs that share K per (tile, 64 of the joined ranks)
+//   lora_shrink_*_kernel  h: CTAs that share K per (tile, some of the joined ranks)
 //   lora_expand_kernel    z: a CTA per (tile, run of column groups)
 // so that many small pieces of work even out adapters of unlike ranks (one cluster per tile for both, h in distributed shared
 // memory, took 56 us where this takes 15: 128 tokens of 31 adapters of ranks 8 to 64).  The second is launched while the first
 // runs and has its first y and factors at hand by the time h is there.  Measured (us, and the time of the bytes at 6.56 TB/s):
-// one token 4.6; 128 tokens of 128 adapters of rank 16, 14336 to 4096 18.3 / 12.4; 8192 tokens of 8, 4096 to 6144 56 / 42;
-// the same to 2 x 14336 with silu, rank 32 167 / 121.  Ranks above some 32 are bound by the matrix instructions and what
-// they read from shared memory: 8192 tokens of rank 64, 4096 to 6144 117 / 42.
+// one token 4.6; 128 tokens of 128 adapters of rank 16, 14336 to 4096 18.4 / 12.4; 8192 tokens of 8, 4096 to 6144 56 / 42;
+// the same to 2 x 14336 with silu, rank 32 165 / 121.  Ranks above some 32 are bound by the second kernel's matrix instructions:
+// 8192 tokens of rank 64, 4096 to 6144 90 / 42 (117 before the first kernel used tcgen05).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -35,12 +34,13 @@
 #include "../common/device_once.h"
 #include "../common/pdl.cuh"
 #include "../common/ptx.cuh"
+#include "../common/tensormap.h"
 #include "../gemm/gated_act.cuh"
 
 namespace b200 {
 
 static constexpr int kLoraMaxSlices = 4;
-static constexpr int kFewChunk = 4, kManyChunk = 8;   // 8-wide tiles of h that a CTA computes
+static constexpr int kFewChunk = 4, kManyChunk = 16;  // 8-wide tiles of h that a CTA computes
 static constexpr int kPlanThreads = 1024;
 
 // ----------------------------------------------------------------------------------------------- grouping
@@ -147,7 +147,10 @@ struct LoraParams {
   void* h;
   long long h_plane;                             // T * h_width
   int h_width;                                   // slices * largest rank
-  int K, slices, parts;
+  int T, K, slices, parts;
+  int stages, stage_bytes;                       // many rows: the first kernel's ring
+  int boxes;                                     // 1: rows of x that follow one another are copied as a box
+  int* status;
   int per;                                       // column groups of a CTA of the second kernel
   int n[kLoraMaxSlices];
   int h_pitch;                                   // elements between rows of h in shared memory
@@ -219,25 +222,28 @@ static constexpr int kFewThreads = 128, kFewWarps = kFewThreads / 32, kFewRing =
 template <int NT>
 __device__ __forceinline__ void shrink_rows(const LoraParams& p, const LoraTile& tl, int n0, int sum_r, int s_lo, int s_hi,
                                             uint32_t ring, float* d) {
-  constexpr int STAGE = (NT + 2) * 512, D = kFewRing / STAGE;          // NT / 2 x 2 pieces of A, two rows of x
+  constexpr int STAGE = (NT + 2) * 512, D = kFewRing / STAGE;          // NT pieces of A, two rows of x
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + (n0 / 16) * 512 + lane * 8;
+  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + (n0 / 8) * 256 + lane * 8;
   const long long a_step = sum_r * 32;
+  const int swap = g >> 1 & 3;                                         // places of the pieces of x: ldmatrix without bank conflicts
   const bool ok0 = g < tl.count, ok1 = g + 8 < tl.count;               // (the other rows of h are not used)
   const __nv_bfloat16* x0 = p.x + (ok0 ? p.order[tl.start + g] : 0) * p.x_stride + t4 * 8;
   const __nv_bfloat16* x1 = p.x + (ok1 ? p.order[tl.start + g + 8] : 0) * p.x_stride + t4 * 8;
-  ring += lane * 16;
+  const uint32_t at = ring + lane * 16, x_put = ring + NT * 512 + (g * 4 + (t4 ^ swap)) * 16;
+  // 16 rows of x as four matrices: rows 0 - 7 and 8 - 15 of one piece of 8 of K, then of the next
+  const uint32_t x_get = ring + NT * 512 + (lane >> 3 & 1) * 512 + ((lane & 7) * 4 + (lane >> 4 ^ (lane >> 1 & 3))) * 16;
   int put = 0;
   auto copy = [&](int s) {
     if (s < s_hi) {
-      const uint32_t st = ring + put * STAGE;
+      const uint32_t st = put * STAGE;
       put = put + 1 == D ? 0 : put + 1;
 #pragma unroll
-      for (int u = 0; u < NT; ++u) cp16(st + u * 512, a + s * a_step + u * 256);
+      for (int u = 0; u < NT; ++u) cp16(at + st + u * 512, a + s * a_step + u * 256);
       const bool in = s * 32 + t4 * 8 < p.K;                           // K is a multiple of 8
       const int k = in ? s * 32 : 0;
-      if (ok0) cp16_or_zero(st + NT * 512, x0 + k, in);
-      if (ok1) cp16_or_zero(st + NT * 512 + 512, x1 + k, in);
+      if (ok0) cp16_or_zero(x_put + st, x0 + k, in);
+      if (ok1) cp16_or_zero(x_put + st + 512, x1 + k, in);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -250,16 +256,18 @@ __device__ __forceinline__ void shrink_rows(const LoraParams& p, const LoraTile&
   int get = 0;
   for (int s = s_lo; s < s_hi; s += kFewWarps) {
     asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
-    const uint32_t st = ring + get * STAGE;
+    __syncwarp();
+    const uint32_t st = get * STAGE;
     get = get + 1 == D ? 0 : get + 1;
-    const uint4 v0 = lds16(st + NT * 512), v1 = lds16(st + NT * 512 + 512);
+    uint32_t v[4], w[4];
+    ldmatrix4(v, x_get + st);
+    ldmatrix4(w, x_get + st ^ 32);
 #pragma unroll
-    for (int j = 0; j < NT; j += 2) {
-      const uint4 b = lds16(st + j * 512), c = lds16(st + j * 512 + 512);
-      mma_bf16(acc[j], v0.x, v1.x, v0.y, v1.y, b.x, b.y);
-      mma_bf16(acc[j + 1], v0.x, v1.x, v0.y, v1.y, b.z, b.w);
-      mma_bf16(acc[j], v0.z, v1.z, v0.w, v1.w, c.x, c.y);
-      mma_bf16(acc[j + 1], v0.z, v1.z, v0.w, v1.w, c.z, c.w);
+    for (int j = 0; j < NT; ++j) {
+      uint32_t b[4];                                                   // eight ranks, 32 of K
+      ldmatrix4(b, at + st + j * 512);
+      mma_bf16(acc[j], v[0], v[1], v[2], v[3], b[0], b[1]);
+      mma_bf16(acc[j], w[0], w[1], w[2], w[3], b[2], b[3]);
     }
     copy(s + (D - 1) * kFewWarps);                                     // where the stage before this one was
   }
@@ -308,157 +316,210 @@ __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const Lora
   }
 }
 
-// ---- h of many rows: 64 rows of x and 64 of the joined ranks, in slabs of 128 of K through a ring in shared memory, so that
-// what is in flight does not depend on registers.  Warps: two halves of every slab's K, then 32 rows x 32 ranks each (a fragment
-// of x and one of A serve two and two pairs of matrix instructions).  128 rows a CTA, or 128 ranks, halve what is read once more
-// from L2 but were no faster (8192 tokens, K 4096, 48 ranks: 26.2 us, 25.3 so; 192 ranks 60 and 61), nor were 64 of K a slab.
-// The parts of K meet in distributed shared memory: with fp32 parts in global memory that every CTA of the second kernel
-// adds up, 2847 tokens of ranks 33 to 128 took 66 us, 57 so.
-static constexpr int kManyThreads = 256, kManyRows = 64, kSlab = 128, kStages = 3, kStageBytes = 2 * kManyRows * kSlab * 2;
+// ---- h of many rows: 128 rows of x and up to 128 of the joined ranks on tcgen05, the sum in tensor memory, in slabs of 64 of K
+// through a ring of stages.  Rows of x that follow one another (a prompt's) are one TMA box a slab; others are gathered by eight
+// warps in copies of 16 bytes (rows behind the tile's last are not copied: what lies there only reaches rows of h that nobody
+// reads).  The factors lie in the order of unswizzled operands, so a slab of them is two bulk copies.  The parts of K, a CTA of
+// the cluster each, meet in distributed shared memory.  Alone, 8192 tokens, K 4096: 20 us for 48 joined ranks, 27 for 192, 42 for
+// 384 (x's bytes alone 10; some 8 us are the start, the first copies and the joining); with mma.sync, where every warp reads x
+// from shared memory again for 32 of the ranks, 25 for 48 and 60 for 192.  Also slower: the fence between copies and products
+// issued by the copying threads, which then wait for all their copies (384 ranks: 80), and TMA's gathers of four rows (85
+// cycles each; both kernels 66 us for 56).
+static constexpr int kManyCopies = 256, kManyThreads = kManyCopies + 64, kManyRows = 128, kSlab = 64, kManyRing = 208 * 1024;
+static constexpr int kManyStages = 8, kXBytes = kManyRows * kSlab * 2;
 
-__global__ void __launch_bounds__(kManyThreads, 2) lora_shrink_many_kernel(const LoraParams p) {
+// Arrive on an mbarrier once all of this thread's copies so far have landed (the arrival is one of the expected).
+__device__ __forceinline__ void arrive_when_copied(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Products of 16 of K: x in rows of 128 bytes in the 128-byte swizzle, the factors unswizzled (128 bytes to the next eight of K, 512
+// to the next eight ranks).  Descriptors' low words; ACC: added to what is there.
+template <bool ACC>
+__device__ __forceinline__ void umma_factors(uint32_t d_tmem, uint32_t x_lo, uint32_t f_lo, uint32_t idesc) {
+  asm volatile(
+      "{\n\t"
+      ".reg .b64 dx, df;\n\t"
+      ".reg .pred p;\n\t"
+      "mov.b64 dx, {%1, %3};\n\t"
+      "mov.b64 df, {%2, %4};\n\t"
+      "setp.eq.u32 p, %6, 1;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], dx, df, %5, p;\n\t"
+      "}"
+      :
+      : "r"(d_tmem), "r"(x_lo), "r"(f_lo), "r"(kSmemDescHiSw128), "r"((512u >> 4) | (1u << 14)), "r"(idesc), "n"(ACC ? 1 : 0)
+      : "memory");
+}
+
+__global__ void __launch_bounds__(kManyThreads, 2)
+lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ LoraParams p) {
   constexpr int W = kManyChunk * 8;
   extern __shared__ __align__(128) char smem[];
+  __shared__ uint64_t full[kManyStages], empty[kManyStages], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int gave_up;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t ring = (smem_u32(smem) + 1023) & ~1023u;
+  char* ring_ptr = smem + (ring - smem_u32(smem));
   pdl_wait();
   pdl_trigger();
   LoraTile tl;
   if (!lora_tile(p, blockIdx.z, tl) || tl.slot < 0) return;
+  const int first = p.order[tl.start];
+  const bool box = p.boxes && p.order[tl.start + tl.count - 1] - first == tl.count - 1;   // (the order is ascending)
+  // copies: eight lanes a row of 128 bytes, 32 rows at once
+  const int crow = threadIdx.x >> 3, piece = threadIdx.x & 7;
+  int order[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) order[i] = crow < 32 && crow + 32 * i < tl.count ? p.order[tl.start + crow + 32 * i] : 0;
   int sum_r = 0;
   for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * (p.slices + 1) + s];
+  const float scale = lora_scale(p, tl.slot);
   const int n0 = blockIdx.y * W;
   if (n0 >= sum_r) return;
   const int width = min(W, sum_r - n0);                                // a multiple of 16
   const int slabs = (p.K + kSlab - 1) / kSlab, blocks = (p.K + 31) / 32;
   const int s_lo = static_cast<int>(static_cast<long long>(slabs) * blockIdx.x / p.parts);
-  const int s_hi = static_cast<int>(static_cast<long long>(slabs) * (blockIdx.x + 1) / p.parts);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-
-  // copies: sixteen lanes a row of 256 bytes, its 16-byte pieces at piece ^ 4 (row % 2), so that the eight lanes that read two
-  // rows at once find 128 bytes in different banks; A as it lies.  (Rows behind the tile's last are copies of its first.)
-  const int crow = threadIdx.x >> 4, piece = threadIdx.x & 15;
-  const __nv_bfloat16* xs[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = crow + 16 * i;
-    xs[i] = p.x + p.order[tl.start + (row < tl.count ? row : 0)] * p.x_stride + s_lo * kSlab + piece * 8;
-  }
-  const long long a_step = sum_r * 32;
-  const __nv_bfloat16* a = p.a + tl.slot * p.a_slot + (n0 / 16) * 512 + threadIdx.x * 8 + s_lo * 4 * a_step;
-  const bool aok = threadIdx.x < width * 4;
-  const uint32_t base = smem_u32(smem);
-  const uint32_t xdst = base + crow * 256 + ((piece ^ (crow & 1) << 2) << 4), adst = base + 16384 + threadIdx.x * 16;
-  uint32_t put = 0;
-  int next = s_lo;                                                     // slab that is copied next
-  auto copy = [&]() {
-    if (next < s_hi) {
-      if (next * kSlab + kSlab <= p.K) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cp16(xdst + put + i * 4096, xs[i]);
-        if (aok) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) cp16(adst + put + i * 4096, a + i * a_step);
-        }
-      } else {                                                         // the end of K, a multiple of 8
-        const bool in = next * kSlab + piece * 8 < p.K;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cp16_or_zero(xdst + put + i * 4096, in ? xs[i] : p.x, in);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (aok) cp16_or_zero(adst + put + i * 4096, next * 4 + i < blocks ? a + i * a_step : p.a, next * 4 + i < blocks);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xs[i] += kSlab;
-      a += 4 * a_step;
-      put = put + kStageBytes == kStages * kStageBytes ? 0 : put + kStageBytes;
-      ++next;
+  const int count = static_cast<int>(static_cast<long long>(slabs) * (blockIdx.x + 1) / p.parts) - s_lo;   // one at least
+  const uint32_t tmem_cols = width > 64 ? 128 : width > 32 ? 64 : 32;
+  if (threadIdx.x == kManyCopies + 32) {
+    tma_prefetch_desc(&tm_x);
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&full[i], box ? 1 : kManyCopies + 1);
+      mbar_init(&empty[i], 1);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  for (int i = 0; i < kStages - 1; ++i) copy();
+    mbar_init(&done, 1);
+    gave_up = 0;
+    fence_barrier_init();
+  }
+  if (warp == kManyCopies / 32) {
+    tmem_alloc(&tmem_slot, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
 
-  const int kw = warp >> 2, m0 = (warp & 1) * 32, j0 = (warp >> 1 & 1) * 32;
-  const bool live = j0 < width && m0 < tl.count;
-  float acc[2][4][4];
+  if (warp < kManyCopies / 32 && !box) {
+    const __nv_bfloat16* xs[4];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+    for (int i = 0; i < 4; ++i) xs[i] = p.x + order[i] * p.x_stride + s_lo * kSlab + piece * 8;
+    const uint32_t dst = ring + crow * 128 + ((piece ^ (crow & 7)) << 4);
+    int put = 0;
+    uint32_t phase = 1;                                                // (the first pass over the ring does not wait)
+    for (int i = 0; i < count; ++i) {
+      if (!__shfl_sync(0xffffffffu, lane > 0 || mbar_wait(&empty[put], phase), 0)) {
+        if (lane == 0) atomicCAS(p.status, 0, kStatusTimeoutEmptyBarrier);
+        break;
+      }
+      const bool in = (s_lo + i) * kSlab + piece * 8 < p.K;            // K is a multiple of 8
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
-  // (32 of K at 4 pieces; the exchange of pieces swaps neighbouring 32 in odd rows)
-  const uint32_t xf = base + (m0 + g) * 256 + kw * 128 + t4 * 16, x_swap = (g & 1) * 64;
-  const uint32_t af = base + 16384 + kw * 8192 + (j0 / 16) * 1024 + lane * 16;
-  uint32_t get = 0;
-  for (int s = s_lo; s < s_hi; ++s) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    __syncthreads();
-    copy();
-    if (live) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint4 xv[4], av[2][2];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) xv[i] = lds16(xf + get + (q * 64 ^ x_swap) + i * 2048);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) av[j][u] = lds16(af + get + q * 4096 + j * 1024 + u * 512);
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint4 &v = xv[2 * m], &w = xv[2 * m + 1];
-            mma_bf16(acc[m][2 * j], v.x, w.x, v.y, w.y, av[j][0].x, av[j][0].y);
-            mma_bf16(acc[m][2 * j + 1], v.x, w.x, v.y, w.y, av[j][0].z, av[j][0].w);
-            mma_bf16(acc[m][2 * j], v.z, w.z, v.w, w.w, av[j][1].x, av[j][1].y);
-            mma_bf16(acc[m][2 * j + 1], v.z, w.z, v.w, w.w, av[j][1].z, av[j][1].w);
-          }
+      for (int u = 0; u < 4; ++u)
+        if (crow + 32 * u < tl.count) cp16_or_zero(dst + put * p.stage_bytes + u * 4096, in ? xs[u] + i * kSlab : p.x, in);
+      arrive_when_copied(&full[put]);
+      if (++put == p.stages) put = 0, phase ^= 1;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kManyCopies / 32 + 1 && lane == 0) {
+    const char* a = reinterpret_cast<const char*>(p.a + tl.slot * p.a_slot) + n0 * 64;
+    const long long a_step = static_cast<long long>(sum_r) * 64;
+    int put = 0, i = 0;
+    uint32_t phase = 1;
+    for (; i < count; ++i) {
+      if (!mbar_wait(&empty[put], phase)) {
+        atomicCAS(p.status, 0, kStatusTimeoutEmptyBarrier);
+        break;
+      }
+      const int s = (s_lo + i) * 2, steps = min(2, blocks - s);
+      char* st = ring_ptr + put * p.stage_bytes;
+      mbar_arrive_expect_tx(&full[put], steps * width * 64 + (box ? kXBytes : 0));
+      if (box) tma_load_2d(st, &tm_x, &full[put], (s_lo + i) * kSlab, first);
+      for (int u = 0; u < steps; ++u) bulk_load_1d(st + kXBytes + u * width * 64, a + (s + u) * a_step, width * 64, &full[put]);
+      if (++put == p.stages) put = 0, phase ^= 1;
+    }
+    if (*static_cast<volatile int*>(&gave_up)) {
+      // what was copied for nobody has landed before this CTA ends
+      for (int j = 0; j < min(i, p.stages); ++j) {
+        if (put-- == 0) put = p.stages - 1, phase ^= 1;
+        mbar_wait(&full[put], phase ^ 1);
       }
     }
-    get = get + kStageBytes == kStages * kStageBytes ? 0 : get + kStageBytes;
-  }
-  // the two halves of K in order
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  float* mine = reinterpret_cast<float*>(smem) + (warp & 3) * 32 * 36;
-  float* part = reinterpret_cast<float*>(smem) + 4 * 32 * 36;
-  if (kw == 1 && live) {
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        *reinterpret_cast<float2*>(mine + (m * 16 + g) * 36 + j * 8 + t4 * 2) = make_float2(acc[m][j][0], acc[m][j][1]);
-        *reinterpret_cast<float2*>(mine + (m * 16 + g + 8) * 36 + j * 8 + t4 * 2) = make_float2(acc[m][j][2], acc[m][j][3]);
+  } else if (warp == kManyCopies / 32 && lane == 0) {
+    const uint32_t idesc = make_idesc(1, 1, kManyRows, width);
+    // (above 18 bits, an address holds the CTA's rank in its cluster)
+    const uint32_t lo = (ring & 0x3FFFF) >> 4, stage_lo = p.stage_bytes >> 4, f_at = (kXBytes >> 4) + ((128u >> 4) << 16);
+    int get = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < count; ++i) {
+      if (!mbar_wait(&full[get], phase)) {
+        atomicCAS(p.status, 0, kStatusTimeoutFullBarrier);
+        gave_up = 1;
+        break;
       }
+      // Gathered rows were written through another proxy than the products read them.  (Here: a fence of the copying threads would
+      // wait for all of their copies in flight.)
+      if (!box) fence_proxy_async();
+      tc_fence_after_sync();
+      const uint32_t x_lo = lo + get * stage_lo, f_lo = x_lo + f_at, f_next = f_lo + width * 4;
+      if ((s_lo + i) * 2 + 1 < blocks) {
+        if (i == 0) umma_factors<false>(tmem, x_lo, f_lo, idesc);
+        else umma_factors<true>(tmem, x_lo, f_lo, idesc);
+        umma_factors<true>(tmem, x_lo + 2, f_lo + 16, idesc);
+        umma_factors<true>(tmem, x_lo + 4, f_next, idesc);
+        umma_factors<true>(tmem, x_lo + 6, f_next + 16, idesc);
+      } else {                                                         // the last 32 of K
+        if (i == 0) umma_factors<false>(tmem, x_lo, f_lo, idesc);
+        else umma_factors<true>(tmem, x_lo, f_lo, idesc);
+        umma_factors<true>(tmem, x_lo + 2, f_lo + 16, idesc);
+      }
+      tc_commit(&empty[get]);
+      if (++get == p.stages) get = 0, phase ^= 1;
+    }
+    tc_commit(&done);
+    if (!mbar_wait(&done, 0)) atomicCAS(p.status, 0, kStatusTimeoutTmemFull);
+    tc_fence_before_sync();
   }
+  // Every product is through, and the ring free.  (The other warps wait here and not at the mbarrier: eight warps that poll it
+  // slow down the two that work.)
   __syncthreads();
-  if (kw == 0 && live) {
+  tc_fence_after_sync();
+  float* part = reinterpret_cast<float*>(ring_ptr);
+  const int pitch = width + 4;
+  if (warp < kManyCopies / 32 && (warp & 3) * 32 < tl.count) {         // a quarter of the rows, every other 32 columns
+    const int row = (warp & 3) * 32 + lane;
+    for (int c = (warp >> 2) * 32; c < width; c += 64) {
+      uint32_t v[32];
+      tmem_ld_32x32b_x32(tmem + ((warp & 3) << 21) + c, v);
+      tmem_ld_wait();
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = m * 16 + g + e * 8, col = j * 8 + t4 * 2;
-          const float2 o = *reinterpret_cast<const float2*>(mine + r * 36 + col);
-          *reinterpret_cast<float2*>(part + (m0 + r) * W + j0 + col) =
-              make_float2(acc[m][j][2 * e] + o.x, acc[m][j][2 * e + 1] + o.y);
-        }
+      for (int j = 0; j < 32; j += 4)
+        if (c + j < width)
+          *reinterpret_cast<uint4*>(part + row * pitch + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    }
   }
+  tc_fence_before_sync();
   // The cluster's CTAs have summed a part of K each.  Every one adds up its share of the elements in the order of the parts and
   // leaves them ready for the second kernel, whose many CTAs then need no more than copy them.
   cluster_arrive_release();
   cluster_wait_acquire();
+  if (warp == kManyCopies / 32) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, tmem_cols);
+  }
   const int C = p.parts, rank = blockIdx.x, vecs = width / 4;
-  const float scale = lora_scale(p, tl.slot);
   __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p.h) + static_cast<long long>(tl.start) * p.h_width + n0;
   for (int i = rank * kManyThreads + threadIdx.x; i < tl.count * vecs; i += C * kManyThreads) {
     const int row = i / vecs, v = i % vecs * 4;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < C; ++c) {
-      const float4 q = ld_shared_cluster_f4(mapa_shared(smem_u32(part + row * W + v), c));
-      sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
-    }
+    const uint32_t at = smem_u32(part + row * pitch + v);
+    float4 q[8];                                                       // (8 parts at most)
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < C) q[c] = ld_shared_cluster_f4(mapa_shared(at, c));
+    float4 sum = q[0];
+#pragma unroll
+    for (int c = 1; c < 8; ++c)
+      if (c < C) sum.x += q[c].x, sum.y += q[c].y, sum.z += q[c].z, sum.w += q[c].w;
     uint2 hi, lo;
     split_h(sum, scale, hi, lo);
     __nv_bfloat16* dst = h + static_cast<long long>(row) * p.h_width + v;
@@ -488,7 +549,14 @@ __global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_ker
   const bool in_place = !GATED && p.out == p.y;
   // Everything but h is older than the first kernel, which has started only behind it: no wait yet.
   LoraTile tl;
-  if (!lora_tile(p, blockIdx.y, tl)) {
+  bool any = lora_tile(p, MANY ? blockIdx.y >> 1 : blockIdx.y, tl);
+  if constexpr (MANY) {                                                // a half of the rows
+    const int from = (blockIdx.y & 1) * BM;
+    any = any && from < tl.count;
+    tl.start += from;
+    tl.count = min(BM, tl.count - from);
+  }
+  if (!any) {
     pdl_wait();
     return;
   }
@@ -659,14 +727,16 @@ __global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_ker
   };
   // step k of h of rows m times its B
   auto multiply = [&](float (&acc)[8][4], int m, int k, const uint4& p0, const uint4& p1, const uint4& q0, const uint4& q1) {
+    uint32_t hi[4], lo[4];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       if (GATED && k >= (s ? k1 : k0)) continue;
       const uint4 &v = s ? q0 : p0, &w = s ? q1 : p1;
-      uint32_t hi[4], lo[4];
       const uint32_t at = hf + m * m_step + k * 32 + (GATED && s ? r0 * 2 : 0);
-      ldmatrix4(hi, at);
-      ldmatrix4(lo, at + lo_at);
+      if (GATED || s == 0) {
+        ldmatrix4(hi, at);
+        ldmatrix4(lo, at + lo_at);
+      }
       float(*c)[4] = acc + 4 * s;
       mma_bf16(c[0], hi[0], hi[1], hi[2], hi[3], v.x, v.y);
       mma_bf16(c[1], hi[0], hi[1], hi[2], hi[3], v.z, v.w);
@@ -762,28 +832,36 @@ __global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_ker
   }
 }
 
-static constexpr int kShrinkFewSmem = kFewWarps * kFewRing, kShrinkManySmem = kStages * kStageBytes, kExpandSmem = 168 * 1024;
+static constexpr int kShrinkFewSmem = kFewWarps * kFewRing, kExpandSmem = 168 * 1024;
 
 template <bool MANY, int ACT, bool PAIRS>
 static int launch_lora(const LoraParams& p, unsigned tiles, unsigned chunks, unsigned blocks, cudaStream_t stream) {
-  auto shrink = MANY ? lora_shrink_many_kernel : lora_shrink_few_kernel;
   auto expand = lora_expand_kernel<MANY, ACT, PAIRS>;
   static DeviceOnce once;
   int dev;
   if (once.needed(&dev)) {
     const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    if (cudaFuncSetAttribute(shrink, attr, MANY ? kShrinkManySmem : kShrinkFewSmem) != cudaSuccess ||
+    if ((MANY ? cudaFuncSetAttribute(lora_shrink_many_kernel, attr, kManyRing + 1024)
+              : cudaFuncSetAttribute(lora_shrink_few_kernel, attr, kShrinkFewSmem)) != cudaSuccess ||
         cudaFuncSetAttribute(expand, attr, kExpandSmem) != cudaSuccess)
       return -3;
     once.mark(dev);
   }
   const size_t smem = 4 * (PAIRS ? 6 : 4) * (MANY ? 2048 : 6144) + 2 * sizeof(__nv_bfloat16) * (MANY ? 64 : 16) * p.h_pitch;
   const dim3 grid(p.parts, chunks, tiles);
-  if (smem > kExpandSmem || tiles > 65535) return -2;
-  if (launch_pdl(shrink, grid, dim3(MANY ? kManyThreads : kFewThreads), MANY ? kShrinkManySmem : kShrinkFewSmem, stream,
-                 MANY ? p.parts : 1, p) != cudaSuccess)
+  if (smem > kExpandSmem || tiles > (MANY ? 32767 : 65535)) return -2;
+  if constexpr (MANY) {
+    CUtensorMap tm_x = {};
+    if (p.boxes && make_tensormap_2d(&tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.x, p.T, p.K, p.x_stride, kManyRows, kSlab,
+                                     CU_TENSOR_MAP_SWIZZLE_128B) != 0)
+      return -4;
+    if (launch_pdl(lora_shrink_many_kernel, grid, dim3(kManyThreads), p.stages * p.stage_bytes + 1024, stream, p.parts, tm_x, p) !=
+        cudaSuccess)
+      return -3;
+  } else if (launch_pdl(lora_shrink_few_kernel, grid, dim3(kFewThreads), kShrinkFewSmem, stream, 1, p) != cudaSuccess) {
     return -3;
-  return launch_pdl(expand, dim3(blocks, tiles), dim3(kExpandThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
+  }
+  return launch_pdl(expand, dim3(blocks, MANY ? 2 * tiles : tiles), dim3(kExpandThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
 }
 
 template <int ACT>
@@ -796,7 +874,7 @@ static int launch_lora(const LoraParams& p, bool many, int max_rank, unsigned ti
 
 // Parts of K that a step's h is summed from, a CTA each (many rows: of a cluster).  Few rows (tiles of 16): as many as the slots
 // let be resident, whatever the number of tokens, so that a row does not depend on it.  Many rows: as many as fill the SMs, given
-// the pieces of 64 ranks that a tile has on average.
+// the pieces of 128 ranks that a tile has on average.
 static int lora_parts(int K, int rows, int max_tiles, int num_slots, int chunks) {
   const int pieces = max_tiles * chunks;
   const int want = rows < kManyRows ? std::min((K + 511) / 512, 592 / num_slots)
@@ -829,7 +907,7 @@ extern "C" int b200_lora_plan(const int* slots, int T, int L, int rows, int* ord
                     reinterpret_cast<LoraTile*>(tiles), num_tiles, status) == cudaSuccess ? 0 : -3;
 }
 
-// ranks: [L, slices + 1], a slot's ranks and the bits of its scale.  max_tiles: tiles that the plan may have, of `rows` (16 or 64)
+// ranks: [L, slices + 1], a slot's ranks and the bits of its scale.  max_tiles: tiles that the plan may have, of `rows` (16 or 128)
 // tokens each.  h: scratch of b200_lora_scratch_bytes.  n: columns of each slice.  max_rank: bound of the ranks; mean_rank: about
 // what a tile's joined ranks are (16 at least).  act: 0 adds, a gated kind of gemm/gated_act.cuh joins gate and up (alternating
 // groups of eight columns of y).
@@ -837,7 +915,7 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
                          const void* a, long long a_slot, const void* b, long long b_slot, const int* ranks, const int* order,
                          const int* tiles, const int* num_tiles, int max_tiles, int rows, void* h, int T, int num_slots, int K,
                          int slices, const int* n, int max_rank, int mean_rank, int act, float act_alpha, float act_limit,
-                         cudaStream_t stream) {
+                         int* status, cudaStream_t stream) {
   using namespace b200;
   if (slices < 1 || slices > kLoraMaxSlices || (K & 7) || max_rank < 16 || mean_rank < 16 || (max_rank & 15) || max_tiles < 1 ||
       (rows != 16 && rows != kManyRows))
@@ -861,14 +939,21 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   p.h = h;
   p.h_width = slices * max_rank;
   p.h_plane = static_cast<long long>(T) * p.h_width;
+  p.T = T;
   p.K = K;
+  p.boxes = x_stride >= K;                       // (not where rows overlap)
   p.slices = slices;
+  p.status = status;
   const bool many = rows == kManyRows, gated = act != kActNone;
   p.act_alpha = act_alpha;
   p.act_limit = act_limit;
   const int width = (many ? kManyChunk : kFewChunk) * 8;
   const unsigned chunks = (p.h_width + width - 1) / width, tiles_n = static_cast<unsigned>(max_tiles);
   p.parts = lora_parts(K, rows, max_tiles, num_slots, (mean_rank + width - 1) / width);
+  // the first kernel's ring: two CTAs an SM, or all of it for one where there are too few
+  const long long ctas = static_cast<long long>(p.parts) * max_tiles * ((mean_rank + width - 1) / width);
+  p.stage_bytes = kXBytes + std::min(p.h_width, width) * kSlab * 2;
+  p.stages = std::min((ctas > 148 ? kManyRing / 2 : kManyRing) / p.stage_bytes, kManyStages);
   p.h_pitch = (gated ? 2 : 1) * max_rank + 8;    // eight rows of 16 bytes are in banks of their own
   // column groups of a CTA: two rounds of the resident CTAs in all, or for few rows one, where a CTA's start is most of its
   // time (128 adapters of rank 16, 4096 columns: 7.7 us, with two rounds 9.6); a group a warp at least
@@ -878,7 +963,8 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
     if (p.n[s] & 7) return -1;
     if (!gated || s == 0) groups += gated ? (p.n[s] + 31) / 32 : (p.n[s] + 63) / 64;
   }
-  const long long want = static_cast<long long>(groups) * max_tiles / (148 * (many ? 8 : 2));
+  const int row_tiles = many ? max_tiles + T / kManyRows : max_tiles;   // of the second kernel: 64 rows
+  const long long want = static_cast<long long>(groups) * row_tiles / (148 * (many ? 8 : 2));
   p.per = static_cast<int>(std::max(1LL, (want + 3) / 4)) * 4;
   unsigned blocks = 0;
   for (int s = 0; s < slices; ++s)

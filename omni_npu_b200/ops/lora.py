@@ -16,10 +16,11 @@ from . import SILU, _C, _act_kind, _count, device_state, ref
 MAX_SLOTS, MAX_SLICES, MAX_RANK = 512, 4, 256
 
 # Tokens of one adapter that are taken together.  Up to this many tokens of a step: tiles of 16, one matrix instruction high,
-# through kernels that stream the factors; above, tiles of 64.  Us, tiles of 64 / 16: 200 tokens of 32 adapters of rank 16,
-# 4096 to 4096 + 1024 + 1024 13.3 / 9.7, 14336 to 4096 18.2 / 9.0; 700 tokens 15.2 / 15.2 and 18.2 / 13.5; 1000 tokens of 4 of
-# rank 64 22.9 / 34.1 and 28.4 / 26.5.  A row's result does not depend on the rows beside it as long as these are no more.
-FEW_TOKENS, FEW_ROWS, MANY_ROWS = 768, 16, 64
+# through kernels that stream the factors; above, tiles of 128.  Us, tiles of 128 / 16: 200 tokens of 8 adapters of rank 16,
+# 4096 to 4096 + 1024 + 1024 12.7 / 8.2, 14336 to 4096 19.2 / 8.8; 768 tokens 17.3 / 14.3 and 22.9 / 14.7; 1000 tokens 17.8 /
+# 19.6 and 23.3 / 16.6; 768 tokens of 8 of rank 64 21.7 / 26.9.  A row's result does not depend on the rows beside it as long as
+# these are no more.
+FEW_TOKENS, FEW_ROWS, MANY_ROWS = 768, 16, 128
 
 
 def _padded(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
@@ -56,7 +57,7 @@ class LoraStack:
         self.max_rank = (max_rank + 15) // 16 * 16
         self.dtype = dtype
         with torch.inference_mode(False):
-            # in the order of the matrix instructions' lanes (csrc/lora/lora.cu), K and columns in whole 32
+            # in the order of the matrix instructions (csrc/lora/lora.cu), K and columns in whole 32
             self._k = (in_features + 31) // 32
             self.a = torch.zeros(num_slots, len(slices) * self.max_rank * self._k * 32, dtype=dtype, device=device)
             self.b = torch.zeros(num_slots, sum((n + 31) // 32 * 32 for n in slices) * self.max_rank, dtype=dtype, device=device)
@@ -92,7 +93,7 @@ class LoraStack:
         with torch.inference_mode():
             for p, view in zip(a, self._views_a(slot, ranks)):
                 if view is not None:
-                    view.copy_(_padded(p, view.shape[0] * 16, self._k * 32).view(view.shape))
+                    view.copy_(_padded(p, view.shape[0] * 8, self._k * 32).view(view.shape))
             for q, view in zip(b, self._views_b(slot, ranks)):
                 if view is not None:
                     view.copy_(_padded(q, view.shape[0] * 32, view.shape[5] * 16).view(view.shape))
@@ -103,13 +104,13 @@ class LoraStack:
         self._set_ranks(slot, ranks)
 
     def _views_a(self, slot: int, ranks):
-        """A of each slice as [ranks, K] in the shape (rank / 16, 2, 8, K / 32, 4, 2, 4) over its packed place."""
-        total = sum(ranks) // 16
-        packed = self.a[slot, : total * 16 * self._k * 32].view(self._k, total, 2, 8, 4, 2, 4)   # k32, r16, u, g, q, half, 4
+        """A of each slice as [ranks, K] in the shape (rank / 8, 8, K / 32, 4, 8) over its packed place."""
+        total = sum(ranks) // 8
+        packed = self.a[slot, : total * 8 * self._k * 32].view(self._k, total, 4, 8, 8)   # k32, r8, k8, rank, 8
         at = 0
         for r in ranks:
-            yield packed[:, at: at + r // 16].permute(1, 5, 3, 0, 4, 2, 6) if r else None
-            at += r // 16
+            yield packed[:, at: at + r // 8].permute(1, 3, 0, 2, 4) if r else None
+            at += r // 8
 
     def _views_b(self, slot: int, ranks):
         """B of each slice as [columns, rank] in the shape (columns / 32, 4, 2, 2, 2, rank / 16, 2, 4, 2) over its packed place."""
@@ -207,7 +208,7 @@ def _launch(y, x, stack: LoraStack, plan: LoraPlan, out, kind, alpha, limit) -> 
     if plan.num_tokens:
         _count(2)
     return _C().lora(x, y, out, stack.a, stack.b, stack.ranks, plan.buffer,
-                     [plan.num_tokens, plan.num_slots, plan.rows, kind] + stack.sizes, alpha, limit)
+                     [plan.num_tokens, plan.num_slots, plan.rows, kind] + stack.sizes, alpha, limit, device_state(x.device).status)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan,

@@ -256,3 +256,52 @@ def test_copy_blocks_refusals(pairs):
     with pytest.raises(ValueError):
         ops.copy_blocks(cache, pairs)
     assert torch.equal(c, want)
+
+
+@pytest.mark.parametrize("contiguous", [False, True])
+@pytest.mark.parametrize("k,slices,ranks", [(8, [8], [16]), (40, [16, 24], [1, 0, 17]), (1032, [64, 8], [33, 128]),
+                                            (4096, [256, 72, 64], [16, 0, 64, 100]), (14336, [64], [8, 256])])
+@pytest.mark.parametrize("tokens", [769, 1000, 2177])
+def test_many_rows(tokens, k, slices, ranks, contiguous):
+    """Tiles of 128 rows: rows that follow one another, or gathered; ends of K inside a slab; parts of K; 16 to 500 joined ranks."""
+    run_add(tokens, 4, ranks, k, slices, slots_of(tokens, 4, seed=tokens, contiguous=contiguous))
+    if contiguous:                                             # no gaps: whole tiles follow one another
+        run_add(tokens, 4, ranks, k, slices, slots_of(tokens, 4, none=0, contiguous=True))
+
+
+@pytest.mark.parametrize("stride", [0, 64, 256, 264])
+def test_many_rows_of_any_stride(stride):
+    tokens, k = 900, 256
+    _, y, ad = make_case(tokens, 2, [16, 48], k, [72], device=DEV)
+    data = torch.randn(tokens * max(stride, 8) + k, generator=torch.Generator().manual_seed(5)).bfloat16().to(DEV)
+    x = torch.as_strided(data, (tokens, k), (stride, 1))
+    slots = slots_of(tokens, 2, none=0, contiguous=True).to(DEV)
+    out = ops.lora_add(y, x, load(ops, ad, 48, k, [72], DEV), ops.lora_plan(slots, 2))
+    z, bound = exact(x, y, ad, slots, [72])
+    check_sum(out, z, bound)
+
+
+@pytest.mark.parametrize("contiguous", [False, True])
+@pytest.mark.parametrize("tokens,n,k,ranks", [(800, 104, 520, [16, 0, 40]), (1500, 1000, 2048, [32])])
+def test_gated_many_rows(tokens, n, k, ranks, contiguous):
+    x, y, ad = make_case(tokens, 3, ranks, k, [n, n], device=DEV)
+    slots = slots_of(tokens, 3, contiguous=contiguous).to(DEV)
+    out = ops.lora_gated(y, x, load(ops, ad, 40, k, [n, n], DEV, True), ops.lora_plan(slots, 3))
+    z, bound = exact(x, y, ad, slots, [n, n], interleaved=True)
+    check_silu(out, z, bound)
+
+
+def test_many_rows_keep_their_values_to_themselves():
+    """NaN of a row of a tile, and of the rows behind a tile's last, stay in their rows."""
+    tokens, k = 1000, 256
+    x, y, ad = make_case(tokens, 2, [16], k, [64], device=DEV)
+    slots = torch.full((tokens,), -1, dtype=torch.int32, device=DEV)
+    slots[:300], slots[400:777] = 0, 1
+    bad = torch.tensor([3, 129, 300, 301, 777, 500], device=DEV)
+    x[bad] = float("nan")
+    out = ops.lora_add(y, x, load(ops, ad, 16, k, [64], DEV), ops.lora_plan(slots, 2))
+    z, bound = exact(x, y, ad, slots, [64])
+    keep = torch.ones(tokens, dtype=torch.bool, device=DEV)
+    keep[torch.tensor([3, 129, 500], device=DEV)] = False
+    check_sum(out[keep], z[keep], bound[keep])
+    assert bool(out[~keep].isnan().all())
