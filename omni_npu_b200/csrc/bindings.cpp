@@ -794,7 +794,7 @@ Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given
   int64_t width = 0, padded = 0;
   for (int64_t i = 0; i < S; ++i) {
     width += n[i] = (int)slices[i];
-    padded += (slices[i] + 31) / 32 * 32;
+    padded += act || max_rank <= 32 ? (slices[i] + 31) / 32 * 32 : (slices[i] + 63) / 64 * 64;
   }
   TORCH_CHECK_VALUE(x.dim() == 2 && y.dim() == 2 && x.size(0) == y.size(0) && x.size(1) == K && y.size(1) == width,
                     "lora: x ", x.sizes(), " and y ", y.sizes(), " do not fit a projection of ", K, " to ", width);
@@ -805,7 +805,7 @@ Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given
     TORCH_CHECK_VALUE(t->device() == x.device(), "lora: tensors on ", x.device(), " and ", t->device());
   TORCH_CHECK(a.is_contiguous() && b.is_contiguous() && a.dim() == 2 && b.dim() == 2 && a.size(0) == L && b.size(0) == L &&
                         a.size(1) == S * max_rank * ((K + 31) / 32 * 32) && b.size(1) == padded * max_rank,
-              "lora: factors [slots, slices * rank * K] and [slots, columns * rank], K and columns in whole 32");
+              "lora: factors [slots, slices * rank * K] and [slots, columns * rank], K in whole 32, columns in whole 64 (32)");
   CHECK_I32(ranks);
   CHECK_I32(plan);
   CHECK_I32(status);

@@ -8,22 +8,24 @@
 // adapter; the slices' A of a slot are joined along the rank.
 //
 // The factors lie in the order in which the matrix instructions take them, so that they are read in whole kilobytes and need no
-// shuffling: A as 8 x 8 matrices (rows of ldmatrix, unswizzled operands of tcgen05), B as lanes hold it (g = lane / 4, q = lane % 4):
+// shuffling: as 8 x 8 matrices (rows of ldmatrix, unswizzled operands of tcgen05), B of stacks up to rank 32, whose products all are
+// mma.sync's, as lanes hold it (g = lane / 4, q = lane % 4):
 //   A  [K / 32][rank / 8][4][rank % 8][8]        8 of K each of eight ranks, four times
-//   B  [N / 32][rank / 16][v = 0, 1][lane][8]    columns 8 (g / 2) + 2 j + g % 2 of 32 for j = 2 v, 2 v + 1 times
+//   B  [N / 64][rank / 8][2][4][8][8]            (interleaved columns: [N / 32][rank / 8][1]...) 8 ranks each of eight columns,
+//                                                the columns of matrix j of a block of 32: 8 (i / 2) + 2 j + i % 2
+//   or [N / 32][rank / 16][v = 0, 1][lane][8]    columns 8 (g / 2) + 2 j + g % 2 of 32 for j = 2 v, 2 v + 1 times
 //                                                k = 2 q, 2 q + 1, 2 q + 8, 2 q + 9 of 16
-// K and N padded with zeros.  The columns of a lane's results are eight neighbours.
+// K and N padded with zeros.  So the columns of a lane's results are eight neighbours.
 //
 // Tokens are grouped by adapter once a step (lora_plan_kernel: a stable counting sort, then tiles of up to `rows` tokens of one
 // adapter).  Two launches apply the adapters, both bound by what they read and write:
 //   lora_shrink_*_kernel  h: CTAs that share K per (tile, some of the joined ranks)
-//   lora_expand_kernel    z: a CTA per (tile, run of column groups)
+//   lora_expand_*_kernel  z: a CTA per (tile, run of column groups)
 // so that many small pieces of work even out adapters of unlike ranks (one cluster per tile for both, h in distributed shared
 // memory, took 56 us where this takes 15: 128 tokens of 31 adapters of ranks 8 to 64).  The second is launched while the first
 // runs and has its first y and factors at hand by the time h is there.  Measured (us, and the time of the bytes at 6.56 TB/s):
-// one token 4.6; 128 tokens of 128 adapters of rank 16, 14336 to 4096 18.4 / 12.4; 8192 tokens of 8, 4096 to 6144 56 / 42;
-// the same to 2 x 14336 with silu, rank 32 165 / 121.  Ranks above some 32 are bound by the second kernel's matrix instructions:
-// 8192 tokens of rank 64, 4096 to 6144 90 / 42 (117 before the first kernel used tcgen05).
+// one token 4.5; 128 tokens of 128 adapters of rank 16, 14336 to 4096 18.2 / 12.4; 8192 tokens of 8, 4096 to 6144 56 / 42;
+// the same to 2 x 14336 with silu, rank 32 167 / 121; 8192 tokens of rank 64, 4096 to 6144 72 / 42, of rank 128 100.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -40,6 +42,7 @@
 namespace b200 {
 
 static constexpr int kLoraMaxSlices = 4;
+static constexpr int kLanesRank = 32;            // up to this largest rank B lies in the order of lanes
 static constexpr int kFewChunk = 4, kManyChunk = 16;  // 8-wide tiles of h that a CTA computes
 static constexpr int kPlanThreads = 1024;
 
@@ -142,13 +145,14 @@ struct LoraParams {
   const int* order;
   const LoraTile* tiles;
   const int* num_tiles;
-  // h, rows in the order of the plan: few rows fp32 [parts][T][h_width], to be summed; many rows bf16 [2][T][h_width], h times the
-  // scale rounded and what that leaves
+  // h, rows in the order of the plan: few rows fp32 [parts][T][h_width], to be summed; many rows bf16 [2][h_width / 8][T][8], h
+  // times the scale rounded and what that leaves
   void* h;
   long long h_plane;                             // T * h_width
   int h_width;                                   // slices * largest rank
   int T, K, slices, parts;
   int stages, stage_bytes;                       // many rows: the first kernel's ring
+  int groups, buffers, max_rank;                         // many rows: groups in flight in the second kernel
   int boxes;                                     // 1: rows of x that follow one another are copied as a box
   int* status;
   int per;                                       // column groups of a CTA of the second kernel
@@ -333,21 +337,25 @@ __device__ __forceinline__ void arrive_when_copied(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Products of 16 of K: x in rows of 128 bytes in the 128-byte swizzle, the factors unswizzled (128 bytes to the next eight of K, 512
-// to the next eight ranks).  Descriptors' low words; ACC: added to what is there.
-template <bool ACC>
-__device__ __forceinline__ void umma_factors(uint32_t d_tmem, uint32_t x_lo, uint32_t f_lo, uint32_t idesc) {
+// Words of descriptors of unswizzled operands: 128 bytes from eight rows to the next eight (high word, SBO) or `rows` times that
+// of 16 bytes of a row to the next 16 (low word, LBO).  Above 18 bits, an address holds the CTA's rank in its cluster.
+__device__ __forceinline__ constexpr uint32_t plain_hi(uint32_t sbo) { return sbo >> 4 | 1u << 14; }
+__device__ __forceinline__ uint32_t plain_lo(uint32_t addr, uint32_t lbo) { return (addr & 0x3FFFF) >> 4 | (lbo >> 4) << 16; }
+
+// A product of 16 of K.  HA, HB: the descriptors' high words; ACC: added to what is there.
+template <uint32_t HA, uint32_t HB, bool ACC>
+__device__ __forceinline__ void umma_words(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
   asm volatile(
       "{\n\t"
-      ".reg .b64 dx, df;\n\t"
+      ".reg .b64 da, db;\n\t"
       ".reg .pred p;\n\t"
-      "mov.b64 dx, {%1, %3};\n\t"
-      "mov.b64 df, {%2, %4};\n\t"
+      "mov.b64 da, {%1, %3};\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
       "setp.eq.u32 p, %6, 1;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], dx, df, %5, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t"
       "}"
       :
-      : "r"(d_tmem), "r"(x_lo), "r"(f_lo), "r"(kSmemDescHiSw128), "r"((512u >> 4) | (1u << 14)), "r"(idesc), "n"(ACC ? 1 : 0)
+      : "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(HA), "r"(HB), "r"(idesc), "n"(ACC ? 1 : 0)
       : "memory");
 }
 
@@ -362,7 +370,6 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
   const uint32_t ring = (smem_u32(smem) + 1023) & ~1023u;
   char* ring_ptr = smem + (ring - smem_u32(smem));
   pdl_wait();
-  pdl_trigger();
   LoraTile tl;
   if (!lora_tile(p, blockIdx.z, tl) || tl.slot < 0) return;
   const int first = p.order[tl.start];
@@ -400,6 +407,7 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
+  pdl_trigger();                                                       // (not before tensor memory is held: the second kernel takes some too)
 
   if (warp < kManyCopies / 32 && !box) {
     const __nv_bfloat16* xs[4];
@@ -447,8 +455,9 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
     }
   } else if (warp == kManyCopies / 32 && lane == 0) {
     const uint32_t idesc = make_idesc(1, 1, kManyRows, width);
-    // (above 18 bits, an address holds the CTA's rank in its cluster)
-    const uint32_t lo = (ring & 0x3FFFF) >> 4, stage_lo = p.stage_bytes >> 4, f_at = (kXBytes >> 4) + ((128u >> 4) << 16);
+    // x in rows of 128 bytes in the 128-byte swizzle; the factors: 128 bytes to the next eight of K, 512 to the next eight ranks
+    constexpr uint32_t HX = kSmemDescHiSw128, HF = plain_hi(512);
+    const uint32_t lo = plain_lo(ring, 0), stage_lo = p.stage_bytes >> 4, f_at = (kXBytes >> 4) + ((128u >> 4) << 16);
     int get = 0;
     uint32_t phase = 0;
     for (int i = 0; i < count; ++i) {
@@ -463,15 +472,15 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
       tc_fence_after_sync();
       const uint32_t x_lo = lo + get * stage_lo, f_lo = x_lo + f_at, f_next = f_lo + width * 4;
       if ((s_lo + i) * 2 + 1 < blocks) {
-        if (i == 0) umma_factors<false>(tmem, x_lo, f_lo, idesc);
-        else umma_factors<true>(tmem, x_lo, f_lo, idesc);
-        umma_factors<true>(tmem, x_lo + 2, f_lo + 16, idesc);
-        umma_factors<true>(tmem, x_lo + 4, f_next, idesc);
-        umma_factors<true>(tmem, x_lo + 6, f_next + 16, idesc);
+        if (i == 0) umma_words<HX, HF, false>(tmem, x_lo, f_lo, idesc);
+        else umma_words<HX, HF, true>(tmem, x_lo, f_lo, idesc);
+        umma_words<HX, HF, true>(tmem, x_lo + 2, f_lo + 16, idesc);
+        umma_words<HX, HF, true>(tmem, x_lo + 4, f_next, idesc);
+        umma_words<HX, HF, true>(tmem, x_lo + 6, f_next + 16, idesc);
       } else {                                                         // the last 32 of K
-        if (i == 0) umma_factors<false>(tmem, x_lo, f_lo, idesc);
-        else umma_factors<true>(tmem, x_lo, f_lo, idesc);
-        umma_factors<true>(tmem, x_lo + 2, f_lo + 16, idesc);
+        if (i == 0) umma_words<HX, HF, false>(tmem, x_lo, f_lo, idesc);
+        else umma_words<HX, HF, true>(tmem, x_lo, f_lo, idesc);
+        umma_words<HX, HF, true>(tmem, x_lo + 2, f_lo + 16, idesc);
       }
       tc_commit(&empty[get]);
       if (++get == p.stages) get = 0, phase ^= 1;
@@ -507,10 +516,13 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
     tc_fence_after_sync();
     tmem_dealloc(tmem, tmem_cols);
   }
-  const int C = p.parts, rank = blockIdx.x, vecs = width / 4;
-  __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p.h) + static_cast<long long>(tl.start) * p.h_width + n0;
-  for (int i = rank * kManyThreads + threadIdx.x; i < tl.count * vecs; i += C * kManyThreads) {
-    const int row = i / vecs, v = i % vecs * 4;
+  // A warp takes four rows x 32 ranks: 128 bytes of a row at once from every part, 64 of h for eight ranks.  (With eight rows x 16
+  // ranks, whole 16 bytes of h a lane but half as much of a part's row at once, the kernel takes 2 to 4 us more.)
+  const int C = p.parts, rank = blockIdx.x, across = (width + 31) / 32, units = (tl.count + 3) / 4 * across;
+  __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p.h) + (static_cast<long long>(n0 / 8) * p.T + tl.start) * 8;
+  for (int i = rank * (kManyThreads / 32) + warp; i < units; i += C * (kManyThreads / 32)) {
+    const int row = i / across * 4 + (lane >> 3), v = i % across * 32 + (lane & 7) * 4;
+    if (row >= tl.count || v >= width) continue;
     const uint32_t at = smem_u32(part + row * pitch + v);
     float4 q[8];                                                       // (8 parts at most)
 #pragma unroll
@@ -522,7 +534,7 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
       if (c < C) sum.x += q[c].x, sum.y += q[c].y, sum.z += q[c].z, sum.w += q[c].w;
     uint2 hi, lo;
     split_h(sum, scale, hi, lo);
-    __nv_bfloat16* dst = h + static_cast<long long>(row) * p.h_width + v;
+    __nv_bfloat16* dst = h + (static_cast<long long>(v / 8) * p.T + row) * 8 + (v & 4);
     *reinterpret_cast<uint2*>(dst) = hi;
     *reinterpret_cast<uint2*>(dst + p.h_plane) = lo;
   }
@@ -531,166 +543,183 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
 }
 
 // ---- z: a CTA has a tile's rows and a run of column groups of one slice, 64 columns of y each (gated: 32 of gate and their 32 of
-// up).  A warp takes every fourth group, 16 rows at a time: y, which comes through a ring of the lane's own, starts its
-// accumulators; a lane's results are eight neighbouring columns twice, so y and the result move 16 bytes a lane, 512 of a row
-// by the four warps.  Many rows: up to 32 ranks B stays in registers for the 64 rows; above (PAIRS), every step of 16 ranks
-// is used for 32 rows, and the registers take the step after next meanwhile (8192 tokens of rank 64, 4096 columns: 43.6 us,
-// with 16 rows 47.3).  Few rows: B comes through the ring as well, 32 ranks a stage.
+// up).  A warp takes 16 rows of a group at a time.  y comes through a ring of the lane's own; a lane's results are eight
+// neighbouring columns twice, so y and the result move 16 bytes a lane.
 static constexpr int kExpandThreads = 128;
 
-template <bool MANY, int ACT, bool PAIRS>
-__global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_kernel(const LoraParams p) {
+// What both kernels find out first: the CTA's slice and groups in it.
+struct LoraRun {
+  int h0, first, r0, r1, N, groups, ga, gb;      // first rank in h, first column of y, ranks (of gate and of up), columns
+  const __nv_bfloat16 *b, *b_up;                 // factors, in blocks of 64 columns (gated: 32)
+};
+
+// per > 0: `at` is a CTA's number among the slices' runs of `per` groups; 0: the run starts at group `at` of all of the slices'.
+template <bool GATED, bool LANES>
+__device__ __forceinline__ LoraRun lora_run(const LoraParams& p, int slot, int at, int per) {
+  constexpr int GW = GATED ? 32 : 64, BC = GATED || LANES ? 32 : 64;   // columns of a group, of a block of B
+  LoraRun c;
+  int slice = 0;
+  c.h0 = c.first = 0;
+  c.b = p.b + max(slot, 0) * p.b_slot;
+  const int* ranks = p.ranks + max(slot, 0) * (p.slices + 1);
+  if constexpr (GATED) {
+    c.r0 = slot >= 0 ? ranks[0] : 0;
+    c.r1 = slot >= 0 ? ranks[1] : 0;
+  } else {
+    for (;; ++slice) {
+      c.r0 = slot >= 0 ? ranks[slice] : 0;
+      const int groups = (p.n[slice] + 63) / 64, steps = per ? (groups + per - 1) / per : groups;
+      if (at < steps) break;
+      at -= steps;
+      c.h0 += c.r0;
+      c.first += p.n[slice];
+      c.b += static_cast<long long>((p.n[slice] + BC - 1) / BC) * c.r0 * BC;
+    }
+    c.r1 = c.r0;
+  }
+  c.N = p.n[slice];
+  c.groups = (c.N + GW - 1) / GW;
+  c.b_up = c.b + (GATED ? static_cast<long long>(c.groups) * c.r0 * 32 : 0);
+  c.ga = per ? at * per : at;
+  c.gb = per ? min(c.groups, c.ga + per) : c.groups;
+  return c;
+}
+
+// 16 rows (g, g + 8 of a lane) x 64 columns of y: into a ring's stage, `st` this lane's place of four of 512 bytes.  Columns behind
+// the slice's last eight are read there; their results are not stored.
+// Gated: the eight pieces of 16 bytes of a row are gate and up in turn, and a lane needs two neighbours; copied so, every request
+// would be for halves of sectors, twice.  So lane q copies pieces q and 4 + q, the latter one place off, and finds its own without
+// bank conflicts (other lanes' copies: a __syncwarp).
+template <bool GATED>
+__device__ __forceinline__ void copy_y(uint32_t st, const __nv_bfloat16* y, int group, int N, int t4, long long at0, long long at1) {
+  const int col = group * 64 + t4 * 8, end = (GATED ? 2 : 1) * N - 8;
+  const __nv_bfloat16 *src0 = y + min(col, end), *src1 = y + min(col + 32, end);
+  constexpr uint32_t swap = GATED ? 16 : 0;
+  cp16(st, src0 + at0);
+  cp16((st + 512) ^ swap, src1 + at0);
+  cp16(st + 1024, src0 + at1);
+  cp16((st + 1536) ^ swap, src1 + at1);
+}
+template <bool GATED>
+__device__ __forceinline__ void get_y(float (&v)[8][4], uint32_t st, int t4) {
+  const uint32_t own = GATED ? (t4 >> 1) * 512 + ((t4 & 1) * 2 ^ t4 >> 1) * 16 - t4 * 16 : 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint4 u = lds16(GATED ? (st + own + i * 1024) ^ s * 16 : st + i * 1024 + s * 512);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[4 * s + j][2 * i] = lo_f(w[j]);
+        v[4 * s + j][2 * i + 1] = hi_f(w[j]);
+      }
+    }
+}
+
+// A lane's results; out_row -1: not a row of the tile.
+template <int ACT>
+__device__ __forceinline__ void store_z(const LoraParams& p, const float (&acc)[8][4], __nv_bfloat16* out, int group, int left,
+                                        long long at0, long long at1) {
   constexpr bool GATED = ACT != kActNone;
-  constexpr int BM = MANY ? 64 : 16, STEP = 4, D = PAIRS ? 6 : 4, STAGE = MANY ? 2048 : 2048 + 4096;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = 2 * i;
+    const long long at = i ? at1 : at0;
+    uint32_t o0[4], o1[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (GATED) {
+        o0[j] = pack_bf16x2(gated_act(ACT, acc[j][e], acc[4 + j][e], p.act_alpha, p.act_limit),
+                            gated_act(ACT, acc[j][e + 1], acc[4 + j][e + 1], p.act_alpha, p.act_limit));
+      } else {
+        o0[j] = pack_bf16x2(acc[j][e], acc[j][e + 1]);
+        o1[j] = pack_bf16x2(acc[4 + j][e], acc[4 + j][e + 1]);
+      }
+    }
+    __nv_bfloat16* row = out + at + group * (GATED ? 32 : 64);
+    if (at >= 0 && left > 0) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+    if (!GATED && at >= 0 && left > 32) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+  }
+}
+
+// ---- few rows: a warp has every fourth group.  B comes through the ring as well, 32 ranks a stage; y starts the accumulators.
+template <int ACT, bool LANES>
+__global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_few_kernel(const LoraParams p) {
+  constexpr bool GATED = ACT != kActNone;
+  constexpr int BM = 16, STEP = 4, D = 4, STAGE = 2048 + 4096;
   constexpr int GW = GATED ? 32 : 64;                                  // columns of a slice in a group
   extern __shared__ __align__(128) char smem[];
-  __shared__ long long y_row[BM], out_row[BM];                         // where a row of the tile starts; out_row -1: none
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const bool in_place = !GATED && p.out == p.y;
   // Everything but h is older than the first kernel, which has started only behind it: no wait yet.
   LoraTile tl;
-  bool any = lora_tile(p, MANY ? blockIdx.y >> 1 : blockIdx.y, tl);
-  if constexpr (MANY) {                                                // a half of the rows
-    const int from = (blockIdx.y & 1) * BM;
-    any = any && from < tl.count;
-    tl.start += from;
-    tl.count = min(BM, tl.count - from);
-  }
-  if (!any) {
+  if (!lora_tile(p, blockIdx.y, tl)) {
     pdl_wait();
     return;
   }
-  if (threadIdx.x < BM) {
-    const bool ok = threadIdx.x < tl.count;
-    const int t = p.order[tl.start + (ok ? threadIdx.x : 0)];          // (rows behind the last read what the first does)
-    y_row[threadIdx.x] = t * p.y_stride;
-    out_row[threadIdx.x] = ok ? t * p.out_stride : -1;
-  }
-  // this CTA's slice and groups in it; of the slice: first rank in h, first column of y, factors (in blocks of 32 columns)
-  int slice = 0, block = blockIdx.x, h0 = 0, first = 0, r0 = 0, r1 = 0;
-  const __nv_bfloat16* b = p.b + max(tl.slot, 0) * p.b_slot + lane * 8;
-  const int* ranks = p.ranks + max(tl.slot, 0) * (p.slices + 1);
-  if constexpr (GATED) {
-    r0 = tl.slot >= 0 ? ranks[0] : 0;
-    r1 = tl.slot >= 0 ? ranks[1] : 0;
-  } else {
-    for (;; ++slice) {
-      r0 = tl.slot >= 0 ? ranks[slice] : 0;
-      const int blocks = ((p.n[slice] + 63) / 64 + p.per - 1) / p.per;
-      if (block < blocks) break;
-      block -= blocks;
-      h0 += r0;
-      first += p.n[slice];
-      b += static_cast<long long>((p.n[slice] + 31) / 32) * r0 * 32;
-    }
-    r1 = r0;
-  }
-  const int N = p.n[slice], b_last = (N + 31) / 32 - 1, k0 = r0 / 16, k1 = r1 / 16, ks = max(k0, k1);
+  // where a lane's two rows start (rows behind the last read what the first does, and are not stored)
+  const int t0 = p.order[tl.start + (g < tl.count ? g : 0)], t1 = p.order[tl.start + (g + 8 < tl.count ? g + 8 : 0)];
+  const long long y0 = t0 * p.y_stride, y1 = t1 * p.y_stride;
+  const long long o0 = g < tl.count ? t0 * p.out_stride : -1, o1 = g + 8 < tl.count ? t1 * p.out_stride : -1;
+  const LoraRun c = lora_run<GATED, LANES>(p, tl.slot, blockIdx.x, p.per);
+  const int k0 = c.r0 / 16, k1 = c.r1 / 16, ks = max(k0, k1);
   if (ks == 0 && in_place) {
     pdl_wait();
     return;
   }
-  const __nv_bfloat16* b_up = b + (GATED ? static_cast<long long>(b_last + 1) * r0 * 32 : 0);
-  const int ga = block * p.per + warp, gb = min((N + GW - 1) / GW, (block + 1) * p.per);
-  const int ms = (tl.count + 15) / 16;
-  const float scale = !MANY && tl.slot >= 0 ? lora_scale(p, tl.slot) : 0.f;
+  const float scale = tl.slot >= 0 ? lora_scale(p, tl.slot) : 0.f;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * D * STAGE + lane * 16;
-  const __nv_bfloat16* y = p.y + first;
-  __nv_bfloat16* out = p.out + first + t4 * 8;
-  // Gated: the eight pieces of 16 bytes of a row are gate and up in turn, and a lane needs two neighbours; copied so, every
-  // request would be for halves of sectors, twice.  So lane q copies pieces q and 4 + q, the latter one place off, and finds
-  // its own without bank conflicts at y_at and y_at ^ 16.
-  constexpr uint32_t y_swap = GATED ? 16 : 0;
-  const uint32_t y_at = GATED ? (t4 >> 1) * 512 + ((t4 & 1) * 2 ^ t4 >> 1) * 16 - t4 * 16 : 0;
-  // 16 ranks (step k) of 32 columns of group gi: its half s, or gate / up.  Past the end: any others, whose results are not used
-  auto b_at = [&](int gi, int s, int k) {
-    if constexpr (GATED) return (s ? b_up : b) + (static_cast<long long>(gi) * (s ? k1 : k0) + min(k, max((s ? k1 : k0) - 1, 0))) * 512;
-    return b + (static_cast<long long>(min(2 * gi + s, b_last)) * k0 + min(k, k0 - 1)) * 512;
-  };
-  __syncthreads();
-  // the ring's next stage: group cg and its rows cm (few rows: steps ck, ck + 1).  Columns behind the slice's last eight are read
-  // there; their results are not stored.
-  int cg = ga, cm = 0, ck = 0;
+  const __nv_bfloat16* y = p.y + c.first;
+  __nv_bfloat16* out = p.out + c.first + t4 * 8;
+  // the ring's next stage: group cg, steps ck, ck + 1 of 16 ranks
+  int cg = c.ga + warp, ck = 0;
   uint32_t put = ring;
   auto copy = [&]() {
-    if (cg < gb) {
+    if (cg < c.gb) {
       const uint32_t st = put;
       put = put + STAGE == ring + D * STAGE ? ring : put + STAGE;
-      if (MANY || ck == 0) {
-        const int col = cg * 64 + t4 * 8, end = (GATED ? 2 : 1) * N - 8;
-        const __nv_bfloat16 *src0 = y + min(col, end), *src1 = y + min(col + 32, end);
-        const long long at0 = y_row[cm * 16 + g], at1 = y_row[cm * 16 + g + 8];
-        cp16(st, src0 + at0);
-        cp16((st + 512) ^ y_swap, src1 + at0);
-        cp16(st + 1024, src0 + at1);
-        cp16((st + 1536) ^ y_swap, src1 + at1);
-      }
-      if constexpr (MANY) {
-        if (++cm == ms) {
-          cm = 0;
-          cg += STEP;
-        }
-      } else {
+      if (ck == 0) copy_y<GATED>(st, y, cg, c.N, t4, y0, y1);
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (ck + k < ks) {
+      for (int k = 0; k < 2; ++k)
+        if (ck + k < ks) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              const __nv_bfloat16* src = b_at(cg, s, ck + k);
-              cp16(st + 2048 + k * 2048 + s * 1024, src);
-              cp16(st + 2048 + k * 2048 + s * 1024 + 512, src + 256);
-            }
+          for (int s = 0; s < 2; ++s) {                                // gated: gate and up; past the end of one, its last
+            const int steps = GATED && s ? k1 : k0;
+            const __nv_bfloat16* src =
+                GATED   ? (s ? c.b_up : c.b) + (static_cast<long long>(cg) * steps + min(ck + k, max(steps - 1, 0))) * 512
+                : LANES ? c.b + (static_cast<long long>(min(2 * cg + s, (c.N - 1) / 32)) * k0 + ck + k) * 512
+                        : c.b + (static_cast<long long>(cg) * k0 + ck + k) * 1024 + s * 512;
+            cp16(st + 2048 + k * 2048 + s * 1024, src + lane * 8);
+            cp16(st + 2048 + k * 2048 + s * 1024 + 512, src + lane * 8 + 256);
           }
-        ck += 2;
-        if (ck >= ks) {
-          ck = 0;
-          cg += STEP;
         }
+      ck += 2;
+      if (ck >= ks) {
+        ck = 0;
+        cg += STEP;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
   for (int i = 0; i < D - 1; ++i) copy();
-  uint4 bv[2][4];                                                      // many rows: B of two steps, half s at 2 s
-  auto load_b = [&](uint4 (&v)[4], int gi, int k) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const __nv_bfloat16* src = b_at(gi, s, k);
-      v[2 * s] = *reinterpret_cast<const uint4*>(src);
-      v[2 * s + 1] = *reinterpret_cast<const uint4*>(src + 256);
-    }
-  };
-  if (MANY && ks > 0 && ga < gb) {
-    load_b(bv[0], ga, 0);
-    if (ks > 1) load_b(bv[1], ga, 1);
-  }
   pdl_wait();
   pdl_trigger();
 
   // h of this slice (gated: of both) into shared memory, [2][BM][h_pitch]
   const uint32_t h_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + 4 * D * STAGE;
-  const int sum_r = GATED ? r0 + r1 : r0;
-  if constexpr (MANY) {
-    const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(p.h) + static_cast<long long>(tl.start) * p.h_width + h0;
-    const int pieces = sum_r / 8;
-    for (int i = threadIdx.x; i < 2 * tl.count * pieces; i += kExpandThreads) {
-      const int piece = i % pieces, row = i / pieces >> 1, rest = i / pieces & 1;
-      cp16(h_at + ((rest * BM + row) * p.h_pitch + piece * 8) * 2,
-           h + rest * p.h_plane + static_cast<long long>(row) * p.h_width + piece * 8);
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  } else {
-    const float* h = static_cast<const float*>(p.h) + static_cast<long long>(tl.start) * p.h_width + h0;
+  {
+    const float* h = static_cast<const float*>(p.h) + static_cast<long long>(tl.start) * p.h_width + c.h0;
     __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(smem + 4 * D * STAGE);
-    const int vecs = sum_r / 4;
+    const int vecs = (GATED ? c.r0 + c.r1 : c.r0) / 4;
     for (int i = threadIdx.x; i < tl.count * vecs; i += kExpandThreads) {
       const int row = i / vecs, v = i % vecs * 4;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       const float* src = h + static_cast<long long>(row) * p.h_width + v;
 #pragma unroll 4
-      for (int c = 0; c < p.parts; ++c) {
-        const float4 q = *reinterpret_cast<const float4*>(src + c * p.h_plane);
+      for (int part = 0; part < p.parts; ++part) {
+        const float4 q = *reinterpret_cast<const float4*>(src + part * p.h_plane);
         sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
       }
       uint2 hi, lo;
@@ -700,75 +729,192 @@ __global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_ker
     }
   }
   __syncthreads();
-  const uint32_t hf = h_at + ((lane & 15) * p.h_pitch + (lane >> 4) * 8) * 2;
-  const uint32_t lo_at = 2 * BM * p.h_pitch, m_step = 32 * p.h_pitch;
+  const uint32_t hf = h_at + ((lane & 15) * p.h_pitch + (lane >> 4) * 8) * 2, lo_at = 2 * BM * p.h_pitch;
+  // two tiles of eight columns, 16 ranks of each as two matrices
+  const uint32_t b_lane = 2048 + (lane >> 3 & 1) * (GATED ? 512 : 1024) + (lane >> 4) * 128 + (lane & 7) * 16 - lane * 16;
   uint32_t get = ring;
   auto next = [&]() {
     asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
-    if (GATED) __syncwarp();
+    __syncwarp();
     const uint32_t st = get;
     get = get + STAGE == ring + D * STAGE ? ring : get + STAGE;
     return st;
   };
-  // the accumulators of 16 rows, from a stage of the ring
-  auto start = [&](float (&acc)[8][4], uint32_t st) {
+  for (int gi = c.ga + warp; gi < c.gb; gi += STEP) {
+    float acc[8][4];
+    uint32_t st = next();
+    get_y<GATED>(acc, st, t4);
+    for (int k = 0;;) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int u = 0; u < 2; ++u)
+        if (k + u < ks) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (GATED && k + u >= (s ? k1 : k0)) continue;
+            if (GATED || s == 0) {
+              const uint32_t at = hf + (k + u) * 32 + (GATED && s ? c.r0 * 2 : 0);
+              ldmatrix4(hi, at);
+              ldmatrix4(lo, at + lo_at);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+              uint32_t b[4];
+              if constexpr (LANES) {
+                const uint4 v = lds16(st + 2048 + u * 2048 + s * 1024 + j * 256);
+                b[0] = v.x, b[1] = v.y, b[2] = v.z, b[3] = v.w;
+              } else {
+                ldmatrix4(b, st + b_lane + u * 2048 + (GATED ? s * 1024 + j * 128 : (4 * s + j) * 128));
+              }
+              mma_bf16(acc[4 * s + j], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
+              mma_bf16(acc[4 * s + j + 1], hi[0], hi[1], hi[2], hi[3], b[2], b[3]);
+              mma_bf16(acc[4 * s + j], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
+              mma_bf16(acc[4 * s + j + 1], lo[0], lo[1], lo[2], lo[3], b[2], b[3]);
+            }
+          }
+        }
+      copy();
+      k += 2;
+      if (k >= ks) break;
+      st = next();
+    }
+    store_z<ACT>(p, acc, out, gi, c.N - gi * GW - t4 * 8, o0, o1);
+  }
+}
+
+// ---- many rows, up to 32 ranks: mma.sync, half a tile's rows, a warp has every fourth group.  y starts the accumulators, and B stays
+// in registers for the 64 rows: little to compute, so that four CTAs an SM keep memory busy (8192 tokens of rank 16, 4096 to
+// 6144: 33 us for 31 of bytes; the tcgen05 kernel takes 4 to 10 more, gated 9 to 35).
+// PAIRS: gated ranks above 144, whose h the tcgen05 kernel has no room for.  Every step of 16 ranks is used for 32 rows, and the
+// registers take the step after next meanwhile.
+template <int ACT, bool PAIRS>
+__global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_many_kernel(const LoraParams p) {
+  constexpr bool GATED = ACT != kActNone, LANES = !PAIRS;
+  constexpr int BM = 64, STEP = 4, D = PAIRS ? 6 : 4, STAGE = 2048;
+  constexpr int GW = GATED ? 32 : 64;                                  // columns of a slice in a group
+  extern __shared__ __align__(128) char smem[];
+  __shared__ long long y_row[BM], out_row[BM];                         // where a row of the tile starts; out_row -1: none
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const bool in_place = !GATED && p.out == p.y;
+  // Everything but h is older than the first kernel, which has started only behind it: no wait yet.
+  LoraTile tl;
+  const int from = (blockIdx.y & 1) * BM;
+  if (!lora_tile(p, blockIdx.y >> 1, tl) || from >= tl.count) {
+    pdl_wait();
+    return;
+  }
+  tl.start += from;
+  tl.count = min(BM, tl.count - from);
+  if (threadIdx.x < BM) {
+    const bool ok = threadIdx.x < tl.count;
+    const int t = p.order[tl.start + (ok ? threadIdx.x : 0)];          // (rows behind the last read what the first does)
+    y_row[threadIdx.x] = t * p.y_stride;
+    out_row[threadIdx.x] = ok ? t * p.out_stride : -1;
+  }
+  const LoraRun c = lora_run<GATED, LANES>(p, tl.slot, blockIdx.x, p.per);
+  const int k0 = c.r0 / 16, k1 = c.r1 / 16, ks = max(k0, k1);
+  if (ks == 0 && in_place) {
+    pdl_wait();
+    return;
+  }
+  const int ga = c.ga + warp, gb = c.gb, ms = (tl.count + 15) / 16;
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * D * STAGE + lane * 16;
+  const __nv_bfloat16* y = p.y + c.first;
+  __nv_bfloat16* out = p.out + c.first + t4 * 8;
+  __syncthreads();
+  int cg = ga, cm = 0;                                                 // the ring's next stage: group cg and its rows cm
+  uint32_t put = ring;
+  auto copy = [&]() {
+    if (cg < gb) {
+      copy_y<GATED>(put, y, cg, c.N, t4, y_row[cm * 16 + g], y_row[cm * 16 + g + 8]);
+      put = put + STAGE == ring + D * STAGE ? ring : put + STAGE;
+      if (++cm == ms) {
+        cm = 0;
+        cg += STEP;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < D - 1; ++i) copy();
+  // B of two steps: eight times eight columns.  Gated, past the end of one of the two: its last, not used
+  uint2 bv[2][8];
+  auto load_b = [&](uint2 (&v)[8], int gi, int k) {
+    if constexpr (LANES) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const uint4 v = lds16(GATED ? (st + y_at + i * 1024) ^ s * 16 : st + i * 1024 + s * 512);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const int steps = GATED && s ? k1 : k0, block = GATED ? gi : min(2 * gi + s, (c.N - 1) / 32);
+        const __nv_bfloat16* src =
+            (s && GATED ? c.b_up : c.b) + (static_cast<long long>(block) * steps + min(k, max(steps - 1, 0))) * 512 + lane * 8;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          acc[4 * s + j][2 * i] = lo_f(w[j]);
-          acc[4 * s + j][2 * i + 1] = hi_f(w[j]);
+        for (int j = 0; j < 2; ++j) {
+          const uint4 q = *reinterpret_cast<const uint4*>(src + j * 256);
+          v[4 * s + 2 * j] = make_uint2(q.x, q.y);
+          v[4 * s + 2 * j + 1] = make_uint2(q.z, q.w);
         }
       }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int steps = GATED && j >= 4 ? k1 : k0;
+      const __nv_bfloat16* src =
+          GATED ? (j >= 4 ? c.b_up : c.b) + (static_cast<long long>(gi) * steps + min(k, max(steps - 1, 0))) * 512 + (j & 3) * 64
+                : c.b + (static_cast<long long>(gi) * k0 + min(k, k0 - 1)) * 1024 + j * 64;
+      v[j].x = *reinterpret_cast<const uint32_t*>(src + lane * 2);
+      v[j].y = *reinterpret_cast<const uint32_t*>(src + lane * 2 + (GATED ? 256 : 512));
+    }
+  };
+  if (ks > 0 && ga < gb) {
+    load_b(bv[0], ga, 0);
+    if (ks > 1) load_b(bv[1], ga, 1);
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  // h of this slice (gated: of both) into shared memory, [2][BM][h_pitch]
+  const uint32_t h_at = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + 4 * D * STAGE;
+  {
+    const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(p.h) + (static_cast<long long>(c.h0 / 8) * p.T + tl.start) * 8;
+    const int pieces = (GATED ? c.r0 + c.r1 : c.r0) / 8;
+    for (int i = threadIdx.x; i < 2 * tl.count * pieces; i += kExpandThreads) {
+      const int row = i % tl.count, q = i / tl.count, rest = q >= pieces, piece = q - rest * pieces;
+      cp16(h_at + ((rest * BM + row) * p.h_pitch + piece * 8) * 2,
+           h + rest * p.h_plane + (static_cast<long long>(piece) * p.T + row) * 8);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  __syncthreads();
+  const uint32_t hf = h_at + ((lane & 15) * p.h_pitch + (lane >> 4) * 8) * 2;
+  const uint32_t lo_at = 2 * BM * p.h_pitch, m_step = 32 * p.h_pitch;
+  uint32_t get = ring;
+  // the accumulators of 16 rows, from a stage of the ring
+  auto start = [&](float (&acc)[8][4]) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+    if (GATED) __syncwarp();
+    get_y<GATED>(acc, get, t4);
+    get = get + STAGE == ring + D * STAGE ? ring : get + STAGE;
+    copy();
   };
   // step k of h of rows m times its B
-  auto multiply = [&](float (&acc)[8][4], int m, int k, const uint4& p0, const uint4& p1, const uint4& q0, const uint4& q1) {
+  auto multiply = [&](float (&acc)[8][4], int m, int k, const uint2 (&b)[8]) {
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       if (GATED && k >= (s ? k1 : k0)) continue;
-      const uint4 &v = s ? q0 : p0, &w = s ? q1 : p1;
-      const uint32_t at = hf + m * m_step + k * 32 + (GATED && s ? r0 * 2 : 0);
       if (GATED || s == 0) {
+        const uint32_t at = hf + m * m_step + k * 32 + (GATED && s ? c.r0 * 2 : 0);
         ldmatrix4(hi, at);
         ldmatrix4(lo, at + lo_at);
       }
-      float(*c)[4] = acc + 4 * s;
-      mma_bf16(c[0], hi[0], hi[1], hi[2], hi[3], v.x, v.y);
-      mma_bf16(c[1], hi[0], hi[1], hi[2], hi[3], v.z, v.w);
-      mma_bf16(c[2], hi[0], hi[1], hi[2], hi[3], w.x, w.y);
-      mma_bf16(c[3], hi[0], hi[1], hi[2], hi[3], w.z, w.w);
-      mma_bf16(c[0], lo[0], lo[1], lo[2], lo[3], v.x, v.y);
-      mma_bf16(c[1], lo[0], lo[1], lo[2], lo[3], v.z, v.w);
-      mma_bf16(c[2], lo[0], lo[1], lo[2], lo[3], w.x, w.y);
-      mma_bf16(c[3], lo[0], lo[1], lo[2], lo[3], w.z, w.w);
+#pragma unroll
+      for (int j = 4 * s; j < 4 * s + 4; ++j) mma_bf16(acc[j], hi[0], hi[1], hi[2], hi[3], b[j].x, b[j].y);
+#pragma unroll
+      for (int j = 4 * s; j < 4 * s + 4; ++j) mma_bf16(acc[j], lo[0], lo[1], lo[2], lo[3], b[j].x, b[j].y);
     }
   };
   auto store = [&](const float (&acc)[8][4], int gi, int m) {
-    const int left = N - gi * GW - t4 * 8;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int e = 2 * i;
-      const long long at = out_row[m * 16 + i * 8 + g];
-      uint32_t o0[4], o1[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (GATED) {
-          o0[j] = pack_bf16x2(gated_act(ACT, acc[j][e], acc[4 + j][e], p.act_alpha, p.act_limit),
-                              gated_act(ACT, acc[j][e + 1], acc[4 + j][e + 1], p.act_alpha, p.act_limit));
-        } else {
-          o0[j] = pack_bf16x2(acc[j][e], acc[j][e + 1]);
-          o1[j] = pack_bf16x2(acc[4 + j][e], acc[4 + j][e + 1]);
-        }
-      }
-      __nv_bfloat16* row = out + at + gi * GW;
-      if (at >= 0 && left > 0) *reinterpret_cast<uint4*>(row) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
-      if (!GATED && at >= 0 && left > 32) *reinterpret_cast<uint4*>(row + 32) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
-    }
+    store_z<ACT>(p, acc, out, gi, c.N - gi * GW - t4 * 8, out_row[m * 16 + g], out_row[m * 16 + g + 8]);
   };
   for (int gi = ga; gi < gb; gi += STEP) {
     const bool more = gi + STEP < gb;
@@ -777,20 +923,16 @@ __global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_ker
       for (int m = 0; m < ms; m += 2) {
         const bool two = m + 1 < ms, last = m + 2 >= ms;
         float acc[2][8][4];
-        start(acc[0], next());
-        copy();
-        if (two) {
-          start(acc[1], next());
-          copy();
-        }
+        start(acc[0]);
+        if (two) start(acc[1]);
         for (int k = 0; k < ks; k += 2) {
           const bool tail = k + 2 >= ks;
           const int ng = tail && last && more ? gi + STEP : gi, nk = tail ? 0 : k + 2;
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             if (k + u < ks) {
-              multiply(acc[0], m, k + u, bv[u][0], bv[u][1], bv[u][2], bv[u][3]);
-              if (two) multiply(acc[1], m + 1, k + u, bv[u][0], bv[u][1], bv[u][2], bv[u][3]);
+              multiply(acc[0], m, k + u, bv[u]);
+              if (two) multiply(acc[1], m + 1, k + u, bv[u]);
             }
             load_b(bv[u], ng, nk + u);
           }
@@ -801,75 +943,357 @@ __global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_ker
     } else {
       for (int m = 0; m < ms; ++m) {
         float acc[8][4];
-        uint32_t st = next();
-        start(acc, st);
-        if constexpr (MANY) {
-          copy();
+        start(acc);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (u < ks) multiply(acc, m, u, bv[u]);
+        if (m + 1 == ms && more)
 #pragma unroll
           for (int u = 0; u < 2; ++u)
-            if (u < ks) multiply(acc, m, u, bv[u][0], bv[u][1], bv[u][2], bv[u][3]);
-          if (m + 1 == ms && more)
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              if (u < ks) load_b(bv[u], gi + STEP, u);
-        } else {
-          for (int k = 0;;) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              if (k + u < ks) {
-                const uint32_t at = st + 2048 + u * 2048;
-                multiply(acc, m, k + u, lds16(at), lds16(at + 512), lds16(at + 1024), lds16(at + 1536));
-              }
-            copy();
-            k += 2;
-            if (k >= ks) break;
-            st = next();
-          }
-        }
+            if (u < ks) load_b(bv[u], gi + STEP, u);
         store(acc, gi, m);
       }
     }
   }
 }
 
-static constexpr int kShrinkFewSmem = kFewWarps * kFewRing, kExpandSmem = 168 * 1024;
+// ---- many rows, more than 32 ranks: the products on tcgen05 (h's two parts one after the other along K), 64 columns of tensor
+// memory a group, NB groups in flight.  CTAs stay for the whole kernel and share out (tiles x groups) evenly.  Four warps add y to
+// what they read from tensor memory, 32 rows each; one thread issues the products, one warp copies h and, in bulk, B of each
+// group.  Both kernels, 4096 to 6144: 8192 tokens of rank 64 72 us (94 with mma.sync), of rank 128 100 (149); 4096 tokens of rank
+// 64 to 2 x 14336 with silu 103 (196); 1024 tokens of rank 64 22 (28).  Two CTAs an SM even if the ring of y is short for it: 2847
+// tokens of ranks 33 to 128 40 us, 44 with one.
+static constexpr int kExpandTcThreads = 192;
 
-template <bool MANY, int ACT, bool PAIRS>
-static int launch_lora(const LoraParams& p, unsigned tiles, unsigned chunks, unsigned blocks, cudaStream_t stream) {
-  auto expand = lora_expand_kernel<MANY, ACT, PAIRS>;
+__device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, float (&v)[8][4]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
+        "=f"(v[2][0]), "=f"(v[2][1]), "=f"(v[2][2]), "=f"(v[2][3]), "=f"(v[3][0]), "=f"(v[3][1]), "=f"(v[3][2]), "=f"(v[3][3]),
+        "=f"(v[4][0]), "=f"(v[4][1]), "=f"(v[4][2]), "=f"(v[4][3]), "=f"(v[5][0]), "=f"(v[5][1]), "=f"(v[5][2]), "=f"(v[5][3]),
+        "=f"(v[6][0]), "=f"(v[6][1]), "=f"(v[6][2]), "=f"(v[6][3]), "=f"(v[7][0]), "=f"(v[7][1]), "=f"(v[7][2]), "=f"(v[7][3])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Products of one group: `steps` of 16 ranks, for both parts of h.
+template <int ROWS, int BW>
+__device__ __forceinline__ void expand_group(uint32_t d, uint32_t h_lo, uint32_t h_part, uint32_t b_lo, int steps) {
+  constexpr uint32_t HI = plain_hi(128), idesc = make_idesc(1, 1, ROWS, BW);
+  constexpr uint32_t h_step = ROWS * 32 / 16, b_step = BW * 32 / 16;
+  umma_words<HI, HI, false>(d, h_lo, b_lo, idesc);
+  umma_words<HI, HI, true>(d, h_lo + h_part, b_lo, idesc);
+  for (int k = 1; k < steps; ++k) {
+    umma_words<HI, HI, true>(d, h_lo + k * h_step, b_lo + k * b_step, idesc);
+    umma_words<HI, HI, true>(d, h_lo + h_part + k * h_step, b_lo + k * b_step, idesc);
+  }
+}
+
+template <int ACT, int D>
+__global__ void __launch_bounds__(kExpandTcThreads, D == 8 ? 1 : 2)
+lora_expand_tc_kernel(const __grid_constant__ LoraParams p) {
+  constexpr bool GATED = ACT != kActNone;
+  constexpr int ROWS = 128, STAGE = 2048, GW = GATED ? 32 : 64;
+  extern __shared__ __align__(128) char smem[];
+  __shared__ uint64_t b_full[4], d_full[4], d_empty[4], h_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int token[ROWS], gave_up;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const bool in_place = !GATED && p.out == p.y;
+  // Everything but h is older than the first kernel, which has started only behind it: no wait yet.
+  const long long work = static_cast<long long>(*p.num_tiles) * p.groups;
+  long long pos = work * blockIdx.x / gridDim.x;
+  const long long end = work * (blockIdx.x + 1) / gridDim.x;
+  const int NB = p.buffers;
+  if (threadIdx.x == 160) {
+    for (int i = 0; i < NB; ++i) {
+      mbar_init(&b_full[i], 1);
+      mbar_init(&d_full[i], 1);
+      mbar_init(&d_empty[i], 4);
+    }
+    mbar_init(&h_full, 1);
+    gave_up = 0;
+    fence_barrier_init();
+  }
+  // shared memory: rings of the four warps, NB times B of a group, h [2][ranks / 8][ROWS][8]
+  char* b_ptr = smem + 4 * D * STAGE;
+  const int b_bytes = p.max_rank * 128;
+  char* h_ptr = b_ptr + NB * b_bytes;
+  bool started = false;
+  // (no kernel behind this one starts before tensor memory is held: it may take some too)
+  auto ready = [&]() {
+    if (started) return;
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    pdl_wait();
+    pdl_trigger();
+  };
+  // each role's place among the NB, and in the warps' rings
+  int buf = 0;
+  uint32_t phase = warp == 5 ? 1 : 0, h_phase = 0, tmem = 0;
+  const uint32_t ring = smem_u32(smem) + warp * D * STAGE + lane * 16;
+  uint32_t put = ring, get = ring;
+
+  while (pos < end) {
+    // a stretch: one tile, one slice
+    const int tile = static_cast<int>(pos / p.groups);
+    const int4 entry = *reinterpret_cast<const int4*>(p.tiles + tile);
+    const int slot = entry.x, start = entry.y, rows = entry.z;
+    LoraRun c = lora_run<GATED, false>(p, slot, static_cast<int>(pos % p.groups), 0);
+    const int n = static_cast<int>(min(static_cast<long long>(c.gb - c.ga), end - pos));
+    pos += n;
+    const int k0 = c.r0 / 16, k1 = c.r1 / 16;
+    const bool products = k0 + k1 > 0;
+    if (!products && in_place) continue;
+    const int hk = GATED ? c.r0 + c.r1 : c.r0;
+    __syncthreads();                                                   // the stretch before is through
+    if (threadIdx.x < ROWS) token[threadIdx.x] = p.order[start + (threadIdx.x < rows ? threadIdx.x : 0)];
+    if (warp < 4) {
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const int row0 = warp * (ROWS / 4), ms = min(ROWS / 64, max(0, (rows - row0 + 15) / 16));
+      const __nv_bfloat16* y = p.y + c.first;
+      __nv_bfloat16* out = p.out + c.first + t4 * 8;
+      int cg = ms ? 0 : n, cm = 0;
+      auto copy = [&]() {
+        if (cg < n) {
+          const int row = row0 + cm * 16 + g;
+          copy_y<GATED>(put, y, c.ga + cg, c.N, t4, token[row] * p.y_stride, token[row + 8] * p.y_stride);
+          put = put + STAGE == ring + D * STAGE ? ring : put + STAGE;
+          if (++cm == ms) cm = 0, ++cg;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+#pragma unroll
+      for (int i = 0; i < D - 1; ++i) copy();
+      ready();
+      tmem = tmem_slot;
+      for (int i = 0; i < n; ++i) {
+        if (products) {
+          if (!*static_cast<volatile int*>(&gave_up) && !mbar_wait(&d_full[buf], phase)) {
+            atomicCAS(p.status, 0, kStatusTimeoutTmemFull);
+            gave_up = 1;
+          }
+          tc_fence_after_sync();
+          __syncwarp();
+          if (ms == 0 && lane == 0) mbar_arrive(&d_empty[buf]);
+        }
+#pragma unroll 1
+        for (int m = 0; m < ms; ++m) {
+          float acc[8][4], v[8][4];
+          if (products) {
+            tmem_ld_16x256b_x8(tmem + ((warp * 32 + m * 16) << 16) + buf * 64, acc);
+            tmem_ld_wait();
+            if (m + 1 == ms) {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&d_empty[buf]);
+            }
+          }
+          asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+          if (GATED) __syncwarp();
+          get_y<GATED>(v, get, t4);
+          get = get + STAGE == ring + D * STAGE ? ring : get + STAGE;
+          copy();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[j][e] = (GATED ? (j < 4 ? k0 : k1) != 0 : products) ? acc[j][e] + v[j][e] : v[j][e];
+          const int row = row0 + m * 16 + g;
+          store_z<ACT>(p, acc, out, c.ga + i, c.N - (c.ga + i) * GW - t4 * 8, row < rows ? token[row] * p.out_stride : -1,
+                       row + 8 < rows ? token[row + 8] * p.out_stride : -1);
+        }
+        if (products && ++buf == NB) buf = 0, phase ^= 1;
+      }
+    } else if (warp == 4) {
+      if (!started) {
+        tmem_alloc(&tmem_slot, NB * 64);
+        tmem_relinquish();
+      }
+      ready();
+      tmem = tmem_slot;
+      if (products && lane == 0) {
+        const uint32_t h_lo = plain_lo(smem_u32(h_ptr), ROWS * 16), b_base = plain_lo(smem_u32(b_ptr), GW * 16);
+        const uint32_t h_part = hk / 8 * ROWS;                         // (in 16 bytes)
+        const uint32_t h_up = h_lo + c.r0 / 8 * ROWS, b_up = c.r0 * 4; // gated: r0 / 8 times 32 columns
+        bool ok = !*static_cast<volatile int*>(&gave_up) && mbar_wait(&h_full, h_phase);
+        for (int i = 0; i < n && ok; ++i) {
+          ok = mbar_wait(&b_full[buf], phase) && mbar_wait(&d_empty[buf], phase ^ 1);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint32_t d = tmem + buf * 64, b_lo = b_base + buf * (b_bytes >> 4);
+          if (k0) expand_group<ROWS, GW>(d, h_lo, h_part, b_lo, k0);
+          if (GATED && k1) expand_group<ROWS, GW>(d + 32, h_up, h_part, b_lo + b_up, k1);
+          tc_commit(&d_full[buf]);
+          if (++buf == NB) buf = 0, phase ^= 1;
+        }
+        if (!ok) {
+          atomicCAS(p.status, 0, kStatusTimeoutFullBarrier);
+          gave_up = 1;
+        }
+      }
+      h_phase ^= products;
+    } else {
+      int i = 0;
+      // B of a group (gated: of gate and of up), when the products that were before in its place are through
+      auto load = [&]() {
+        if (*static_cast<volatile int*>(&gave_up) || !mbar_wait(&d_full[buf], phase)) return false;
+        char* dst = b_ptr + buf * b_bytes;
+        mbar_arrive_expect_tx(&b_full[buf], (GATED ? hk * 32 : hk * 64) * 2);
+        const long long at = c.ga + i;
+        if (GATED) {
+          if (c.r0) bulk_load_1d(dst, c.b + at * c.r0 * 32, c.r0 * 64, &b_full[buf]);
+          if (c.r1) bulk_load_1d(dst + c.r0 * 64, c.b_up + at * c.r1 * 32, c.r1 * 64, &b_full[buf]);
+        } else {
+          bulk_load_1d(dst, c.b + at * c.r0 * 64, c.r0 * 128, &b_full[buf]);
+        }
+        if (++buf == NB) buf = 0, phase ^= 1;
+        return true;
+      };
+      bool ok = true;
+      if (products && lane == 0)
+        for (; i < min(n, NB) && ok; ++i) ok = load();
+      __syncwarp();
+      ready();
+      if (products) {
+        const int pieces = hk / 8;
+        if (lane == 0) mbar_arrive_expect_tx(&h_full, 2 * pieces * rows * 16);
+        __syncwarp();
+        const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(p.h) + (static_cast<long long>(c.h0 / 8) * p.T + start) * 8;
+        for (int q = lane; q < 2 * pieces; q += 32)
+          bulk_load_1d(h_ptr + q * ROWS * 16, h + q / pieces * p.h_plane + static_cast<long long>(q % pieces) * p.T * 8,
+                       rows * 16, &h_full);
+        __syncwarp();
+        if (lane == 0) {
+          for (; i < n && ok; ++i) ok = load();
+          if (!ok) {
+            atomicCAS(p.status, 0, kStatusTimeoutEmptyBarrier);
+            gave_up = 1;
+          }
+        }
+        __syncwarp();
+      }
+    }
+    started = true;
+  }
+  if (!started) {
+    pdl_wait();
+    return;
+  }
+  __syncthreads();
+  if (*static_cast<volatile int*>(&gave_up)) {                         // what is in flight ends first (bounded waits)
+    if (threadIdx.x == 0)
+      for (int q = 0; q < 2; ++q) {
+        mbar_wait(&h_full, q);
+        for (int i = 0; i < NB; ++i) mbar_wait(&b_full[i], q), mbar_wait(&d_full[i], q);
+      }
+    __syncthreads();
+  }
+  if (warp == 4) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, NB * 64);
+  }
+}
+
+static constexpr int kShrinkFewSmem = kFewWarps * kFewRing, kExpandFewSmem = 140 * 1024, kExpandManySmem = 184 * 1024, kExpandTcSmem = 224 * 1024;
+
+template <int ACT, bool LANES>
+static int launch_few(const LoraParams& p, unsigned tiles, unsigned chunks, unsigned blocks, cudaStream_t stream) {
+  auto expand = lora_expand_few_kernel<ACT, LANES>;
   static DeviceOnce once;
   int dev;
   if (once.needed(&dev)) {
     const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    if ((MANY ? cudaFuncSetAttribute(lora_shrink_many_kernel, attr, kManyRing + 1024)
-              : cudaFuncSetAttribute(lora_shrink_few_kernel, attr, kShrinkFewSmem)) != cudaSuccess ||
-        cudaFuncSetAttribute(expand, attr, kExpandSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(lora_shrink_few_kernel, attr, kShrinkFewSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(expand, attr, kExpandFewSmem) != cudaSuccess)
       return -3;
     once.mark(dev);
   }
-  const size_t smem = 4 * (PAIRS ? 6 : 4) * (MANY ? 2048 : 6144) + 2 * sizeof(__nv_bfloat16) * (MANY ? 64 : 16) * p.h_pitch;
-  const dim3 grid(p.parts, chunks, tiles);
-  if (smem > kExpandSmem || tiles > (MANY ? 32767 : 65535)) return -2;
-  if constexpr (MANY) {
-    CUtensorMap tm_x = {};
-    if (p.boxes && make_tensormap_2d(&tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.x, p.T, p.K, p.x_stride, kManyRows, kSlab,
-                                     CU_TENSOR_MAP_SWIZZLE_128B) != 0)
-      return -4;
-    if (launch_pdl(lora_shrink_many_kernel, grid, dim3(kManyThreads), p.stages * p.stage_bytes + 1024, stream, p.parts, tm_x, p) !=
-        cudaSuccess)
-      return -3;
-  } else if (launch_pdl(lora_shrink_few_kernel, grid, dim3(kFewThreads), kShrinkFewSmem, stream, 1, p) != cudaSuccess) {
+  const size_t smem = 4 * 4 * 6144 + 2 * sizeof(__nv_bfloat16) * 16 * p.h_pitch;
+  if (smem > kExpandFewSmem || tiles > 65535) return -2;
+  if (launch_pdl(lora_shrink_few_kernel, dim3(p.parts, chunks, tiles), dim3(kFewThreads), kShrinkFewSmem, stream, 1, p) != cudaSuccess ||
+      launch_pdl(expand, dim3(blocks, tiles), dim3(kExpandThreads), smem, stream, 1, p) != cudaSuccess)
     return -3;
+  return 0;
+}
+
+template <int ACT, typename Kernel>
+static int launch_many(const LoraParams& p, Kernel expand, int attr_smem, unsigned tiles, unsigned chunks, dim3 grid, int threads,
+                       size_t smem, DeviceOnce& once, cudaStream_t stream) {
+  int dev;
+  if (once.needed(&dev)) {
+    const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    if (cudaFuncSetAttribute(lora_shrink_many_kernel, attr, kManyRing + 1024) != cudaSuccess ||
+        cudaFuncSetAttribute(expand, attr, attr_smem) != cudaSuccess)
+      return -3;
+    once.mark(dev);
   }
-  return launch_pdl(expand, dim3(blocks, MANY ? 2 * tiles : tiles), dim3(kExpandThreads), smem, stream, 1, p) == cudaSuccess ? 0 : -3;
+  if (smem > static_cast<size_t>(attr_smem) || tiles > 32767) return -2;
+  CUtensorMap tm_x = {};
+  if (p.boxes && make_tensormap_2d(&tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.x, p.T, p.K, p.x_stride, kManyRows, kSlab,
+                                   CU_TENSOR_MAP_SWIZZLE_128B) != 0)
+    return -4;
+  if (launch_pdl(lora_shrink_many_kernel, dim3(p.parts, chunks, tiles), dim3(kManyThreads), p.stages * p.stage_bytes + 1024, stream,
+                 p.parts, tm_x, p) != cudaSuccess ||
+      launch_pdl(expand, grid, dim3(threads), smem, stream, 1, p) != cudaSuccess)
+    return -3;
+  return 0;
+}
+
+// Shared memory of the tcgen05 kernel: h of 128 rows, two or four groups' B, and a ring of y; two CTAs an SM, or one with a ring of
+// twice the depth.  ctas 0: too much.
+struct TcPlan {
+  int buffers, depth, ctas;
+  size_t smem;
+};
+static TcPlan tc_plan(bool gated, int max_rank) {
+  const size_t h = (gated ? 2 : 1) * max_rank * 128 * 4, b = max_rank * 128, ring = 4 * 2048;
+  const size_t half = 114 * 1024 - 1792;
+  for (int depth = 4; depth > 1; depth /= 2)
+    for (int buffers = 4; buffers > 1; buffers /= 2)
+      if (h + buffers * b + depth * ring <= half) return {buffers, depth, 2, h + buffers * b + depth * ring};
+  for (int depth = 8; depth > 2; depth /= 2)
+    if (h + 2 * b + depth * ring <= kExpandTcSmem) return {2, depth, 1, h + 2 * b + depth * ring};
+  return {2, 0, 0, 0};
 }
 
 template <int ACT>
-static int launch_lora(const LoraParams& p, bool many, int max_rank, unsigned tiles, unsigned chunks, unsigned blocks,
-                       cudaStream_t stream) {
-  if (!many) return launch_lora<false, ACT, false>(p, tiles, chunks, blocks, stream);
-  return max_rank > 32 ? launch_lora<true, ACT, true>(p, tiles, chunks, blocks, stream)
-                       : launch_lora<true, ACT, false>(p, tiles, chunks, blocks, stream);
+static int launch_lora(LoraParams& p, bool many, int max_tiles, unsigned chunks, int slices, int groups, cudaStream_t stream) {
+  constexpr bool GATED = ACT != kActNone;
+  const unsigned tiles = static_cast<unsigned>(max_tiles);
+  const TcPlan tc = tc_plan(GATED, p.max_rank);
+  const long long work = static_cast<long long>(groups) * max_tiles;
+  if (many && p.max_rank > kLanesRank && tc.ctas) {
+    static DeviceOnce once2, once4, once8;
+    p.buffers = tc.buffers;
+    const auto launch = [&](auto kernel, DeviceOnce& once) {
+      return launch_many<ACT>(p, kernel, kExpandTcSmem, tiles, chunks, dim3(sm_count() * tc.ctas), kExpandTcThreads, tc.smem, once, stream);
+    };
+    return tc.depth == 2   ? launch(lora_expand_tc_kernel<ACT, 2>, once2)
+           : tc.depth == 4 ? launch(lora_expand_tc_kernel<ACT, 4>, once4)
+                           : launch(lora_expand_tc_kernel<ACT, 8>, once8);
+  }
+  // column groups of a CTA: two rounds of the resident CTAs in all, or for few rows one, where a CTA's start is most of its
+  // time (128 adapters of rank 16, 4096 columns: 7.7 us, with two rounds 9.6); a group a warp at least
+  const long long want = many ? static_cast<long long>(groups) * (max_tiles + p.T / kManyRows) / (148 * 8) : work / (148 * 2);
+  p.per = static_cast<int>(std::max(1LL, (want + 3) / 4)) * 4;
+  unsigned blocks = 0;
+  for (int s = 0; s < (GATED ? 1 : slices); ++s) blocks += ((GATED ? (p.n[s] + 31) / 32 : (p.n[s] + 63) / 64) + p.per - 1) / p.per;
+  if (!many)
+    return p.max_rank > kLanesRank ? launch_few<ACT, false>(p, tiles, chunks, blocks, stream)
+                                   : launch_few<ACT, true>(p, tiles, chunks, blocks, stream);
+  static DeviceOnce once;
+  const size_t smem = 4 * (p.max_rank > kLanesRank ? 6 : 4) * 2048 + 2 * sizeof(__nv_bfloat16) * 64 * p.h_pitch;
+  const dim3 grid(blocks, 2 * tiles);
+  if constexpr (GATED)
+    if (p.max_rank > kLanesRank) {
+      static DeviceOnce pairs;
+      return launch_many<ACT>(p, lora_expand_many_kernel<ACT, true>, kExpandManySmem, tiles, chunks, grid, kExpandThreads, smem, pairs, stream);
+    }
+  return launch_many<ACT>(p, lora_expand_many_kernel<ACT, false>, kExpandManySmem, tiles, chunks, grid, kExpandThreads, smem, once, stream);
 }
 
 // Parts of K that a step's h is summed from, a CTA each (many rows: of a cluster).  Few rows (tiles of 16): as many as the slots
@@ -948,32 +1372,26 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   p.act_alpha = act_alpha;
   p.act_limit = act_limit;
   const int width = (many ? kManyChunk : kFewChunk) * 8;
-  const unsigned chunks = (p.h_width + width - 1) / width, tiles_n = static_cast<unsigned>(max_tiles);
+  const unsigned chunks = (p.h_width + width - 1) / width;
   p.parts = lora_parts(K, rows, max_tiles, num_slots, (mean_rank + width - 1) / width);
   // the first kernel's ring: two CTAs an SM, or all of it for one where there are too few
   const long long ctas = static_cast<long long>(p.parts) * max_tiles * ((mean_rank + width - 1) / width);
   p.stage_bytes = kXBytes + std::min(p.h_width, width) * kSlab * 2;
   p.stages = std::min((ctas > 148 ? kManyRing / 2 : kManyRing) / p.stage_bytes, kManyStages);
   p.h_pitch = (gated ? 2 : 1) * max_rank + 8;    // eight rows of 16 bytes are in banks of their own
-  // column groups of a CTA: two rounds of the resident CTAs in all, or for few rows one, where a CTA's start is most of its
-  // time (128 adapters of rank 16, 4096 columns: 7.7 us, with two rounds 9.6); a group a warp at least
   int groups = 0;
   for (int s = 0; s < kLoraMaxSlices; ++s) {
     p.n[s] = s < slices ? n[s] : 0;
     if (p.n[s] & 7) return -1;
     if (!gated || s == 0) groups += gated ? (p.n[s] + 31) / 32 : (p.n[s] + 63) / 64;
   }
-  const int row_tiles = many ? max_tiles + T / kManyRows : max_tiles;   // of the second kernel: 64 rows
-  const long long want = static_cast<long long>(groups) * row_tiles / (148 * (many ? 8 : 2));
-  p.per = static_cast<int>(std::max(1LL, (want + 3) / 4)) * 4;
-  unsigned blocks = 0;
-  for (int s = 0; s < slices; ++s)
-    if (!gated || s == 0) blocks += ((gated ? (n[s] + 31) / 32 : (n[s] + 63) / 64) + p.per - 1) / p.per;
+  p.groups = groups;
+  p.max_rank = max_rank;
   switch (act) {
-    case kActNone: return launch_lora<kActNone>(p, many, max_rank, tiles_n, chunks, blocks, stream);
-    case kActSilu: return launch_lora<kActSilu>(p, many, max_rank, tiles_n, chunks, blocks, stream);
-    case kActClampedGlu: return launch_lora<kActClampedGlu>(p, many, max_rank, tiles_n, chunks, blocks, stream);
-    case kActGeluTanh: return launch_lora<kActGeluTanh>(p, many, max_rank, tiles_n, chunks, blocks, stream);
-    default: return launch_lora<kActReluGate>(p, many, max_rank, tiles_n, chunks, blocks, stream);
+    case kActNone: return launch_lora<kActNone>(p, many, max_tiles, chunks, slices, groups, stream);
+    case kActSilu: return launch_lora<kActSilu>(p, many, max_tiles, chunks, slices, groups, stream);
+    case kActClampedGlu: return launch_lora<kActClampedGlu>(p, many, max_tiles, chunks, slices, groups, stream);
+    case kActGeluTanh: return launch_lora<kActGeluTanh>(p, many, max_tiles, chunks, slices, groups, stream);
+    default: return launch_lora<kActReluGate>(p, many, max_tiles, chunks, slices, groups, stream);
   }
 }

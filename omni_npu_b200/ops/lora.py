@@ -13,7 +13,7 @@ import torch
 
 from . import SILU, _C, _act_kind, _count, device_state, ref
 
-MAX_SLOTS, MAX_SLICES, MAX_RANK = 512, 4, 256
+MAX_SLOTS, MAX_SLICES, MAX_RANK, LANES_RANK = 512, 4, 256, 32
 
 # Tokens of one adapter that are taken together.  Up to this many tokens of a step: tiles of 16, one matrix instruction high,
 # through kernels that stream the factors; above, tiles of 128.  Us, tiles of 128 / 16: 200 tokens of 8 adapters of rank 16,
@@ -57,10 +57,13 @@ class LoraStack:
         self.max_rank = (max_rank + 15) // 16 * 16
         self.dtype = dtype
         with torch.inference_mode(False):
-            # in the order of the matrix instructions (csrc/lora/lora.cu), K and columns in whole 32
+            # in the order of the matrix instructions (csrc/lora/lora.cu), K in whole 32, columns in whole blocks
             self._k = (in_features + 31) // 32
             self.a = torch.zeros(num_slots, len(slices) * self.max_rank * self._k * 32, dtype=dtype, device=device)
-            self.b = torch.zeros(num_slots, sum((n + 31) // 32 * 32 for n in slices) * self.max_rank, dtype=dtype, device=device)
+            self._lanes = self.max_rank <= LANES_RANK
+            self._block = 32 if interleaved or self._lanes else 64
+            self.b = torch.zeros(num_slots, sum((n + self._block - 1) // self._block for n in slices) * self._block * self.max_rank,
+                                 dtype=dtype, device=device)
             # of every slot the ranks (in whole 16) and the bits of the scale
             self.ranks = torch.zeros(num_slots, len(slices) + 1, dtype=torch.int32, device=device)
         self.device = self.a.device
@@ -96,7 +99,7 @@ class LoraStack:
                     view.copy_(_padded(p, view.shape[0] * 8, self._k * 32).view(view.shape))
             for q, view in zip(b, self._views_b(slot, ranks)):
                 if view is not None:
-                    view.copy_(_padded(q, view.shape[0] * 32, view.shape[5] * 16).view(view.shape))
+                    view.copy_(_padded(q, view.shape[0] * self._block, view.shape[5] * (16 if self._lanes else 8)).view(view.shape))
             row = torch.tensor(ranks + [0], dtype=torch.int32)
             row[-1:].view(torch.float32).fill_(scale)
             self.ranks[slot].copy_(row)
@@ -113,14 +116,19 @@ class LoraStack:
             at += r // 8
 
     def _views_b(self, slot: int, ranks):
-        """B of each slice as [columns, rank] in the shape (columns / 32, 4, 2, 2, 2, rank / 16, 2, 4, 2) over its packed place."""
+        """B of each slice as [columns, rank] over its packed place: (columns / 32, 4, 2, 2, 2, rank / 16, 2, 4, 2) in the order
+        of lanes, else (columns / block, block / 32, 4, 4, 2, rank / 8, 8)."""
         at = 0
         for r, n in zip(ranks, self.slices):
-            c = (n + 31) // 32
-            # n32, r16, v, g / 2, g % 2, q, j % 2, half, 2
-            yield (self.b[slot, at: at + c * 32 * r].view(c, r // 16, 2, 4, 2, 4, 2, 2, 2).permute(0, 3, 2, 6, 4, 1, 7, 5, 8)
-                   if r else None)
-            at += c * 32 * r
+            c = (n + self._block - 1) // self._block
+            packed = self.b[slot, at: at + c * self._block * r]
+            if not r:
+                yield None
+            elif self._lanes:                                 # n32, r16, j / 2, i / 2, i % 2, q, j % 2, half, 2
+                yield packed.view(c, r // 16, 2, 4, 2, 4, 2, 2, 2).permute(0, 3, 2, 6, 4, 1, 7, 5, 8)
+            else:                                             # block, r8, 32 columns, j, i / 2, i % 2, 8
+                yield packed.view(c, r // 8, self._block // 32, 4, 4, 2, 8).permute(0, 2, 4, 3, 5, 1, 6)
+            at += c * self._block * r
 
     def clear(self, slot: int) -> None:
         """Empty a slot."""

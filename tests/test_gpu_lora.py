@@ -282,11 +282,12 @@ def test_many_rows_of_any_stride(stride):
 
 
 @pytest.mark.parametrize("contiguous", [False, True])
-@pytest.mark.parametrize("tokens,n,k,ranks", [(800, 104, 520, [16, 0, 40]), (1500, 1000, 2048, [32])])
+@pytest.mark.parametrize("tokens,n,k,ranks", [(800, 104, 520, [16, 0, 40]), (1500, 1000, 2048, [32]), (900, 1000, 256, [64, 0, 0, 8]),
+                                              (1300, 520, 264, [128, 16, 0, 100, 128]), (800, 96, 128, [150, 0]), (1000, 200, 64, [256, 17])])
 def test_gated_many_rows(tokens, n, k, ranks, contiguous):
     x, y, ad = make_case(tokens, 3, ranks, k, [n, n], device=DEV)
     slots = slots_of(tokens, 3, contiguous=contiguous).to(DEV)
-    out = ops.lora_gated(y, x, load(ops, ad, 40, k, [n, n], DEV, True), ops.lora_plan(slots, 3))
+    out = ops.lora_gated(y, x, load(ops, ad, max(ranks), k, [n, n], DEV, True), ops.lora_plan(slots, 3))
     z, bound = exact(x, y, ad, slots, [n, n], interleaved=True)
     check_silu(out, z, bound)
 
@@ -305,3 +306,17 @@ def test_many_rows_keep_their_values_to_themselves():
     keep[torch.tensor([3, 129, 500], device=DEV)] = False
     check_sum(out[keep], z[keep], bound[keep])
     assert bool(out[~keep].isnan().all())
+
+
+@pytest.mark.parametrize("ranks", [[16], [48], [64, 16], [128], [200, 0, 40]])
+def test_many_rows_in_and_out_of_place(ranks):
+    """Both ways give the same; rows without an adapter keep their bits."""
+    tokens, k, slices = 3000, 128, [328, 64]
+    x, y, ad = make_case(tokens, 2, ranks, k, slices, device=DEV)
+    slots = slots_of(tokens, 2, none=0.5).to(DEV)
+    st, plan = load(ops, ad, max(ranks), k, slices, DEV), ops.lora_plan(slots, 2)
+    out = ops.lora_add(y, x, st, plan)
+    z, bound = exact(x, y, ad, slots, slices)
+    check_sum(out, z, bound)
+    assert torch.equal(out[slots < 0].view(torch.int16), y[slots < 0].view(torch.int16))
+    assert torch.equal(ops.lora_add(y, x, st, plan, out=y), out)
