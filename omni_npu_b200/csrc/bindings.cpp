@@ -115,6 +115,9 @@ int b200_lora(const void* x, long long x_stride, const void* y, long long y_stri
               const int* tiles, const int* num_tiles, int max_tiles, int rows, void* h, int T, int num_slots, int K, int slices,
               const int* n, int max_rank, int mean_rank, int act, float act_alpha, float act_limit, int* status,
               cudaStream_t stream);
+int b200_lora_pack(const void* const* a, const void* const* b, const long long* a_strides, const long long* b_strides,
+                   const int* a_types, const int* b_types, const int* r, const int* n, int slices, int K, bool lanes, int block,
+                   float scale, void* out_a, void* out_b, int* out_ranks, cudaStream_t stream);
 size_t b200_mla_decode_scratch_bytes(int total_tokens, int N, int splits);
 int b200_mla_decode(const void* q, const void* cache, void* out, float* lse, const int* block_tables,
                     const int* seq_lens, const int* topk_indices, int topk, int B, int q_len, int N,
@@ -842,6 +845,49 @@ Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given
   return out;
 }
 
+// An adapter's factors into slot `slot` of a stack's a, b and ranks.  fa[i] [r, K] and fb[i] [n, r] of each slice, bf16, fp16 or
+// fp32, or none; slices: columns.
+void lora_pack(const Tensor& a, const Tensor& b, const Tensor& ranks, int64_t slot, const std::vector<c10::optional<Tensor>>& fa,
+               const std::vector<c10::optional<Tensor>>& fb, at::IntArrayRef slices, int64_t K, bool lanes, int64_t block,
+               double scale) {
+  const int64_t S = (int64_t)slices.size();
+  TORCH_CHECK(S >= 1 && S <= 4 && (int64_t)fa.size() == S && (int64_t)fb.size() == S, "lora_pack: one to four slices");
+  TORCH_CHECK(a.scalar_type() == at::kBFloat16 && b.scalar_type() == at::kBFloat16 && a.is_contiguous() && b.is_contiguous() &&
+                  slot >= 0 && slot < a.size(0) && ranks.size(0) == a.size(0) && ranks.size(1) == S + 1,
+              "lora_pack: bf16 factors [slots, ...] and ranks [slots, slices + 1]");
+  CHECK_I32(ranks);
+  const auto type = [](const Tensor& t) {
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat,
+                "lora_pack: factors are bf16, fp16 or fp32");
+    return t.scalar_type() == at::kBFloat16 ? 0 : t.scalar_type() == at::kHalf ? 1 : 2;
+  };
+  const void *pa[4] = {}, *pb[4] = {};
+  long long sa[8] = {}, sb[8] = {};
+  int ta[4] = {}, tb[4] = {}, r[4] = {}, n[4] = {};
+  int64_t sum_r = 0, packed = 0;
+  for (int64_t i = 0; i < S; ++i) {
+    n[i] = (int)slices[i];
+    if (!fa[i].has_value()) continue;
+    const Tensor &p = *fa[i], &q = *fb[i];
+    TORCH_CHECK(p.dim() == 2 && q.dim() == 2 && p.size(1) == K && q.size(0) == slices[i] && q.size(1) == p.size(0) &&
+                    p.device() == a.device() && q.device() == a.device(),
+                "lora_pack: factors of other sizes or on another device");
+    pa[i] = p.data_ptr(), pb[i] = q.data_ptr();
+    sa[2 * i] = p.stride(0), sa[2 * i + 1] = p.stride(1), sb[2 * i] = q.stride(0), sb[2 * i + 1] = q.stride(1);
+    ta[i] = type(p), tb[i] = type(q);
+    r[i] = (int)p.size(0);
+    sum_r += (r[i] + 15) / 16 * 16;
+    packed += (slices[i] + block - 1) / block * block * ((r[i] + 15) / 16 * 16);
+  }
+  TORCH_CHECK(sum_r * ((K + 31) / 32 * 32) <= a.size(1) && packed <= b.size(1), "lora_pack: ranks above the stack's");
+  c10::cuda::CUDAGuard guard(a.device());
+  check(b200_lora_pack(pa, pb, sa, sb, ta, tb, r, n, (int)S, (int)K, lanes, (int)block, (float)scale,
+                       static_cast<at::BFloat16*>(a.data_ptr()) + slot * a.size(1),
+                       static_cast<at::BFloat16*>(b.data_ptr()) + slot * b.size(1), ranks.data_ptr<int>() + slot * (S + 1),
+                       cur_stream()),
+        "lora_pack");
+}
+
 int64_t mla_decode_scratch_bytes(int64_t T, int64_t N, int64_t splits) {
   return (int64_t)b200_mla_decode_scratch_bytes((int)T, (int)N, (int)splits);
 }
@@ -922,6 +968,7 @@ TORCH_LIBRARY_FRAGMENT(omni_b200, m) {
   m.def("cache_copy", &cache_copy);
   m.def("lora_plan", &lora_plan);
   m.def("lora", &lora);
+  m.def("lora_pack", &lora_pack);
   m.def("mla_decode_scratch_bytes", &mla_decode_scratch_bytes);
   m.def("mla_decode", &mla_decode);
 }

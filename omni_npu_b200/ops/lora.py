@@ -93,18 +93,32 @@ class LoraStack:
             if not 1 <= r <= self.max_rank:
                 raise ValueError(f"LoraStack.load: rank {r}, at most {self.max_rank}")
             ranks.append((r + 15) // 16 * 16)
-        with torch.inference_mode():
-            for p, view in zip(a, self._views_a(slot, ranks)):
-                if view is not None:
-                    view.copy_(_padded(p, view.shape[0] * 8, self._k * 32).view(view.shape))
-            for q, view in zip(b, self._views_b(slot, ranks)):
-                if view is not None:
-                    view.copy_(_padded(q, view.shape[0] * self._block, view.shape[5] * (16 if self._lanes else 8)).view(view.shape))
-            row = torch.tensor(ranks + [0], dtype=torch.int32)
-            row[-1:].view(torch.float32).fill_(scale)
-            self.ranks[slot].copy_(row)
+        if self.device.type == "cuda":
+            _count(1)
+            _C().lora_pack(self.a, self.b, self.ranks, slot, [self._here(p) for p in a], [self._here(q) for q in b], self.slices,
+                           self.in_features, self._lanes, self._block, scale)
+        else:
+            with torch.inference_mode():
+                for p, view in zip(a, self._views_a(slot, ranks)):
+                    if view is not None:
+                        view.copy_(_padded(p, view.shape[0] * 8, self._k * 32).view(view.shape))
+                for q, view in zip(b, self._views_b(slot, ranks)):
+                    if view is not None:
+                        view.copy_(_padded(q, view.shape[0] * self._block,
+                                           view.shape[5] * (16 if self._lanes else 8)).view(view.shape))
+                row = torch.tensor(ranks + [0], dtype=torch.int32)
+                row[-1:].view(torch.float32).fill_(scale)
+                self.ranks[slot].copy_(row)
         self._scales[slot] = float(scale)
         self._set_ranks(slot, ranks)
+
+    def _here(self, t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        """A factor on the stack's device, of a type that the packing kernel reads."""
+        if t is None:
+            return None
+        if t.device != self.device:
+            t = t.to(self.device)
+        return t if t.dtype in (torch.bfloat16, torch.float16, torch.float32) else t.to(self.dtype)
 
     def _views_a(self, slot: int, ranks):
         """A of each slice as [ranks, K] in the shape (rank / 8, 8, K / 32, 4, 8) over its packed place."""

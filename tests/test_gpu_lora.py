@@ -320,3 +320,23 @@ def test_many_rows_in_and_out_of_place(ranks):
     check_sum(out, z, bound)
     assert torch.equal(out[slots < 0].view(torch.int16), y[slots < 0].view(torch.int16))
     assert torch.equal(ops.lora_add(y, x, st, plan, out=y), out)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float64])
+@pytest.mark.parametrize("max_rank", [32, 128])
+@pytest.mark.parametrize("k,slices,interleaved", [(8, [8], False), (40, [72, 8, 136], False), (264, [40, 40], True), (520, [16, 24, 8, 64], False)])
+def test_factors_are_laid_out_as_on_the_host(dtype, max_rank, k, slices, interleaved):
+    gen = torch.Generator().manual_seed(k)
+    host = ops.LoraStack(3, max_rank, k, slices, interleaved=interleaved)
+    card = ops.LoraStack(3, max_rank, k, slices, device=DEV, interleaved=interleaved)
+    for slot, ranks in enumerate([[1, 16, 17, 32], [max_rank, 0, 5, 8], [0, 9, 0, max_rank]]):
+        a = [torch.randn(r, k, generator=gen).to(dtype) if r else None for r in ranks[: len(slices)]]
+        b = [torch.randn(n, r, generator=gen).to(dtype) if r else None for n, r in zip(slices, ranks)]
+        host.load(slot, a, b, 0.3)
+        if slot == 0:                                          # other strides
+            a = [t if t is None else t.t().contiguous().t() for t in a]
+            b = [t if t is None else torch.cat([t, t], 1)[:, t.shape[1]:] for t in b]
+        card.load(slot, [t if t is None or slot == 2 else t.to(DEV) for t in a], [t if t is None else t.to(DEV) for t in b], 0.3)
+    assert torch.equal(card.a.cpu(), host.a) and torch.equal(card.b.cpu(), host.b) and torch.equal(card.ranks.cpu(), host.ranks)
+    card.load(0, [None] * len(slices), [None] * len(slices))   # nothing left but the scale
+    assert card.ranks[0].tolist() == [0] * len(slices) + [0x3F800000]
