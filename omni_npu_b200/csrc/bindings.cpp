@@ -3,6 +3,8 @@
 // pointers + stream); this file only validates tensors and forwards.
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 #include <torch/torch.h>
@@ -762,7 +764,7 @@ Tensor lora_plan(const Tensor& slots, int64_t num_slots, int64_t rows, const Ten
   CHECK_I32(status);
   const int64_t T = slots.numel(), at = lora_tiles_at(T);
   c10::cuda::CUDAGuard guard(slots.device());
-  Tensor plan = torch::empty({at + 4 * lora_max_tiles(T, num_slots, rows)}, slots.options());
+  Tensor plan(at::detail::empty_cuda({at + 4 * lora_max_tiles(T, num_slots, rows)}, at::kInt, slots.device(), c10::nullopt));
   int* p = plan.data_ptr<int>();
   check(b200_lora_plan(slots.data_ptr<int>(), (int)T, (int)num_slots, (int)rows, p, p + at, p + T, status.data_ptr<int>(),
                        cur_stream()),
@@ -819,7 +821,8 @@ Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given
   TORCH_CHECK_VALUE(max_tiles <= (rows == 16 ? 65535 : 32767), "lora: ", T, " tokens are too many at once");
   c10::cuda::CUDAGuard guard(x.device());
   const int64_t cols = act ? slices[0] : width;
-  const Tensor out = given.has_value() ? *given : torch::empty({T, cols}, y.options());
+  // (allocations without the dispatcher: small steps wait for the host, and it takes some 0.5 us each)
+  const Tensor out = given.has_value() ? *given : Tensor(at::detail::empty_cuda({T, cols}, at::kBFloat16, y.device(), c10::nullopt));
   for (const Tensor* t : {&x, &y, &out})
     TORCH_CHECK_VALUE(t->stride(1) == 1 && (T < 2 || t->stride(0) % 8 == 0) && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0,
                       "lora: rows of x, y and out are contiguous and start at 16-byte boundaries");
@@ -833,12 +836,11 @@ Tensor lora(const Tensor& x, const Tensor& y, const c10::optional<Tensor>& given
     TORCH_CHECK_VALUE(T < 2 || out.stride(0) >= out.size(1), "lora: rows of out overlap");
   }
   if (T == 0) return out;
-  const Tensor h = torch::empty(
-      {b200_lora_scratch_bytes((int)T, (int)K, (int)rows, (int)max_tiles, (int)L, (int)S, (int)max_rank)},
-      x.options().dtype(at::kByte));
+  const c10::DataPtr h = c10::cuda::CUDACachingAllocator::get()->allocate(
+      b200_lora_scratch_bytes((int)T, (int)K, (int)rows, (int)max_tiles, (int)L, (int)S, (int)max_rank));
   const int* p = plan.data_ptr<int>();
   check(b200_lora(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(), out.stride(0), a.data_ptr(), a.size(1),
-                  b.data_ptr(), b.size(1), ranks.data_ptr<int>(), p, p + at, p + T, (int)max_tiles, (int)rows, h.data_ptr(),
+                  b.data_ptr(), b.size(1), ranks.data_ptr<int>(), p, p + at, p + T, (int)max_tiles, (int)rows, h.get(),
                   (int)T, (int)L, (int)K, (int)S, n, (int)max_rank, (int)std::max<int64_t>(mean_rank, 16), (int)act,
                   (float)act_alpha, (float)act_limit, status.data_ptr<int>(), cur_stream()),
         "lora");

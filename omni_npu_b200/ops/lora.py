@@ -17,8 +17,8 @@ MAX_SLOTS, MAX_SLICES, MAX_RANK, LANES_RANK = 512, 4, 256, 32
 
 # Tokens of one adapter that are taken together.  Up to this many tokens of a step: tiles of 16, one matrix instruction high,
 # through kernels that stream the factors; above, tiles of 128.  Us, tiles of 128 / 16: 200 tokens of 8 adapters of rank 16,
-# 4096 to 4096 + 1024 + 1024 12.7 / 8.2, 14336 to 4096 19.2 / 8.8; 768 tokens 17.3 / 14.3 and 22.9 / 14.7; 1000 tokens 17.8 /
-# 19.6 and 23.3 / 16.6; 768 tokens of 8 of rank 64 21.7 / 26.9.  A row's result does not depend on the rows beside it as long as
+# 4096 to 4096 + 1024 + 1024 12.3 / 8.1, 14336 to 4096 17.8 / 8.5; 768 tokens 16.7 / 13.9 and 20.8 / 14.7; 1000 tokens 17.1 /
+# 19.1 and 21.8 / 16.3; 768 tokens of 8 of rank 64 21.1 / 26.5.  A row's result does not depend on the rows beside it as long as
 # these are no more.
 FEW_TOKENS, FEW_ROWS, MANY_ROWS = 768, 16, 128
 
@@ -176,10 +176,12 @@ class LoraStack:
 class LoraPlan:
     """A step's tokens grouped by adapter slot (:func:`lora_plan`)."""
 
-    __slots__ = ("slots", "num_slots", "num_tokens", "rows", "buffer")
+    __slots__ = ("slots", "num_slots", "num_tokens", "rows", "buffer", "status")
 
-    def __init__(self, slots: torch.Tensor, num_slots: int, rows: int = 0, buffer: Optional[torch.Tensor] = None) -> None:
+    def __init__(self, slots: torch.Tensor, num_slots: int, rows: int = 0, buffer: Optional[torch.Tensor] = None,
+                 status: Optional[torch.Tensor] = None) -> None:
         self.slots, self.num_slots, self.num_tokens, self.rows, self.buffer = slots, num_slots, slots.shape[0], rows, buffer
+        self.status = status                                  # where the device's kernels report (on a GPU)
 
     @property
     def order(self) -> torch.Tensor:
@@ -208,10 +210,11 @@ def lora_plan(slots: torch.Tensor, num_slots: int) -> LoraPlan:
             raise ValueError(f"lora_plan: slots outside -1 .. {num_slots - 1}")
         return LoraPlan(slots, num_slots)
     rows = FEW_ROWS if t <= FEW_TOKENS else MANY_ROWS
+    status = device_state(slots.device).status
     if t == 0:
-        return LoraPlan(slots, num_slots, rows, slots.new_empty(4))
+        return LoraPlan(slots, num_slots, rows, slots.new_empty(4), status)
     _count(1)
-    return LoraPlan(slots, num_slots, rows, _C().lora_plan(slots, num_slots, rows, device_state(slots.device).status))
+    return LoraPlan(slots, num_slots, rows, _C().lora_plan(slots, num_slots, rows, status), status)
 
 
 def _check(what: str, y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan) -> None:
@@ -230,7 +233,7 @@ def _launch(y, x, stack: LoraStack, plan: LoraPlan, out, kind, alpha, limit) -> 
     if plan.num_tokens:
         _count(2)
     return _C().lora(x, y, out, stack.a, stack.b, stack.ranks, plan.buffer,
-                     [plan.num_tokens, plan.num_slots, plan.rows, kind] + stack.sizes, alpha, limit, device_state(x.device).status)
+                     [plan.num_tokens, plan.num_slots, plan.rows, kind] + stack.sizes, alpha, limit, plan.status)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, plan: LoraPlan,
