@@ -389,6 +389,17 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
   const int s_lo = static_cast<int>(static_cast<long long>(slabs) * blockIdx.x / p.parts);
   const int count = static_cast<int>(static_cast<long long>(slabs) * (blockIdx.x + 1) / p.parts) - s_lo;   // one at least
   const uint32_t tmem_cols = width > 64 ? 128 : width > 32 ? 64 : 32;
+  // a slab's factors, and its rows of x where these are a box
+  const char* a = reinterpret_cast<const char*>(p.a + tl.slot * p.a_slot) + n0 * 64;
+  const long long a_step = static_cast<long long>(sum_r) * 64;
+  int loaded = 0;
+  auto load = [&](int i, int put) {
+    const int s = (s_lo + i) * 2, steps = min(2, blocks - s);
+    char* st = ring_ptr + put * p.stage_bytes;
+    mbar_arrive_expect_tx(&full[put], steps * width * 64 + (box ? kXBytes : 0));
+    if (box) tma_load_2d(st, &tm_x, &full[put], (s_lo + i) * kSlab, first);
+    for (int u = 0; u < steps; ++u) bulk_load_1d(st + kXBytes + u * width * 64, a + (s + u) * a_step, width * 64, &full[put]);
+  };
   if (threadIdx.x == kManyCopies + 32) {
     tma_prefetch_desc(&tm_x);
     for (int i = 0; i < p.stages; ++i) {
@@ -398,6 +409,8 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
     mbar_init(&done, 1);
     gave_up = 0;
     fence_barrier_init();
+    fence_proxy_async();
+    for (; loaded < min(count, p.stages); ++loaded) load(loaded, loaded);   // (this thread's barriers, and places nobody has used)
   }
   if (warp == kManyCopies / 32) {
     tmem_alloc(&tmem_slot, tmem_cols);
@@ -430,28 +443,16 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kManyCopies / 32 + 1 && lane == 0) {
-    const char* a = reinterpret_cast<const char*>(p.a + tl.slot * p.a_slot) + n0 * 64;
-    const long long a_step = static_cast<long long>(sum_r) * 64;
-    int put = 0, i = 0;
-    uint32_t phase = 1;
+    // (the first pass over the ring went before)
+    int put = loaded == p.stages ? 0 : loaded, i = loaded;
+    uint32_t phase = loaded == p.stages ? 0 : 1;
     for (; i < count; ++i) {
       if (!mbar_wait(&empty[put], phase)) {
         atomicCAS(p.status, 0, kStatusTimeoutEmptyBarrier);
         break;
       }
-      const int s = (s_lo + i) * 2, steps = min(2, blocks - s);
-      char* st = ring_ptr + put * p.stage_bytes;
-      mbar_arrive_expect_tx(&full[put], steps * width * 64 + (box ? kXBytes : 0));
-      if (box) tma_load_2d(st, &tm_x, &full[put], (s_lo + i) * kSlab, first);
-      for (int u = 0; u < steps; ++u) bulk_load_1d(st + kXBytes + u * width * 64, a + (s + u) * a_step, width * 64, &full[put]);
+      load(i, put);
       if (++put == p.stages) put = 0, phase ^= 1;
-    }
-    if (*static_cast<volatile int*>(&gave_up)) {
-      // what was copied for nobody has landed before this CTA ends
-      for (int j = 0; j < min(i, p.stages); ++j) {
-        if (put-- == 0) put = p.stages - 1, phase ^= 1;
-        mbar_wait(&full[put], phase ^ 1);
-      }
     }
   } else if (warp == kManyCopies / 32 && lane == 0) {
     const uint32_t idesc = make_idesc(1, 1, kManyRows, width);
@@ -492,6 +493,11 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
   // Every product is through, and the ring free.  (The other warps wait here and not at the mbarrier: eight warps that poll it
   // slow down the two that work.)
   __syncthreads();
+  if (*static_cast<volatile int*>(&gave_up)) {                         // what is in flight ends first (bounded waits)
+    if (threadIdx.x == 0)
+      for (int i = 0; i < p.stages; ++i) mbar_wait(&full[i], 0), mbar_wait(&full[i], 1);
+    __syncthreads();
+  }
   tc_fence_after_sync();
   float* part = reinterpret_cast<float*>(ring_ptr);
   const int pitch = width + 4;
