@@ -16,8 +16,9 @@ LM head and sampling.  Prefill steps run eagerly.
 from __future__ import annotations
 
 import time
+from contextlib import nullcontext
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import ContextManager, Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -235,8 +236,11 @@ class ModelRunner:
                               for _ in range(getattr(self.model, "num_kv_layers", mc.num_layers))]
         self.num_blocks = num_blocks
 
-    def initialize_kv_cache(self, num_blocks: int) -> None:
-        self._init_kv_cache_tensors(num_blocks)
+    def initialize_kv_cache(self, num_blocks: int, pool: Optional[ContextManager] = None) -> None:
+        """Allocate the cache, in the memory pool ``pool`` if given.  Only what a step fills again may lie there (sleep mode
+        drops the pool's contents), so the table of addresses for page copies does not."""
+        with pool or nullcontext():
+            self._init_kv_cache_tensors(num_blocks)
         self.page_cache = self._page_cache()
         if self.kv_connector is not None:
             self.kv_connector.register_kv_caches(self.kv_caches)

@@ -102,12 +102,11 @@ class Worker:
             from ..kv_transfer.connector import create_connector
             self.model_runner.kv_connector = create_connector(self.config, role="worker",
                                                               device=self.device)
+        pool = None
         if self.config.enable_sleep_mode and self.device.type == "cuda":
             from .mem_pool import B200MemAllocator
-            with B200MemAllocator.get_instance().use_memory_pool(tag="kv_cache"):
-                self.model_runner.initialize_kv_cache(num_blocks)
-        else:
-            self.model_runner.initialize_kv_cache(num_blocks)
+            pool = B200MemAllocator.get_instance().use_memory_pool(tag="kv_cache")
+        self.model_runner.initialize_kv_cache(num_blocks, pool)
 
     def compile_or_warm_up_model(self) -> None:
         if self.device.type == "cuda":

@@ -1,0 +1,74 @@
+"""What sleep mode discards and what has to outlive it."""
+from contextlib import contextmanager
+
+import pytest
+import torch
+
+from omni_npu_b200 import ops
+from omni_npu_b200.config import ModelConfig
+from omni_npu_b200.engine.llm import LLM
+from omni_npu_b200.worker import mem_pool
+
+
+class FakePool:
+    """Records which tag is active, and what was asked of it."""
+
+    def __init__(self):
+        self.tag, self.calls, self._sleeping = None, [], False
+
+    @contextmanager
+    def use_memory_pool(self, tag=None):
+        old, self.tag = self.tag, tag
+        try:
+            yield
+        finally:
+            self.tag = old
+
+    def sleep(self, offload_tags=None):
+        self.calls.append(("sleep", tuple(offload_tags)))
+        self._sleeping = True
+        return 1
+
+    def wake_up(self, tags=None):
+        self.calls.append(("wake", tags))
+        self._sleeping = tags is not None
+        return 1
+
+
+@pytest.fixture
+def pool(monkeypatch):
+    fake = FakePool()
+    monkeypatch.setattr(mem_pool.B200MemAllocator, "get_instance", staticmethod(lambda: fake))
+    monkeypatch.setattr(mem_pool.B200MemAllocator, "instance", fake)
+    return fake
+
+
+def _llm(**kw):
+    cfg = ModelConfig(hidden_size=64, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=16, intermediate_size=96, vocab_size=97,
+                      rope_theta=10000.0, max_position_embeddings=512, dtype=torch.float32)
+    args = dict(model=cfg, device="cpu", max_num_seqs=8, max_num_batched_tokens=64, max_model_len=128, num_gpu_blocks=64,
+                block_size=4, seed=3)
+    args.update(kw)
+    return LLM(**args)
+
+
+def test_the_addresses_of_page_copies_lie_outside_the_pool_that_is_discarded(pool, monkeypatch):
+    """A table of raw pointers in discarded memory would be read as pointers after the wake-up."""
+    worker = _llm().engine.worker
+    made = []
+
+    class Recording(ops.CacheBlocks):
+        def __init__(self, tensors):
+            made.append(("addresses", pool.tag))
+            super().__init__(tensors)
+
+    def init(num_blocks, inner=worker.model_runner._init_kv_cache_tensors):
+        made.append(("cache", pool.tag))
+        inner(num_blocks)
+    monkeypatch.setattr(ops, "CacheBlocks", Recording)
+    monkeypatch.setattr(worker.model_runner, "_init_kv_cache_tensors", init)
+    monkeypatch.setattr(worker, "device", torch.device("cuda"))
+    worker.config.enable_sleep_mode = True
+    worker.initialize_from_config(16)
+    assert made == [("cache", "kv_cache"), ("addresses", None)]
+    assert worker.model_runner.page_cache.num_blocks == 16
