@@ -54,6 +54,7 @@ class AdapterManager:
         self.slots: Dict[str, int] = {}
         self.keys: Dict[str, bytes] = {}             # told apart in the prefix cache, also from an earlier load of the name
         self._loads = itertools.count()
+        self._lost = False                           # the stacks hold nothing that may be read
         self.layers: Dict[str, LinearBase] = {}
         self.stacks: Dict[str, ops.LoraStack] = {}
         # checkpoint module name -> (projection, its slice)
@@ -114,6 +115,10 @@ class AdapterManager:
             found.setdefault(proj, [[None] * n, [None] * n])["AB".index(m["which"])][i] = tensor
         if not found:
             raise ValueError(f"adapter {name!r} has no factors")
+        if self._lost:
+            for stack in self.stacks.values():
+                stack.reset()
+            self._lost = False
         slot = next(i for i in range(self.num_slots) if i not in self.slots.values())
         try:
             for proj, (a, b) in found.items():
@@ -130,6 +135,13 @@ class AdapterManager:
     def unload(self, name: str) -> None:
         self._clear(self.slot(name))
         del self.slots[name], self.keys[name]
+
+    def forget(self) -> None:
+        """The stacks' memory is about to lose its contents: no adapter is loaded any more.  (No token names a slot before the
+        next load, which empties them on the device first.)"""
+        self.slots.clear()
+        self.keys.clear()
+        self._lost = True
 
     def slot(self, name: str) -> int:
         if name not in self.slots:

@@ -151,6 +151,13 @@ class LoraStack:
             self.ranks[slot].zero_()
         self._set_ranks(slot, [0] * len(self.slices))
 
+    def reset(self) -> None:
+        """Empty every slot, whatever the memory holds."""
+        with torch.inference_mode():
+            self.ranks.zero_()
+        for slot in range(self.num_slots):
+            self._set_ranks(slot, [0] * len(self.slices))
+
     def factors(self, slot: int):
         """(A, B) of each slice of a slot (ranks padded to 16), None where it has none."""
         ranks = self._ranks[slot]

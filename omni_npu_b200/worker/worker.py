@@ -206,11 +206,14 @@ class Worker:
             on_trace_ready=torch.profiler.tensorboard_trace_handler(trace_dir, use_gzip=True))
 
     def sleep(self, level: int = 1) -> int:
-        """Level 1: weights are kept in pinned host memory, the KV cache is discarded; level 2: both
-        are discarded.  Returns the device bytes released.
+        """Level 1: weights and loaded adapters are kept in pinned host memory, the KV cache is discarded; level 2: all
+        are discarded, adapters have to be loaded again.  Returns the device bytes released.
         (reference: sleep-mode pool, omni_npu/worker/npu_mem_pool.py:109-284, wired in
         omni_npu/worker/npu_worker.py:164-179)"""
         from .mem_pool import B200MemAllocator
+        adapters = getattr(self.model_runner, "adapters", None)
+        if level != 1 and adapters is not None:
+            adapters.forget()                        # their factors lie beside the weights
         return B200MemAllocator.get_instance().sleep(offload_tags=("weights",) if level == 1 else ())
 
     def wake_up(self, tags=None) -> int:

@@ -4,7 +4,7 @@ from contextlib import contextmanager
 import pytest
 import torch
 
-from omni_npu_b200 import ops
+from omni_npu_b200 import SamplingParams, ops
 from omni_npu_b200.config import ModelConfig
 from omni_npu_b200.engine.llm import LLM
 from omni_npu_b200.worker import mem_pool
@@ -72,3 +72,36 @@ def test_the_addresses_of_page_copies_lie_outside_the_pool_that_is_discarded(poo
     worker.initialize_from_config(16)
     assert made == [("cache", "kv_cache"), ("addresses", None)]
     assert worker.model_runner.page_cache.num_blocks == 16
+
+
+def adapter(rank=4):
+    g = torch.Generator().manual_seed(rank)
+    tensors = {}
+    for layer in range(2):
+        name = f"base_model.model.model.layers.{layer}.self_attn.q_proj.lora_"
+        tensors[name + "A.weight"] = torch.randn(rank, 64, generator=g)
+        tensors[name + "B.weight"] = torch.randn(64, rank, generator=g)
+    return {"r": rank, "lora_alpha": 2 * rank}, tensors
+
+
+def test_adapters_outlive_the_first_level_and_not_the_second(pool):
+    llm = _llm(enable_lora=True, max_loras=2)
+    m = llm.engine.adapters()
+    config, tensors = adapter()
+    m.load_tensors("a", config, tensors.items())
+    sp = SamplingParams(max_tokens=5, ignore_eos=True)
+    want = llm.generate([[5, 6, 7]], sp, adapter="a")[0].output_token_ids
+    llm.sleep(1)
+    llm.wake_up()
+    assert llm.generate([[5, 6, 7]], sp, adapter="a")[0].output_token_ids == want
+    llm.sleep(2)
+    for s in m.stacks.values():                                 # what the device may hold after the wake-up
+        s.a.fill_(7), s.b.fill_(7), s.ranks.fill_(1 << 20)
+    llm.wake_up()
+    assert not m.slots and not m.keys
+    with pytest.raises(ValueError):
+        llm.generate([[5, 6, 7]], sp, adapter="a")
+    assert m.load_tensors("a", config, tensors.items()) == 0
+    # also where the adapter has no factors
+    assert all(not s.ranks[1].any() and (s.ranks[0, :-1] <= 16).all() for s in m.stacks.values())
+    assert llm.generate([[5, 6, 7]], sp, adapter="a")[0].output_token_ids == want
