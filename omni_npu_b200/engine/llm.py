@@ -119,13 +119,20 @@ class LLMEngine:
             raise ValueError("low-rank adapters are off (enable_lora=True turns them on)")
         return manager
 
+    def _awake_adapters(self):
+        """The adapter slots, to be written: their memory has to be there."""
+        adapters = self.adapters()
+        if self.worker.asleep:
+            raise ValueError("adapters are loaded and unloaded while the engine is awake: its memory has been given back")
+        return adapters
+
     def load_adapter(self, name: str, path: str) -> int:
         """Load a low-rank adapter (a directory in the PEFT layout) into a free slot; returns the slot."""
-        return self.adapters().load(name, path)
+        return self._awake_adapters().load(name, path)
 
     def unload_adapter(self, name: str) -> None:
         """Empty an adapter's slot; refused while requests use it."""
-        self.adapters().slot(name)
+        self._awake_adapters().slot(name)
         users = sum(r.adapter == name for r in self.scheduler.requests.values())
         if users or self._inflight is not None and any(r.adapter == name for r in self._inflight[1]["reqs"]):
             raise ValueError(f"adapter {name!r} is in use by {max(users, 1)} requests")

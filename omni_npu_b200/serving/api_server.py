@@ -319,13 +319,15 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
     @app.post("/sleep")
     async def sleep(level: int = 1):
         try:
-            return {"status": "asleep", "released_bytes": llm.sleep(level)}
+            with loop.lock:                                  # (not while an adapter is loaded into that memory)
+                return {"status": "asleep", "released_bytes": llm.sleep(level)}
         except RuntimeError as e:
             return JSONResponse({"error": str(e)}, status_code=409)
 
     @app.post("/wake_up")
     async def wake_up():
-        return {"status": "awake", "mapped_bytes": llm.wake_up()}
+        with loop.lock:
+            return {"status": "awake", "mapped_bytes": llm.wake_up()}
 
     @app.get("/ping")
     def ping():

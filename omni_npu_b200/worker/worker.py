@@ -220,6 +220,15 @@ class Worker:
         from .mem_pool import B200MemAllocator
         return B200MemAllocator.get_instance().wake_up(tags)
 
+    @property
+    def asleep(self) -> bool:
+        """Whether some of the engine's memory has been given back and not mapped again."""
+        if not self.config.enable_sleep_mode:
+            return False
+        from .mem_pool import B200MemAllocator
+        pool = B200MemAllocator.instance
+        return pool is not None and pool._sleeping
+
     def shutdown(self) -> None:
         if self.model_runner is not None and self.model_runner.kv_connector is not None:
             self.model_runner.kv_connector.close()

@@ -1,4 +1,5 @@
 """What sleep mode discards and what has to outlive it."""
+import json
 from contextlib import contextmanager
 
 import pytest
@@ -105,3 +106,47 @@ def test_adapters_outlive_the_first_level_and_not_the_second(pool):
     # also where the adapter has no factors
     assert all(not s.ranks[1].any() and (s.ranks[0, :-1] <= 16).all() for s in m.stacks.values())
     assert llm.generate([[5, 6, 7]], sp, adapter="a")[0].output_token_ids == want
+
+
+def test_adapters_are_not_written_while_their_memory_is_away(pool, tmp_path):
+    from safetensors.torch import save_file
+    config, tensors = adapter()
+    (tmp_path / "adapter_config.json").write_text(json.dumps(config))
+    save_file(tensors, str(tmp_path / "adapter_model.safetensors"))
+    llm = _llm(enable_lora=True, max_loras=2, enable_sleep_mode=True)
+    llm.load_adapter("a", str(tmp_path))
+    llm.sleep(1)
+    for _ in range(2):
+        with pytest.raises(ValueError, match="awake"):
+            llm.load_adapter("b", str(tmp_path))
+        with pytest.raises(ValueError, match="awake"):
+            llm.unload_adapter("a")
+        llm.wake_up(["kv_cache"])                               # the factors are still away
+    assert list(llm.engine.adapters().slots) == ["a"]
+    llm.wake_up()
+    assert llm.load_adapter("b", str(tmp_path)) == 1
+    llm.unload_adapter("a")
+    # an engine whose memory never lies in the pool
+    other = _llm(enable_lora=True, max_loras=1)
+    llm.sleep(1)
+    assert other.load_adapter("a", str(tmp_path)) == 0
+
+
+def test_the_server_sleeps_when_no_adapter_is_being_loaded(pool):
+    pytest.importorskip("fastapi")
+    from starlette.testclient import TestClient
+    from omni_npu_b200.serving.api_server import build_app
+    llm = _llm(enable_lora=True, max_loras=1, enable_sleep_mode=True)
+    app = build_app(llm, model_name="base")
+    lock, held = app.state.engine_loop.lock, []
+    for name in ("sleep", "wake_up"):
+        def call(*a, inner=getattr(llm, name)):
+            held.append(lock.locked())
+            return inner(*a)
+        setattr(llm, name, call)
+    with TestClient(app) as client:
+        assert client.post("/sleep").status_code == 200
+        assert client.post("/v1/load_lora_adapter", json={"lora_name": "a", "lora_path": "/nowhere"}).status_code == 400
+        assert client.post("/wake_up").status_code == 200
+    app.state.engine_loop.shutdown()
+    assert held == [True, True]
