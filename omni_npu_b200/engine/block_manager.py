@@ -12,7 +12,7 @@ so a remote consumer can still pull them
 from __future__ import annotations
 
 import time
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
 
 def chain_block_hashes(token_ids: Sequence[int], block_size: int, prev: Optional[List[bytes]] = None,
@@ -38,9 +38,10 @@ def chain_block_hashes(token_ids: Sequence[int], block_size: int, prev: Optional
 
 
 class BlockPool:
-    """Free list of KV blocks.  A block may be shared (``share``): it returns with its last user.  With ``prefix_caching`` a block may be shared by several requests
-    (reference counts) and a full block whose content hash was registered stays findable after its
-    last user frees it, until the block is needed again (least recently freed first)."""
+    """Free list of KV blocks.  A block may be shared by several requests (``share``, reference
+    counts): it returns with its last user.  With ``prefix_caching`` a full block whose content hash
+    was registered stays findable after its last user frees it, until the block is needed again
+    (least recently freed first)."""
 
     def __init__(self, num_blocks: int, block_size: int, num_reserved: int = 0, prefix_caching: bool = False) -> None:
         if num_blocks <= num_reserved:
@@ -127,6 +128,16 @@ class BlockPool:
             return
         self._hash_of[block] = content_hash
         self._block_of[content_hash] = block
+
+    def unregister(self, blocks: Iterable[int]) -> None:
+        """These blocks no longer hold what was registered: nobody finds them by it any more."""
+        for b in blocks:
+            content_hash = self._hash_of.pop(b, None)
+            if content_hash is not None:
+                del self._block_of[content_hash]
+            if b in self._cached_free:
+                del self._cached_free[b]
+                self._free.append(b)
 
     def match_prefix(self, hashes: Sequence[bytes]) -> List[int]:
         """Blocks holding the longest cached prefix of the hash chain (not yet acquired)."""

@@ -326,20 +326,20 @@ class LLMEngine:
     def _after_recovered_step(self, out, verdict: dict) -> List[RequestOutput]:
         """The step failed and the workers recovered (token recovery).  ``recompute``: nothing
         of the step is kept, every scheduled request is recomputed from scratch (its KV may be
-        half-written); ``abort``: requests that own a damaged KV block are aborted, the rest
-        recomputed."""
+        half-written); ``abort``: running requests that own a damaged KV block are aborted (blocks are
+        shared, so some of them may not be part of the step), the rest of the step is recomputed."""
         self.stats["recovered_steps"] = self.stats.get("recovered_steps", 0) + 1
-        bad = set(verdict.get("bad_blocks") or [])
+        damaged: List[Request] = []
+        if verdict.get("opt") == "abort":
+            damaged = self.scheduler.lose_blocks(set(verdict.get("bad_blocks") or []))
         finished: List[RequestOutput] = []
+        for req in damaged:
+            self.scheduler.abort_request(req.request_id)
+            self.worker.model_runner.input_batch.remove_request(req.request_id)
+            finished.append(RequestOutput.from_request(req))
         for seq in list(out.seqs):
             req = seq.request
-            if req.is_finished:
-                continue
-            if verdict.get("opt") == "abort" and bad & set(req.block_ids):
-                self.scheduler.abort_request(req.request_id)
-                self.worker.model_runner.input_batch.remove_request(req.request_id)
-                finished.append(RequestOutput.from_request(req))
-            else:
+            if not req.is_finished:
                 self.scheduler.preempt_for_recompute(req)
                 self.worker.model_runner.input_batch.remove_request(req.request_id)
         return finished

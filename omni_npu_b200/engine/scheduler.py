@@ -13,7 +13,7 @@ from __future__ import annotations
 import time
 from collections import deque
 from dataclasses import dataclass, field
-from typing import Any, Deque, Dict, List, Optional, Tuple
+from typing import Any, Deque, Dict, List, Optional, Set, Tuple
 
 from ..config import CacheConfig, SchedulerConfig
 from .block_manager import BlockPool, StateSlotPool
@@ -186,17 +186,28 @@ class Scheduler:
             self.pool.free([req.fork_source[0]])
             req.fork_source = None
 
+    def _drop_shared_blocks(self, req: Request) -> bool:
+        """Take the shared blocks back from a sample that waits for admission (it computes the prompt then)."""
+        if not req.block_ids and req.fork_source is None:
+            return False
+        self._drop_fork_source(req)
+        self.pool.free(req.block_ids)
+        req.block_ids = []
+        req.num_computed_tokens = 0
+        return True
+
     def _drop_waiting_forks(self) -> bool:
-        """Take the shared blocks back from samples that wait for admission (they compute the prompt then)."""
-        dropped = False
+        """The same of all such samples."""
+        return any([self._drop_shared_blocks(req) for req in self.waiting]) if self.can_fork else False
+
+    def lose_blocks(self, blocks: Set[int]) -> List[Request]:
+        """The contents of these blocks are lost: nobody finds them in the prefix cache any more, and samples that wait for
+        admission with them compute their prompt again.  Returns the running requests that own one."""
+        self.pool.unregister(blocks)
         for req in self.waiting if self.can_fork else ():
-            if req.block_ids or req.fork_source is not None:
-                dropped = True
-                self._drop_fork_source(req)
-                self.pool.free(req.block_ids)
-                req.block_ids = []
-                req.num_computed_tokens = 0
-        return dropped
+            if not blocks.isdisjoint(req.block_ids) or req.fork_source is not None and req.fork_source[0] in blocks:
+                self._drop_shared_blocks(req)
+        return [req for req in self.running if not blocks.isdisjoint(req.block_ids)]
 
     # ---------------------------------------------------------------- blocks
     def _ensure_blocks(self, req: Request, total_tokens: int) -> bool:
