@@ -95,7 +95,7 @@ class ModelRunner:
         self._plp_capture = None
         # logits at chosen rows of a step (trace replay): the rows asked for, and what was computed there
         self.keep_logits = False              # captured decode graphs also keep their logits
-        self._graph_logits: Dict[int, torch.Tensor] = {}
+        self._graph_logits: Dict[Tuple[int, bool], torch.Tensor] = {}    # by size, and whether with adapters
         self._want_rows: Optional[List[int]] = None
         self.last_logits: Optional[torch.Tensor] = None
         self.last_prompt_logprobs: Dict[int, Tuple[int, list]] = {}
@@ -295,7 +295,7 @@ class ModelRunner:
                     rows = torch.tensor(self._want_rows, dtype=torch.long, device=hidden_all.device)
                     self.last_logits = self.model.compute_logits(hidden_all.index_select(0, rows))
             elif self.keep_logits and not md.is_prefill:
-                self._graph_logits[num_samples] = logits
+                self._graph_logits[num_samples, bool(md.extra.get("adapters"))] = logits
             if self._logits_fn is not None:
                 logits = self._logits_fn(logits)
             # (no step offset: the staged seed of a row already carries the index of the token it samples)
@@ -797,7 +797,7 @@ class ModelRunner:
             got = self.last_logits
             if out.kind == "decode":
                 if got is None:                     # the step ran as a graph
-                    got = self._graph_logits[self._pad_decode_size(len(out.seqs))]
+                    got = self._graph_logits[self._pad_decode_size(len(out.seqs)), self._uses_adapters(out.seqs)]
                 got = got.index_select(0, torch.tensor(self._want_rows, dtype=torch.long, device=got.device))
             return got.float().cpu()
         finally:
