@@ -519,7 +519,6 @@ class EngineConfig:
     compilation: CompilationConfig = field(default_factory=CompilationConfig)
     kv_transfer: Optional[KVTransferConfig] = None
     speculative: SpeculativeConfig = field(default_factory=SpeculativeConfig)
-    adapters: AdapterConfig = field(default_factory=AdapterConfig)
     model_path: Optional[str] = None          # HF directory with safetensors; None = random init
     load_format: str = "auto"                 # auto | dummy
     seed: int = 0
@@ -527,6 +526,7 @@ class EngineConfig:
     enforce_eager: bool = False
     enable_sleep_mode: bool = False
     additional_config: Dict[str, Any] = field(default_factory=dict)
+    adapters: AdapterConfig = field(default_factory=AdapterConfig)
 
     def __post_init__(self) -> None:
         ac = self.additional_config

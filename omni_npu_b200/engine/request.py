@@ -35,8 +35,6 @@ class SamplingParams:
     # token sequences that must not appear in the output: once the output ends with all but the last
     # token of one of them, that last token cannot be sampled
     bad_words_token_ids: Optional[Sequence[Sequence[int]]] = None
-    # samples drawn from this prompt (offline front end); each has a seed of its own
-    n: int = 1
     # scheduling priority under SchedulerConfig.policy == "priority": lower values are admitted first
     # and preempted last (ties: earlier arrival first)
     priority: int = 0
@@ -44,6 +42,8 @@ class SamplingParams:
     # {"grammar": ebnf} (sample/structured.py); needs a tokenizer given to the engine
     structured: Optional[Dict[str, Any]] = None
     extra_args: Dict[str, Any] = field(default_factory=dict)
+    # samples drawn from this prompt (offline front end); each has a seed of its own
+    n: int = 1
 
     @property
     def greedy(self) -> bool:

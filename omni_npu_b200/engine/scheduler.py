@@ -40,10 +40,10 @@ class SchedulerOutput:
     preempted: List[str] = field(default_factory=list)
     finished_req_ids: List[str] = field(default_factory=list)
     kv_connector_metadata: Any = None
-    # cache pages to copy before the step: (source, destination, rows)
-    block_copies: List[Tuple[int, int, int]] = field(default_factory=list)
     step_index: int = 0
     pending_pos: List[int] = field(default_factory=list)   # asynchronous scheduling: output index of each placeholder
+    # cache pages to copy before the step: (source, destination, rows)
+    block_copies: List[Tuple[int, int, int]] = field(default_factory=list)
 
     @property
     def total_num_scheduled_tokens(self) -> int:
