@@ -96,17 +96,20 @@ class Scheduler:
         self._enqueue(req)
 
     def add_fork(self, req: Request, parent_id: str) -> None:
-        """A request with the prompt of another one: it waits until that prompt has been computed and then shares its
-        blocks, computing the last token alone.  Without such a parent, or where blocks cannot be shared, an ordinary
-        request."""
+        """A request with the prompt of another one: it shares that prompt's blocks, once they have been computed, and
+        computes the last token alone.  Without such a parent, or where blocks cannot be shared, an ordinary request."""
         parent = self.requests.get(parent_id)
-        if (not self.can_fork or parent is None or parent.is_finished or parent.num_computed_tokens >= parent.num_prompt_tokens
+        if (not self.can_fork or parent is None or parent.is_finished
                 or parent.prompt_token_ids != req.prompt_token_ids or parent.adapter != req.adapter
                 or req.sampling_params.prompt_logprobs is not None or parent.request_id in self.held):
             return self.add_request(req)
         self.requests[req.request_id] = req
-        self.held[req.request_id] = req
-        parent.forks.append(req)
+        if parent.num_computed_tokens >= parent.num_prompt_tokens:
+            self._share_prompt(parent, req)
+            self._enqueue(req)
+        else:
+            self.held[req.request_id] = req
+            parent.forks.append(req)
 
     def _enqueue(self, req: Request) -> None:
         if self.cfg.policy == "priority":
@@ -153,27 +156,31 @@ class Scheduler:
 
     # ------------------------------------------------- several samples of one prompt
     def _fork_prompt(self, parent: Request) -> None:
-        """The prompt of ``parent`` has been computed: its further samples take its blocks over and may be admitted.  They share
-        the whole blocks; of the last one they get a copy of the rows before the prompt's last token, which
-        each computes itself (it writes there, and its logits are what the sample is drawn from)."""
+        """The prompt of ``parent`` has been computed: its further samples take its blocks over and may be admitted."""
         forks, parent.forks = parent.forks, []
         front = self.cfg.policy != "priority"          # they arrived with their parent, before what waits now
-        full, rows = divmod(parent.num_prompt_tokens - 1, self.block_size)
         for req in reversed(forks) if front else forks:
             del self.held[req.request_id]
-            req.block_ids = parent.block_ids[:full]
-            self.pool.share(req.block_ids)
-            req.num_computed_tokens = full * self.block_size
-            if rows and self.copies_pages:
-                req.fork_source = (parent.block_ids[full], rows)
-                self.pool.share([parent.block_ids[full]])
-                req.num_computed_tokens += rows
-            self.fork_stats["requests"] += 1
-            self.fork_stats["shared_tokens"] += req.num_computed_tokens
+            self._share_prompt(parent, req)
             if front:
                 self.waiting.appendleft(req)
             else:
                 self._enqueue(req)
+
+    def _share_prompt(self, parent: Request, req: Request) -> None:
+        """A further sample shares the whole blocks of its parent's computed prompt; of the last one it gets a copy of the
+        rows before the prompt's last token, which it computes itself (it writes there, and its logits are what the sample
+        is drawn from)."""
+        full, rows = divmod(parent.num_prompt_tokens - 1, self.block_size)
+        req.block_ids = parent.block_ids[:full]
+        self.pool.share(req.block_ids)
+        req.num_computed_tokens = full * self.block_size
+        if rows and self.copies_pages:
+            req.fork_source = (parent.block_ids[full], rows)
+            self.pool.share([parent.block_ids[full]])
+            req.num_computed_tokens += rows
+        self.fork_stats["requests"] += 1
+        self.fork_stats["shared_tokens"] += req.num_computed_tokens
 
     def _release_fork_sources(self) -> None:
         """The last step's page copies have been launched: what they read may be given out again."""
