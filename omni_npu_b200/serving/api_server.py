@@ -70,27 +70,41 @@ class EngineLoop:
         """``stop``: strings that end the request when they appear in its decoded output (needs
         ``self.tokenizer``); the answer's text is cut before the first of them.  ``adapter``, ``fork_of``: as in
         ``LLMEngine.add_request``."""
-        self.engine.validate_sampling_params(sp)        # ValueError -> HTTP 400, before anything is queued
+        return self.submit_samples(prompt_ids, [sp], kv_transfer_params, stop, adapter, fork_of)[0]
+
+    def submit_samples(self, prompt_ids: List[int], sps: List[SamplingParams], kv_transfer_params=None,
+                       stop: Optional[List[str]] = None, adapter: Optional[str] = None,
+                       fork_of: Optional[str] = None) -> List[str]:
+        """Several samples of one prompt, which share its blocks (``fork_of``, else the first one's).  No step runs in
+        between: all of them are added, or none."""
+        for sp in sps:
+            self.engine.validate_sampling_params(sp)    # ValueError -> HTTP 400, before anything is queued
         if stop and self.tokenizer is None:
             raise ValueError("stop strings need a tokenizer (use stop_token_ids on a server without one)")
-        rid = f"cmpl-{uuid.uuid4().hex}"
-        slot = {"event": threading.Event(), "output": None, "seen": 0, "queue": [], "request": None,
-                "stop": [s for s in (stop or []) if s], "text": None}
+        rids: List[str] = []
         with self.lock:
-            self.waiters[rid] = slot
-            if self.group is None:
-                try:
-                    self.engine.add_request(prompt_ids, sp, request_id=rid, kv_transfer_params=kv_transfer_params,
-                                            adapter=adapter, fork_of=fork_of)
-                except ValueError:
-                    del self.waiters[rid]
-                    raise
-                slot["request"] = self.engine.scheduler.requests[rid]
-            else:                                   # added on every rank by the next broadcast
-                self._new.append((rid, list(prompt_ids), sp, kv_transfer_params, fork_of))
-            self.counters["requests"] += 1
+            for sp in sps:
+                rid = f"cmpl-{uuid.uuid4().hex}"
+                slot = {"event": threading.Event(), "output": None, "seen": 0, "queue": [], "request": None,
+                        "stop": [s for s in (stop or []) if s], "text": None}
+                if self.group is None:
+                    try:
+                        self.engine.add_request(prompt_ids, sp, request_id=rid, kv_transfer_params=kv_transfer_params,
+                                                adapter=adapter, fork_of=fork_of)
+                    except ValueError:
+                        for earlier in rids:
+                            self.engine.abort_request(earlier)
+                            del self.waiters[earlier]
+                        raise
+                    slot["request"] = self.engine.scheduler.requests[rid]
+                else:                                   # added on every rank by the next broadcast
+                    self._new.append((rid, list(prompt_ids), sp, kv_transfer_params, fork_of))
+                self.waiters[rid] = slot
+                rids.append(rid)
+                fork_of = fork_of or rid
+            self.counters["requests"] += len(rids)
         self.wake.set()
-        return rid
+        return rids
 
     def abort(self, rid: str) -> None:
         with self.lock:
@@ -411,13 +425,15 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
         manager = llm.engine.worker.model_runner.adapters
         return body.get("model") if manager is not None and body.get("model") in manager.slots else None
 
-    def _submit(ids, body, fork_of: Optional[str] = None) -> str:
+    def _submit(ids, body, n: int = 1) -> List[str]:
         stop = body.get("stop")
         stop = [stop] if isinstance(stop, str) else list(stop or [])
         adapter = _adapter(body)
+        # (each sample draws from its own default seed, or from seed + index)
+        bodies = [dict(body, seed=body["seed"] + i) if i and body.get("seed") is not None else body for i in range(n)]
         try:
-            return loop.submit(ids, sampling_from_body(body, tokenizer), body.get("kv_transfer_params"), stop=stop,
-                               adapter=adapter, fork_of=fork_of)
+            return loop.submit_samples(ids, [sampling_from_body(b, tokenizer) for b in bodies],
+                                       body.get("kv_transfer_params"), stop=stop, adapter=adapter)
         except ValueError as e:
             raise HTTPException(400, str(e))
 
@@ -482,18 +498,14 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
         name = _adapter(body) or model_name
         n = _n_choices(body)
         if n > 1:
-            # n requests that share the first one's prompt (each draws from its own default seed, or from seed + index)
-            rids: List[str] = []
-            for i in range(n):
-                rids.append(_submit(ids, dict(body, seed=body["seed"] + i) if body.get("seed") is not None else body,
-                                    rids[0] if rids else None))
+            rids = _submit(ids, body, n)
             outs = [await _finish(r) for r in rids]
             done = sum(len(o.output_token_ids) for o in outs)
             return JSONResponse({
                 "id": rids[0], "object": "text_completion", "created": int(time.time()), "model": name,
                 "choices": [_completion_choice(i, o) for i, o in enumerate(outs)],
                 "usage": {"prompt_tokens": len(ids), "completion_tokens": done, "total_tokens": len(ids) + done}})
-        rid = _submit(ids, body)
+        rid = _submit(ids, body)[0]
         created = int(time.time())
         if body.get("stream"):
             def chunk(toks, finish):
@@ -518,7 +530,7 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
         else:
             raise HTTPException(400, "chat needs a tokenizer with a chat template")
         name = _adapter(body) or model_name
-        rid = _submit(ids, body)
+        rid = _submit(ids, body)[0]
         if body.get("stream"):
             # chat.completion.chunk events: the role first, then the text of the new tokens as they
             # arrive (reasoning / tool-call parsing needs the whole text and applies to the plain answer)
