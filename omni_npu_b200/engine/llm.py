@@ -128,7 +128,15 @@ class LLMEngine:
 
     def load_adapter(self, name: str, path: str) -> int:
         """Load a low-rank adapter (a directory in the PEFT layout) into a free slot; returns the slot."""
-        return self._awake_adapters().load(name, path)
+        return self.install_adapter(self.read_adapter(name, path))
+
+    def read_adapter(self, name: str, path: str):
+        """The first, long part of ``load_adapter``: files are read and checked, factors brought to the device.  It may run
+        beside steps; what it returns is for ``install_adapter``, which may not."""
+        return self._awake_adapters().read(name, path)
+
+    def install_adapter(self, adapter) -> int:
+        return self._awake_adapters().install(adapter)
 
     def unload_adapter(self, name: str) -> None:
         """Empty an adapter's slot; refused while requests use it."""

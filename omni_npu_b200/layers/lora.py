@@ -11,6 +11,7 @@ import itertools
 import json
 import os
 import re
+from dataclasses import dataclass
 from typing import Dict, Iterable, List, Optional, Tuple
 
 import torch
@@ -41,6 +42,14 @@ class LoraLinearMethod:
 
 
 _TENSOR = re.compile(r"^(?:base_model\.model\.)?(?P<module>.+)\.lora_(?P<which>[AB])(?:\.default)?\.weight$")
+
+
+@dataclass
+class Adapter:
+    """A checked adapter whose factors are on the device, in no slot yet."""
+    name: str
+    scale: float
+    factors: Dict[str, List[List[Optional[torch.Tensor]]]]       # of a projection: A of each slice, B of each slice
 
 
 class AdapterManager:
@@ -85,17 +94,23 @@ class AdapterManager:
     # ------------------------------------------------------------------ adapters
     def load(self, name: str, path: str) -> int:
         """Load a PEFT directory under ``name``; returns its slot."""
-        with open(os.path.join(path, "adapter_config.json")) as f:
-            config = json.load(f)
-        from ..models.utils import iter_safetensors
-        return self.load_tensors(name, config, iter_safetensors(path))
+        return self.install(self.read(name, path))
 
     def load_tensors(self, name: str, config: dict, tensors: Iterable[Tuple[str, torch.Tensor]]) -> int:
         """Load an adapter from its configuration and (name, tensor) pairs."""
-        if not name or name in self.slots:
-            raise ValueError(f"adapter {name!r} is already loaded" if name else "an adapter needs a name")
-        if len(self.slots) == self.num_slots:
-            raise ValueError(f"all {self.num_slots} adapter slots are taken")
+        return self.install(self.prepare(name, config, tensors))
+
+    def read(self, name: str, path: str) -> Adapter:
+        """The adapter of a PEFT directory.  Like ``prepare`` it changes nothing here, so steps may run meanwhile."""
+        self._check_free(name)
+        with open(os.path.join(path, "adapter_config.json")) as f:
+            config = json.load(f)
+        from ..models.utils import iter_safetensors
+        return self.prepare(name, config, iter_safetensors(path))
+
+    def prepare(self, name: str, config: dict, tensors: Iterable[Tuple[str, torch.Tensor]]) -> Adapter:
+        """Check an adapter and bring its factors to the device."""
+        self._check_free(name)
         for key, off in (("use_dora", False), ("bias", "none"), ("fan_in_fan_out", False), ("modules_to_save", None),
                          ("rank_pattern", {}), ("alpha_pattern", {}), ("peft_type", "LORA")):
             if config.get(key) and config[key] != off:
@@ -111,26 +126,37 @@ class AdapterManager:
             if part is None:
                 raise ValueError(f"adapter {name!r}: {key} belongs to no projection that takes adapters")
             proj, i = part
-            n = len(self.stacks[proj].slices)
-            found.setdefault(proj, [[None] * n, [None] * n])["AB".index(m["which"])][i] = tensor
+            stack = self.stacks[proj]
+            n = len(stack.slices)
+            found.setdefault(proj, [[None] * n, [None] * n])["AB".index(m["which"])][i] = tensor.to(stack.device, stack.dtype)
         if not found:
             raise ValueError(f"adapter {name!r} has no factors")
+        return Adapter(name, scale, found)
+
+    def install(self, adapter: Adapter) -> int:
+        """Put an adapter into a free slot; returns it."""
+        name = adapter.name
+        self._check_free(name)
         if self._lost:
             for stack in self.stacks.values():
                 stack.reset()
             self._lost = False
         slot = next(i for i in range(self.num_slots) if i not in self.slots.values())
         try:
-            for proj, (a, b) in found.items():
-                dtype = self.stacks[proj].dtype
-                a, b = ([None if t is None else t.to(self.stacks[proj].device, dtype) for t in f] for f in (a, b))
-                self.stacks[proj].load(slot, a, b, scale)
+            for proj, (a, b) in adapter.factors.items():
+                self.stacks[proj].load(slot, a, b, adapter.scale)
         except Exception as e:
             self._clear(slot)
             raise ValueError(f"adapter {name!r}: {e}") if isinstance(e, ValueError) else e
         self.slots[name] = slot
         self.keys[name] = f"adapter {next(self._loads)} {name}".encode()
         return slot
+
+    def _check_free(self, name: str) -> None:
+        if not name or name in self.slots:
+            raise ValueError(f"adapter {name!r} is already loaded" if name else "an adapter needs a name")
+        if len(self.slots) == self.num_slots:
+            raise ValueError(f"all {self.num_slots} adapter slots are taken")
 
     def unload(self, name: str) -> None:
         self._clear(self.slot(name))

@@ -382,8 +382,10 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
     def load_adapter(body: Dict[str, Any]):
         """Load a low-rank adapter: ``lora_name`` as requests will ask for it (``model``), ``lora_path`` its directory."""
         try:
+            # (steps go on while the files are read)
+            adapter = llm.engine.read_adapter(str(body.get("lora_name") or ""), str(body.get("lora_path") or ""))
             with loop.lock:
-                slot = llm.load_adapter(str(body.get("lora_name") or ""), str(body.get("lora_path") or ""))
+                slot = llm.engine.install_adapter(adapter)
         except (ValueError, KeyError, OSError) as e:
             raise HTTPException(400, str(e))
         return {"status": "loaded", "slot": slot}

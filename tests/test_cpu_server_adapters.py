@@ -1,0 +1,74 @@
+"""Adapters that a server loads while it answers."""
+import json
+
+import pytest
+import torch
+
+from omni_npu_b200.config import ModelConfig
+from omni_npu_b200.engine.llm import LLM
+from omni_npu_b200.ops.lora import LoraStack
+
+pytest.importorskip("fastapi")
+from starlette.testclient import TestClient  # noqa: E402
+
+from omni_npu_b200.serving.api_server import build_app  # noqa: E402
+
+
+def _llm(**kw):
+    cfg = ModelConfig(hidden_size=64, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=16, intermediate_size=96, vocab_size=97,
+                      rope_theta=10000.0, max_position_embeddings=512, dtype=torch.float32)
+    args = dict(model=cfg, device="cpu", max_num_seqs=8, max_num_batched_tokens=64, max_model_len=128, num_gpu_blocks=64,
+                block_size=4, seed=3, enable_lora=True, max_loras=2)
+    args.update(kw)
+    return LLM(**args)
+
+
+def tensors(rank=4):
+    g = torch.Generator().manual_seed(rank)
+    return {f"base_model.model.model.layers.{i}.self_attn.q_proj.lora_{w}.weight": torch.randn(*s, generator=g)
+            for i in range(2) for w, s in (("A", (rank, 64)), ("B", (64, rank)))}
+
+
+def save(path, config=None, factors=None):
+    from safetensors.torch import save_file
+    path.mkdir()
+    (path / "adapter_config.json").write_text(config if isinstance(config, str) else json.dumps(config or {"r": 4, "lora_alpha": 8}))
+    save_file(factors or tensors(), str(path / "adapter_model.safetensors"))
+    return str(path)
+
+
+@pytest.fixture
+def server():
+    llm = _llm()
+    app = build_app(llm, model_name="base")
+    with TestClient(app, raise_server_exceptions=False) as client:
+        yield llm, app.state.engine_loop, client
+    app.state.engine_loop.shutdown()
+
+
+def test_files_are_read_beside_the_steps(server, tmp_path, monkeypatch):
+    llm, loop, client = server
+    seen = []
+    from omni_npu_b200.models import utils
+
+    def reading(path, inner=utils.iter_safetensors):
+        seen.append(("read", loop.lock.locked()))
+        return inner(path)
+
+    def load(self, *a, inner=LoraStack.load):
+        seen.append(("packed", loop.lock.locked()))
+        inner(self, *a)
+    monkeypatch.setattr(utils, "iter_safetensors", reading)
+    monkeypatch.setattr(LoraStack, "load", load)
+    path = save(tmp_path / "a")
+    assert client.post("/v1/load_lora_adapter", json={"lora_name": "a", "lora_path": path}).status_code == 200
+    assert seen == [("read", False)] + [("packed", True)] * 2
+    assert [m["id"] for m in client.get("/v1/models").json()["data"]] == ["base", "a"]
+    # a name or a slot that was taken meanwhile
+    b, c = (llm.engine.read_adapter(n, path) for n in "bc")
+    llm.engine.install_adapter(b)
+    with pytest.raises(ValueError):
+        llm.engine.install_adapter(b)
+    with pytest.raises(ValueError):
+        llm.engine.install_adapter(c)
+    assert llm.engine.adapters().slots == {"a": 0, "b": 1}
