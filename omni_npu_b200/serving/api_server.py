@@ -375,8 +375,10 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
     @app.get("/v1/models")
     def models():
         manager = llm.engine.worker.model_runner.adapters
+        with loop.lock:                                      # (another thread may be loading one)
+            names = list(manager.slots) if manager else []
         return {"object": "list", "data": [{"id": model_name, "object": "model"}]
-                + [{"id": name, "object": "model", "parent": model_name} for name in (manager.slots if manager else ())]}
+                + [{"id": name, "object": "model", "parent": model_name} for name in names]}
 
     @app.post("/v1/load_lora_adapter")
     def load_adapter(body: Dict[str, Any]):

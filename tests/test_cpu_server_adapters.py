@@ -72,3 +72,21 @@ def test_files_are_read_beside_the_steps(server, tmp_path, monkeypatch):
     with pytest.raises(ValueError):
         llm.engine.install_adapter(c)
     assert llm.engine.adapters().slots == {"a": 0, "b": 1}
+
+
+def test_models_are_listed_while_one_is_loaded(server, tmp_path):
+    llm, loop, client = server
+    path = save(tmp_path / "a")
+    adapters = llm.engine.adapters()
+
+    class Slots(dict):
+        """Another thread's load, as soon as the first name has been listed."""
+        def __iter__(self):
+            for i, name in enumerate(super().__iter__()):
+                yield name
+                if i == 0 and not loop.lock.locked():
+                    self["b"] = 1
+    adapters.slots = Slots()
+    assert client.post("/v1/load_lora_adapter", json={"lora_name": "a", "lora_path": path}).status_code == 200
+    got = client.get("/v1/models")
+    assert got.status_code == 200 and [m["id"] for m in got.json()["data"]] == ["base", "a"]
