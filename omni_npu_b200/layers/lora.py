@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import itertools
 import json
+import math
 import os
 import re
 from dataclasses import dataclass
@@ -105,17 +106,29 @@ class AdapterManager:
         self._check_free(name)
         with open(os.path.join(path, "adapter_config.json")) as f:
             config = json.load(f)
+        from safetensors import SafetensorError
         from ..models.utils import iter_safetensors
-        return self.prepare(name, config, iter_safetensors(path))
+        try:
+            return self.prepare(name, config, iter_safetensors(path))
+        except SafetensorError as e:
+            raise ValueError(f"adapter {name!r}: damaged file: {e}")
 
     def prepare(self, name: str, config: dict, tensors: Iterable[Tuple[str, torch.Tensor]]) -> Adapter:
         """Check an adapter and bring its factors to the device."""
         self._check_free(name)
+        if not isinstance(config, dict):
+            raise ValueError(f"adapter {name!r}: its configuration is not an object")
         for key, off in (("use_dora", False), ("bias", "none"), ("fan_in_fan_out", False), ("modules_to_save", None),
                          ("rank_pattern", {}), ("alpha_pattern", {}), ("peft_type", "LORA")):
             if config.get(key) and config[key] != off:
                 raise ValueError(f"adapter {name!r}: {key} = {config[key]!r} is not supported")
-        rank, alpha = int(config["r"]), float(config.get("lora_alpha", config["r"]))
+        try:
+            rank = int(config["r"])
+            alpha = float(config.get("lora_alpha", rank))
+        except (KeyError, TypeError, ValueError):
+            raise ValueError(f"adapter {name!r}: r = {config.get('r')!r} and lora_alpha = {config.get('lora_alpha')!r} are not numbers")
+        if not math.isfinite(alpha):
+            raise ValueError(f"adapter {name!r}: lora_alpha = {alpha}")
         if not 1 <= rank <= self.max_rank:
             raise ValueError(f"adapter {name!r} has rank {rank}, the engine takes 1 to {self.max_rank}")
         scale = alpha / rank ** 0.5 if config.get("use_rslora") else alpha / rank

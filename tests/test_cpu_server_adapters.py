@@ -90,3 +90,21 @@ def test_models_are_listed_while_one_is_loaded(server, tmp_path):
     assert client.post("/v1/load_lora_adapter", json={"lora_name": "a", "lora_path": path}).status_code == 200
     got = client.get("/v1/models")
     assert got.status_code == 200 and [m["id"] for m in got.json()["data"]] == ["base", "a"]
+
+
+@pytest.mark.parametrize("config", ["[1]", "{", json.dumps({"r": None}), json.dumps({"r": 4, "lora_alpha": None}),
+                                    json.dumps({"lora_alpha": 4}), json.dumps({"r": [4]}), json.dumps({"r": 4, "lora_alpha": float("nan")})])
+def test_a_configuration_that_is_none_is_the_callers_mistake(server, tmp_path, config):
+    llm, loop, client = server
+    got = client.post("/v1/load_lora_adapter", json={"lora_name": "a", "lora_path": save(tmp_path / "a", config)})
+    assert got.status_code == 400 and not llm.engine.adapters().slots
+
+
+@pytest.mark.parametrize("keep", [0, 4, 100, -10])
+def test_a_damaged_file_is_the_callers_mistake(server, tmp_path, keep):
+    llm, loop, client = server
+    path = save(tmp_path / "a")
+    file = tmp_path / "a" / "adapter_model.safetensors"
+    file.write_bytes(file.read_bytes()[:keep])
+    got = client.post("/v1/load_lora_adapter", json={"lora_name": "a", "lora_path": path})
+    assert got.status_code == 400 and not llm.engine.adapters().slots
