@@ -138,6 +138,9 @@ class AdapterManager:
             part = self.parts.get(m["module"]) if m else None
             if part is None:
                 raise ValueError(f"adapter {name!r}: {key} belongs to no projection that takes adapters")
+            if tensor.dim() != 2 or tensor.shape["AB".index(m["which"])] != rank:
+                # (the scale is the configuration's)
+                raise ValueError(f"adapter {name!r}: {key} is {tuple(tensor.shape)}, its rank should be {rank}")
             proj, i = part
             stack = self.stacks[proj]
             n = len(stack.slices)

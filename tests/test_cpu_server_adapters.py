@@ -108,3 +108,13 @@ def test_a_damaged_file_is_the_callers_mistake(server, tmp_path, keep):
     file.write_bytes(file.read_bytes()[:keep])
     got = client.post("/v1/load_lora_adapter", json={"lora_name": "a", "lora_path": path})
     assert got.status_code == 400 and not llm.engine.adapters().slots
+
+
+def test_factors_of_another_rank_than_the_configurations():
+    """They would be scaled by a rank that is not theirs."""
+    m = _llm().engine.adapters()
+    with pytest.raises(ValueError, match="rank should be 8"):
+        m.load_tensors("a", {"r": 8, "lora_alpha": 16}, tensors(4).items())
+    with pytest.raises(ValueError, match="rank should be 4"):
+        m.load_tensors("a", {"r": 4}, {k: v[0] for k, v in tensors(4).items()}.items())
+    assert not m.slots and m.load_tensors("a", {"r": 4}, tensors(4).items()) == 0
