@@ -297,7 +297,10 @@ def sampling_from_body(body: Dict[str, Any], tokenizer=None) -> SamplingParams:
                           logit_bias={int(k): float(v) for k, v in (body.get("logit_bias") or {}).items()} or None)
 
 
-def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=None, tool_parser=None):
+def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=None, tool_parser=None,
+              adapter_routes: bool = True):
+    """The server's application.  ``adapter_routes``: whether adapters may be loaded, from any directory that this process
+    can read, and unloaded over HTTP."""
     from fastapi import FastAPI, HTTPException
     from fastapi.responses import JSONResponse, PlainTextResponse, StreamingResponse
 
@@ -380,26 +383,27 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
         return {"object": "list", "data": [{"id": model_name, "object": "model"}]
                 + [{"id": name, "object": "model", "parent": model_name} for name in names]}
 
-    @app.post("/v1/load_lora_adapter")
-    def load_adapter(body: Dict[str, Any]):
-        """Load a low-rank adapter: ``lora_name`` as requests will ask for it (``model``), ``lora_path`` its directory."""
-        try:
-            # (steps go on while the files are read)
-            adapter = llm.engine.read_adapter(str(body.get("lora_name") or ""), str(body.get("lora_path") or ""))
-            with loop.lock:
-                slot = llm.engine.install_adapter(adapter)
-        except (ValueError, KeyError, OSError) as e:
-            raise HTTPException(400, str(e))
-        return {"status": "loaded", "slot": slot}
+    if adapter_routes:
+        @app.post("/v1/load_lora_adapter")
+        def load_adapter(body: Dict[str, Any]):
+            """Load a low-rank adapter: ``lora_name`` as requests will ask for it (``model``), ``lora_path`` its directory."""
+            try:
+                # (steps go on while the files are read)
+                adapter = llm.engine.read_adapter(str(body.get("lora_name") or ""), str(body.get("lora_path") or ""))
+                with loop.lock:
+                    slot = llm.engine.install_adapter(adapter)
+            except (ValueError, KeyError, OSError) as e:
+                raise HTTPException(400, str(e))
+            return {"status": "loaded", "slot": slot}
 
-    @app.post("/v1/unload_lora_adapter")
-    def unload_adapter(body: Dict[str, Any]):
-        try:
-            with loop.lock:
-                llm.unload_adapter(str(body.get("lora_name") or ""))
-        except ValueError as e:
-            raise HTTPException(400, str(e))
-        return {"status": "unloaded"}
+        @app.post("/v1/unload_lora_adapter")
+        def unload_adapter(body: Dict[str, Any]):
+            try:
+                with loop.lock:
+                    llm.unload_adapter(str(body.get("lora_name") or ""))
+            except ValueError as e:
+                raise HTTPException(400, str(e))
+            return {"status": "unloaded"}
 
     @app.get("/metrics")
     def metrics():
@@ -606,6 +610,7 @@ def make_parser() -> argparse.ArgumentParser:
     ap.add_argument("--enable-lora", action="store_true", help="take low-rank adapters beside the model's weights")
     ap.add_argument("--max-loras", type=int, default=8, help="adapters loaded at once")
     ap.add_argument("--max-lora-rank", type=int, default=16)
+    ap.add_argument("--no-lora-routes", action="store_true", help="adapters are those of --lora-modules, none over HTTP")
     ap.add_argument("--lora-modules", nargs="*", default=[], metavar="NAME=PATH", help="adapters to load at the start")
     ap.add_argument("--compilation-config", type=json.loads, default=None)
     ap.add_argument("--kv-transfer-config", type=json.loads, default=None)
@@ -673,7 +678,8 @@ def main(argv=None) -> None:
             proc.__init__(proc.cfg, device=proc.device)
     rp = get_reasoning_parser(args.reasoning_parser)(tokenizer) if args.reasoning_parser and tokenizer else None
     tp = get_tool_parser(args.tool_call_parser)(tokenizer) if args.tool_call_parser and tokenizer else None
-    app = build_app(llm, tokenizer, args.served_model_name or os.path.basename(str(args.model)), rp, tp)
+    app = build_app(llm, tokenizer, args.served_model_name or os.path.basename(str(args.model)), rp, tp,
+                    adapter_routes=not args.no_lora_routes)
     uvicorn.run(app, host=args.host, port=args.port, log_level="info")
 
 

@@ -118,3 +118,20 @@ def test_factors_of_another_rank_than_the_configurations():
     with pytest.raises(ValueError, match="rank should be 4"):
         m.load_tensors("a", {"r": 4}, {k: v[0] for k, v in tensors(4).items()}.items())
     assert not m.slots and m.load_tensors("a", {"r": 4}, tensors(4).items()) == 0
+
+
+def test_a_server_without_routes_for_adapters(tmp_path):
+    from omni_npu_b200.serving.api_server import make_parser
+    llm = _llm()
+    path = save(tmp_path / "a")
+    llm.load_adapter("a", path)
+    app = build_app(llm, model_name="base", adapter_routes=False)
+    with TestClient(app) as client:
+        assert client.post("/v1/load_lora_adapter", json={"lora_name": "b", "lora_path": path}).status_code == 404
+        assert client.post("/v1/unload_lora_adapter", json={"lora_name": "a"}).status_code == 404
+        assert [m["id"] for m in client.get("/v1/models").json()["data"]] == ["base", "a"]
+        body = {"prompt": [5, 6, 7, 8], "max_tokens": 3, "ignore_eos": True, "model": "a"}
+        assert client.post("/v1/completions", json=body).json()["model"] == "a"
+    app.state.engine_loop.shutdown()
+    args = make_parser().parse_args(["--model", "m"])
+    assert not args.no_lora_routes and make_parser().parse_args(["--model", "m", "--no-lora-routes"]).no_lora_routes
