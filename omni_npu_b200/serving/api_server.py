@@ -387,6 +387,8 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
         @app.post("/v1/load_lora_adapter")
         def load_adapter(body: Dict[str, Any]):
             """Load a low-rank adapter: ``lora_name`` as requests will ask for it (``model``), ``lora_path`` its directory."""
+            if body.get("lora_name") == model_name:
+                raise HTTPException(400, f"{model_name!r} is the served model's name")
             try:
                 # (steps go on while the files are read)
                 adapter = llm.engine.read_adapter(str(body.get("lora_name") or ""), str(body.get("lora_path") or ""))
@@ -429,9 +431,9 @@ def build_app(llm, tokenizer=None, model_name: str = "model", reasoning_parser=N
         return PlainTextResponse("\n".join(lines) + "\n")
 
     def _adapter(body) -> Optional[str]:
-        """A request names an adapter as its model; any other name stands for the served model."""
-        manager = llm.engine.worker.model_runner.adapters
-        return body.get("model") if manager is not None and body.get("model") in manager.slots else None
+        """A request names an adapter as its model; the served model's name, and any other, stands for the served model."""
+        manager, name = llm.engine.worker.model_runner.adapters, body.get("model")
+        return name if manager is not None and name != model_name and name in manager.slots else None
 
     def _submit(ids, body, n: int = 1) -> List[str]:
         stop = body.get("stop")

@@ -4,6 +4,7 @@ import json
 import pytest
 import torch
 
+from omni_npu_b200 import SamplingParams
 from omni_npu_b200.config import ModelConfig
 from omni_npu_b200.engine.llm import LLM
 from omni_npu_b200.ops.lora import LoraStack
@@ -135,3 +136,15 @@ def test_a_server_without_routes_for_adapters(tmp_path):
     app.state.engine_loop.shutdown()
     args = make_parser().parse_args(["--model", "m"])
     assert not args.no_lora_routes and make_parser().parse_args(["--model", "m", "--no-lora-routes"]).no_lora_routes
+
+
+def test_the_served_models_name_stays_the_served_models(server, tmp_path):
+    llm, loop, client = server
+    path = save(tmp_path / "a", factors={k: 3 * v for k, v in tensors().items()})
+    body = {"prompt": [5, 6, 7, 8], "max_tokens": 6, "ignore_eos": True, "model": "base"}
+    want = client.post("/v1/completions", json=body).json()["choices"][0]["token_ids"]
+    assert client.post("/v1/load_lora_adapter", json={"lora_name": "base", "lora_path": path}).status_code == 400
+    llm.load_adapter("base", path)                            # (not over HTTP)
+    assert llm.generate([[5, 6, 7, 8]], adapter="base", sampling_params=SamplingParams(max_tokens=6, ignore_eos=True)
+                        )[0].output_token_ids != want
+    assert client.post("/v1/completions", json=body).json()["choices"][0]["token_ids"] == want
