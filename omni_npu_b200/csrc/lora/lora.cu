@@ -5,7 +5,7 @@
 //
 // for tokens t with adapter s = slots[t] (none: z = y).  y is the shared product; p(n) is the slice of column n (query, key and
 // value of a joined projection have factors of their own).  Ranks are multiples of 16 (zero padded), 0 for a slice without an
-// adapter; the slices' A of a slot are joined along the rank.
+// adapter; the slices' A of a slot are joined along the rank.  The padded ranks' h is 0 also where x holds an infinity.
 //
 // The factors lie in the order in which the matrix instructions take them, so that they are read in whole kilobytes and need no
 // shuffling: as 8 x 8 matrices (rows of ldmatrix, unswizzled operands of tcgen05), B of stacks up to rank 32, whose products all are
@@ -141,7 +141,7 @@ struct LoraParams {
   const __nv_bfloat16* a;                        // [L, a_slot]
   const __nv_bfloat16* b;                        // [L, b_slot]
   long long a_slot, b_slot;
-  const int* ranks;                              // [L, slices + 1]: of each slice, then the scale's bits
+  const int* ranks;                              // [L, slices + 1]: of each slice, not padded, then the scale's bits
   const int* order;
   const LoraTile* tiles;
   const int* num_tiles;
@@ -171,6 +171,13 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 
 __device__ __forceinline__ float lo_f(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float hi_f(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+__device__ __forceinline__ constexpr int padded_rank(int r) { return (r + 15) & ~15; }
+// The slices' ranks of an adapter together.
+__device__ __forceinline__ int joined_ranks(const LoraParams& p, int slot) {
+  int sum = 0;
+  for (int s = 0; s < p.slices; ++s) sum += padded_rank(p.ranks[slot * (p.slices + 1) + s]);
+  return sum;
+}
 __device__ __forceinline__ float lora_scale(const LoraParams& p, int slot) {
   return __int_as_float(p.ranks[slot * (p.slices + 1) + p.slices]);
 }
@@ -198,6 +205,24 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
+}
+
+// Whether joined rank `col` is a rank, not padding.  An infinity or NaN in x times the zeros of a padded rank is NaN, which would
+// go on to every column: the padded ranks' h is taken as 0.
+__device__ __forceinline__ bool is_rank(const LoraParams& p, int slot, int col) {
+  const int* ranks = p.ranks + slot * (p.slices + 1);
+  for (int s = 0; s < p.slices; ++s) {
+    const int pad = padded_rank(ranks[s]);
+    if (col < pad) return col < ranks[s];
+    col -= pad;
+  }
+  return false;
+}
+__device__ __forceinline__ void keep_ranks(float4& v, int left) {
+  v.x = left > 0 ? v.x : 0.f;
+  v.y = left > 1 ? v.y : 0.f;
+  v.z = left > 2 ? v.z : 0.f;
+  v.w = left > 3 ? v.w : 0.f;
 }
 
 // Four of h times the scale as the sum of two bf16 (17 bits of the fp32 values), so that the product with B adds no rounding
@@ -290,8 +315,7 @@ __global__ void __launch_bounds__(kFewThreads) lora_shrink_few_kernel(const Lora
   pdl_trigger();                                                       // (the second kernel reads what was there before this one)
   LoraTile tl;
   if (!lora_tile(p, blockIdx.z, tl) || tl.slot < 0) return;
-  int sum_r = 0;
-  for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * (p.slices + 1) + s];
+  const int sum_r = joined_ranks(p, tl.slot);
   const int n0 = blockIdx.y * W;
   if (n0 >= sum_r) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
@@ -364,7 +388,7 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
   constexpr int W = kManyChunk * 8;
   extern __shared__ __align__(128) char smem[];
   __shared__ uint64_t full[kManyStages], empty[kManyStages], done;
-  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t tmem_slot, ranks_are[W / 32];                    // bits: not padding
   __shared__ int gave_up;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = (smem_u32(smem) + 1023) & ~1023u;
@@ -379,8 +403,7 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
   int order[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) order[i] = crow < 32 && crow + 32 * i < tl.count ? p.order[tl.start + crow + 32 * i] : 0;
-  int sum_r = 0;
-  for (int s = 0; s < p.slices; ++s) sum_r += p.ranks[tl.slot * (p.slices + 1) + s];
+  const int sum_r = joined_ranks(p, tl.slot);
   const float scale = lora_scale(p, tl.slot);
   const int n0 = blockIdx.y * W;
   if (n0 >= sum_r) return;
@@ -490,6 +513,10 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
     if (!mbar_wait(&done, 0)) atomicCAS(p.status, 0, kStatusTimeoutTmemFull);
     tc_fence_before_sync();
   }
+  if (warp < W / 32) {                                                 // (while the last products run)
+    const uint32_t bits = __ballot_sync(0xffffffffu, is_rank(p, tl.slot, n0 + threadIdx.x));
+    if (lane == 0) ranks_are[warp] = bits;
+  }
   // Every product is through, and the ring free.  (The other warps wait here and not at the mbarrier: eight warps that poll it
   // slow down the two that work.)
   __syncthreads();
@@ -538,6 +565,8 @@ lora_shrink_many_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_c
 #pragma unroll
     for (int c = 1; c < 8; ++c)
       if (c < C) sum.x += q[c].x, sum.y += q[c].y, sum.z += q[c].z, sum.w += q[c].w;
+    const uint32_t is = ranks_are[v >> 5] >> (v & 31);                 // (ranks behind a padded one of the four are padded)
+    keep_ranks(sum, __popc(is & 15));
     uint2 hi, lo;
     split_h(sum, scale, hi, lo);
     __nv_bfloat16* dst = h + (static_cast<long long>(v / 8) * p.T + row) * 8 + (v & 4);
@@ -555,7 +584,8 @@ static constexpr int kExpandThreads = 128;
 
 // What both kernels find out first: the CTA's slice and groups in it.
 struct LoraRun {
-  int h0, first, r0, r1, N, groups, ga, gb;      // first rank in h, first column of y, ranks (of gate and of up), columns
+  int h0, first, r0, r1, N, groups, ga, gb;      // first rank in h, first column of y, padded ranks (of gate and of up), columns
+  int real0, real1;                              // the ranks that are not padding
   const __nv_bfloat16 *b, *b_up;                 // factors, in blocks of 64 columns (gated: 32)
 };
 
@@ -569,11 +599,14 @@ __device__ __forceinline__ LoraRun lora_run(const LoraParams& p, int slot, int a
   c.b = p.b + max(slot, 0) * p.b_slot;
   const int* ranks = p.ranks + max(slot, 0) * (p.slices + 1);
   if constexpr (GATED) {
-    c.r0 = slot >= 0 ? ranks[0] : 0;
-    c.r1 = slot >= 0 ? ranks[1] : 0;
+    c.real0 = slot >= 0 ? ranks[0] : 0;
+    c.real1 = slot >= 0 ? ranks[1] : 0;
+    c.r0 = padded_rank(c.real0);
+    c.r1 = padded_rank(c.real1);
   } else {
     for (;; ++slice) {
-      c.r0 = slot >= 0 ? ranks[slice] : 0;
+      c.real0 = slot >= 0 ? ranks[slice] : 0;
+      c.r0 = padded_rank(c.real0);
       const int groups = (p.n[slice] + 63) / 64, steps = per ? (groups + per - 1) / per : groups;
       if (at < steps) break;
       at -= steps;
@@ -582,6 +615,7 @@ __device__ __forceinline__ LoraRun lora_run(const LoraParams& p, int slot, int a
       c.b += static_cast<long long>((p.n[slice] + BC - 1) / BC) * c.r0 * BC;
     }
     c.r1 = c.r0;
+    c.real1 = c.real0;
   }
   c.N = p.n[slice];
   c.groups = (c.N + GW - 1) / GW;
@@ -728,6 +762,7 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_few_kernel(cons
         const float4 q = *reinterpret_cast<const float4*>(src + part * p.h_plane);
         sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
       }
+      keep_ranks(sum, GATED && v >= c.r0 ? c.real1 - (v - c.r0) : c.real0 - v);
       uint2 hi, lo;
       split_h(sum, scale, hi, lo);
       *reinterpret_cast<uint2*>(dst + row * p.h_pitch + v) = hi;

@@ -24,7 +24,7 @@ struct PackParams {
   const void* b[kPackSlices];                    // [n, r]
   long long a_row[kPackSlices], a_col[kPackSlices], b_row[kPackSlices], b_col[kPackSlices];
   int a_type[kPackSlices], b_type[kPackSlices];  // 0 bf16, 1 fp16, 2 fp32
-  int r[kPackSlices], rank[kPackSlices], n[kPackSlices];   // ranks, in whole 16; columns
+  int r[kPackSlices], rank[kPackSlices], n[kPackSlices];   // ranks, the same in whole 16, columns
   __nv_bfloat16 *out_a, *out_b;
   int* out_ranks;
   long long a_units, units;                      // of 16 bytes: of A, of both
@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kPackThreads) lora_pack_kernel(const __grid_co
   pdl_wait();
   pdl_trigger();
   const long long u = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x;
-  if (u <= p.slices) p.out_ranks[u] = u < p.slices ? p.rank[u] : p.scale;
+  if (u <= p.slices) p.out_ranks[u] = u < p.slices ? p.r[u] : p.scale;
   if (u >= p.units) return;
   if (u < p.a_units) {
     // [K / 32][rank / 8][4][8][8]

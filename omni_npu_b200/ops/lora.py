@@ -64,10 +64,11 @@ class LoraStack:
             self._block = 32 if interleaved or self._lanes else 64
             self.b = torch.zeros(num_slots, sum((n + self._block - 1) // self._block for n in slices) * self._block * self.max_rank,
                                  dtype=dtype, device=device)
-            # of every slot the ranks (in whole 16) and the bits of the scale
+            # of every slot the ranks and the bits of the scale
             self.ranks = torch.zeros(num_slots, len(slices) + 1, dtype=torch.int32, device=device)
         self.device = self.a.device
         self._ranks = [[0] * len(slices) for _ in range(num_slots)]
+        self._padded = [[0] * len(slices) for _ in range(num_slots)]       # in whole 16, as the factors lie
         self._scales = [0.0] * num_slots
         self.sizes = [in_features, self.max_rank, 0, *slices]
 
@@ -92,17 +93,18 @@ class LoraStack:
                                  f"(r, {self.in_features}) and ({self.slices[i]}, r)")
             if not 1 <= r <= self.max_rank:
                 raise ValueError(f"LoraStack.load: rank {r}, at most {self.max_rank}")
-            ranks.append((r + 15) // 16 * 16)
+            ranks.append(r)
+        padded = [(r + 15) // 16 * 16 for r in ranks]
         if self.device.type == "cuda":
             _count(1)
             _C().lora_pack(self.a, self.b, self.ranks, slot, [self._here(p) for p in a], [self._here(q) for q in b], self.slices,
                            self.in_features, self._lanes, self._block, scale)
         else:
             with torch.inference_mode():
-                for p, view in zip(a, self._views_a(slot, ranks)):
+                for p, view in zip(a, self._views_a(slot, padded)):
                     if view is not None:
                         view.copy_(_padded(p, view.shape[0] * 8, self._k * 32).view(view.shape))
-                for q, view in zip(b, self._views_b(slot, ranks)):
+                for q, view in zip(b, self._views_b(slot, padded)):
                     if view is not None:
                         view.copy_(_padded(q, view.shape[0] * self._block,
                                            view.shape[5] * (16 if self._lanes else 8)).view(view.shape))
@@ -160,7 +162,7 @@ class LoraStack:
 
     def factors(self, slot: int):
         """(A, B) of each slice of a slot (ranks padded to 16), None where it has none."""
-        ranks = self._ranks[slot]
+        ranks = self._padded[slot]
         return [None if a is None else (a.reshape(r, -1)[:, : self.in_features], b.reshape(-1, r)[:n])
                 for a, b, r, n in zip(self._views_a(slot, ranks), self._views_b(slot, ranks), ranks, self.slices)]
 
@@ -171,7 +173,8 @@ class LoraStack:
 
     def _set_ranks(self, slot: int, ranks) -> None:
         self._ranks[slot] = ranks
-        used = [sum(r) for r in self._ranks if any(r)]
+        self._padded[slot] = [(r + 15) // 16 * 16 for r in ranks]
+        used = [sum(r) for r in self._padded if any(r)]
         # input features; largest rank; mean of the loaded adapters' ranks, the slices' together (only speed depends on it); slices
         self.sizes = [self.in_features, self.max_rank, sum(used) // max(1, len(used)), *self.slices]
 

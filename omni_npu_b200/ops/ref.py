@@ -882,6 +882,7 @@ def lora_sum(y: torch.Tensor, x: torch.Tensor, stack, slots: torch.Tensor) -> to
         rows = (slots == s).nonzero().flatten()
         for i, f in enumerate(stack.factors(s)):
             if f is not None:
-                d = (x[rows].float() @ f[0].float().t()) @ f[1].float().t()
+                r = stack._ranks[s][i]                         # (an infinity times a padded rank's zeros would be NaN)
+                d = (x[rows].float() @ f[0][:r].float().t()) @ f[1][:, :r].float().t()
                 z[rows[:, None], stack.columns(i)[None, :]] += d * stack._scales[s]
     return z
