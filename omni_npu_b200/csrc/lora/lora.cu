@@ -1337,14 +1337,16 @@ static int launch_lora(LoraParams& p, bool many, int max_tiles, unsigned chunks,
   return launch_many<ACT>(p, lora_expand_many_kernel<ACT, false>, kExpandManySmem, tiles, chunks, grid, kExpandThreads, smem, once, stream);
 }
 
-// Parts of K that a step's h is summed from, a CTA each (many rows: of a cluster).  Few rows (tiles of 16): as many as the slots
-// let be resident, whatever the number of tokens, so that a row does not depend on it.  Many rows: as many as fill the SMs, given
-// the pieces of 128 ranks that a tile has on average.
+// Parts of K that a step's h is summed from, a CTA each (many rows: of a cluster).  They set the order of the sums, so they follow
+// from the step and the stack's bounds alone, not from the adapters that happen to be loaded beside a token's own.  Few rows (tiles
+// of 16): as many as the slots let be resident, whatever the number of tokens, so that a row does not depend on it.  Many rows: as
+// many as fill the SMs, given the pieces of 128 ranks that a tile may have, in a power of two (clusters of seven: 2048 tokens to
+// 2 x 14336 of a stack of rank 128 79 us, of four or eight 73).  Going by the ranks that are loaded, 8192 tokens of rank 16 in a
+// stack of 128 took 81 us for 84, and with the stack's own rank the same.
 static int lora_parts(int K, int rows, int max_tiles, int num_slots, int chunks) {
-  const int pieces = max_tiles * chunks;
-  const int want = rows < kManyRows ? std::min((K + 511) / 512, 592 / num_slots)
-                                    : std::min((K + 127) / 128, (296 + pieces / 2) / pieces);
-  return std::min(std::max(want, 1), rows < kManyRows ? 16 : 8);
+  if (rows < kManyRows) return std::min(std::max(std::min((K + 511) / 512, 592 / num_slots), 1), 16);
+  const int pieces = max_tiles * chunks, want = std::min((K + 127) / 128, (296 + pieces / 2) / pieces);
+  return want >= 8 ? 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
 }
 
 }  // namespace b200
@@ -1414,7 +1416,7 @@ extern "C" int b200_lora(const void* x, long long x_stride, const void* y, long 
   p.act_limit = act_limit;
   const int width = (many ? kManyChunk : kFewChunk) * 8;
   const unsigned chunks = (p.h_width + width - 1) / width;
-  p.parts = lora_parts(K, rows, max_tiles, num_slots, (mean_rank + width - 1) / width);
+  p.parts = lora_parts(K, rows, max_tiles, num_slots, chunks);
   // the first kernel's ring: two CTAs an SM, or all of it for one where there are too few
   const long long ctas = static_cast<long long>(p.parts) * max_tiles * ((mean_rank + width - 1) / width);
   p.stage_bytes = kXBytes + std::min(p.h_width, width) * kSlab * 2;
