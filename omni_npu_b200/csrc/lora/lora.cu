@@ -152,7 +152,7 @@ struct LoraParams {
   int h_width;                                   // slices * largest rank
   int T, K, slices, parts;
   int stages, stage_bytes;                       // many rows: the first kernel's ring
-  int groups, buffers, max_rank;                         // many rows: groups in flight in the second kernel
+  int groups, buffers, max_rank;                 // many rows, tcgen05: column groups of all slices, groups in flight, bound of the ranks
   int boxes;                                     // 1: rows of x that follow one another are copied as a box
   int* status;
   int per;                                       // column groups of a CTA of the second kernel
@@ -831,6 +831,7 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_few_kernel(cons
 template <int ACT, bool PAIRS>
 __global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_many_kernel(const LoraParams p) {
   constexpr bool GATED = ACT != kActNone, LANES = !PAIRS;
+  static_assert(GATED || LANES, "without an activation, ranks above 32 take the tcgen05 kernel");
   constexpr int BM = 64, STEP = 4, D = PAIRS ? 6 : 4, STAGE = 2048;
   constexpr int GW = GATED ? 32 : 64;                                  // columns of a slice in a group
   extern __shared__ __align__(128) char smem[];
@@ -898,12 +899,11 @@ __global__ void __launch_bounds__(kExpandThreads, PAIRS ? 3 : 4) lora_expand_man
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int steps = GATED && j >= 4 ? k1 : k0;
+      const int steps = j >= 4 ? k1 : k0;
       const __nv_bfloat16* src =
-          GATED ? (j >= 4 ? c.b_up : c.b) + (static_cast<long long>(gi) * steps + min(k, max(steps - 1, 0))) * 512 + (j & 3) * 64
-                : c.b + (static_cast<long long>(gi) * k0 + min(k, k0 - 1)) * 1024 + j * 64;
+          (j >= 4 ? c.b_up : c.b) + (static_cast<long long>(gi) * steps + min(k, max(steps - 1, 0))) * 512 + (j & 3) * 64;
       v[j].x = *reinterpret_cast<const uint32_t*>(src + lane * 2);
-      v[j].y = *reinterpret_cast<const uint32_t*>(src + lane * 2 + (GATED ? 256 : 512));
+      v[j].y = *reinterpret_cast<const uint32_t*>(src + lane * 2 + 256);
     }
   };
   if (ks > 0 && ga < gb) {
