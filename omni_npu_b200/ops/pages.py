@@ -30,6 +30,11 @@ class CacheBlocks:
             if t.stride(-1) != 1 or t.stride(-2) != t.shape[-1] or row % 16 or head % 16 or t.stride(0) * size % 16 \
                     or t.data_ptr() % 16 or t.numel() == 0:
                 raise ValueError("CacheBlocks: rows of a head lie one after another and are multiples of 16 bytes, not none")
+            span = t.shape[-2] * t.shape[-1]                   # elements of a head, then from the first to the last of several
+            for stride, n in sorted((t.stride(i), t.shape[i]) for i in range(t.dim() - 2) if t.shape[i] > 1):
+                if stride < span:
+                    raise ValueError("CacheBlocks: pages or heads of a tensor overlap")
+                span += (n - 1) * stride
             desc.append([t.data_ptr(), t.stride(0) * size, head, heads | (row // 16) << 32])
             self._max_vecs = max(self._max_vecs, heads * self.block_size * (row // 16))
         self._desc = torch.tensor(desc, dtype=torch.int64, device=self.device) if first.is_cuda else None
