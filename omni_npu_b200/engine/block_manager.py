@@ -139,6 +139,9 @@ class BlockPool:
                 del self._cached_free[b]
                 self._free.append(b)
 
+    def unregister_all(self) -> None:
+        self.unregister(list(self._hash_of))
+
     def match_prefix(self, hashes: Sequence[bytes]) -> List[int]:
         """Blocks holding the longest cached prefix of the hash chain (not yet acquired)."""
         out: List[int] = []

@@ -430,6 +430,7 @@ class LLM:
         only between requests.  Returns the bytes released."""
         if self.engine.has_unfinished_requests():
             raise RuntimeError("sleep() while requests are running")
+        self.engine.scheduler.pool.unregister_all()          # (what cached prefixes held is discarded)
         return self.engine.worker.sleep(level)
 
     def wake_up(self, tags=None) -> int:

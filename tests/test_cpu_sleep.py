@@ -150,3 +150,19 @@ def test_the_server_sleeps_when_no_adapter_is_being_loaded(pool):
         assert client.post("/wake_up").status_code == 200
     app.state.engine_loop.shutdown()
     assert held == [True, True]
+
+
+def test_cached_prefixes_are_forgotten_with_the_cache(pool):
+    p = list(range(5, 25))
+    sp = SamplingParams(max_tokens=5, ignore_eos=True)
+    want = _llm().generate([p], sp)[0].output_token_ids
+    llm = _llm(enable_prefix_caching=True)
+    assert llm.generate([p], sp)[0].output_token_ids == want
+    for t in llm.engine.worker.model_runner.page_cache.tensors:
+        t.fill_(7.0)                                            # what the device may hold after the wake-up
+    llm.sleep(1)
+    llm.wake_up()
+    stats = llm.engine.scheduler.prefix_stats
+    assert llm.generate([p], sp)[0].output_token_ids == want and stats["hit_tokens"] == 0
+    assert llm.generate([p], sp)[0].output_token_ids == want and stats["hit_tokens"] == 16
+    assert llm.engine.scheduler.pool.num_free == 64
