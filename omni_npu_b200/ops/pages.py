@@ -31,7 +31,8 @@ class CacheBlocks:
                     or t.data_ptr() % 16 or t.numel() == 0:
                 raise ValueError("CacheBlocks: rows of a head lie one after another and are multiples of 16 bytes, not none")
             span = t.shape[-2] * t.shape[-1]                   # elements of a head, then from the first to the last of several
-            for stride, n in sorted((t.stride(i), t.shape[i]) for i in range(t.dim() - 2) if t.shape[i] > 1):
+            outer = () if t.is_contiguous() else range(t.dim() - 2)
+            for stride, n in sorted((t.stride(i), t.shape[i]) for i in outer if t.shape[i] > 1):
                 if stride < span:
                     raise ValueError("CacheBlocks: pages or heads of a tensor overlap")
                 span += (n - 1) * stride
