@@ -145,6 +145,7 @@ def test_the_served_models_name_stays_the_served_models(server, tmp_path):
     want = client.post("/v1/completions", json=body).json()["choices"][0]["token_ids"]
     assert client.post("/v1/load_lora_adapter", json={"lora_name": "base", "lora_path": path}).status_code == 400
     llm.load_adapter("base", path)                            # (not over HTTP)
-    assert llm.generate([[5, 6, 7, 8]], adapter="base", sampling_params=SamplingParams(max_tokens=6, ignore_eos=True)
-                        )[0].output_token_ids != want
+    with loop.lock:                                           # (the server's thread steps the engine otherwise)
+        other = llm.generate([[5, 6, 7, 8]], SamplingParams(max_tokens=6, ignore_eos=True), adapter="base")[0].output_token_ids
+    assert other != want
     assert client.post("/v1/completions", json=body).json()["choices"][0]["token_ids"] == want
