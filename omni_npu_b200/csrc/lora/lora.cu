@@ -24,8 +24,9 @@
 // so that many small pieces of work even out adapters of unlike ranks (one cluster per tile for both, h in distributed shared
 // memory, took 56 us where this takes 15: 128 tokens of 31 adapters of ranks 8 to 64).  The second is launched while the first
 // runs and has its first y and factors at hand by the time h is there.  Measured (us, and the time of the bytes at 6.56 TB/s):
-// one token 4.5; 128 tokens of 128 adapters of rank 16, 14336 to 4096 18.2 / 12.4; 8192 tokens of 8, 4096 to 6144 56 / 42;
-// the same to 2 x 14336 with silu, rank 32 167 / 121; 8192 tokens of rank 64, 4096 to 6144 72 / 42, of rank 128 100.
+// one token 4.5; 128 tokens of 128 adapters of rank 16, 14336 to 4096 18.1 / 12.4; 8192 tokens of 8, 4096 to 6144 56 / 42;
+// the same to 2 x 14336 with silu, rank 32 166 / 121 in a short graph at 1.97 GHz, 185 called without a pause, which reaches the
+// power limit (1.70 GHz); 8192 tokens of rank 64, 4096 to 6144 72 / 42, of rank 128 102.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -826,6 +827,8 @@ __global__ void __launch_bounds__(kExpandThreads, 4) lora_expand_few_kernel(cons
 // ---- many rows, up to 32 ranks: mma.sync, half a tile's rows, a warp has every fourth group.  y starts the accumulators, and B stays
 // in registers for the 64 rows: little to compute, so that four CTAs an SM keep memory busy (8192 tokens of rank 16, 4096 to
 // 6144: 33 us for 31 of bytes; the tcgen05 kernel takes 4 to 10 more, gated 9 to 35).
+// Gated, rank 32, 14336 columns: 147 us, issue slots half busy; four CTAs are too few warps (14.6 counted) for the chain of loads,
+// products, activation and store, whose fixed latencies are what they wait for first.
 // PAIRS: gated ranks above 144, whose h the tcgen05 kernel has no room for.  Every step of 16 ranks is used for 32 rows, and the
 // registers take the step after next meanwhile.
 template <int ACT, bool PAIRS>

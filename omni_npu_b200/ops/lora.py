@@ -16,10 +16,10 @@ from . import SILU, _C, _act_kind, _count, device_state, ref
 MAX_SLOTS, MAX_SLICES, MAX_RANK, LANES_RANK = 512, 4, 256, 32
 
 # Tokens of one adapter that are taken together.  Up to this many tokens of a step: tiles of 16, one matrix instruction high,
-# through kernels that stream the factors; above, tiles of 128.  Us, tiles of 128 / 16: 200 tokens of 8 adapters of rank 16,
-# 4096 to 4096 + 1024 + 1024 12.3 / 8.1, 14336 to 4096 17.8 / 8.5; 768 tokens 16.7 / 13.9 and 20.8 / 14.7; 1000 tokens 17.1 /
-# 19.1 and 21.8 / 16.3; 768 tokens of 8 of rank 64 21.1 / 26.5.  A row's result does not depend on the rows beside it as long as
-# these are no more.
+# through kernels that stream the factors; above, tiles of 128.  The rule sees the number of tokens alone.  Us, tiles of 128 / 16:
+# 200 tokens of 8 adapters of rank 16, 4096 to 4096 + 1024 + 1024 12.3 / 8.1, 14336 to 4096 17.8 / 8.5; 768 tokens 16.7 / 13.9 and
+# 20.8 / 14.7; 1000 tokens 17.1 / 19.1.  Where it loses: 768 tokens of 8 of rank 64 21.1 / 26.5 (taken in 16), 1000 tokens 14336
+# to 4096 21.8 / 16.3 (taken in 128).  A row's result does not depend on the rows beside it as long as these are no more.
 FEW_TOKENS, FEW_ROWS, MANY_ROWS = 768, 16, 128
 
 
@@ -34,7 +34,9 @@ class LoraStack:
 
     ``slices``: columns of the parts of a joined projection (query, key and value; gate and up), each with factors of its
     own.  ``interleaved``: two equal slices whose columns alternate in groups of eight, gate first, as the gated products
-    store them.  Slots start empty: tokens of an empty slot get the shared product alone."""
+    store them.  Slots start empty: tokens of an empty slot get the shared product alone.  Factors are finite.
+
+    The kernels are chosen, and the work is dealt, by ``max_rank`` and ``num_slots``: neither larger than needed."""
 
     def __init__(self, num_slots: int, max_rank: int, in_features: int, slices: Sequence[int], device=None,
                  dtype: torch.dtype = torch.bfloat16, interleaved: bool = False) -> None:
